@@ -169,6 +169,73 @@ int matmul_launch_noalloc(void *context, int implementation, int precision,
                           const void *a, const void *b, float *c, int m, int k, int n,
                           void *stream, char *error, size_t error_size);
 
+/* ------------------------------------------------------------------ operators
+ * No counterparts in the reference.  Products with more fused to them, on the
+ * tensor cores, in the manner of matmul_launch: asynchronous on `stream`, graph
+ * capturable, matrices row-major and owned by the caller, base pointers aligned
+ * to their element, any sizes >= 1 that fit in an int.  `precision` is 1 (tf32),
+ * 2 (fp16) or 3 (bf16) and names the format of the product's operands; sums and
+ * everything else inside are FP32.  An output or an auxiliary operand followed by
+ * a flag `x_fp32` is FP32 when the flag is not 0, otherwise in the input format
+ * (rounded to it once, to nearest even).  Operands that TMA cannot address are
+ * repacked first, and other scratch is stream-ordered, as in matmul_launch.  The
+ * caller's current device is the same after the call.  A wait that runs out is
+ * reported and leaves NaN as in matmul_set_wait_limit.  Outputs must not overlap
+ * inputs or each other unless said otherwise.
+ *
+ * Activations: 0 none, 1 relu, 2 gelu (erf), 3 gelu by tanh, 4 silu. */
+
+/* out = act(a b + bias) + residual, a m x k, b k x n, out m x n.  bias (n
+ * values), residual (m x n, in out's format) and preact may be null; preact
+ * receives a b + bias, which the backward pass needs.  residual may be out. */
+int matmul_epilogue(void *context, int precision, const void *a, const void *b, const void *bias, int bias_fp32,
+                    int activation, const void *residual, void *out, int out_fp32, void *preact, int preact_fp32,
+                    int m, int k, int n, void *stream, char *error, size_t error_size);
+
+/* Gradients of matmul_epilogue for dout (m x n, input format): dz = dout *
+ * act'(preact), da = dz b^T, db = a^T dz, dbias = dz's column sums.  Null for a
+ * gradient leaves it out (a is read for db only, b for da only); preact is not
+ * read when the activation is 0.  dz is rounded to the input format for the two
+ * products; dbias sums the unrounded values, in a fixed order. */
+int matmul_epilogue_backward(void *context, int precision, const void *dout, const void *a, const void *b,
+                             const void *preact, int preact_fp32, int activation, void *da, int da_fp32, void *db,
+                             int db_fp32, void *dbias, int dbias_fp32, int m, int k, int n, void *stream, char *error,
+                             size_t error_size);
+
+/* Products grouped by expert: out[i] = a[i] b[g] for the rows offsets[g] <= i <
+ * offsets[g + 1] of a (rows x k), b groups x k x n, out rows x n.  offsets:
+ * groups + 1 values on the device (int64 when offsets64, else int32), read when
+ * the kernel runs; values outside [0, rows] are clipped and one below an earlier
+ * one counts as equal to it.  Rows of no group are not written. */
+int matmul_grouped(void *context, int precision, const void *a, const void *b, const void *offsets, int offsets64,
+                   int groups, void *out, int out_fp32, int rows, int k, int n, void *stream, char *error,
+                   size_t error_size);
+
+/* Gradients of matmul_grouped for dout (rows x n): da[i] = dout[i] b[g]^T (rows
+ * of no group are not written), db[g] = sum over g's rows of a[i]^T dout[i]
+ * (zeros for an empty group).  Null for either leaves it out. */
+int matmul_grouped_backward(void *context, int precision, const void *dout, const void *a, const void *b,
+                            const void *offsets, int offsets64, int groups, void *da, int da_fp32, void *db,
+                            int db_fp32, int rows, int k, int n, void *stream, char *error, size_t error_size);
+
+/* Softmax cross entropy of the logits z = hidden weight (m x k, k x v), which are
+ * not stored: lse = log sum exp of each row, loss = lse - z[label].  labels: m
+ * values (int64 when labels64, else int32); a row whose label is ignore_index has
+ * loss 0, any other label outside [0, v) gives NaN. */
+int matmul_cross_entropy(void *context, int precision, const void *hidden, const void *weight, const void *labels,
+                         int labels64, long long ignore_index, float *loss, float *lse, int m, int k, int v,
+                         void *stream, char *error, size_t error_size);
+
+/* Gradients of matmul_cross_entropy for grad (m values): dz = grad (exp(z - lse) -
+ * [column == label]), zero for ignored rows, dhidden = dz weight^T, dweight =
+ * hidden^T dz, in pieces of the vocabulary with z computed again.  dz is held in
+ * the input format, so fp16, which cannot hold the small ones, is refused.  Null
+ * for either gradient leaves it out. */
+int matmul_cross_entropy_backward(void *context, int precision, const float *grad, const void *hidden,
+                                  const void *weight, const void *labels, int labels64, long long ignore_index,
+                                  const float *lse, void *dhidden, int dhidden_fp32, void *dweight, int dweight_fp32,
+                                  int m, int k, int v, void *stream, char *error, size_t error_size);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,7 +2,7 @@
 
     python matrix-multiplication_b200/build.py [--verbose-ptxas]
 
-Compiles ``csrc/matmul_b200.cu`` for sm_100a only into ``build/b200_matmul.so``
+Compiles ``csrc/*.cu`` (in parallel) for sm_100a only into ``build/b200_matmul.so``
 at the repository root (the same place relative to the loader as the
 reference's ``build/matmul.so``).  The CUDA runtime is linked statically and
 the driver API is reached through ``cudaGetDriverEntryPoint``, so the library
@@ -17,11 +17,13 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
-SOURCE = PACKAGE / "csrc" / "matmul_b200.cu"
+SOURCES = sorted((PACKAGE / "csrc").glob("*.cu"))
 HEADERS = sorted((PACKAGE / "csrc").glob("*.cuh")) + [ROOT / "include" / "b200_matmul.h"]
 OUTPUT = ROOT / "build" / "b200_matmul.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -34,18 +36,40 @@ def nvcc() -> str:
 
 
 def command(output: Path = OUTPUT, verbose_ptxas: bool = False) -> list[str]:
+    """The one-step form of the build: every source into the shared library."""
     cmd = [nvcc(), "-O3", "-std=c++17", *ARCH_FLAGS, "-lineinfo", "-shared", "-Xcompiler", "-fPIC",
-           "-cudart", "static", "-I", str(ROOT / "include"), "-o", str(output), str(SOURCE)]
+           "-cudart", "static", "-I", str(ROOT / "include"), "-o", str(output), *map(str, SOURCES)]
     if verbose_ptxas:
         cmd[1:1] = ["-Xptxas", "-v"]
     return cmd
+
+
+def compile_command(source: Path, target: Path, verbose_ptxas: bool = False) -> list[str]:
+    """One source into an object file."""
+    cmd = [nvcc(), "-O3", "-std=c++17", *ARCH_FLAGS, "-lineinfo", "-Xcompiler", "-fPIC", "-I", str(ROOT / "include"),
+           "-c", "-o", str(target), str(source)]
+    if verbose_ptxas:
+        cmd[1:1] = ["-Xptxas", "-v"]
+    return cmd
+
+
+def link_command(objects: list[Path], output: Path) -> list[str]:
+    return [nvcc(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-cudart", "static", "-o", str(output),
+            *map(str, objects)]
 
 
 def up_to_date(output: Path = OUTPUT) -> bool:
     if not output.exists():
         return False
     built = output.stat().st_mtime
-    return all(path.stat().st_mtime <= built for path in [SOURCE, *HEADERS, Path(__file__)])
+    return all(path.stat().st_mtime <= built for path in [*SOURCES, *HEADERS, Path(__file__)])
+
+
+def _run(cmd: list[str]) -> str:
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"nvcc failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
+    return result.stderr
 
 
 def build(force: bool = False, verbose_ptxas: bool = False, output: Path = OUTPUT) -> Path:
@@ -53,13 +77,15 @@ def build(force: bool = False, verbose_ptxas: bool = False, output: Path = OUTPU
     if not force and not verbose_ptxas and up_to_date(output):
         return output
     output.parent.mkdir(parents=True, exist_ok=True)
-    tmp = output.with_suffix(".so.tmp")
-    result = subprocess.run(command(tmp, verbose_ptxas), capture_output=True, text=True)
-    if result.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
-    if verbose_ptxas:
-        print(result.stderr, file=sys.stderr)
-    os.replace(tmp, output)
+    with tempfile.TemporaryDirectory(dir=output.parent) as folder:
+        objects = [Path(folder) / f"{source.stem}.o" for source in SOURCES]
+        tmp = Path(folder) / output.name
+        with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
+            texts = list(pool.map(_run, [compile_command(s, o, verbose_ptxas) for s, o in zip(SOURCES, objects)]))
+        _run(link_command(objects, tmp))
+        if verbose_ptxas:
+            print("\n".join(texts), file=sys.stderr)
+        os.replace(tmp, output)
     return output
 
 

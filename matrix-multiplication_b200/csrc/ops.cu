@@ -1,0 +1,878 @@
+// C-ABI of the operators next to matmul_launch: the product with bias, activation and
+// residual in its epilogue, products grouped by expert, and softmax cross entropy over
+// a large vocabulary, each with its gradient.  Declarations and contracts:
+// include/b200_matmul.h; kernels: tc_ops.cuh, ops_aux.cuh.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <initializer_list>
+
+#include "context.cuh"
+#include "ops.cuh"
+#include "ops_plan.cuh"
+
+namespace {
+
+using namespace b200;
+
+constexpr int kTf32 = 1, kFp16 = 2, kBf16 = 3;     // precision ids of the ABI
+
+// Makes a device current for a call and puts the caller's back.
+struct DeviceScope {
+    int previous = -1;
+    cudaError_t status;
+    explicit DeviceScope(int device)
+    {
+        status = cudaGetDevice(&previous);
+        if (status == cudaSuccess && previous != device)
+            status = cudaSetDevice(device);
+        else if (status == cudaSuccess)
+            previous = -1;
+    }
+    ~DeviceScope()
+    {
+        if (previous >= 0)
+            cudaSetDevice(previous);
+    }
+};
+
+const OpKernels &kernels_of(int precision)
+{
+    return precision == kTf32 ? kOpKernelsTF32 : precision == kFp16 ? kOpKernelsF16 : kOpKernelsBF16;
+}
+
+int element(int precision)
+{
+    return precision == kTf32 ? 4 : 2;
+}
+
+CUtensorMapDataType operand_type(int precision)
+{
+    return precision == kTf32   ? CU_TENSOR_MAP_DATA_TYPE_TFLOAT32
+           : precision == kFp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// A row-major matrix, or `groups` of them `slab` elements apart.
+struct Matrix {
+    const void *ptr = nullptr;
+    int64_t rows = 0, cols = 0, pitch = 0;
+    int64_t groups = 1, slab = 0;
+};
+
+// One call: its context, format, stream and stream-ordered scratch.  Scratch is asked
+// for with reserve() first, taken by one allocation, and given back to the stream when
+// the call returns, after everything it enqueued.
+struct Call {
+    Context *ctx;
+    int precision;
+    cudaStream_t stream;
+    const char *name;
+    char *error;
+    size_t error_size;
+    uint8_t *scratch = nullptr;
+    size_t scratch_bytes = 0;
+
+    ~Call()
+    {
+        if (scratch)
+            cudaFreeAsync(scratch, stream);
+    }
+    int failed(const char *detail) { return fail(error, error_size, name, detail); }
+    int failed(cudaError_t st) { return fail_cuda(error, error_size, name, st); }
+    const OpKernels &kernels() const { return kernels_of(precision); }
+    int elem() const { return element(precision); }
+
+    size_t reserve(size_t bytes)
+    {
+        const size_t at = scratch_bytes;
+        scratch_bytes += (bytes + 255) / 256 * 256;
+        return at;
+    }
+    int allocate()
+    {
+        if (!scratch_bytes)
+            return 0;
+        void *ptr = nullptr;
+        const cudaError_t st = scratch_alloc(ctx, &ptr, scratch_bytes, stream);
+        if (st != cudaSuccess)
+            return fail_cuda(error, error_size, name, st);
+        scratch = static_cast<uint8_t *>(ptr);
+        return 0;
+    }
+};
+
+// An operand that TMA can address: the caller's matrix, or its copy in scratch with rows
+// padded to 16 bytes (unaligned bases and row pitches).
+struct Operand {
+    Matrix source;
+    Matrix ready;
+    bool direct = true;
+    size_t at = 0;
+
+    void plan(Call &c, const void *ptr, int64_t rows, int64_t cols, int64_t groups = 1)
+    {
+        source = Matrix{ptr, rows, cols, cols, groups, rows * cols};
+        direct = aligned16(ptr) && cols * c.elem() % 16 == 0;
+        ready = source;
+        if (!direct) {
+            ready.pitch = round_up(cols, 16 / c.elem());
+            ready.slab = rows * ready.pitch;
+            at = c.reserve(static_cast<size_t>(groups * ready.slab * c.elem()));
+        }
+    }
+    int prepare(Call &c)
+    {
+        if (direct)
+            return 0;
+        ready.ptr = c.scratch + at;
+        const cudaError_t st = c.kernels().repack(source.ptr, c.scratch + at, source.rows * source.groups, source.cols,
+                                                  ready.pitch, c.ctx->sm_count, c.stream);
+        return st == cudaSuccess ? 0 : c.failed(st);
+    }
+};
+
+bool encode_3d(const Context *ctx, CUtensorMap *map, CUtensorMapDataType type, const Matrix &m, int elem,
+               uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle)
+{
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(m.cols), static_cast<cuuint64_t>(m.rows),
+                                static_cast<cuuint64_t>(m.groups)};
+    const cuuint64_t row = static_cast<cuuint64_t>(m.pitch) * elem;
+    const cuuint64_t slab = m.groups > 1 ? static_cast<cuuint64_t>(m.slab) * elem : row * m.rows;
+    const cuuint64_t strides[2] = {row, slab};
+    const cuuint32_t box[3] = {box_inner, box_rows, 1};
+    const cuuint32_t steps[3] = {1, 1, 1};
+    return ctx->encode(map, type, 3, const_cast<void *>(m.ptr), dims, strides, box, steps,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// An operand's map: K-major tiles are boxes of 128 bytes of K x `extent` rows,
+// MN-major tiles boxes of 128 bytes of M/N x one K block of rows.
+bool operand_map(const Call &c, CUtensorMap *map, const Matrix &m, bool mn_major, int extent)
+{
+    const uint32_t inner = static_cast<uint32_t>(OP_ROW_BYTES / c.elem());
+    const CUtensorMapSwizzle swizzle = mn_major && c.precision == kTf32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
+                                                                        : CU_TENSOR_MAP_SWIZZLE_128B;
+    return encode_3d(c.ctx, map, operand_type(c.precision), m, c.elem(), inner,
+                     mn_major ? inner : static_cast<uint32_t>(extent), swizzle);
+}
+
+// Whether TMA can write an output, and its map (boxes of 128 rows x 128 bytes).
+bool output_tma(const Matrix &m, int elem)
+{
+    return aligned16(m.ptr) && m.pitch * elem % 16 == 0 && (m.groups == 1 || m.slab * elem % 16 == 0);
+}
+
+bool output_map(const Call &c, CUtensorMap *map, const Matrix &m, bool half)
+{
+    const CUtensorMapDataType type = half ? operand_type(c.precision) : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    return encode_3d(c.ctx, map, type, m, half ? 2 : 4, half ? 64 : 32, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+struct TileShape {
+    int ctas, bm, bn;     // CTAs per tile, D's rows and columns per tile
+};
+constexpr TileShape kTileShapes[] = {{2, 256, 256}, {1, 128, 128}, {1, 128, 64}, {1, 128, 16},
+                                     {1, 128, 32},  {1, 128, 64},  {1, 128, 128}};
+
+bool is_swap(int tile)
+{
+    return tile >= kSwap16;
+}
+
+// Estimated cycles of `tiles` tiles of a kind with K blocks of 128 bytes: the model and
+// the constants of the plain product's plan (matmul_b200.cu): a K block costs the most
+// of its MMA time, its operand bytes into one SM at 55 B/cycle, and all running CTAs'
+// bytes out of L2 at 8 KB/cycle.
+double tile_cycles(const Context *ctx, int tile, double tiles, double k_blocks)
+{
+    const TileShape &t = kTileShapes[tile];
+    const double units = t.ctas == 2 ? ctx->max_pairs : ctx->sm_count;
+    const double active = t.ctas * std::min(tiles, units);
+    const double rounds = std::max(1.0, std::ceil(tiles / units));
+    const double bytes = static_cast<double>(OP_BM + t.bn / t.ctas) * OP_ROW_BYTES;
+    const double k_cycles = std::max({2.0 * t.bn, bytes / 55.0, active * bytes / 8000.0});
+    return 2000.0 + rounds * (k_blocks * k_cycles + 4000.0 * t.bn / 256.0) + (t.ctas == 2 ? 10000.0 : 0.0);
+}
+
+int choose_tile(const Context *ctx, int64_t m, int64_t n, int64_t k_blocks, int64_t groups = 1)
+{
+    int best = kSingle64;
+    double best_cycles = 0.0;
+    for (int tile : {kPair256, kSingle128, kSingle64}) {
+        const TileShape &t = kTileShapes[tile];
+        if (t.ctas == 2 && (ctx->max_pairs < 1 || m <= OP_BM))
+            continue;
+        const double tiles = static_cast<double>((m + t.bm - 1) / t.bm) * static_cast<double>((n + t.bn - 1) / t.bn) *
+                             static_cast<double>(groups);
+        const double cycles = tile_cycles(ctx, tile, tiles, static_cast<double>(k_blocks));
+        if (best_cycles == 0.0 || cycles < best_cycles) {
+            best = tile;
+            best_cycles = cycles;
+        }
+    }
+    return best;
+}
+
+// A product with everything but its tile-dependent parts: operands as stored, sizes, and
+// in `launch` the epilogue's parameters.
+struct Product {
+    Matrix a, b;             // kNN: M x K, K x N;  kNT: M x K, N x K;  kTN: K x M, K x N
+    int64_t m = 0, n = 0, k = 0;
+    OpLaunch launch;
+};
+
+int enqueue(Call &c, Product &q)
+{
+    OpLaunch &l = q.launch;
+    const TileShape &t = kTileShapes[l.tile];
+    const bool swap = is_swap(l.tile);
+    const bool a_mn = l.layout == kTN, b_mn = l.layout != kNT;
+    const int b_cols = t.bn / t.ctas;
+    bool ok;
+    if (swap)     // D = B^T A^T: B's columns on the M side, A's rows on the N side
+        ok = operand_map(c, &l.map_a, q.b, true, OP_BM) && operand_map(c, &l.map_b, q.a, false, b_cols);
+    else
+        ok = operand_map(c, &l.map_a, q.a, a_mn, OP_BM) && operand_map(c, &l.map_b, q.b, b_mn, b_cols);
+    if (!ok) {
+        cudaGetLastError();
+        return c.failed("cuTensorMapEncodeTiled rejected an operand");
+    }
+    OpParams &p = l.p;
+    p.m = static_cast<int>(q.m);
+    p.n = static_cast<int>(q.n);
+    const int64_t side_m = swap ? q.n : q.m, side_n = swap ? q.m : q.n;
+    p.num_m_blocks = static_cast<int>((side_m + t.bm - 1) / t.bm);
+    p.num_n_blocks = static_cast<int>((side_n + t.bn - 1) / t.bn);
+    const int bk = OP_ROW_BYTES / c.elem();
+    p.num_k_blocks = static_cast<int>((q.k + bk - 1) / bk);
+    int64_t tiles = static_cast<int64_t>(p.num_m_blocks) * p.num_n_blocks;
+    if (p.grouping == kGroupedK)
+        tiles *= p.groups;
+    else if (p.grouping == kGroupedRows)     // at most this many; the plan on the device has the number
+        tiles = (q.m / (swap ? t.bn : t.bm) + std::min<int64_t>(p.groups, q.m)) *
+                (swap ? p.num_m_blocks : p.num_n_blocks);
+    if (tiles > 0x7fffffff)
+        return c.failed("too many output tiles");
+    p.num_tiles = static_cast<int>(tiles);
+    if (p.raster == 0)
+        p.raster = swap ? p.num_m_blocks : t.ctas == 2 ? 8 : 16;
+    p.status = c.ctx->status;
+    p.wait_limit_ns = wait_limit(c.ctx);
+    const int64_t units = t.ctas == 2 ? c.ctx->max_pairs : c.ctx->sm_count;
+    l.grid = static_cast<int>(std::min(tiles, units)) * t.ctas;
+    const cudaError_t st = c.kernels().product(l, c.stream);
+    return st == cudaSuccess ? 0 : c.failed(st);
+}
+
+// Points a product's epilogue at an output matrix.
+int set_output(Call &c, OpLaunch &l, const Matrix &out, bool half)
+{
+    OpParams &p = l.p;
+    p.out = const_cast<void *>(out.ptr);
+    p.out_pitch = out.pitch;
+    p.out_slab = out.slab;
+    p.out_half = half ? 1 : 0;
+    p.out_tma = output_tma(out, half ? 2 : 4) ? 1 : 0;
+    if (p.out_tma && !output_map(c, &l.map_c, out, half)) {
+        cudaGetLastError();
+        return c.failed("cuTensorMapEncodeTiled rejected an output");
+    }
+    return 0;
+}
+
+// ---------------------------------------------------------------- argument checks
+int check_call(void *opaque, int precision, const char *name, char *error, size_t error_size)
+{
+    clear_error(error, error_size);
+    if (!opaque)
+        return fail(error, error_size, name, "context is null");
+    if (precision != kTf32 && precision != kFp16 && precision != kBf16)
+        return fail(error, error_size, name, "the precision must be 1 (tf32), 2 (fp16) or 3 (bf16)");
+    return 0;
+}
+
+bool misaligned(const void *ptr, int bytes)
+{
+    return reinterpret_cast<uintptr_t>(ptr) % static_cast<uintptr_t>(bytes) != 0;
+}
+
+bool aligned_to(std::initializer_list<std::pair<const void *, int>> pointers)
+{
+    for (const auto &p : pointers)
+        if (p.first && misaligned(p.first, p.second))
+            return false;
+    return true;
+}
+
+} // namespace
+
+namespace b200 {
+
+// Called by matmul_create with the device current.
+cudaError_t setup_operators()
+{
+    for (const OpKernels *k : {&kOpKernelsF16, &kOpKernelsBF16, &kOpKernelsTF32}) {
+        const cudaError_t st = k->setup();
+        if (st != cudaSuccess)
+            return st;
+    }
+    return cudaSuccess;
+}
+
+} // namespace b200
+
+extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const void *b, const void *bias,
+                               int bias_fp32, int activation, const void *residual, void *out, int out_fp32,
+                               void *preact, int preact_fp32, int m, int k, int n, void *stream, char *error,
+                               size_t error_size)
+{
+    const char *name = "matmul_epilogue";
+    if (check_call(opaque, precision, name, error, error_size))
+        return 1;
+    Call c{static_cast<Context *>(opaque), precision, static_cast<cudaStream_t>(stream), name, error, error_size};
+    if (!a || !b || !out)
+        return c.failed("matrix pointer is null");
+    if (m <= 0 || k <= 0 || n <= 0)
+        return c.failed("dimensions must be positive");
+    if (activation < kActNone || activation > kActSilu)
+        return c.failed("unknown activation");
+    const int e = c.elem();
+    const bool out_half = e == 2 && !out_fp32, preact_half = e == 2 && !preact_fp32, bias_half = e == 2 && !bias_fp32;
+    if (!aligned_to({{a, e}, {b, e}, {out, out_half ? 2 : 4}, {residual, out_half ? 2 : 4},
+                     {preact, preact_half ? 2 : 4}, {bias, bias_half ? 2 : 4}}))
+        return c.failed("a pointer is not aligned to its element size");
+    DeviceScope device(c.ctx->device);
+    if (device.status != cudaSuccess)
+        return c.failed(device.status);
+    Operand oa, ob;
+    oa.plan(c, a, m, k);
+    ob.plan(c, b, k, n);
+    if (c.allocate() || oa.prepare(c) || ob.prepare(c))
+        return 1;
+    Product q;
+    q.a = oa.ready;
+    q.b = ob.ready;
+    q.m = m;
+    q.n = n;
+    q.k = k;
+    OpLaunch &l = q.launch;
+    const int bk = OP_ROW_BYTES / e;
+    if (m <= 64) {
+        l.tile = m <= 16 ? kSwap16 : m <= 32 ? kSwap32 : kSwap64;
+        l.epilogue = kEpiStoreT;
+    } else {
+        l.tile = choose_tile(c.ctx, m, n, (static_cast<int64_t>(k) + bk - 1) / bk);
+        l.epilogue = kEpiStore;
+    }
+    const Matrix mo{out, m, n, n};
+    if (set_output(c, l, mo, out_half))
+        return 1;
+    OpParams &p = l.p;
+    p.bias = bias;
+    p.bias_half = bias_half ? 1 : 0;
+    p.activation = activation;
+    p.residual = residual;
+    p.residual_half = p.out_half;
+    p.residual_vec = residual && aligned16(residual) && static_cast<int64_t>(n) * (out_half ? 2 : 4) % 16 == 0;
+    if (preact) {
+        const Matrix mz{preact, m, n, n};
+        p.preact = preact;
+        p.preact_half = preact_half ? 1 : 0;
+        p.preact_tma = output_tma(mz, preact_half ? 2 : 4) ? 1 : 0;
+        if (p.preact_tma && !output_map(c, &l.map_z, mz, preact_half)) {
+            cudaGetLastError();
+            return c.failed("cuTensorMapEncodeTiled rejected an output");
+        }
+    }
+    return enqueue(c, q);
+}
+
+namespace {
+
+// dz = dout * act'(preact) into `dz` (pitch dz_pitch; null without an activation) and
+// dbias, the column sums, through `partial` ([chunks][n]) when there are several chunks.
+struct ActGradPlan {
+    int chunks = 1, rows_per_chunk = 0;
+    void choose(const Context *ctx, int m, int n)
+    {
+        // About eight blocks per SM, at least 32 rows each.
+        const int64_t column_blocks = (static_cast<int64_t>(n) + AG_COLS - 1) / AG_COLS;
+        const int64_t wanted = std::max<int64_t>(1, 8LL * ctx->sm_count / column_blocks);
+        int64_t rows = std::max<int64_t>(32, (m + wanted - 1) / wanted);
+        rows = (rows + 7) / 8 * 8;
+        chunks = static_cast<int>((m + rows - 1) / rows);
+        rows_per_chunk = static_cast<int>(rows);
+    }
+};
+
+} // namespace
+
+extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void *dout, const void *a, const void *b,
+                                        const void *preact, int preact_fp32, int activation, void *da, int da_fp32,
+                                        void *db, int db_fp32, void *dbias, int dbias_fp32, int m, int k, int n,
+                                        void *stream, char *error, size_t error_size)
+{
+    const char *name = "matmul_epilogue_backward";
+    if (check_call(opaque, precision, name, error, error_size))
+        return 1;
+    Call c{static_cast<Context *>(opaque), precision, static_cast<cudaStream_t>(stream), name, error, error_size};
+    if (!dout || (da && !b) || (db && !a) || (activation != kActNone && !preact))
+        return c.failed("matrix pointer is null");
+    if (!da && !db && !dbias)
+        return c.failed("no gradient is asked for");
+    if (m <= 0 || k <= 0 || n <= 0)
+        return c.failed("dimensions must be positive");
+    if (activation < kActNone || activation > kActSilu)
+        return c.failed("unknown activation");
+    const int e = c.elem();
+    const bool da_half = e == 2 && !da_fp32, db_half = e == 2 && !db_fp32, dbias_half = e == 2 && !dbias_fp32;
+    const bool preact_half = e == 2 && !preact_fp32;
+    if (!aligned_to({{dout, e}, {a, e}, {b, e}, {preact, preact_half ? 2 : 4}, {da, da_half ? 2 : 4},
+                     {db, db_half ? 2 : 4}, {dbias, dbias_half ? 2 : 4}}))
+        return c.failed("a pointer is not aligned to its element size");
+    DeviceScope device(c.ctx->device);
+    if (device.status != cudaSuccess)
+        return c.failed(device.status);
+
+    const bool own_dz = activation != kActNone && (da || db);
+    Operand oa, ob, od;
+    if (db)
+        oa.plan(c, a, m, k);
+    if (da)
+        ob.plan(c, b, k, n);
+    size_t dz_at = 0;
+    const int64_t dz_pitch = round_up(n, 16 / e);
+    if (own_dz)
+        dz_at = c.reserve(static_cast<size_t>(m * dz_pitch * e));
+    else if (da || db)
+        od.plan(c, dout, m, n);
+    ActGradPlan plan;
+    plan.choose(c.ctx, m, n);
+    size_t partial_at = 0;
+    const bool partial = dbias && plan.chunks > 1;
+    if (partial)
+        partial_at = c.reserve(static_cast<size_t>(plan.chunks) * n * sizeof(float));
+    if (c.allocate() || (db && oa.prepare(c)) || (da && ob.prepare(c)) || (!own_dz && (da || db) && od.prepare(c)))
+        return 1;
+
+    if (own_dz || dbias) {
+        ActGradParams g{};
+        g.dout = dout;
+        g.preact = activation != kActNone ? preact : nullptr;
+        g.preact_half = preact_half ? 1 : 0;
+        g.dz = own_dz ? c.scratch + dz_at : nullptr;
+        g.dz_pitch = dz_pitch;
+        g.partial = partial ? reinterpret_cast<float *>(c.scratch + partial_at) : nullptr;
+        g.dbias = dbias;
+        g.dbias_half = dbias_half ? 1 : 0;
+        g.m = m;
+        g.n = n;
+        g.rows_per_chunk = plan.rows_per_chunk;
+        g.activation = activation;
+        g.vec = aligned16(dout) && static_cast<int64_t>(n) * e % 16 == 0 && (!g.preact || aligned16(preact)) &&
+                (!g.preact || static_cast<int64_t>(n) * (preact_half ? 2 : 4) % 16 == 0);
+        cudaError_t st = c.kernels().act_grad(g, dim3(static_cast<unsigned int>((n + AG_COLS - 1) / AG_COLS),
+                                                      static_cast<unsigned int>(plan.chunks)),
+                                              c.stream);
+        if (st == cudaSuccess && partial)
+            st = c.kernels().bias_grad(g.partial, plan.chunks, n, dbias, g.dbias_half, c.stream);
+        if (st != cudaSuccess)
+            return c.failed(st);
+    }
+    const Matrix dz = own_dz ? Matrix{c.scratch + dz_at, m, n, dz_pitch} : od.ready;
+    const int64_t bk = OP_ROW_BYTES / e;
+    if (da) {
+        Product q;
+        q.a = dz;
+        q.b = ob.ready;
+        q.m = m;
+        q.n = k;
+        q.k = n;
+        q.launch.layout = kNT;
+        q.launch.tile = choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk);
+        if (set_output(c, q.launch, Matrix{da, m, k, k}, da_half) || enqueue(c, q))
+            return 1;
+    }
+    if (db) {
+        Product q;
+        q.a = oa.ready;
+        q.b = dz;
+        q.m = k;
+        q.n = n;
+        q.k = m;
+        q.launch.layout = kTN;
+        q.launch.tile = choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk);
+        if (set_output(c, q.launch, Matrix{db, k, n, n}, db_half) || enqueue(c, q))
+            return 1;
+    }
+    return 0;
+}
+
+namespace {
+
+// The device-side plan of a grouped product in scratch: row tiles (or group bounds) and
+// the groups' tensor maps.
+struct GroupPlan {
+    int tile_rows = 0, maps = 0;
+    size_t maps_at = 0, tiles_at = 0, count_at = 0;
+
+    // tile_rows 0: ragged-K mode.
+    void plan(Call &c, int groups, int rows, int tile, int map_count)
+    {
+        tile_rows = tile;
+        maps = map_count;
+        const int64_t entries = tile ? rows / tile + std::min(groups, rows) : groups;
+        maps_at = c.reserve(static_cast<size_t>(groups) * std::max(maps, 1) * sizeof(CUtensorMap));
+        tiles_at = c.reserve(static_cast<size_t>(entries) * sizeof(OpRowTile));
+        count_at = c.reserve(sizeof(int));
+    }
+    int enqueue(Call &c, const void *offsets, int offsets64, int groups, int rows, const CUtensorMap &map0,
+                const CUtensorMap &map1, OpParams &p)
+    {
+        GroupPlanParams g{};
+        g.offsets = offsets;
+        g.offsets64 = offsets64;
+        g.groups = groups;
+        g.rows = rows;
+        g.tile_rows = tile_rows;
+        g.maps = maps;
+        g.count = reinterpret_cast<int *>(c.scratch + count_at);
+        g.tiles = reinterpret_cast<OpRowTile *>(c.scratch + tiles_at);
+        g.group_maps = reinterpret_cast<CUtensorMap *>(c.scratch + maps_at);
+        p.grouping = tile_rows ? kGroupedRows : kGroupedK;
+        p.groups = groups;
+        p.row_tile_count = g.count;
+        p.row_tiles = g.tiles;
+        p.group_maps = g.group_maps;
+        const cudaError_t st = launch_pdl(group_plan_kernel, dim3(1), dim3(GP_THREADS), 0, c.stream, map0, map1, g);
+        return st == cudaSuccess ? 0 : c.failed(st);
+    }
+};
+
+int check_groups(Call &c, int groups, int rows, int k, int n, const void *offsets, int offsets64)
+{
+    if (rows <= 0 || k <= 0 || n <= 0 || groups <= 0)
+        return c.failed("dimensions must be positive");
+    if (!offsets)
+        return c.failed("offsets pointer is null");
+    if (misaligned(offsets, offsets64 ? 8 : 4))
+        return c.failed("a pointer is not aligned to its element size");
+    return 0;
+}
+
+// Rows per tile follow the mean group: with few rows they take the MMA's N side (16 to
+// 128 wide) and the weight's columns its M side, so that a tile wastes little.
+int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_t n, int64_t k_blocks)
+{
+    const int64_t mean = (rows + groups - 1) / groups;
+    if (mean <= 16)
+        return kSwap16;
+    if (mean <= 32)
+        return kSwap32;
+    if (mean <= 64)
+        return kSwap64;
+    if (mean <= 128)
+        return kSwap128;
+    return choose_tile(ctx, mean, n, k_blocks, groups);
+}
+
+// A product over row groups: out[i] = a[i] . b[g] (layout kNN) or a[i] . b[g]^T (kNT).
+int grouped_rows(Call &c, GroupPlan &plan, Product &q, const void *offsets, int offsets64, int groups, int rows,
+                 const Matrix &out, bool half)
+{
+    if (set_output(c, q.launch, out, half))
+        return 1;
+    if (plan.enqueue(c, offsets, offsets64, groups, rows, q.launch.map_c, q.launch.map_c, q.launch.p))
+        return 1;
+    return enqueue(c, q);
+}
+
+} // namespace
+
+extern "C" int matmul_grouped(void *opaque, int precision, const void *a, const void *b, const void *offsets,
+                              int offsets64, int groups, void *out, int out_fp32, int rows, int k, int n, void *stream,
+                              char *error, size_t error_size)
+{
+    const char *name = "matmul_grouped";
+    if (check_call(opaque, precision, name, error, error_size))
+        return 1;
+    Call c{static_cast<Context *>(opaque), precision, static_cast<cudaStream_t>(stream), name, error, error_size};
+    if (!a || !b || !out)
+        return c.failed("matrix pointer is null");
+    if (check_groups(c, groups, rows, k, n, offsets, offsets64))
+        return 1;
+    const int e = c.elem();
+    const bool half = e == 2 && !out_fp32;
+    if (!aligned_to({{a, e}, {b, e}, {out, half ? 2 : 4}}))
+        return c.failed("a pointer is not aligned to its element size");
+    DeviceScope device(c.ctx->device);
+    if (device.status != cudaSuccess)
+        return c.failed(device.status);
+    const int64_t bk = OP_ROW_BYTES / e;
+    Product q;
+    OpLaunch &l = q.launch;
+    l.tile = choose_grouped_tile(c.ctx, rows, groups, n, (k + bk - 1) / bk);
+    const bool swap = is_swap(l.tile);
+    l.epilogue = swap ? kEpiStoreT : kEpiStore;
+    Operand oa, ob;
+    oa.plan(c, a, rows, k);
+    ob.plan(c, b, k, n, groups);
+    const Matrix mo{out, rows, n, n};
+    GroupPlan plan;
+    plan.plan(c, groups, rows, swap ? kTileShapes[l.tile].bn : kTileShapes[l.tile].bm,
+              !swap && output_tma(mo, half ? 2 : 4) ? 1 : 0);
+    if (c.allocate() || oa.prepare(c) || ob.prepare(c))
+        return 1;
+    q.a = oa.ready;
+    q.b = ob.ready;
+    q.m = rows;
+    q.n = n;
+    q.k = k;
+    return grouped_rows(c, plan, q, offsets, offsets64, groups, rows, mo, half);
+}
+
+extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *dout, const void *a, const void *b,
+                                       const void *offsets, int offsets64, int groups, void *da, int da_fp32, void *db,
+                                       int db_fp32, int rows, int k, int n, void *stream, char *error,
+                                       size_t error_size)
+{
+    const char *name = "matmul_grouped_backward";
+    if (check_call(opaque, precision, name, error, error_size))
+        return 1;
+    Call c{static_cast<Context *>(opaque), precision, static_cast<cudaStream_t>(stream), name, error, error_size};
+    if (!dout || (da && !b) || (db && !a))
+        return c.failed("matrix pointer is null");
+    if (!da && !db)
+        return c.failed("no gradient is asked for");
+    if (check_groups(c, groups, rows, k, n, offsets, offsets64))
+        return 1;
+    const int e = c.elem();
+    const bool da_half = e == 2 && !da_fp32, db_half = e == 2 && !db_fp32;
+    if (!aligned_to({{dout, e}, {a, e}, {b, e}, {da, da_half ? 2 : 4}, {db, db_half ? 2 : 4}}))
+        return c.failed("a pointer is not aligned to its element size");
+    DeviceScope device(c.ctx->device);
+    if (device.status != cudaSuccess)
+        return c.failed(device.status);
+    const int64_t bk = OP_ROW_BYTES / e;
+    Operand oa, ob, od;
+    od.plan(c, dout, rows, n);
+    GroupPlan rows_plan, k_plan;
+    Product qa, qb;
+    const Matrix ma{da, rows, k, k};
+    if (da) {
+        ob.plan(c, b, k, n, groups);
+        const int64_t mean = (rows + groups - 1) / groups;
+        qa.launch.layout = kNT;
+        qa.launch.tile = choose_tile(c.ctx, mean, k, (n + bk - 1) / bk, groups);
+        rows_plan.plan(c, groups, rows, kTileShapes[qa.launch.tile].bm, output_tma(ma, da_half ? 2 : 4) ? 1 : 0);
+    }
+    if (db) {
+        oa.plan(c, a, rows, k);
+        const int64_t mean = (rows + groups - 1) / groups;
+        qb.launch.layout = kTN;
+        qb.launch.tile = choose_tile(c.ctx, k, n, (mean + bk - 1) / bk, groups);
+        k_plan.plan(c, groups, rows, 0, 2);
+    }
+    if (c.allocate() || od.prepare(c) || (da && ob.prepare(c)) || (db && oa.prepare(c)))
+        return 1;
+    if (da) {
+        qa.a = od.ready;
+        qa.b = ob.ready;
+        qa.m = rows;
+        qa.n = k;
+        qa.k = n;
+        if (grouped_rows(c, rows_plan, qa, offsets, offsets64, groups, rows, ma, da_half))
+            return 1;
+    }
+    if (db) {
+        qb.a = oa.ready;
+        qb.b = od.ready;
+        qb.m = k;
+        qb.n = n;
+        qb.k = rows;
+        const TileShape &t = kTileShapes[qb.launch.tile];
+        CUtensorMap map0, map1;
+        if (!operand_map(c, &map0, qb.a, true, OP_BM) || !operand_map(c, &map1, qb.b, true, t.bn / t.ctas)) {
+            cudaGetLastError();
+            return c.failed("cuTensorMapEncodeTiled rejected an operand");
+        }
+        if (set_output(c, qb.launch, Matrix{db, k, n, n, groups, static_cast<int64_t>(k) * n}, db_half) ||
+            k_plan.enqueue(c, offsets, offsets64, groups, rows, map0, map1, qb.launch.p) || enqueue(c, qb))
+            return 1;
+    }
+    return 0;
+}
+
+namespace {
+
+int check_loss(Call &c, int m, int k, int v, const void *labels, int labels64)
+{
+    if (m <= 0 || k <= 0 || v <= 0)
+        return c.failed("dimensions must be positive");
+    if (!labels)
+        return c.failed("labels pointer is null");
+    if (misaligned(labels, labels64 ? 8 : 4))
+        return c.failed("a pointer is not aligned to its element size");
+    return 0;
+}
+
+} // namespace
+
+extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hidden, const void *weight,
+                                    const void *labels, int labels64, long long ignore_index, float *loss, float *lse,
+                                    int m, int k, int v, void *stream, char *error, size_t error_size)
+{
+    const char *name = "matmul_cross_entropy";
+    if (check_call(opaque, precision, name, error, error_size))
+        return 1;
+    Call c{static_cast<Context *>(opaque), precision, static_cast<cudaStream_t>(stream), name, error, error_size};
+    if (!hidden || !weight || !loss || !lse)
+        return c.failed("pointer is null");
+    if (check_loss(c, m, k, v, labels, labels64))
+        return 1;
+    const int e = c.elem();
+    if (!aligned_to({{hidden, e}, {weight, e}, {loss, 4}, {lse, 4}}))
+        return c.failed("a pointer is not aligned to its element size");
+    DeviceScope device(c.ctx->device);
+    if (device.status != cudaSuccess)
+        return c.failed(device.status);
+    const int64_t bk = OP_ROW_BYTES / e;
+    Product q;
+    OpLaunch &l = q.launch;
+    l.epilogue = kEpiLse;
+    l.tile = choose_tile(c.ctx, m, v, (k + bk - 1) / bk);
+    const int tiles = (v + kTileShapes[l.tile].bn - 1) / kTileShapes[l.tile].bn;
+    Operand oh, ow;
+    oh.plan(c, hidden, m, k);
+    ow.plan(c, weight, k, v);
+    const size_t partial_at = c.reserve(static_cast<size_t>(tiles) * m * sizeof(float2));
+    const size_t logit_at = c.reserve(static_cast<size_t>(m) * sizeof(float));
+    if (c.allocate() || oh.prepare(c) || ow.prepare(c))
+        return 1;
+    q.a = oh.ready;
+    q.b = ow.ready;
+    q.m = m;
+    q.n = v;
+    q.k = k;
+    OpParams &p = l.p;
+    p.labels = labels;
+    p.labels64 = labels64;
+    p.ignore = ignore_index;
+    p.classes = v;
+    p.partial = reinterpret_cast<float2 *>(c.scratch + partial_at);
+    p.label_logit = reinterpret_cast<float *>(c.scratch + logit_at);
+    if (enqueue(c, q))
+        return 1;
+    const cudaError_t st = launch_pdl(loss_join_kernel, dim3(static_cast<unsigned int>((m + 31) / 32)), dim3(256), 0,
+                                      c.stream, static_cast<const float2 *>(p.partial), tiles,
+                                      static_cast<const float *>(p.label_logit), loss, lse, p);
+    return st == cudaSuccess ? 0 : c.failed(st);
+}
+
+extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const float *grad, const void *hidden,
+                                             const void *weight, const void *labels, int labels64,
+                                             long long ignore_index, const float *lse, void *dhidden, int dhidden_fp32,
+                                             void *dweight, int dweight_fp32, int m, int k, int v, void *stream,
+                                             char *error, size_t error_size)
+{
+    const char *name = "matmul_cross_entropy_backward";
+    if (check_call(opaque, precision, name, error, error_size))
+        return 1;
+    Call c{static_cast<Context *>(opaque), precision, static_cast<cudaStream_t>(stream), name, error, error_size};
+    if (precision == kFp16)
+        return c.failed("the gradient of each logit is held in the input format, and fp16 cannot hold the small ones; "
+                        "use bf16 or tf32");
+    if (!grad || !hidden || !weight || !lse)
+        return c.failed("pointer is null");
+    if (!dhidden && !dweight)
+        return c.failed("no gradient is asked for");
+    if (check_loss(c, m, k, v, labels, labels64))
+        return 1;
+    const int e = c.elem();
+    const bool dh_half = e == 2 && !dhidden_fp32, dw_half = e == 2 && !dweight_fp32;
+    if (!aligned_to({{hidden, e}, {weight, e}, {grad, 4}, {lse, 4}, {dhidden, dh_half ? 2 : 4}, {dweight, dw_half ? 2 : 4}}))
+        return c.failed("a pointer is not aligned to its element size");
+    DeviceScope device(c.ctx->device);
+    if (device.status != cudaSuccess)
+        return c.failed(device.status);
+    const int64_t bk = OP_ROW_BYTES / e;
+    // Vocabulary pieces: the logits' gradients of one piece (m x width, input format) take
+    // about 64 MB, so that the two products that read them find them in L2.
+    constexpr int64_t kPieceBytes = int64_t{64} << 20;
+    int64_t width = kPieceBytes / (static_cast<int64_t>(m) * e) / 256 * 256;
+    width = std::max<int64_t>(width, 4096);
+    width = std::min<int64_t>(width, round_up(v, 256));
+    const int64_t pieces = (v + width - 1) / width;
+    Operand oh, ow;
+    oh.plan(c, hidden, m, k);
+    ow.plan(c, weight, k, v);
+    const size_t dz_at = c.reserve(static_cast<size_t>(m) * width * e);
+    // dH is summed over the pieces in FP32: in the output itself where it is FP32.
+    const bool own_sum = dhidden && dh_half && pieces > 1;
+    const size_t sum_at = own_sum ? c.reserve(static_cast<size_t>(m) * k * sizeof(float)) : 0;
+    if (c.allocate() || oh.prepare(c) || ow.prepare(c))
+        return 1;
+    const Matrix dh{dhidden, m, k, k};
+    const Matrix sum = own_sum ? Matrix{c.scratch + sum_at, m, k, k} : dh;
+    for (int64_t piece = 0; piece < pieces; ++piece) {
+        const int64_t v0 = piece * width, cols = std::min<int64_t>(width, v - v0);
+        const Matrix w{static_cast<const uint8_t *>(ow.ready.ptr) + v0 * e, k, cols, ow.ready.pitch};
+        const Matrix dz{c.scratch + dz_at, m, cols, width};
+        {
+            Product q;
+            q.a = oh.ready;
+            q.b = w;
+            q.m = m;
+            q.n = cols;
+            q.k = k;
+            q.launch.epilogue = kEpiSoftmaxGrad;
+            q.launch.tile = choose_tile(c.ctx, m, cols, (k + bk - 1) / bk);
+            OpParams &p = q.launch.p;
+            p.labels = labels;
+            p.labels64 = labels64;
+            p.ignore = ignore_index;
+            p.classes = v;
+            p.column0 = static_cast<int>(v0);
+            p.lse = lse;
+            p.grad = grad;
+            if (set_output(c, q.launch, dz, e == 2) || enqueue(c, q))
+                return 1;
+        }
+        if (dhidden) {
+            Product q;
+            q.a = dz;
+            q.b = w;
+            q.m = m;
+            q.n = k;
+            q.k = cols;
+            q.launch.layout = kNT;
+            q.launch.tile = choose_tile(c.ctx, m, k, (cols + bk - 1) / bk);
+            const bool last = piece == pieces - 1;
+            if (set_output(c, q.launch, last ? dh : sum, last && dh_half))
+                return 1;
+            if (piece > 0) {
+                q.launch.p.residual = sum.ptr;
+                q.launch.p.residual_half = 0;
+                q.launch.p.residual_vec = aligned16(sum.ptr) && static_cast<int64_t>(k) * 4 % 16 == 0;
+            }
+            if (enqueue(c, q))
+                return 1;
+        }
+        if (dweight) {
+            Product q;
+            q.a = oh.ready;
+            q.b = dz;
+            q.m = k;
+            q.n = cols;
+            q.k = m;
+            q.launch.layout = kTN;
+            q.launch.tile = choose_tile(c.ctx, k, cols, (m + bk - 1) / bk);
+            const Matrix dw{static_cast<uint8_t *>(dweight) + v0 * (dw_half ? 2 : 4), k, cols, v};
+            if (set_output(c, q.launch, dw, dw_half) || enqueue(c, q))
+                return 1;
+        }
+    }
+    return 0;
+}

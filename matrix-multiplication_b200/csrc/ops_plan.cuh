@@ -1,0 +1,168 @@
+// Small kernels around the operators' products (tc_ops.cuh): the tile plan of grouped
+// products and the join of the loss's per-tile maxima and sums.  Both are bound by
+// launch latency.  Included by ops.cu alone.
+#pragma once
+
+#include <cuda.h>
+#include <cstdint>
+
+#include "ptx.cuh"
+#include "tc_ops.cuh"
+
+namespace b200 {
+
+// ---------------------------------------------------------------- plan of a grouped product
+constexpr int GP_THREADS = 1024;
+
+struct GroupPlanParams {
+    const void *offsets;      // groups + 1 row offsets
+    int offsets64;
+    int groups, rows;
+    int tile_rows;            // rows mode: rows per tile; 0: one entry per group (ragged-K mode)
+    int maps;                 // tensor maps per group (0, 1 or 2)
+    int *count;               // number of row tiles
+    OpRowTile *tiles;
+    CUtensorMap *group_maps;  // [groups][maps]
+};
+
+// One block: group g's rows are [max(offsets[0..g]), max(offsets[0..g+1])) clipped to
+// [0, rows], so that whatever the offsets hold, groups are disjoint, in order and in
+// range.  Rows mode writes ceil(rows of g / tile_rows) entries per group, in order;
+// ragged-K mode one entry per group.  Each group's tensor maps are the templates with
+// the row extent cut at the group's end.
+__global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_constant__ CUtensorMap map0,
+                                                                const __grid_constant__ CUtensorMap map1,
+                                                                const GroupPlanParams p)
+{
+    __shared__ int warp_max[32], warp_sum[32];
+    __shared__ int carry_max, carry_sum;
+    __shared__ int ends[GP_THREADS];
+    __shared__ __align__(128) uint8_t map_s[32][128];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    wait_for_prior_grid();
+    allow_next_grid();
+    auto offset = [&](int i) {
+        const long long v = p.offsets64 ? static_cast<const long long *>(p.offsets)[i]
+                                        : static_cast<long long>(static_cast<const int *>(p.offsets)[i]);
+        return static_cast<int>(v < 0 ? 0 : v > p.rows ? p.rows : v);
+    };
+    if (threadIdx.x == 0) {
+        carry_max = offset(0);
+        carry_sum = 0;
+    }
+    __syncthreads();
+    for (int g0 = 0; g0 < p.groups; g0 += GP_THREADS) {
+        const int g = g0 + threadIdx.x;
+        // Running maximum of the ends.
+        int end = g < p.groups ? offset(g + 1) : 0;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, end, d);
+            if (lane >= d)
+                end = max(end, o);
+        }
+        if (lane == 31)
+            warp_max[warp] = end;
+        __syncthreads();
+        int before = carry_max;
+        for (int i = 0; i < warp; ++i)
+            before = max(before, warp_max[i]);
+        end = max(end, before);
+        ends[threadIdx.x] = end;
+        __syncthreads();
+        const int begin = threadIdx.x ? ends[threadIdx.x - 1] : carry_max;
+        const int count = g < p.groups && p.tile_rows ? (end - begin + p.tile_rows - 1) / p.tile_rows : 0;
+        // Running sum of the tile counts.
+        int sum = count;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d)
+                sum += o;
+        }
+        if (lane == 31)
+            warp_sum[warp] = sum;
+        __syncthreads();
+        int first = carry_sum + sum - count;
+        for (int i = 0; i < warp; ++i)
+            first += warp_sum[i];
+        if (g < p.groups) {
+            if (p.tile_rows) {
+                for (int i = 0; i < count; ++i)
+                    p.tiles[first + i] = OpRowTile{g, begin + i * p.tile_rows, end, 0};
+            } else {
+                p.tiles[g] = OpRowTile{g, begin, end, 0};
+            }
+        }
+        // Tensor maps of this chunk's groups, one warp each.
+        if (p.maps) {
+            for (int i = warp; i < GP_THREADS && g0 + i < p.groups; i += 32) {
+                for (int j = 0; j < p.maps; ++j) {
+                    const uint32_t s = smem_addr(map_s[warp]);
+                    const uint32_t *src = reinterpret_cast<const uint32_t *>(j ? &map1 : &map0);
+                    reinterpret_cast<uint32_t *>(map_s[warp])[lane] = src[lane];
+                    __syncwarp();
+                    if (lane == 0) {
+                        const uint32_t extent = static_cast<uint32_t>(max(ends[i], 1));
+                        asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"l"(
+                                         static_cast<uint64_t>(s)),
+                                     "r"(extent)
+                                     : "memory");
+                    }
+                    __syncwarp();
+                    asm volatile(
+                        "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned "
+                        "[%0], [%1], 128;" ::"l"(reinterpret_cast<uint64_t>(p.group_maps + (g0 + i) * p.maps + j)),
+                        "r"(s)
+                        : "memory");
+                    __syncwarp();
+                }
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == GP_THREADS - 1) {
+            carry_max = end;
+            carry_sum = first + count;
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0 && p.count)
+        *p.count = carry_sum;
+}
+
+// ---------------------------------------------------------------- loss
+// lse = log sum exp over the column tiles' (maximum, sum) pairs in base 2, loss = lse -
+// the label's logit; 32 rows per block, eight warps each take every eighth tile and
+// join in a fixed order.
+__global__ void __launch_bounds__(256) loss_join_kernel(const float2 *partial, int tiles, const float *label_logit,
+                                                        float *loss, float *lse, const OpParams p)
+{
+    __shared__ float tops[8][32], sums[8][32];
+    wait_for_prior_grid();
+    allow_next_grid();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = static_cast<int>(blockIdx.x) * 32 + lane;
+    float top = -INFINITY, sum = 0.0f;
+    auto join = [&](float t, float s) {
+        const float next = fmaxf(top, t);
+        const float origin = next == -INFINITY ? 0.0f : next;
+        sum = sum * exp2f(top - origin) + s * exp2f(t - origin);
+        top = next;
+    };
+    if (row < p.m)
+        for (int i = warp; i < tiles; i += 8) {
+            const float2 v = partial[static_cast<long long>(i) * p.m + row];
+            join(v.x, v.y);
+        }
+    tops[warp][lane] = top;
+    sums[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && row < p.m) {
+        for (int i = 1; i < 8; ++i)
+            join(tops[i][lane], sums[i][lane]);
+        const float total = (top + log2f(sum)) * 0.69314718055994531f;
+        const int label = op_label(p, row);
+        lse[row] = total;
+        loss[row] = label == -1 ? 0.0f : label == -2 ? __int_as_float(0x7fc00000) : total - label_logit[row];
+    }
+}
+
+} // namespace b200

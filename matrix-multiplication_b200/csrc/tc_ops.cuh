@@ -1,0 +1,862 @@
+// Tensor-core product with a fused epilogue, the main loop of the operators next to
+// matmul_launch (ops.cu): D = Aop * Bop, FP32 accumulation in tensor memory, where
+//
+//   * either operand may be stored with its K index contiguous ("K-major") or its
+//     M/N index contiguous ("MN-major"), so A.B, A.B^T and A^T.B of row-major
+//     matrices are read in place;
+//   * the rows may belong to groups (experts) of any size, each with its own B:
+//     - rows mode: a row tile lies in one group, whose table entry names the group,
+//       its first row and the end of its rows;
+//     - ragged-K mode (gradient of B): one product per group over the group's rows.
+//       Operand tensor maps of that group end at its last row, so TMA fills the
+//       rest of a K block with zeros and no value of a neighbour enters a sum;
+//   * the epilogue applies bias, activation and residual, reduces each row to a
+//     maximum and a sum of exponentials (loss), or turns logits into gradients.
+//
+// Roles, rings, bounded waits and the pair protocol are those of tc2_gemm.cuh (CTAS
+// = 2: one 256 x BN tile per CTA pair, each CTA staging half of either operand) and
+// tc_gemm.cuh (CTAS = 1: 128 x BN).  All maps are three-dimensional (inner, rows,
+// group): a coordinate past a group's own K rows reads zeros, not the next group.
+//
+// Measured choices stand at the host's plan (ops.cu).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+
+#include "ptx.cuh"
+
+namespace b200 {
+
+enum OpFormat : int { kOpF16 = 0, kOpBF16 = 1, kOpTF32 = 2 };
+enum OpEpilogue : int {
+    kEpiStore = 0,      // out = act(D + bias) + residual, D's rows are out's rows
+    kEpiStoreT = 1,     // the same, D's rows are out's columns (few rows: they take the MMA's N side)
+    kEpiLse = 2,        // per row: maximum and sum of exponentials of this tile's columns, label's logit
+    kEpiSoftmaxGrad = 3 // out = (exp(D - lse) - [column == label]) * grad
+};
+enum OpActivation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
+enum OpGrouping : int { kUngrouped = 0, kGroupedRows = 1, kGroupedK = 2 };
+
+// Status bits of the device status word (matmul_device_status).
+enum : unsigned int { kOpLoadTimeout = 1u, kOpMmaTimeout = 2u, kOpEpilogueTimeout = 4u, kOpDrainTimeout = 8u };
+
+constexpr int OP_BM = 128;                    // M rows per CTA (TMEM lanes)
+constexpr int OP_THREADS = 192;               // TMA warp, MMA warp, four epilogue warps
+constexpr int OP_ROW_BYTES = 128;             // one swizzle row: K depth of a stage (K-major)
+constexpr int OP_A_STAGE = OP_BM * OP_ROW_BYTES;
+constexpr int OP_BOX = 128 * 128;             // epilogue box: 128 rows x 128 bytes
+constexpr int OP_EPI_BYTES = 2 * OP_BOX;
+constexpr int OP_BAR_BYTES = 512;
+
+template <int CTAS, int BN>
+struct OpTile {
+    static constexpr int kBCols = BN / CTAS;                   // N columns staged per CTA
+    static constexpr int kBStage = kBCols * OP_ROW_BYTES;
+    static constexpr int kStages = kBCols >= 256 ? 4 : kBCols >= 128 ? 6 : 8;
+    static constexpr int kBiasBytes = BN * 4 < 256 ? 256 : BN * 4;
+    static constexpr int kSmem = 1024 + kStages * (OP_A_STAGE + kBStage) + OP_EPI_BYTES + OP_BAR_BYTES + kBiasBytes;
+    static constexpr uint32_t kTmemColumns = 2 * BN < 32 ? 32 : 2 * BN;   // two accumulators
+    static_assert(kSmem <= 227 * 1024, "tile exceeds shared memory");
+};
+
+// A row tile of a grouped product: group, first row, end of the group's rows.
+struct OpRowTile {
+    int group, row0, row_end, unused;
+};
+
+struct OpParams {
+    int m, n;                 // rows and columns of the output (of one group in ragged-K mode)
+    int num_m_blocks, num_n_blocks, num_k_blocks;   // M- and N-side tiles of D, K blocks
+    int num_tiles;
+    int raster;               // M-side tiles per raster group
+    int grouping;             // OpGrouping
+    const int *row_tile_count;        // rows mode: number of row tiles (device)
+    const OpRowTile *row_tiles;       // rows mode: table of row tiles; ragged-K mode: one entry per group
+    const CUtensorMap *group_maps;    // rows mode: out's map per group; ragged-K mode: Aop's and Bop's
+    int groups;
+    // kEpiStore / kEpiStoreT / kEpiSoftmaxGrad
+    void *out;
+    long long out_pitch, out_slab;    // elements between rows / between groups' outputs
+    int out_half;                     // 1: the 16-bit input format, 0: FP32
+    int out_tma;                      // 1: out can be written by TMA
+    void *preact;                     // D + bias before the activation, or null (pitch n)
+    int preact_half, preact_tma;
+    const void *residual;             // null, or added after the activation (pitch out_pitch)
+    int residual_half;
+    int residual_vec;                 // 1: 16-byte loads of the residual are aligned
+    const void *bias;                 // n values or null
+    int bias_half;
+    int activation;
+    // kEpiLse / kEpiSoftmaxGrad
+    const void *labels;
+    int labels64;
+    int column0;                      // vocabulary index of column 0
+    long long ignore;
+    long long classes;                // vocabulary size: labels outside [0, classes) that are not `ignore` give NaN
+    float2 *partial;                  // [n tiles][m]: maximum (of logit * log2 e) and sum
+    float *label_logit;               // [m]
+    const float *lse, *grad;          // [m]
+    unsigned int *status;
+    unsigned long long wait_limit_ns;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// The load of a CTA pair: `bar` may be the other CTA's barrier.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_store_3d(const void *map, uint32_t src, int x, int y, int z)
+{
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+
+// A tensor map written by an earlier kernel is read through the tensor-map proxy.
+__device__ __forceinline__ void tensormap_acquire(const void *map)
+{
+    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(reinterpret_cast<uint64_t>(map))
+                 : "memory");
+}
+
+template <int FMT>
+struct OpType;
+template <>
+struct OpType<kOpF16> {
+    using T = __half;
+    static __device__ __forceinline__ float to(T x) { return __half2float(x); }
+    static __device__ __forceinline__ T from(float x) { return __float2half_rn(x); }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi)
+    {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+};
+template <>
+struct OpType<kOpBF16> {
+    using T = __nv_bfloat16;
+    static __device__ __forceinline__ float to(T x) { return __bfloat162float(x); }
+    static __device__ __forceinline__ T from(float x) { return __float2bfloat16_rn(x); }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi)
+    {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+};
+template <>
+struct OpType<kOpTF32> {
+    using T = float;
+    static __device__ __forceinline__ float to(T x) { return x; }
+    static __device__ __forceinline__ T from(float x) { return x; }
+    static __device__ __forceinline__ uint32_t pack(float, float) { return 0u; }   // no 16-bit form
+};
+
+// act(z) in FP32.  relu keeps NaN; gelu_tanh uses 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)).
+__device__ __forceinline__ float op_activation(float z, int act)
+{
+    if (act == kActRelu)
+        return z < 0.0f ? 0.0f : z;
+    if (act == kActGelu)
+        return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    if (act == kActGeluTanh) {
+        const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
+        return z / (1.0f + __expf(-2.0f * u));
+    }
+    if (act == kActSilu)
+        return z / (1.0f + __expf(-z));
+    return z;
+}
+
+// act'(z) in FP32.
+__device__ __forceinline__ float op_activation_slope(float z, int act)
+{
+    if (act == kActRelu)
+        return z > 0.0f ? 1.0f : 0.0f;
+    if (act == kActGelu)
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    if (act == kActGeluTanh) {
+        const float s = 1.0f / (1.0f + __expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));
+        return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
+    }
+    if (act == kActSilu) {
+        const float s = 1.0f / (1.0f + __expf(-z));
+        return s * (1.0f + z * (1.0f - s));
+    }
+    return 1.0f;
+}
+
+// A row's label: its column, -1 for an ignored row, -2 for a label outside the vocabulary.
+__device__ __forceinline__ int op_label(const OpParams &p, int row)
+{
+    const long long y = p.labels64 ? static_cast<const long long *>(p.labels)[row]
+                                   : static_cast<long long>(static_cast<const int *>(p.labels)[row]);
+    if (y == p.ignore)
+        return -1;
+    return y >= 0 && y < p.classes ? static_cast<int>(y) : -2;
+}
+
+// Where a tile of D lies: M-side and N-side origin, group, K blocks and K origin, and
+// the end of the output rows it may write.
+struct OpWhere {
+    int m0, n0, group, nkb, k0, row_end;
+    int n_block;
+};
+
+template <int CTAS, int BN, bool SWAP>
+__device__ __forceinline__ OpWhere op_where(int tile, int row_tile_count, int bk, const OpParams &p)
+{
+    constexpr int kBM = OP_BM * CTAS;
+    OpWhere w;
+    int local = tile, blocks_m = p.num_m_blocks, blocks_n = p.num_n_blocks;
+    w.group = 0;
+    w.k0 = 0;
+    w.nkb = p.num_k_blocks;
+    w.row_end = p.m;
+    if (p.grouping == kGroupedK) {
+        const int per_group = blocks_m * blocks_n;
+        w.group = tile / per_group;
+        local = tile - w.group * per_group;
+        const OpRowTile t = p.row_tiles[w.group];
+        w.k0 = t.row0;
+        w.nkb = (t.row_end - t.row0 + bk - 1) / bk;
+    } else if (p.grouping == kGroupedRows) {
+        (SWAP ? blocks_n : blocks_m) = row_tile_count;
+    }
+    // Raster groups of `raster` M-side tiles, so that the CTAs at work share panels in L2.
+    const int per = p.raster * blocks_n;
+    const int rg = local / per;
+    const int first = rg * p.raster;
+    const int rows = min(blocks_m - first, p.raster);
+    const int in_group = local - rg * per;
+    const int mb = first + in_group % rows, nb = in_group / rows;
+    w.m0 = mb * kBM;
+    w.n0 = nb * BN;
+    w.n_block = nb;
+    if (p.grouping == kGroupedRows) {
+        const OpRowTile t = p.row_tiles[SWAP ? nb : mb];
+        w.group = t.group;
+        w.row_end = t.row_end;
+        (SWAP ? w.n0 : w.m0) = t.row0;
+    }
+    return w;
+}
+
+template <int FMT, int CTAS, int BN, bool A_MN, bool B_MN, int EPI>
+__global__ void __launch_bounds__(OP_THREADS, 1)
+op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+          const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_z,
+          const __grid_constant__ OpParams p)
+{
+    using Tile = OpTile<CTAS, BN>;
+    using Type = OpType<FMT>;
+    using T = typename Type::T;
+    constexpr bool kPair = CTAS == 2;
+    constexpr bool kSwap = EPI == kEpiStoreT;
+    constexpr bool kTF32 = FMT == kOpTF32;
+    constexpr int kElem = kTF32 ? 4 : 2;
+    constexpr int kBK = OP_ROW_BYTES / kElem;             // K elements per stage (64 or 32)
+    constexpr int kMmaK = 32 / kElem;
+    constexpr int kMmasPerStage = kBK / kMmaK;            // 4
+    constexpr int kBox = OP_ROW_BYTES / kElem;            // M/N elements per MN-major box
+    constexpr uint32_t kBoxBytes = kBK * OP_ROW_BYTES;    // one MN-major box
+    constexpr int kStages = Tile::kStages;
+    constexpr int kBStage = Tile::kBStage;
+    constexpr int kBCols = Tile::kBCols;
+    constexpr uint32_t kStageTx = static_cast<uint32_t>(CTAS) * (OP_A_STAGE + kBStage);
+    // FP32 accumulator, formats, A MN-major (bit 15), B MN-major (bit 16), N >> 3, M >> 4.
+    constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(FMT) << 7) | (static_cast<uint32_t>(FMT) << 10) |
+                                ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                                (static_cast<uint32_t>(BN >> 3) << 17) |
+                                (static_cast<uint32_t>((OP_BM * CTAS) >> 4) << 24);
+    static_assert(!B_MN || kBCols % kBox == 0, "whole MN-major boxes");
+    static_assert(!kPair || !kSwap, "the transposed epilogue runs on single CTAs");
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_addr(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    const uint32_t s_a = base;
+    const uint32_t s_b = s_a + kStages * OP_A_STAGE;
+    const uint32_t s_epi = s_b + kStages * kBStage;
+    const uint32_t s_bar = s_epi + OP_EPI_BYTES;
+    const uint32_t s_bias = s_bar + OP_BAR_BYTES;
+    auto full_bar = [&](int s) { return s_bar + 8u * s; };
+    auto empty_bar = [&](int s) { return s_bar + 8u * (kStages + s); };
+    auto accf_bar = [&](int i) { return s_bar + 8u * (2 * kStages + i); };
+    auto acce_bar = [&](int i) { return s_bar + 8u * (2 * kStages + 2 + i); };
+    const uint32_t drain_bar = s_bar + 8u * (2 * kStages + 4);
+    const uint32_t tmem_slot = s_bar + 8u * (2 * kStages + 5);
+    uint32_t *tmem_slot_ptr = reinterpret_cast<uint32_t *>(smem_raw + (tmem_slot - raw));
+    float *bias_s = reinterpret_cast<float *>(smem_raw + (s_bias - raw));
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = kPair ? cluster_cta_rank() : 0u;
+    const bool leader = rank == 0;
+    const int unit = static_cast<int>(blockIdx.x) / CTAS;       // this CTA's or pair's first tile
+    const int units = static_cast<int>(gridDim.x) / CTAS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(accf_bar(i), 1);
+            mbar_init(acce_bar(i), 4 * CTAS);
+        }
+        mbar_init(drain_bar, 1);
+        fence_mbarrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_map(&map_a);
+        tma_prefetch_map(&map_b);
+    }
+    if (warp == 1) {
+        if constexpr (kPair) {
+            tmem_alloc_pair(tmem_slot, Tile::kTmemColumns);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, Tile::kTmemColumns);
+            tmem_relinquish();
+        }
+    }
+    tc_fence_before();
+    if constexpr (kPair)
+        cluster_sync_all();        // both CTAs' barriers exist before either signals the other
+    else
+        __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(tmem_slot_ptr);
+    wait_for_prior_grid();
+    allow_next_grid();
+
+    const int row_tile_count = p.grouping == kGroupedRows ? *p.row_tile_count : 0;
+    const int num_tiles = p.grouping == kGroupedRows ? row_tile_count * (kSwap ? p.num_m_blocks : p.num_n_blocks)
+                                                     : p.num_tiles;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0, filled = 0, fill_parity = 0;
+            bool ok = true;
+            int acquired = -1;     // ragged-K mode: the group whose maps this thread has acquired
+            const uint32_t leader_full0 = kPair ? map_to_cta(full_bar(0), 0) : full_bar(0);
+            for (int tile = unit; ok && tile < num_tiles; tile += units) {
+                const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
+                const void *ma = &map_a, *mb = &map_b;
+                int za = 0, zb = 0;
+                if (p.grouping == kGroupedK) {
+                    ma = p.group_maps + 2 * w.group;
+                    mb = p.group_maps + 2 * w.group + 1;
+                    if (acquired != w.group) {
+                        tensormap_acquire(ma);
+                        tensormap_acquire(mb);
+                        acquired = w.group;
+                    }
+                } else if (p.grouping == kGroupedRows) {
+                    (kSwap ? za : zb) = w.group;
+                }
+                const int am = w.m0 + static_cast<int>(rank) * OP_BM;
+                const int bn = w.n0 + static_cast<int>(rank) * kBCols;
+                for (int kb = 0; kb < w.nkb; ++kb) {
+                    // In a pair this wait keeps the fixed limit: both CTAs then stop at the
+                    // same stage and the leader's drain covers every copy of either.
+                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, kPair ? kWaitLimitNs : p.wait_limit_ns)) {
+                        atomicOr(p.status, kOpLoadTimeout);
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t fb = leader_full0 + 8u * stage;
+                    if (leader)
+                        mbar_arrive_expect_tx(full_bar(stage), kStageTx);
+                    const int k = w.k0 + kb * kBK;
+                    auto load = [&](uint32_t dst, const void *map, int x, int y, int z) {
+                        if constexpr (kPair)
+                            tma_load_3d_pair(dst, map, fb, x, y, z);
+                        else
+                            tma_load_3d(dst, map, fb, x, y, z);
+                    };
+                    const uint32_t sa = s_a + stage * OP_A_STAGE, sb = s_b + stage * kBStage;
+                    if constexpr (A_MN) {
+#pragma unroll
+                        for (int j = 0; j < OP_BM / kBox; ++j)
+                            load(sa + j * kBoxBytes, ma, am + j * kBox, k, za);
+                    } else {
+                        load(sa, ma, k, am, za);
+                    }
+                    if constexpr (B_MN) {
+#pragma unroll
+                        for (int j = 0; j < kBCols / kBox; ++j)
+                            load(sb + j * kBoxBytes, mb, bn + j * kBox, k, zb);
+                    } else {
+                        load(sb, mb, k, bn, zb);
+                    }
+                    filled |= 1u << stage;
+                    fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            // Every issued copy lands before a CTA can exit.
+            if (leader)
+                for (int s = 0; s < kStages; ++s)
+                    if ((filled >> s) & 1u)
+                        if (!mbar_wait(full_bar(s), (fill_parity >> s) & 1u))
+                            atomicOr(p.status, kOpDrainTimeout);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer (a pair's leader)
+        if (leader && lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            const uint64_t a_desc0 = A_MN ? smem_desc_mn<kTF32>(s_a, kBoxBytes) : smem_desc_sw128(s_a, 16, 1024);
+            const uint64_t b_desc0 = B_MN ? smem_desc_mn<kTF32>(s_b, kBoxBytes) : smem_desc_sw128(s_b, 16, 1024);
+            constexpr uint64_t kAStep = A_MN ? (kMmaK * OP_ROW_BYTES) >> 4 : 32 >> 4;
+            constexpr uint64_t kBStep = B_MN ? (kMmaK * OP_ROW_BYTES) >> 4 : 32 >> 4;
+            auto commit = [&](uint32_t bar) {
+                if constexpr (kPair)
+                    tc_commit_pair_both(bar, 3);
+                else
+                    tc_commit(bar);
+            };
+            int acc = 0;
+            uint32_t acc_phase = 0;
+            bool ok = true;
+            for (int tile = unit; ok && tile < num_tiles; tile += units) {
+                const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
+                if (!mbar_wait(acce_bar(acc), acc_phase ^ 1u, p.wait_limit_ns)) {
+                    atomicOr(p.status, kOpMmaTimeout);
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+                for (int kb = 0; kb < w.nkb; ++kb) {
+                    if (!mbar_wait(full_bar(stage), phase, p.wait_limit_ns)) {
+                        atomicOr(p.status, kOpMmaTimeout);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t a_desc = a_desc0 + static_cast<uint64_t>(stage) * (OP_A_STAGE >> 4);
+                    const uint64_t b_desc = b_desc0 + static_cast<uint64_t>(stage) * (kBStage >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < kMmasPerStage; ++kk) {
+                        const uint32_t accumulate = (kb | kk) != 0 ? 1u : 0u;
+                        if constexpr (kPair)
+                            tc_mma_pair<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
+                        else
+                            tc_mma<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
+                    }
+                    commit(empty_bar(stage));
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok)
+                    break;
+                if (w.nkb > 0) {
+                    commit(accf_bar(acc));
+                } else if constexpr (kPair) {     // an empty group: its sum is zero, nothing to wait for
+                    mbar_arrive_cluster(map_to_cta(accf_bar(acc), 0));
+                    mbar_arrive_cluster(map_to_cta(accf_bar(acc), 1));
+                } else {
+                    mbar_arrive(accf_bar(acc));
+                }
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+            // Every MMA issued above completes before TMEM is released.
+            if constexpr (kPair)
+                tc_commit_pair(drain_bar);
+            else
+                tc_commit(drain_bar);
+            if (!mbar_wait(drain_bar, 0))
+                atomicOr(p.status, kOpDrainTimeout);
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------ epilogue
+        const int quarter = warp & 3;                 // TMEM lanes 32 * quarter .. +31
+        const int r = quarter * 32 + lane;
+        const bool issuer = warp == 2 && lane == 0;
+        int acc = 0;
+        uint32_t acc_phase = 0, stores = 0;
+        int failed_tile = -1;
+        int acquired = -1;
+        // Releases the accumulator after this warp's last read of it.
+        auto release = [&]() {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (kPair)
+                    mbar_arrive_cluster(map_to_cta(acce_bar(acc), 0));
+                else
+                    mbar_arrive(acce_bar(acc));
+            }
+        };
+        for (int tile = unit; tile < num_tiles; tile += units) {
+            const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
+            const int row0 = w.m0 + static_cast<int>(rank) * OP_BM;     // D's first row in this CTA
+            const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                   static_cast<uint32_t>(acc * BN);
+            if constexpr (EPI == kEpiStore) {
+                if (p.bias) {       // the tile's bias, read once into shared memory
+                    epilogue_sync();
+                    for (int c = threadIdx.x - 64; c < BN; c += 128) {
+                        const int col = w.n0 + c;
+                        float b = 0.0f;
+                        if (col < p.n)
+                            b = p.bias_half ? Type::to(static_cast<const T *>(p.bias)[col])
+                                            : static_cast<const float *>(p.bias)[col];
+                        bias_s[c] = b;
+                    }
+                    epilogue_sync();
+                }
+            }
+            // Per-row values of the loss epilogues.
+            int label = -1;
+            float row_lse = 0.0f, row_grad = 0.0f;
+            if constexpr (EPI == kEpiLse || EPI == kEpiSoftmaxGrad) {
+                if (row0 + r < p.m) {
+                    label = op_label(p, row0 + r);
+                    if constexpr (EPI == kEpiSoftmaxGrad) {
+                        row_lse = p.lse[row0 + r];
+                        row_grad = p.grad[row0 + r];
+                    }
+                }
+            }
+            int ok = 1;
+            if (lane == 0)
+                ok = mbar_wait(accf_bar(acc), acc_phase, p.wait_limit_ns) ? 1 : 0;
+            ok = epilogue_all(__shfl_sync(0xffffffffu, ok, 0));
+            if (!ok) {
+                if (lane == 0)
+                    atomicOr(p.status, kOpEpilogueTimeout);
+                failed_tile = tile;
+                break;
+            }
+            tc_fence_after();
+
+            if constexpr (EPI == kEpiStore || EPI == kEpiSoftmaxGrad) {
+                const void *mc = &map_c;
+                if (p.grouping == kGroupedRows && p.out_tma) {
+                    mc = p.group_maps + w.group;
+                    if (issuer && acquired != w.group) {
+                        tensormap_acquire(mc);
+                        acquired = w.group;
+                    }
+                }
+                const int zc = p.grouping == kGroupedK ? w.group : 0;
+                // Writes 128 rows x 128 bytes (32 FP32 or 64 16-bit columns) of this CTA's rows
+                // through a shared-memory box: TMA store, or row by row where TMA cannot.
+                auto emit = [&](const uint32_t (&words)[32], const void *map, int z, bool tma, bool half, void *dst,
+                                long long pitch, long long slab, int col0) {
+                    const uint32_t box = s_epi + (stores & 1u) * OP_BOX;
+                    if (issuer)
+                        bulk_wait_group_read<1>();      // the store that last read this box
+                    epilogue_sync();
+                    const uint32_t row_addr = box + r * 128;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        st_shared_v4(row_addr + ((j ^ (r & 7)) << 4), words[4 * j], words[4 * j + 1], words[4 * j + 2],
+                                     words[4 * j + 3]);
+                    if (tma) {
+                        fence_proxy_async_shared();
+                        epilogue_sync();
+                        if (issuer) {
+                            tma_store_3d(map, box, col0, row0, z);
+                            bulk_commit_group();
+                        }
+                    } else {
+                        epilogue_sync();
+                        const uint8_t *box_p = smem_raw + (box - raw);
+                        for (int rr = quarter; rr < OP_BM; rr += 4) {
+                            const int row = row0 + rr;
+                            if (row >= w.row_end)
+                                break;
+                            const long long at = z * slab + row * pitch;
+                            if (half) {
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const int c = lane + 32 * e;
+                                    if (col0 + c < p.n)
+                                        static_cast<T *>(dst)[at + col0 + c] = *reinterpret_cast<const T *>(
+                                            box_p + rr * 128 + (((c >> 3) ^ (rr & 7)) << 4) + (c & 7) * 2);
+                                }
+                            } else if (col0 + lane < p.n) {
+                                static_cast<float *>(dst)[at + col0 + lane] = *reinterpret_cast<const float *>(
+                                    box_p + rr * 128 + (((lane >> 2) ^ (rr & 7)) << 4) + (lane & 3) * 4);
+                            }
+                        }
+                    }
+                    ++stores;
+                };
+                auto emit_columns = [&](const float (&v)[64], const void *map, int z, bool tma, bool half, void *dst,
+                                        long long pitch, long long slab, int col0) {
+                    uint32_t words[32];
+                    if (half) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            words[j] = Type::pack(v[2 * j], v[2 * j + 1]);
+                        emit(words, map, z, tma, true, dst, pitch, slab, col0);
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (col0 + 32 * h >= p.n)
+                                break;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                words[j] = __float_as_uint(v[32 * h + j]);
+                            emit(words, map, z, tma, false, dst, pitch, slab, col0 + 32 * h);
+                        }
+                    }
+                };
+#pragma unroll 1
+                for (int step = 0; step < BN / 64; ++step) {
+                    float v[64];
+                    {
+                        uint32_t u[32];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (w.nkb > 0)
+                                tmem_load_32cols(t_row + step * 64 + h * 32, u);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                v[32 * h + j] = w.nkb > 0 ? __uint_as_float(u[j]) : 0.0f;
+                        }
+                    }
+                    if (step == BN / 64 - 1)
+                        release();
+                    const int col0 = w.n0 + step * 64;
+                    if (col0 >= p.n || row0 >= w.row_end)      // the same for all four warps
+                        continue;
+                    if constexpr (EPI == kEpiSoftmaxGrad) {
+                        // p = exp(z - lse); an ignored row's gradient is zero whatever its logits are.
+                        const int hit = label - p.column0 - col0;
+                        const float scale = label == -2 ? __int_as_float(0x7fc00000) : row_grad;
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) {
+                            const float prob = exp2f((v[j] - row_lse) * 1.4426950408889634f);
+                            v[j] = label == -1 ? 0.0f : (prob - (j == hit ? 1.0f : 0.0f)) * scale;
+                        }
+                    } else {
+                        if (p.bias) {
+                            const float4 *b4 = reinterpret_cast<const float4 *>(bias_s + step * 64);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const float4 b = b4[j];
+                                v[4 * j] += b.x;
+                                v[4 * j + 1] += b.y;
+                                v[4 * j + 2] += b.z;
+                                v[4 * j + 3] += b.w;
+                            }
+                        }
+                        if (p.preact)
+                            emit_columns(v, &map_z, 0, p.preact_tma != 0, p.preact_half != 0, p.preact, p.n, 0, col0);
+                        if (p.activation != kActNone) {
+#pragma unroll
+                            for (int j = 0; j < 64; ++j)
+                                v[j] = op_activation(v[j], p.activation);
+                        }
+                        if (p.residual && row0 + r < w.row_end) {
+                            const long long at = (row0 + r) * p.out_pitch + col0;
+                            if (p.residual_vec && col0 + 64 <= p.n) {
+                                if (p.residual_half) {
+                                    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at);
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) {
+                                        const uint4 q = src[j];
+                                        const T *h = reinterpret_cast<const T *>(&q);
+                                        if constexpr (!kTF32) {
+#pragma unroll
+                                            for (int e = 0; e < 8; ++e)
+                                                v[8 * j + e] += Type::to(h[e]);
+                                        }
+                                    }
+                                } else {
+                                    const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.residual) + at);
+#pragma unroll
+                                    for (int j = 0; j < 16; ++j) {
+                                        const float4 q = src[j];
+                                        v[4 * j] += q.x;
+                                        v[4 * j + 1] += q.y;
+                                        v[4 * j + 2] += q.z;
+                                        v[4 * j + 3] += q.w;
+                                    }
+                                }
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 64; ++j)
+                                    if (col0 + j < p.n)
+                                        v[j] += p.residual_half ? Type::to(static_cast<const T *>(p.residual)[at + j])
+                                                                : static_cast<const float *>(p.residual)[at + j];
+                            }
+                        }
+                    }
+                    emit_columns(v, mc, zc, p.out_tma != 0, p.out_half != 0, p.out, p.out_pitch, p.out_slab, col0);
+                }
+            } else if constexpr (EPI == kEpiStoreT) {
+                // D's rows are output columns: one lane per column, one store of 32 consecutive
+                // elements per output row and warp.
+                const int col = row0 + r;
+                float b = 0.0f;
+                if (p.bias && col < p.n)
+                    b = p.bias_half ? Type::to(static_cast<const T *>(p.bias)[col]) : static_cast<const float *>(p.bias)[col];
+#pragma unroll 1
+                for (int chunk = 0; chunk < BN / 16; ++chunk) {
+                    uint32_t u[16];
+                    tmem_load_16cols(t_row + chunk * 16, u);
+                    if (chunk == BN / 16 - 1)
+                        release();
+                    if (col < p.n) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int row = w.n0 + chunk * 16 + j;
+                            if (row >= w.row_end)
+                                break;
+                            const long long at = row * p.out_pitch + col;
+                            float z = __uint_as_float(u[j]) + b;
+                            if (p.preact) {
+                                if (p.preact_half)
+                                    static_cast<T *>(p.preact)[at] = Type::from(z);
+                                else
+                                    static_cast<float *>(p.preact)[at] = z;
+                            }
+                            z = op_activation(z, p.activation);
+                            if (p.residual)
+                                z += p.residual_half ? Type::to(static_cast<const T *>(p.residual)[at])
+                                                     : static_cast<const float *>(p.residual)[at];
+                            if (p.out_half)
+                                static_cast<T *>(p.out)[at] = Type::from(z);
+                            else
+                                static_cast<float *>(p.out)[at] = z;
+                        }
+                    }
+                }
+            } else {
+                // One pass: running maximum and sum of exponentials in base 2 of this row's
+                // columns in the tile; columns past the vocabulary count as -infinity.
+                float top = -INFINITY, sum = 0.0f;
+                const int row = row0 + r;
+#pragma unroll 1
+                for (int chunk = 0; chunk < BN / 32; ++chunk) {
+                    uint32_t u[32];
+                    tmem_load_32cols(t_row + chunk * 32, u);
+                    if (chunk == BN / 32 - 1)
+                        release();
+                    const int col0 = w.n0 + chunk * 32;
+                    if (col0 >= p.n)
+                        continue;
+                    const int hit = label - col0;
+                    if (label >= 0 && hit >= 0 && hit < 32) {
+                        float z = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            z = j == hit ? __uint_as_float(u[j]) : z;
+                        p.label_logit[row] = z;
+                    }
+                    float t[32], chunk_top = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        t[j] = col0 + j < p.n ? __uint_as_float(u[j]) * 1.4426950408889634f : -INFINITY;
+                        chunk_top = fmaxf(chunk_top, t[j]);
+                    }
+                    const float next = fmaxf(top, chunk_top);
+                    // A row whose logits are all -infinity so far adds nothing; NaN is carried by the sum.
+                    const float origin = next == -INFINITY ? 0.0f : next;
+                    sum *= exp2f(top - origin);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        sum += exp2f(t[j] - origin);
+                    top = next;
+                }
+                if (row < p.m)
+                    p.partial[static_cast<long long>(w.n_block) * p.m + row] = make_float2(top, sum);
+            }
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1u;
+            }
+        }
+        if (issuer) {
+            if (failed_tile >= 0)
+                bulk_wait_group<0>();      // the stored boxes are in memory before the NaN below
+            else
+                bulk_wait_group_read<0>();
+        }
+        __syncwarp();
+        if (failed_tile >= 0) {
+            // NaN over what this CTA did not finish, so that no later step reads stale values.
+            epilogue_sync();
+            const float nan = __int_as_float(0x7fc00000);
+            for (int tile = failed_tile; tile < num_tiles; tile += units) {
+                const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
+                const int row0 = w.m0 + static_cast<int>(rank) * OP_BM;
+                if constexpr (EPI == kEpiLse) {
+                    if (row0 + r < p.m)
+                        p.partial[static_cast<long long>(w.n_block) * p.m + row0 + r] = make_float2(nan, nan);
+                } else {
+                    const int first_row = kSwap ? w.n0 : row0, rows = kSwap ? BN : OP_BM;
+                    const int first_col = kSwap ? row0 : w.n0, cols = kSwap ? OP_BM : BN;
+                    const int row_end = min(w.row_end, first_row + rows), col_end = min(p.n, first_col + cols);
+                    for (int row = first_row + quarter; row < row_end; row += 4)
+                        for (int col = first_col + lane; col < col_end; col += 32) {
+                            const long long at =
+                                (p.grouping == kGroupedK ? w.group : 0) * p.out_slab + row * p.out_pitch + col;
+                            if (p.out_half)
+                                static_cast<T *>(p.out)[at] = Type::from(nan);
+                            else
+                                static_cast<float *>(p.out)[at] = nan;
+                            if (EPI != kEpiSoftmaxGrad && p.preact) {
+                                if (p.preact_half)
+                                    static_cast<T *>(p.preact)[row * static_cast<long long>(p.n) + col] = Type::from(nan);
+                                else
+                                    static_cast<float *>(p.preact)[row * static_cast<long long>(p.n) + col] = nan;
+                            }
+                        }
+                }
+            }
+        }
+    }
+
+    // No CTA (of a pair) releases TMEM before the last MMA and every epilogue are done.
+    tc_fence_before();
+    if constexpr (kPair)
+        cluster_sync_all();
+    else
+        __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (kPair)
+            tmem_dealloc_pair(tmem_base, Tile::kTmemColumns);
+        else
+            tmem_dealloc(tmem_base, Tile::kTmemColumns);
+    }
+}
+
+} // namespace b200

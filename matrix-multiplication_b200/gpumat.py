@@ -43,6 +43,8 @@ from pathlib import Path
 
 import torch
 
+from operators import (ACTIVATION_IDS, validate_cross_entropy, validate_cross_entropy_backward, validate_epilogue,
+                       validate_epilogue_backward, validate_grouped, validate_grouped_backward)
 from precision import INPUT_DTYPES, PRECISION_IDS, unsupported_reason, validate_operands
 
 ABI_VERSION = 3
@@ -55,6 +57,7 @@ _INT_MAX = 2**31 - 1
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _ERROR_ARGS = (ctypes.c_char_p, ctypes.c_size_t)
+_L = ctypes.c_longlong
 _MATRIX_CALL = (_P, _I, _I, _P, _P, _P, _I, _I, _I, _P)
 
 # name -> (argument types without the trailing error buffer, result type, takes an error buffer)
@@ -72,6 +75,14 @@ EXPORTS: dict[str, tuple[tuple, object, bool]] = {
     "matmul_plan": ((_P, _I, _I, _I, _I, _I, ctypes.c_char_p, ctypes.c_size_t), ctypes.c_int, True),
     "matmul_set_sm_limit": ((_P, _I), ctypes.c_int, True),
     "matmul_set_wait_limit": ((_P, ctypes.c_ulonglong), ctypes.c_int, True),
+    "matmul_epilogue": ((_P, _I, _P, _P, _P, _I, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P), ctypes.c_int, True),
+    "matmul_epilogue_backward": ((_P, _I, _P, _P, _P, _P, _I, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P),
+                                 ctypes.c_int, True),
+    "matmul_grouped": ((_P, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _P), ctypes.c_int, True),
+    "matmul_grouped_backward": ((_P, _I, _P, _P, _P, _P, _I, _I, _P, _I, _P, _I, _I, _I, _I, _P), ctypes.c_int, True),
+    "matmul_cross_entropy": ((_P, _I, _P, _P, _P, _I, _L, _P, _P, _I, _I, _I, _P), ctypes.c_int, True),
+    "matmul_cross_entropy_backward": ((_P, _I, _P, _P, _P, _P, _I, _L, _P, _P, _I, _P, _I, _I, _I, _I, _P),
+                                      ctypes.c_int, True),
     "matmul_peer_push": ((_P, _P, ctypes.POINTER(_P), _I, ctypes.c_size_t, _I, _P), ctypes.c_int, True),
 }
 
@@ -174,6 +185,43 @@ class PreparedLaunch:
         return self.out
 
 
+class PreparedOperator:
+    """One call of an operator next to ``matmul_launch`` with its arguments marshalled once.
+
+    Like ``PreparedLaunch``: calling it enqueues the operator on the stream that was
+    current when it was prepared and returns its outputs; it holds every tensor and the
+    stream, so none of them can be freed while it exists.
+    """
+
+    __slots__ = ("_owner", "_name", "_function", "_arguments", "_error", "_tensors", "_stream", "outputs")
+
+    def __init__(self, owner: "NativeMatmul", name: str, arguments: tuple, tensors: tuple, outputs, stream):
+        self._owner = owner
+        self._name = name
+        self._function = getattr(owner.library, name)
+        self._error = ctypes.create_string_buffer(ERROR_BYTES)
+        self._arguments = (*arguments, _P(stream.cuda_stream), self._error, len(self._error))
+        self._tensors = tensors
+        self._stream = stream
+        self.outputs = outputs
+
+    def __call__(self):
+        handle = self._owner._handle
+        if handle is None:
+            raise RuntimeError("NativeMatmul context is closed")
+        if self._function(handle, *self._arguments) != 0:
+            raise Library.failure(self._name, self._error)
+        return self.outputs
+
+
+def _ptr(tensor):
+    return _P(None if tensor is None else tensor.data_ptr())
+
+
+def _fp32(tensor) -> int:
+    return int(tensor is not None and tensor.dtype == torch.float32)
+
+
 class NativeMatmul:
     """A context of the native B200 GEMM library on one CUDA device."""
 
@@ -259,6 +307,122 @@ class NativeMatmul:
         for tensor in (a, b, out):
             tensor.record_stream(stream)
         return PreparedLaunch(self, implementation_id, PRECISION_IDS[precision], a, b, out, m, k, n, stream)
+
+    # ---------------------------------------------------------------- operators next to the product
+    def _operator(self, name: str, arguments: tuple, tensors: tuple, outputs) -> PreparedOperator:
+        stream = torch.cuda.current_stream(self._device)
+        tensors = tuple(t for t in tensors if t is not None)
+        for tensor in tensors:
+            tensor.record_stream(stream)
+        return PreparedOperator(self, name, arguments, tensors, outputs, stream)
+
+    def _operator_precision(self, precision) -> int:
+        self.handle
+        if not isinstance(precision, str) or precision not in PRECISION_IDS:
+            raise ValueError(f"Unknown precision: {precision}")
+        self._require_supported("tcgen05", precision)
+        return PRECISION_IDS[precision]
+
+    def prepare_epilogue(self, a, b, out, *, precision: str, bias=None, activation: str = "none", residual=None,
+                         preact=None) -> PreparedOperator:
+        """``out = activation(a @ b + bias) + residual`` on the tensor cores, in one kernel.
+
+        a (m, k) and b (k, n) have the input dtype of ``precision`` (tf32, fp16 or bf16);
+        out, and preact (receives ``a @ b + bias`` for the backward pass), are FP32 or the
+        input dtype; residual (m, n) has out's dtype and may be out itself; bias (n,) is
+        FP32 or the input dtype.  activation: none, relu, gelu (erf), gelu_tanh or silu.
+        Sums, bias and activation are FP32; out and preact are rounded once.  Returns out.
+        """
+        precision_id = self._operator_precision(precision)
+        m, k, n = validate_epilogue(a, b, out, precision, self._device, bias, activation, residual, preact)
+        return self._operator("matmul_epilogue",
+                              (precision_id, _ptr(a), _ptr(b), _ptr(bias), _fp32(bias), ACTIVATION_IDS[activation],
+                               _ptr(residual), _ptr(out), _fp32(out), _ptr(preact), _fp32(preact), m, k, n),
+                              (a, b, bias, residual, out, preact), out)
+
+    def prepare_epilogue_backward(self, dout, a=None, b=None, *, precision: str, activation: str = "none", preact=None,
+                                  da=None, db=None, dbias=None) -> PreparedOperator:
+        """Gradients of ``prepare_epilogue``: dz = dout * activation'(preact), da = dz @ b.T,
+        db = a.T @ dz, dbias = dz summed over its rows (the residual's gradient is dout).
+
+        Any of da, db, dbias may be left out, and then a (for db) or b (for da) too.  dout
+        (m, n) has the input dtype; preact is needed unless activation is none; the
+        gradients are FP32 or the input dtype.  dz enters the products rounded to the input
+        format; dbias sums the unrounded FP32 values.  Returns (da, db, dbias).
+        """
+        precision_id = self._operator_precision(precision)
+        m, k, n = validate_epilogue_backward(dout, a, b, precision, self._device, activation, preact, da, db, dbias)
+        return self._operator("matmul_epilogue_backward",
+                              (precision_id, _ptr(dout), _ptr(a), _ptr(b), _ptr(preact), _fp32(preact),
+                               ACTIVATION_IDS[activation], _ptr(da), _fp32(da), _ptr(db), _fp32(db), _ptr(dbias),
+                               _fp32(dbias), m, k, n),
+                              (dout, a, b, preact, da, db, dbias), (da, db, dbias))
+
+    def prepare_grouped(self, a, b, offsets, out, *, precision: str) -> PreparedOperator:
+        """``out[i] = a[i] @ b[g]`` for the rows ``offsets[g] <= i < offsets[g + 1]`` of each group g.
+
+        a (rows, k), b (groups, k, n), offsets (groups + 1,) int32 or int64 on the device and
+        read there when the call runs, out (rows, n) FP32 or the input dtype.  Groups may be
+        empty; rows of no group are not written.  Offsets outside [0, rows] are clipped to it
+        and one below an earlier offset counts as equal to it.  Returns out.
+        """
+        precision_id = self._operator_precision(precision)
+        rows, groups, k, n = validate_grouped(a, b, offsets, out, precision, self._device)
+        return self._operator("matmul_grouped",
+                              (precision_id, _ptr(a), _ptr(b), _ptr(offsets), int(offsets.dtype == torch.int64), groups,
+                               _ptr(out), _fp32(out), rows, k, n),
+                              (a, b, offsets, out), out)
+
+    def prepare_grouped_backward(self, dout, a=None, b=None, offsets=None, *, precision: str, da=None,
+                                 db=None) -> PreparedOperator:
+        """Gradients of ``prepare_grouped``: ``da[i] = dout[i] @ b[g].T`` for the rows of each group
+        (other rows are not written) and ``db[g] = a[rows of g].T @ dout[rows of g]`` (zeros for
+        an empty group).  Either may be left out, and then a (for db) or b (for da) too.
+        Returns (da, db).
+        """
+        precision_id = self._operator_precision(precision)
+        rows, groups, k, n = validate_grouped_backward(dout, a, b, offsets, precision, self._device, da, db)
+        return self._operator("matmul_grouped_backward",
+                              (precision_id, _ptr(dout), _ptr(a), _ptr(b), _ptr(offsets),
+                               int(offsets.dtype == torch.int64), groups, _ptr(da), _fp32(da), _ptr(db), _fp32(db),
+                               rows, k, n),
+                              (dout, a, b, offsets, da, db), (da, db))
+
+    def prepare_cross_entropy(self, hidden, weight, labels, loss, lse, *, precision: str,
+                              ignore_index: int = -100) -> PreparedOperator:
+        """Softmax cross entropy of the logits ``hidden @ weight``, which are never stored:
+        ``lse = log(sum(exp(logits), 1))`` and ``loss = lse - logits[label]`` per row.
+
+        hidden (m, k), weight (k, v); labels (m,) int32 or int64; loss and lse (m,) FP32.  A
+        row whose label is ignore_index has loss 0; any other label outside [0, v) gives NaN.
+        Returns (loss, lse).
+        """
+        precision_id = self._operator_precision(precision)
+        m, k, v = validate_cross_entropy(hidden, weight, labels, loss, lse, precision, self._device, ignore_index)
+        return self._operator("matmul_cross_entropy",
+                              (precision_id, _ptr(hidden), _ptr(weight), _ptr(labels), int(labels.dtype == torch.int64),
+                               ignore_index, _ptr(loss), _ptr(lse), m, k, v),
+                              (hidden, weight, labels, loss, lse), (loss, lse))
+
+    def prepare_cross_entropy_backward(self, grad, hidden, weight, labels, lse, *, precision: str, dhidden=None,
+                                       dweight=None, ignore_index: int = -100) -> PreparedOperator:
+        """Gradients of ``prepare_cross_entropy``: with dz = grad * (softmax(logits) - onehot(label)),
+        zero for ignored rows, dhidden = dz @ weight.T and dweight = hidden.T @ dz, computed in
+        pieces of the vocabulary from logits computed again.
+
+        grad (m,) FP32 is the gradient of each row's loss and lse what the forward call wrote.
+        dz enters the products rounded to the input format, so precision is bf16 or tf32: fp16
+        could not hold the small ones.  Either gradient may be left out; they are FP32 or the
+        input dtype.  Returns (dhidden, dweight).
+        """
+        precision_id = self._operator_precision(precision)
+        m, k, v = validate_cross_entropy_backward(grad, hidden, weight, labels, lse, precision, self._device, dhidden,
+                                                  dweight, ignore_index)
+        return self._operator("matmul_cross_entropy_backward",
+                              (precision_id, _ptr(grad), _ptr(hidden), _ptr(weight), _ptr(labels),
+                               int(labels.dtype == torch.int64), ignore_index, _ptr(lse), _ptr(dhidden), _fp32(dhidden),
+                               _ptr(dweight), _fp32(dweight), m, k, v),
+                              (grad, hidden, weight, labels, lse, dhidden, dweight), (dhidden, dweight))
 
     # ---------------------------------------------------------------- this library's additions
     def plan(self, implementation: str, m: int, k: int, n: int, precision: str = "fp32") -> dict:
