@@ -176,6 +176,11 @@ struct TileShape {
 constexpr TileShape kTileShapes[] = {{2, 256, 256}, {1, 128, 128}, {1, 128, 64}, {1, 128, 16},
                                      {1, 128, 32},  {1, 128, 64},  {1, 128, 128}};
 
+int op_epilogue_groups(int tile)
+{
+    return kTileShapes[tile].bn >= 128 ? 2 : 1;
+}
+
 bool is_swap(int tile)
 {
     return tile >= kSwap16;
@@ -375,7 +380,8 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     p.activation = activation;
     p.residual = residual;
     p.residual_half = p.out_half;
-    p.residual_vec = residual && aligned16(residual) && static_cast<int64_t>(n) * (out_half ? 2 : 4) % 16 == 0;
+    if (residual && !aligned16(residual))
+        p.out_tma = 0;
     if (preact) {
         const Matrix mz{preact, m, n, n};
         p.preact = preact;
@@ -743,7 +749,8 @@ extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hid
     OpLaunch &l = q.launch;
     l.epilogue = kEpiLse;
     l.tile = choose_tile(c.ctx, m, v, (k + bk - 1) / bk);
-    const int tiles = (v + kTileShapes[l.tile].bn - 1) / kTileShapes[l.tile].bn;
+    // One (maximum, sum) per row, column tile and epilogue warpgroup of it.
+    const int tiles = (v + kTileShapes[l.tile].bn - 1) / kTileShapes[l.tile].bn * op_epilogue_groups(l.tile);
     Operand oh, ow;
     oh.plan(c, hidden, m, k);
     ow.plan(c, weight, k, v);
@@ -855,7 +862,8 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             if (piece > 0) {
                 q.launch.p.residual = sum.ptr;
                 q.launch.p.residual_half = 0;
-                q.launch.p.residual_vec = aligned16(sum.ptr) && static_cast<int64_t>(k) * 4 % 16 == 0;
+                if (!output_tma(sum, 4))
+                    q.launch.p.out_tma = 0;
             }
             if (enqueue(c, q))
                 return 1;

@@ -1,5 +1,5 @@
-// The elementwise half of the epilogue product's backward pass: the activation gradient
-// with the bias gradient, bound by HBM.
+// Elementwise kernels of the operators, bound by HBM: the activation gradient with the
+// bias gradient, and the copy of operands that TMA cannot address.
 #pragma once
 
 #include <cuda.h>
@@ -9,6 +9,84 @@
 #include "tc_ops.cuh"
 
 namespace b200 {
+
+// ---------------------------------------------------------------- operand copy
+constexpr int RP_THREADS = 256;
+
+struct RepackPlan {
+    unsigned int grid;
+    int log_lanes;
+};
+
+// A power of two of threads per row, at most the block, that covers a row's 16-byte chunks.
+inline RepackPlan repack_plan(int64_t rows, int64_t pitch, int elem, int sms)
+{
+    const int64_t chunks = pitch * elem / 16;
+    int log_lanes = 0;
+    while ((1 << log_lanes) < RP_THREADS && (int64_t{1} << log_lanes) < chunks)
+        ++log_lanes;
+    const int64_t per_block = RP_THREADS >> log_lanes, lanes = int64_t{1} << log_lanes;
+    const int64_t units = (rows + per_block - 1) / per_block * ((chunks + lanes - 1) / lanes);
+    const int64_t cap = 32LL * sms;
+    return {static_cast<unsigned int>(units < cap ? units : cap), log_lanes};
+}
+
+// rows x cols of ELEM-byte elements at any element alignment -> rows x pitch with pitch a
+// multiple of 16 bytes, zero in the added columns.  Each thread writes 16-byte chunks; a
+// source that starts between two 4-byte words is read as a half word, three words and a
+// half word and shifted into place, so that nothing outside the matrix is read.
+template <int ELEM>
+__global__ void __launch_bounds__(RP_THREADS) repack_kernel(const uint8_t *src, uint8_t *dst, int64_t rows,
+                                                            int64_t cols, int64_t pitch, int log_lanes)
+{
+    constexpr int kPer = 16 / ELEM;
+    wait_for_prior_grid();
+    allow_next_grid();
+    const int64_t chunks = pitch / kPer;
+    const int lanes = 1 << log_lanes;
+    const int64_t segments = (chunks + lanes - 1) >> log_lanes;
+    const int per_block = RP_THREADS >> log_lanes;
+    const int64_t units = (rows + per_block - 1) / per_block * segments;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int64_t block_row = u / segments;
+        const int64_t row = block_row * per_block + (threadIdx.x >> log_lanes);
+        const int64_t c = (u - block_row * segments) * lanes + (threadIdx.x & (lanes - 1));
+        if (row >= rows || c >= chunks)
+            continue;
+        const uint8_t *from = src + (row * cols + c * kPer) * ELEM;
+        uint4 q;
+        if ((c + 1) * kPer <= cols) {
+            if (ELEM == 2 && (reinterpret_cast<uintptr_t>(from) & 2u)) {
+                const uint32_t w0 = *reinterpret_cast<const uint16_t *>(from);
+                const uint32_t w1 = *reinterpret_cast<const uint32_t *>(from + 2);
+                const uint32_t w2 = *reinterpret_cast<const uint32_t *>(from + 6);
+                const uint32_t w3 = *reinterpret_cast<const uint32_t *>(from + 10);
+                const uint32_t w4 = *reinterpret_cast<const uint16_t *>(from + 14);
+                q.x = w0 | (w1 << 16);
+                q.y = (w1 >> 16) | (w2 << 16);
+                q.z = (w2 >> 16) | (w3 << 16);
+                q.w = (w3 >> 16) | (w4 << 16);
+            } else {
+                q.x = reinterpret_cast<const uint32_t *>(from)[0];
+                q.y = reinterpret_cast<const uint32_t *>(from)[1];
+                q.z = reinterpret_cast<const uint32_t *>(from)[2];
+                q.w = reinterpret_cast<const uint32_t *>(from)[3];
+            }
+        } else {
+            uint32_t words[4] = {};
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (c * kPer + e < cols) {
+                    if constexpr (ELEM == 2)
+                        words[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(from)[e]) << (16 * (e & 1));
+                    else
+                        words[e] = reinterpret_cast<const uint32_t *>(from)[e];
+                }
+            q = make_uint4(words[0], words[1], words[2], words[3]);
+        }
+        *reinterpret_cast<uint4 *>(dst + (row * pitch + c * kPer) * ELEM) = q;
+    }
+}
 
 // ---------------------------------------------------------------- activation and bias gradient
 constexpr int AG_THREADS = 256;
@@ -74,9 +152,11 @@ __global__ void __launch_bounds__(AG_THREADS) act_grad_kernel(const ActGradParam
         read(p.dout, FMT != kOpTF32, d);
         if (p.preact) {
             read(p.preact, p.preact_half != 0, z);
+            op_with_activation(p.activation, [&](auto act) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                d[e] *= op_activation_slope(z[e], p.activation);
+                for (int e = 0; e < 8; ++e)
+                    d[e] *= op_activation_slope<decltype(act)::value>(z[e]);
+            });
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)

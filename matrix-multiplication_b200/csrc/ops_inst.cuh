@@ -11,11 +11,12 @@ struct OpInstances {
     using T = typename OpType<FMT>::T;
     static constexpr bool kHalf = FMT != kOpTF32;
 
-    // Calls f(kernel, CTAs per tile, shared memory) for the kernel of a launch.
+    // Calls f(kernel, CTAs per tile, threads, shared memory) and shared memory for the kernel of a launch.
     template <int CTAS, int BN, bool A_MN, bool B_MN, int EPI, typename F>
     static cudaError_t with(F &&f)
     {
-        return f(&op_kernel<FMT, CTAS, BN, A_MN, B_MN, EPI>, CTAS, OpTile<CTAS, BN>::kSmem);
+        using Tile = OpTile<CTAS, BN>;
+        return f(&op_kernel<FMT, CTAS, BN, A_MN, B_MN, EPI>, CTAS, Tile::kThreads, Tile::kSmem);
     }
     template <bool A_MN, bool B_MN, int EPI, typename F>
     static cudaError_t with_tile(int tile, F &&f)
@@ -54,7 +55,7 @@ struct OpInstances {
 
     static cudaError_t setup()
     {
-        auto set = [](auto kernel, int, int smem) {
+        auto set = [](auto kernel, int, int, int smem) {
             return cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         };
@@ -74,10 +75,10 @@ struct OpInstances {
 
     static cudaError_t product(const OpLaunch &l, cudaStream_t stream)
     {
-        return with_kernel(l.layout, l.tile, l.epilogue, [&](auto kernel, int ctas, int smem) {
+        return with_kernel(l.layout, l.tile, l.epilogue, [&](auto kernel, int ctas, int threads, int smem) {
             cudaLaunchConfig_t config{};
             config.gridDim = dim3(static_cast<unsigned int>(l.grid));
-            config.blockDim = dim3(OP_THREADS);
+            config.blockDim = dim3(static_cast<unsigned int>(threads));
             config.dynamicSmemBytes = static_cast<size_t>(smem);
             config.stream = stream;
             cudaLaunchAttribute attributes[2]{};
@@ -108,12 +109,10 @@ struct OpInstances {
     static cudaError_t repack(const void *src, void *dst, int64_t rows, int64_t cols, int64_t pitch, int sms,
                               cudaStream_t stream)
     {
-        const PackJob<T> job{static_cast<const T *>(src), static_cast<T *>(dst), rows, cols, pitch};
-        const PackJob<T> none{nullptr, nullptr, 0, 1, 1};
-        const int64_t blocks = (rows * pitch + 255) / 256, cap = 8LL * sms;
-        const int grid = static_cast<int>(blocks < cap ? blocks : cap);
-        return launch_pdl(pack_pair_kernel<T>, dim3(static_cast<unsigned int>(grid)), dim3(256), 0, stream, job, none,
-                          grid);
+        const RepackPlan plan = repack_plan(rows, pitch, static_cast<int>(sizeof(T)), sms);
+        return launch_pdl(repack_kernel<static_cast<int>(sizeof(T))>, dim3(plan.grid), dim3(RP_THREADS), 0, stream,
+                          static_cast<const uint8_t *>(src), static_cast<uint8_t *>(dst), rows, cols, pitch,
+                          plan.log_lanes);
     }
 
     static constexpr OpKernels kTable{setup, product, act_grad, bias_grad, repack};
