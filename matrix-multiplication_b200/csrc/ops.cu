@@ -173,12 +173,14 @@ bool output_map(const Call &c, CUtensorMap *map, const Matrix &m, bool half)
 struct TileShape {
     int ctas, bm, bn;     // CTAs per tile, D's rows and columns per tile
 };
-constexpr TileShape kTileShapes[] = {{2, 256, 256}, {1, 128, 128}, {1, 128, 64}, {1, 128, 16},
-                                     {1, 128, 32},  {1, 128, 64},  {1, 128, 128}};
+constexpr TileShape kTileShapes[] = {{2, 256, 256}, {2, 256, 512}, {1, 128, 128}, {1, 128, 64},
+                                     {1, 128, 16},  {1, 128, 32},  {1, 128, 64},  {1, 128, 128}};
 
-int op_epilogue_groups(int tile)
+// Column ranges of a tile that the loss reduces on its own (halves x epilogue warpgroups).
+int loss_parts(int tile)
 {
-    return kTileShapes[tile].bn >= 128 ? 2 : 1;
+    const int bn = kTileShapes[tile].bn;
+    return bn > 256 ? 4 : bn >= 128 ? 2 : 1;
 }
 
 bool is_swap(int tile)
@@ -186,37 +188,76 @@ bool is_swap(int tile)
     return tile >= kSwap16;
 }
 
-// Estimated cycles of `tiles` tiles of a kind with K blocks of 128 bytes: the model and
-// the constants of the plain product's plan (matmul_b200.cu): a K block costs the most
-// of its MMA time, its operand bytes into one SM at 55 B/cycle, and all running CTAs'
-// bytes out of L2 at 8 KB/cycle.
-double tile_cycles(const Context *ctx, int tile, double tiles, double k_blocks)
+// Estimated cycles of `tiles` tiles of a kind with K blocks of 128 bytes, K split S ways:
+// the model and the constants of the plain product's plan (matmul_b200.cu): a K block
+// costs the most of its MMA time, its operand bytes into one SM at 55 B/cycle, and all
+// running CTAs' bytes out of L2 at 8 KB/cycle; a split adds its exchange.
+double tile_cycles(const Context *ctx, int tile, int splits, double tiles, double k_blocks)
 {
     const TileShape &t = kTileShapes[tile];
     const double units = t.ctas == 2 ? ctx->max_pairs : ctx->sm_count;
-    const double active = t.ctas * std::min(tiles, units);
-    const double rounds = std::max(1.0, std::ceil(tiles / units));
+    const double active = splits > 1 ? tiles * splits : t.ctas * std::min(tiles, units);
+    double rounds = splits > 1 ? 1.0 : std::max(1.0, std::ceil(tiles / units));
     const double bytes = static_cast<double>(OP_BM + t.bn / t.ctas) * OP_ROW_BYTES;
     const double k_cycles = std::max({2.0 * t.bn, bytes / 55.0, active * bytes / 8000.0});
-    return 2000.0 + rounds * (k_blocks * k_cycles + 4000.0 * t.bn / 256.0) + (t.ctas == 2 ? 10000.0 : 0.0);
+    // A 512-column tile's second half is read once the first one's outputs are on their way,
+    // and the next tile's MMAs wait for that: about 24000 cycles a tile where a 256-column
+    // tile, whose two accumulators alternate, loses 4000.  So the wide tile is for long K:
+    // 4096 x 14336 x 4096 BF16 316 us against 345 us, but 4096 x 4096 x 14336 380 against 334.
+    const double epilogue = t.bn == 512 ? 24000.0 : 4000.0 * t.bn / 256.0;
+    // A short last round of 512-column tiles runs as halves (enqueue).
+    if (t.bn == 512 && tiles - std::floor(tiles / units) * units <= units / 2)
+        rounds = std::floor(tiles / units) + (std::fmod(tiles, units) > 0.0 ? 0.5 : 0.0);
+    return 2000.0 + rounds * (std::ceil(k_blocks / splits) * k_cycles + epilogue) +
+           (t.ctas == 2 ? 10000.0 : 0.0) +
+           (splits > 1 ? 1000.0 + static_cast<double>(splits - 1) / splits * OP_BM * t.bn * 4.0 / 8.0 : 0.0);
 }
 
-int choose_tile(const Context *ctx, int64_t m, int64_t n, int64_t k_blocks, int64_t groups = 1)
+struct TileChoice {
+    int tile, splits;
+};
+
+// Whether K blocks split S ways leave every CTA some and fit the device in one wave.
+bool can_split(const Context *ctx, int log_splits, int64_t tiles, int64_t k_blocks)
 {
-    int best = kSingle64;
+    const int64_t splits = int64_t{1} << log_splits, per = (k_blocks + splits - 1) / splits;
+    return tiles * splits <= ctx->max_split_ctas[log_splits] && (splits - 1) * per < k_blocks;
+}
+
+// The tile and K split with the fewest estimated cycles for an m x n product (of one of
+// `groups` groups).  Splits are for ungrouped products whose epilogue can take partial sums.
+TileChoice choose_tile(const Context *ctx, int64_t m, int64_t n, int64_t k_blocks, int64_t groups = 1,
+                       bool splittable = false)
+{
+    TileChoice best{kSingle64, 1};
     double best_cycles = 0.0;
-    for (int tile : {kPair256, kSingle128, kSingle64}) {
+    for (int tile : {kPair256, kPair512, kSingle128, kSingle64}) {
         const TileShape &t = kTileShapes[tile];
-        if (t.ctas == 2 && (ctx->max_pairs < 1 || m <= OP_BM))
+        if (t.ctas == 2 && (ctx->max_pairs < 1 || m <= OP_BM || (tile == kPair512 && n <= 256)))
             continue;
-        const double tiles = static_cast<double>((m + t.bm - 1) / t.bm) * static_cast<double>((n + t.bn - 1) / t.bn) *
-                             static_cast<double>(groups);
-        const double cycles = tile_cycles(ctx, tile, tiles, static_cast<double>(k_blocks));
-        if (best_cycles == 0.0 || cycles < best_cycles) {
-            best = tile;
-            best_cycles = cycles;
+        const int64_t tiles = (m + t.bm - 1) / t.bm * ((n + t.bn - 1) / t.bn) * groups;
+        for (int i = 0; i < (splittable && t.ctas == 1 ? 4 : 1); ++i) {
+            if (i > 0 && !can_split(ctx, i, tiles, k_blocks))
+                continue;
+            const double cycles = tile_cycles(ctx, tile, 1 << i, static_cast<double>(tiles), static_cast<double>(k_blocks));
+            if (best_cycles == 0.0 || cycles < best_cycles) {
+                best = {tile, 1 << i};
+                best_cycles = cycles;
+            }
         }
     }
+    return best;
+}
+
+// At most 64 rows: the transposed tile that holds them, and the most K splits that fit with
+// four K blocks each (bound by the weight's bytes: more SMs streaming them is what counts).
+TileChoice choose_few_rows(const Context *ctx, int64_t m, int64_t n, int64_t k_blocks)
+{
+    TileChoice best{m <= 16 ? kSwap16 : m <= 32 ? kSwap32 : kSwap64, 1};
+    const int64_t tiles = (n + OP_BM - 1) / OP_BM;
+    for (int i = 1; i < 4; ++i)
+        if (can_split(ctx, i, tiles, k_blocks) && (k_blocks >> i) >= 4)
+            best.splits = 1 << i;
     return best;
 }
 
@@ -226,7 +267,22 @@ struct Product {
     Matrix a, b;             // kNN: M x K, K x N;  kNT: M x K, N x K;  kTN: K x M, K x N
     int64_t m = 0, n = 0, k = 0;
     OpLaunch launch;
+    void set_tile(const TileChoice &choice)
+    {
+        launch.tile = choice.tile;
+        launch.splits = choice.splits;
+    }
 };
+
+// Exact quotients by a positive divisor on the device (op_divide).
+OpDivisor divisor(int64_t value)
+{
+    int bits = 0;
+    while ((int64_t{1} << bits) < value)
+        ++bits;
+    const uint64_t magic = (((uint64_t{1} << bits) - static_cast<uint64_t>(value)) << 32) / static_cast<uint64_t>(value) + 1;
+    return {static_cast<uint32_t>(magic), static_cast<uint32_t>(bits > 0 ? bits - 1 : 0), static_cast<int>(value)};
+}
 
 int enqueue(Call &c, Product &q)
 {
@@ -234,7 +290,7 @@ int enqueue(Call &c, Product &q)
     const TileShape &t = kTileShapes[l.tile];
     const bool swap = is_swap(l.tile);
     const bool a_mn = l.layout == kTN, b_mn = l.layout != kNT;
-    const int b_cols = t.bn / t.ctas;
+    const int b_cols = std::min(t.bn, 256) / t.ctas;     // rows of a K-major box of Bop
     bool ok;
     if (swap)     // D = B^T A^T: B's columns on the M side, A's rows on the N side
         ok = operand_map(c, &l.map_a, q.b, true, OP_BM) && operand_map(c, &l.map_b, q.a, false, b_cols);
@@ -261,12 +317,26 @@ int enqueue(Call &c, Product &q)
     if (tiles > 0x7fffffff)
         return c.failed("too many output tiles");
     p.num_tiles = static_cast<int>(tiles);
-    if (p.raster == 0)
-        p.raster = swap ? p.num_m_blocks : t.ctas == 2 ? 8 : 16;
+    p.log_raster = t.ctas == 2 ? 3 : 4;
+    const int64_t per_raster = swap ? p.num_m_blocks : static_cast<int64_t>(p.num_n_blocks) << p.log_raster;
+    const int64_t per_group = static_cast<int64_t>(p.num_m_blocks) * p.num_n_blocks;
+    p.per_raster = divisor(std::min<int64_t>(per_raster, 0x7fffffff));
+    p.per_group = divisor(std::min<int64_t>(per_group, 0x7fffffff));
+    // 512 columns: when the last round has few tiles, they run as halves on twice the pairs
+    // (4096 x 4096 x 14336: 448 tiles on 74 pairs, 6.5 rounds in place of 7).
+    p.full_tiles = p.num_tiles;
+    if (l.tile == kPair512 && p.grouping == kUngrouped) {
+        const int rest = p.num_tiles % c.ctx->max_pairs;
+        if (2 * rest <= c.ctx->max_pairs) {
+            p.full_tiles = p.num_tiles - rest;
+            p.num_tiles += rest;
+            tiles = p.num_tiles;
+        }
+    }
     p.status = c.ctx->status;
     p.wait_limit_ns = wait_limit(c.ctx);
     const int64_t units = t.ctas == 2 ? c.ctx->max_pairs : c.ctx->sm_count;
-    l.grid = static_cast<int>(std::min(tiles, units)) * t.ctas;
+    l.grid = l.splits > 1 ? static_cast<int>(tiles) : static_cast<int>(std::min(tiles, units)) * t.ctas;
     const cudaError_t st = c.kernels().product(l, c.stream);
     return st == cudaSuccess ? 0 : c.failed(st);
 }
@@ -364,13 +434,12 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     q.k = k;
     OpLaunch &l = q.launch;
     const int bk = OP_ROW_BYTES / e;
-    if (m <= 64) {
-        l.tile = m <= 16 ? kSwap16 : m <= 32 ? kSwap32 : kSwap64;
-        l.epilogue = kEpiStoreT;
-    } else {
-        l.tile = choose_tile(c.ctx, m, n, (static_cast<int64_t>(k) + bk - 1) / bk);
-        l.epilogue = kEpiStore;
-    }
+    const int64_t k_blocks = (static_cast<int64_t>(k) + bk - 1) / bk;
+    const TileChoice choice = m <= 64 ? choose_few_rows(c.ctx, m, n, k_blocks)
+                                      : choose_tile(c.ctx, m, n, k_blocks, 1, true);
+    l.tile = choice.tile;
+    l.splits = choice.splits;
+    l.epilogue = m <= 64 ? kEpiStoreT : kEpiStore;
     const Matrix mo{out, m, n, n};
     if (set_output(c, l, mo, out_half))
         return 1;
@@ -497,7 +566,7 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.n = k;
         q.k = n;
         q.launch.layout = kNT;
-        q.launch.tile = choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk);
+        q.set_tile(choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk, 1, true));
         if (set_output(c, q.launch, Matrix{da, m, k, k}, da_half) || enqueue(c, q))
             return 1;
     }
@@ -509,7 +578,7 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.n = n;
         q.k = m;
         q.launch.layout = kTN;
-        q.launch.tile = choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk);
+        q.set_tile(choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk, 1, true));
         if (set_output(c, q.launch, Matrix{db, k, n, n}, db_half) || enqueue(c, q))
             return 1;
     }
@@ -522,7 +591,8 @@ namespace {
 // the groups' tensor maps.
 struct GroupPlan {
     int tile_rows = 0, maps = 0;
-    size_t maps_at = 0, tiles_at = 0, count_at = 0;
+    size_t maps_at = 0, tiles_at = 0, count_at = 0, units_at = 0;
+    int units = 0;
 
     // tile_rows 0: ragged-K mode.
     void plan(Call &c, int groups, int rows, int tile, int map_count)
@@ -533,11 +603,20 @@ struct GroupPlan {
         maps_at = c.reserve(static_cast<size_t>(groups) * std::max(maps, 1) * sizeof(CUtensorMap));
         tiles_at = c.reserve(static_cast<size_t>(entries) * sizeof(OpRowTile));
         count_at = c.reserve(sizeof(int));
+        units_at = c.reserve(static_cast<size_t>(c.ctx->sm_count + 1) * sizeof(int));
     }
+    // `tiles_per_group`, `max_units`: ragged-K mode's tiles and the CTAs or pairs that share them.
     int enqueue(Call &c, const void *offsets, int offsets64, int groups, int rows, const CUtensorMap &map0,
-                const CUtensorMap &map1, OpParams &p)
+                const CUtensorMap &map1, OpParams &p, int64_t tiles_per_group = 0, int64_t max_units = 0)
     {
         GroupPlanParams g{};
+        if (!tile_rows) {
+            g.units = static_cast<int>(std::min(tiles_per_group * groups, max_units));
+            g.unit_first = reinterpret_cast<int *>(c.scratch + units_at);
+            g.tiles_per_group = tiles_per_group;
+            g.k_block = OP_ROW_BYTES / c.elem();
+            p.unit_first = g.unit_first;
+        }
         g.offsets = offsets;
         g.offsets64 = offsets64;
         g.groups = groups;
@@ -547,12 +626,14 @@ struct GroupPlan {
         g.count = reinterpret_cast<int *>(c.scratch + count_at);
         g.tiles = reinterpret_cast<OpRowTile *>(c.scratch + tiles_at);
         g.group_maps = reinterpret_cast<CUtensorMap *>(c.scratch + maps_at);
+        // One warp per tensor map, up to sixteen blocks.
+        const unsigned int blocks = static_cast<unsigned int>(std::min(16, std::max(1, groups * maps / (GP_THREADS / 32))));
         p.grouping = tile_rows ? kGroupedRows : kGroupedK;
         p.groups = groups;
         p.row_tile_count = g.count;
         p.row_tiles = g.tiles;
         p.group_maps = g.group_maps;
-        const cudaError_t st = launch_pdl(group_plan_kernel, dim3(1), dim3(GP_THREADS), 0, c.stream, map0, map1, g);
+        const cudaError_t st = launch_pdl(group_plan_kernel, dim3(blocks), dim3(GP_THREADS), 0, c.stream, map0, map1, g);
         return st == cudaSuccess ? 0 : c.failed(st);
     }
 };
@@ -581,7 +662,7 @@ int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_
         return kSwap64;
     if (mean <= 128)
         return kSwap128;
-    return choose_tile(ctx, mean, n, k_blocks, groups);
+    return choose_tile(ctx, mean, n, k_blocks, groups).tile;
 }
 
 // A product over row groups: out[i] = a[i] . b[g] (layout kNN) or a[i] . b[g]^T (kNT).
@@ -671,14 +752,14 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
         ob.plan(c, b, k, n, groups);
         const int64_t mean = (rows + groups - 1) / groups;
         qa.launch.layout = kNT;
-        qa.launch.tile = choose_tile(c.ctx, mean, k, (n + bk - 1) / bk, groups);
+        qa.launch.tile = choose_tile(c.ctx, mean, k, (n + bk - 1) / bk, groups).tile;
         rows_plan.plan(c, groups, rows, kTileShapes[qa.launch.tile].bm, output_tma(ma, da_half ? 2 : 4) ? 1 : 0);
     }
     if (db) {
         oa.plan(c, a, rows, k);
         const int64_t mean = (rows + groups - 1) / groups;
         qb.launch.layout = kTN;
-        qb.launch.tile = choose_tile(c.ctx, k, n, (mean + bk - 1) / bk, groups);
+        qb.launch.tile = choose_tile(c.ctx, k, n, (mean + bk - 1) / bk, groups).tile;
         k_plan.plan(c, groups, rows, 0, 2);
     }
     if (c.allocate() || od.prepare(c) || (da && ob.prepare(c)) || (db && oa.prepare(c)))
@@ -700,12 +781,15 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
         qb.k = rows;
         const TileShape &t = kTileShapes[qb.launch.tile];
         CUtensorMap map0, map1;
-        if (!operand_map(c, &map0, qb.a, true, OP_BM) || !operand_map(c, &map1, qb.b, true, t.bn / t.ctas)) {
+        if (!operand_map(c, &map0, qb.a, true, OP_BM) || !operand_map(c, &map1, qb.b, true, std::min(t.bn, 256) / t.ctas)) {
             cudaGetLastError();
             return c.failed("cuTensorMapEncodeTiled rejected an operand");
         }
         if (set_output(c, qb.launch, Matrix{db, k, n, n, groups, static_cast<int64_t>(k) * n}, db_half) ||
-            k_plan.enqueue(c, offsets, offsets64, groups, rows, map0, map1, qb.launch.p) || enqueue(c, qb))
+            k_plan.enqueue(c, offsets, offsets64, groups, rows, map0, map1, qb.launch.p,
+                           ((k + t.bm - 1) / t.bm) * ((static_cast<int64_t>(n) + t.bn - 1) / t.bn),
+                           t.ctas == 2 ? c.ctx->max_pairs : c.ctx->sm_count) ||
+            enqueue(c, qb))
             return 1;
     }
     return 0;
@@ -748,9 +832,9 @@ extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hid
     Product q;
     OpLaunch &l = q.launch;
     l.epilogue = kEpiLse;
-    l.tile = choose_tile(c.ctx, m, v, (k + bk - 1) / bk);
-    // One (maximum, sum) per row, column tile and epilogue warpgroup of it.
-    const int tiles = (v + kTileShapes[l.tile].bn - 1) / kTileShapes[l.tile].bn * op_epilogue_groups(l.tile);
+    l.tile = choose_tile(c.ctx, m, v, (k + bk - 1) / bk).tile;
+    // One (maximum, sum) per row and column range of a tile.
+    const int tiles = (v + kTileShapes[l.tile].bn - 1) / kTileShapes[l.tile].bn * loss_parts(l.tile);
     Operand oh, ow;
     oh.plan(c, hidden, m, k);
     ow.plan(c, weight, k, v);
@@ -835,7 +919,7 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = cols;
             q.k = k;
             q.launch.epilogue = kEpiSoftmaxGrad;
-            q.launch.tile = choose_tile(c.ctx, m, cols, (k + bk - 1) / bk);
+            q.launch.tile = choose_tile(c.ctx, m, cols, (k + bk - 1) / bk).tile;
             OpParams &p = q.launch.p;
             p.labels = labels;
             p.labels64 = labels64;
@@ -855,7 +939,7 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = k;
             q.k = cols;
             q.launch.layout = kNT;
-            q.launch.tile = choose_tile(c.ctx, m, k, (cols + bk - 1) / bk);
+            q.set_tile(choose_tile(c.ctx, m, k, (cols + bk - 1) / bk, 1, true));
             const bool last = piece == pieces - 1;
             if (set_output(c, q.launch, last ? dh : sum, last && dh_half))
                 return 1;
@@ -876,7 +960,7 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = cols;
             q.k = m;
             q.launch.layout = kTN;
-            q.launch.tile = choose_tile(c.ctx, k, cols, (m + bk - 1) / bk);
+            q.set_tile(choose_tile(c.ctx, k, cols, (m + bk - 1) / bk, 1, true));
             const Matrix dw{static_cast<uint8_t *>(dweight) + v0 * (dw_half ? 2 : 4), k, cols, v};
             if (set_output(c, q.launch, dw, dw_half) || enqueue(c, q))
                 return 1;

@@ -23,6 +23,7 @@ struct OpInstances {
     {
         switch (tile) {
         case kPair256: return with<2, 256, A_MN, B_MN, EPI>(f);
+        case kPair512: return with<2, 512, A_MN, B_MN, EPI>(f);
         case kSingle128: return with<1, 128, A_MN, B_MN, EPI>(f);
         case kSingle64: return with<1, 64, A_MN, B_MN, EPI>(f);
         }
@@ -77,7 +78,7 @@ struct OpInstances {
     {
         return with_kernel(l.layout, l.tile, l.epilogue, [&](auto kernel, int ctas, int threads, int smem) {
             cudaLaunchConfig_t config{};
-            config.gridDim = dim3(static_cast<unsigned int>(l.grid));
+            config.gridDim = dim3(static_cast<unsigned int>(l.grid), 1, static_cast<unsigned int>(l.splits));
             config.blockDim = dim3(static_cast<unsigned int>(threads));
             config.dynamicSmemBytes = static_cast<size_t>(smem);
             config.stream = stream;
@@ -87,9 +88,9 @@ struct OpInstances {
             attributes[1].id = cudaLaunchAttributeClusterDimension;
             attributes[1].val.clusterDim.x = static_cast<unsigned int>(ctas);
             attributes[1].val.clusterDim.y = 1;
-            attributes[1].val.clusterDim.z = 1;
+            attributes[1].val.clusterDim.z = static_cast<unsigned int>(l.splits);
             config.attrs = attributes;
-            config.numAttrs = ctas > 1 ? 2 : 1;
+            config.numAttrs = ctas > 1 || l.splits > 1 ? 2 : 1;
             return cudaLaunchKernelEx(&config, kernel, l.map_a, l.map_b, l.map_c, l.map_z, l.p);
         });
     }

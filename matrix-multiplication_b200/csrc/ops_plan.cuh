@@ -12,7 +12,8 @@
 namespace b200 {
 
 // ---------------------------------------------------------------- plan of a grouped product
-constexpr int GP_THREADS = 1024;
+constexpr int GP_THREADS = 256;
+constexpr int GP_WARPS = GP_THREADS / 32;
 
 struct GroupPlanParams {
     const void *offsets;      // groups + 1 row offsets
@@ -23,21 +24,34 @@ struct GroupPlanParams {
     int *count;               // number of row tiles
     OpRowTile *tiles;
     CUtensorMap *group_maps;  // [groups][maps]
+    // Ragged-K mode: the first tile of each of `units` CTAs or pairs (and the end).
+    int units;
+    int *unit_first;
+    long long tiles_per_group;
+    int k_block;              // rows per K block
 };
 
-// One block: group g's rows are [max(offsets[0..g]), max(offsets[0..g+1])) clipped to
+// A tile's epilogue in K blocks, for the shares of ragged-K mode.
+constexpr int GP_EPILOGUE_BLOCKS = 6;
+
+// Group g's rows are [max(offsets[0..g]), max(offsets[0..g+1])) clipped to
 // [0, rows], so that whatever the offsets hold, groups are disjoint, in order and in
 // range.  Rows mode writes ceil(rows of g / tile_rows) entries per group, in order;
-// ragged-K mode one entry per group.  Each group's tensor maps are the templates with
-// the row extent cut at the group's end.
+// ragged-K mode one entry per group (`unused` = K blocks and epilogues of a tile of each
+// group before it, summed) and each unit's share: consecutive tiles of about the same
+// total weight, so that a unit meets few groups (each costs it two tensor-map fences
+// before its loads can start: with tiles dealt out in turn, 64 groups of 256 rows took
+// 420 us on 2048 x 2816 outputs).  Each group's tensor maps are the templates with the
+// row extent cut at the group's end.  Every block computes the ends; block 0 writes the
+// tables, all blocks share the maps.
 __global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_constant__ CUtensorMap map0,
                                                                 const __grid_constant__ CUtensorMap map1,
                                                                 const GroupPlanParams p)
 {
-    __shared__ int warp_max[32], warp_sum[32];
+    __shared__ int warp_max[GP_WARPS], warp_sum[GP_WARPS];
     __shared__ int carry_max, carry_sum;
     __shared__ int ends[GP_THREADS];
-    __shared__ __align__(128) uint8_t map_s[32][128];
+    __shared__ __align__(128) uint8_t map_s[GP_WARPS][128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     wait_for_prior_grid();
     allow_next_grid();
@@ -70,7 +84,9 @@ __global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_con
         ends[threadIdx.x] = end;
         __syncthreads();
         const int begin = threadIdx.x ? ends[threadIdx.x - 1] : carry_max;
-        const int count = g < p.groups && p.tile_rows ? (end - begin + p.tile_rows - 1) / p.tile_rows : 0;
+        const int count = g >= p.groups    ? 0
+                          : p.tile_rows ? (end - begin + p.tile_rows - 1) / p.tile_rows
+                                        : (end - begin + p.k_block - 1) / p.k_block + GP_EPILOGUE_BLOCKS;
         // Running sum of the tile counts.
         int sum = count;
         for (int d = 1; d < 32; d <<= 1) {
@@ -84,38 +100,36 @@ __global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_con
         int first = carry_sum + sum - count;
         for (int i = 0; i < warp; ++i)
             first += warp_sum[i];
-        if (g < p.groups) {
+        if (g < p.groups && blockIdx.x == 0) {
             if (p.tile_rows) {
                 for (int i = 0; i < count; ++i)
                     p.tiles[first + i] = OpRowTile{g, begin + i * p.tile_rows, end, 0};
             } else {
-                p.tiles[g] = OpRowTile{g, begin, end, 0};
+                p.tiles[g] = OpRowTile{g, begin, end, first};
             }
         }
         // Tensor maps of this chunk's groups, one warp each.
-        if (p.maps) {
-            for (int i = warp; i < GP_THREADS && g0 + i < p.groups; i += 32) {
-                for (int j = 0; j < p.maps; ++j) {
-                    const uint32_t s = smem_addr(map_s[warp]);
-                    const uint32_t *src = reinterpret_cast<const uint32_t *>(j ? &map1 : &map0);
-                    reinterpret_cast<uint32_t *>(map_s[warp])[lane] = src[lane];
-                    __syncwarp();
-                    if (lane == 0) {
-                        const uint32_t extent = static_cast<uint32_t>(max(ends[i], 1));
-                        asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"l"(
-                                         static_cast<uint64_t>(s)),
-                                     "r"(extent)
-                                     : "memory");
-                    }
-                    __syncwarp();
-                    asm volatile(
-                        "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned "
-                        "[%0], [%1], 128;" ::"l"(reinterpret_cast<uint64_t>(p.group_maps + (g0 + i) * p.maps + j)),
-                        "r"(s)
-                        : "memory");
-                    __syncwarp();
-                }
+        for (int i = warp + GP_WARPS * static_cast<int>(blockIdx.x);
+             i < GP_THREADS * p.maps && g0 + i / p.maps < p.groups; i += GP_WARPS * static_cast<int>(gridDim.x)) {
+            const uint32_t s = smem_addr(map_s[warp]);
+            const int local = i / p.maps;
+            const uint32_t *src = reinterpret_cast<const uint32_t *>(i - local * p.maps ? &map1 : &map0);
+            reinterpret_cast<uint32_t *>(map_s[warp])[lane] = src[lane];
+            __syncwarp();
+            if (lane == 0) {
+                const uint32_t extent = static_cast<uint32_t>(max(ends[local], 1));
+                asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"l"(
+                                 static_cast<uint64_t>(s)),
+                             "r"(extent)
+                             : "memory");
             }
+            __syncwarp();
+            asm volatile(
+                "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned "
+                "[%0], [%1], 128;" ::"l"(reinterpret_cast<uint64_t>(p.group_maps + static_cast<int64_t>(g0) * p.maps + i)),
+                "r"(s)
+                : "memory");
+            __syncwarp();
         }
         __syncthreads();
         if (threadIdx.x == GP_THREADS - 1) {
@@ -124,8 +138,30 @@ __global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_con
         }
         __syncthreads();
     }
-    if (threadIdx.x == 0 && p.count)
-        *p.count = carry_sum;
+    if (blockIdx.x != 0)
+        return;
+    if (p.tile_rows) {
+        if (threadIdx.x == 0)
+            *p.count = carry_sum;
+        return;
+    }
+    // Unit u starts at the first tile at or past u / units of all tiles' weight.
+    for (int u = threadIdx.x; u <= p.units; u += GP_THREADS) {
+        const long long total = carry_sum * p.tiles_per_group;
+        const long long target = total / p.units * u + total % p.units * u / p.units;
+        int lo = 0, hi = p.groups;          // the last group that starts at or before the target
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (p.tiles[mid].unused * p.tiles_per_group <= target)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        const int before = p.tiles[lo].unused;
+        const int weight = (lo + 1 < p.groups ? p.tiles[lo + 1].unused : carry_sum) - before;
+        const long long local = (target - before * p.tiles_per_group + weight - 1) / weight;
+        p.unit_first[u] = static_cast<int>(lo * p.tiles_per_group + min(local, p.tiles_per_group));
+    }
 }
 
 // ---------------------------------------------------------------- loss

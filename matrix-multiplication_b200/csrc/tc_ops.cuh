@@ -50,22 +50,28 @@ constexpr int OP_A_STAGE = OP_BM * OP_ROW_BYTES;
 constexpr int OP_BOX = 128 * 128;             // epilogue box: 128 rows x 128 bytes
 constexpr int OP_BAR_BYTES = 512;
 
-// Geometry of a tile of BN N columns on one CTA or a pair.  Tiles of 128 columns and
-// more have two epilogue warpgroups, each with half of the columns: one warpgroup
-// needs longer for an activation and two outputs than the MMAs of a 4096-deep tile.
-// Five 32 KB stages cover the load latency as well as six do; the sixth's place goes
-// to the second warpgroup's boxes.
+// Geometry of a tile of BN N columns on one CTA or a pair.  A 512-column tile is two
+// halves of 256 that share one accumulator set, freed half by half (tc2_gemm.cuh); the
+// others have two accumulators.  Tiles of 128 columns and more have two epilogue
+// warpgroups, each with half of the columns: one warpgroup needs longer for an
+// activation and two outputs than the MMAs of a 4096-deep 256 x 256 tile (4096 x 4096 x
+// 14336 BF16 with gelu, bias and pre-activation: 609 us with one, 496 us with two).
 template <int CTAS, int BN>
 struct OpTile {
+    static constexpr int kParts = BN > 256 ? 2 : 1;            // 256-column halves
+    static constexpr int kPartCols = BN / kParts;
+    static constexpr int kAccs = BN > 256 ? 1 : 2;
     static constexpr int kBCols = BN / CTAS;                   // N columns staged per CTA
     static constexpr int kBStage = kBCols * OP_ROW_BYTES;
-    static constexpr int kStages = kBCols >= 128 ? 5 : kBCols >= 64 ? 8 : 9;
+    static constexpr int kStages = kBCols >= 256 ? 4 : kBCols >= 128 ? 6 : 8;
     static constexpr int kGroups = BN >= 128 ? 2 : 1;          // epilogue warpgroups
-    static constexpr int kThreads = 64 + 128 * kGroups;        // TMA warp, MMA warp, epilogue
-    static constexpr int kEpiBytes = 2 * kGroups * OP_BOX;     // two boxes each
-    static constexpr int kBiasBytes = BN * 4 < 256 ? 256 : BN * 4;
+    static constexpr int kFirstEpi = kGroups == 2 ? 4 : 2;     // first epilogue warp (after TMA, MMA, two idle ones)
+    static constexpr int kThreads = 32 * (kFirstEpi + 4 * kGroups);
+    static constexpr int kBoxes = 3 - kGroups;                 // boxes per epilogue warpgroup: two in all
+    static constexpr int kEpiBytes = kBoxes * kGroups * OP_BOX;
+    static constexpr int kBiasBytes = kPartCols * 4 < 256 ? 256 : kPartCols * 4;
     static constexpr int kSmem = 1024 + kStages * (OP_A_STAGE + kBStage) + kEpiBytes + OP_BAR_BYTES + kBiasBytes;
-    static constexpr uint32_t kTmemColumns = 2 * BN < 32 ? 32 : 2 * BN;   // two accumulators
+    static constexpr uint32_t kTmemColumns = kAccs * BN < 32 ? 32 : kAccs * BN;
     static_assert(kSmem <= 227 * 1024, "tile exceeds shared memory");
 };
 
@@ -74,15 +80,32 @@ struct OpRowTile {
     int group, row0, row_end, unused;
 };
 
+// Division by a divisor the host knows (Granlund and Montgomery's multiply-and-shift for
+// 32-bit numbers): quotients of numbers below 2^31.
+struct OpDivisor {
+    uint32_t magic, shift;
+    int value;
+};
+
+__device__ __forceinline__ int op_divide(int x, const OpDivisor &d)
+{
+    const uint32_t t = __umulhi(d.magic, static_cast<uint32_t>(x));
+    return d.value == 1 ? x : static_cast<int>((t + ((static_cast<uint32_t>(x) - t) >> 1)) >> d.shift);
+}
+
 struct OpParams {
     int m, n;                 // rows and columns of the output (of one group in ragged-K mode)
     int num_m_blocks, num_n_blocks, num_k_blocks;   // M- and N-side tiles of D, K blocks
     int num_tiles;
-    int raster;               // M-side tiles per raster group
+    int full_tiles;           // 512 columns: tiles from here on are halves of a tile (two indices a tile)
+    int log_raster;           // log2 of the M-side tiles per raster group
+    OpDivisor per_raster;     // raster x N-side tiles (transposed epilogue: M-side tiles)
+    OpDivisor per_group;      // ragged-K mode: tiles of one group
     int grouping;             // OpGrouping
     const int *row_tile_count;        // rows mode: number of row tiles (device)
     const OpRowTile *row_tiles;       // rows mode: table of row tiles; ragged-K mode: one entry per group
     const CUtensorMap *group_maps;    // rows mode: out's map per group; ragged-K mode: Aop's and Bop's
+    const int *unit_first;            // ragged-K mode: the first tile of each CTA or pair, and the end
     int groups;
     // kEpiStore / kEpiStoreT / kEpiSoftmaxGrad
     void *out;
@@ -134,6 +157,38 @@ __device__ __forceinline__ void tma_store_3d(const void *map, uint32_t src, int 
                      reinterpret_cast<uint64_t>(map)),
                  "r"(src), "r"(x), "r"(y), "r"(z)
                  : "memory");
+}
+
+// Arrives on an mbarrier of a CTA of this cluster with CTA-scope release: what the
+// arrival reports is that this warp's TMEM loads have completed (tcgen05.wait::ld).  A
+// cluster-scope release also waits for the stores this thread has under way, 1700 of the
+// 7100 cycles of a 256 x 256 tile with K = 256.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// 64 consecutive FP32 columns of this thread's TMEM lane, waited for in the same asm block.
+__device__ __forceinline__ void tmem_load_64cols(uint32_t taddr, float (&v)[64])
+{
+    uint32_t(&u)[64] = reinterpret_cast<uint32_t(&)[64]>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31]), "=r"(u[32]),
+          "=r"(u[33]), "=r"(u[34]), "=r"(u[35]), "=r"(u[36]), "=r"(u[37]), "=r"(u[38]), "=r"(u[39]), "=r"(u[40]),
+          "=r"(u[41]), "=r"(u[42]), "=r"(u[43]), "=r"(u[44]), "=r"(u[45]), "=r"(u[46]), "=r"(u[47]), "=r"(u[48]),
+          "=r"(u[49]), "=r"(u[50]), "=r"(u[51]), "=r"(u[52]), "=r"(u[53]), "=r"(u[54]), "=r"(u[55]), "=r"(u[56]),
+          "=r"(u[57]), "=r"(u[58]), "=r"(u[59]), "=r"(u[60]), "=r"(u[61]), "=r"(u[62]), "=r"(u[63])
+        : "r"(taddr)
+        : "memory");
 }
 
 // A tensor map written by an earlier kernel is read through the tensor-map proxy.
@@ -275,39 +330,57 @@ __device__ __forceinline__ int op_label(const OpParams &p, int row)
 // the end of the output rows it may write.
 struct OpWhere {
     int m0, n0, group, nkb, k0, row_end;
-    int n_block;
+    int parts;         // 256-column halves
+    int loss_block;    // index of the first half among all column tiles' halves
 };
 
 template <int CTAS, int BN, bool SWAP>
 __device__ __forceinline__ OpWhere op_where(int tile, int row_tile_count, int bk, const OpParams &p)
 {
     constexpr int kBM = OP_BM * CTAS;
+    constexpr bool kHalves = BN > 256;
     OpWhere w;
-    int local = tile, blocks_m = p.num_m_blocks, blocks_n = p.num_n_blocks;
+    int half = 0;
+    w.parts = kHalves ? 2 : 1;
+    if (kHalves && tile >= p.full_tiles) {
+        half = (tile - p.full_tiles) & 1;
+        tile = p.full_tiles + ((tile - p.full_tiles) >> 1);
+        w.parts = 1;
+    }
+    int local = tile;
     w.group = 0;
     w.k0 = 0;
     w.nkb = p.num_k_blocks;
     w.row_end = p.m;
     if (p.grouping == kGroupedK) {
-        const int per_group = blocks_m * blocks_n;
-        w.group = tile / per_group;
-        local = tile - w.group * per_group;
+        w.group = op_divide(tile, p.per_group);
+        local = tile - w.group * p.per_group.value;
         const OpRowTile t = p.row_tiles[w.group];
         w.k0 = t.row0;
         w.nkb = (t.row_end - t.row0 + bk - 1) / bk;
-    } else if (p.grouping == kGroupedRows) {
-        (SWAP ? blocks_n : blocks_m) = row_tile_count;
     }
-    // Raster groups of `raster` M-side tiles, so that the CTAs at work share panels in L2.
-    const int per = p.raster * blocks_n;
-    const int rg = local / per;
-    const int first = rg * p.raster;
-    const int rows = min(blocks_m - first, p.raster);
-    const int in_group = local - rg * per;
-    const int mb = first + in_group % rows, nb = in_group / rows;
+    int mb, nb;
+    if constexpr (SWAP) {       // all M-side tiles (columns) of a row tile, then the next
+        nb = op_divide(local, p.per_raster);
+        mb = local - nb * p.per_raster.value;
+    } else {
+        // Raster groups of 2^log_raster M-side tiles, so that the CTAs at work share panels in L2.
+        const int blocks_m = p.grouping == kGroupedRows ? row_tile_count : p.num_m_blocks;
+        const int rg = op_divide(local, p.per_raster);
+        const int first = rg << p.log_raster;
+        const int in_group = local - rg * p.per_raster.value;
+        const int rows = blocks_m - first;
+        if (rows >> p.log_raster) {
+            nb = in_group >> p.log_raster;
+            mb = first + (in_group & ((1 << p.log_raster) - 1));
+        } else {
+            nb = in_group / rows;
+            mb = first + in_group - nb * rows;
+        }
+    }
     w.m0 = mb * kBM;
-    w.n0 = nb * BN;
-    w.n_block = nb;
+    w.n0 = nb * BN + half * 256;
+    w.loss_block = nb * (kHalves ? 2 : 1) + half;
     if (p.grouping == kGroupedRows) {
         const OpRowTile t = p.row_tiles[SWAP ? nb : mb];
         w.group = t.group;
@@ -339,14 +412,23 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     constexpr int kBStage = Tile::kBStage;
     constexpr int kBCols = Tile::kBCols;
     constexpr int kGroups = Tile::kGroups;
-    constexpr int kGroupCols = BN / kGroups;              // D columns per epilogue warpgroup
+    constexpr int kParts = Tile::kParts;
+    constexpr int kAccs = Tile::kAccs;
+    constexpr int kBoxes = Tile::kBoxes;
+    constexpr int kHalfCols = kBCols / kParts;            // N columns staged per CTA and half
+    constexpr int kMmaN = Tile::kPartCols;
+    constexpr int kDefer = 2;     // 512 columns: K blocks at each end of a tile run on one half first
+    static_assert(kParts == 1 || kDefer < kStages, "deferred K blocks must leave the producer a stage");
+    constexpr bool kSplittable = CTAS == 1 && (EPI == kEpiStore || EPI == kEpiStoreT);
+    constexpr int kGroupCols = Tile::kPartCols / kGroups; // D columns per epilogue warpgroup (and half)
     constexpr uint32_t kStageTx = static_cast<uint32_t>(CTAS) * (OP_A_STAGE + kBStage);
+    constexpr uint32_t kHalfStageTx = static_cast<uint32_t>(CTAS) * (OP_A_STAGE + kBStage / 2);
     // FP32 accumulator, formats, A MN-major (bit 15), B MN-major (bit 16), N >> 3, M >> 4.
     constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(FMT) << 7) | (static_cast<uint32_t>(FMT) << 10) |
                                 ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
-                                (static_cast<uint32_t>(BN >> 3) << 17) |
+                                (static_cast<uint32_t>(kMmaN >> 3) << 17) |
                                 (static_cast<uint32_t>((OP_BM * CTAS) >> 4) << 24);
-    static_assert(!B_MN || kBCols % kBox == 0, "whole MN-major boxes");
+    static_assert(!B_MN || kHalfCols % kBox == 0, "whole MN-major boxes");
     static_assert(!kPair || !kSwap, "the transposed epilogue runs on single CTAs");
 
     extern __shared__ uint8_t smem_raw[];
@@ -363,6 +445,9 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     auto acce_bar = [&](int i) { return s_bar + 8u * (2 * kStages + 2 + i); };
     const uint32_t drain_bar = s_bar + 8u * (2 * kStages + 4);
     const uint32_t tmem_slot = s_bar + 8u * (2 * kStages + 5);
+    const uint32_t recv_bar = s_bar + 8u * (2 * kStages + 6);   // split K: partial rows received
+    const uint32_t fail_flag = s_bar + 8u * (2 * kStages + 7);  // split K: 1 once a progress wait of this CTA ran out
+    volatile uint32_t *fail_flag_ptr = reinterpret_cast<volatile uint32_t *>(smem_raw + (fail_flag - raw));
     uint32_t *tmem_slot_ptr = reinterpret_cast<uint32_t *>(smem_raw + (tmem_slot - raw));
     float *bias_s = reinterpret_cast<float *>(smem_raw + (s_bias - raw));
 
@@ -372,6 +457,12 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const bool leader = rank == 0;
     const int unit = static_cast<int>(blockIdx.x) / CTAS;       // this CTA's or pair's first tile
     const int units = static_cast<int>(gridDim.x) / CTAS;
+    // Split K (clusters of S CTAs along z, one tile per cluster, ungrouped): CTA z runs K
+    // blocks [z * ceil(nk / S), (z + 1) * ceil(nk / S)).
+    const int splits = kSplittable ? static_cast<int>(gridDim.z) : 1;
+    const int kb_per_split = (p.num_k_blocks + splits - 1) / splits;
+    const int kb_begin = splits > 1 ? min(static_cast<int>(blockIdx.z) * kb_per_split, p.num_k_blocks) : 0;
+    auto kb_end = [&](int nkb) { return splits > 1 ? min(nkb, kb_begin + kb_per_split) : nkb; };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -383,6 +474,8 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             mbar_init(acce_bar(i), 4 * CTAS * kGroups);
         }
         mbar_init(drain_bar, 1);
+        mbar_init(recv_bar, 1);
+        *fail_flag_ptr = 0u;
         fence_mbarrier_init();
     }
     if (warp == 0 && lane == 0) {
@@ -448,19 +541,53 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             }
     };
 
+    // NaN over rows x cols elements of the outputs, clipped, one warp per row.
+    auto nan_elements = [&](const OpWhere &w, int first_row, int rows, int first_col, int cols, int warp_index,
+                            int warps, int lane_index) {
+        const float nan = __int_as_float(0x7fc00000);
+        const int row_end = min(w.row_end, first_row + rows), col_end = min(p.n, first_col + cols);
+        for (int row = first_row + warp_index; row < row_end; row += warps)
+            for (int col = first_col + lane_index; col < col_end; col += 32) {
+                const long long at = (p.grouping == kGroupedK ? w.group : 0) * p.out_slab + row * p.out_pitch + col;
+                if (p.out_half)
+                    static_cast<T *>(p.out)[at] = Type::from(nan);
+                else
+                    static_cast<float *>(p.out)[at] = nan;
+                if (EPI != kEpiSoftmaxGrad && p.preact) {
+                    if (p.preact_half)
+                        static_cast<T *>(p.preact)[at] = Type::from(nan);
+                    else
+                        static_cast<float *>(p.preact)[at] = nan;
+                }
+            }
+    };
+
     const int row_tile_count = p.grouping == kGroupedRows ? *p.row_tile_count : 0;
     const int num_tiles = p.grouping == kGroupedRows ? row_tile_count * (kSwap ? p.num_m_blocks : p.num_n_blocks)
                                                      : p.num_tiles;
+    // Tiles are dealt out in turn; in ragged-K mode each unit has consecutive ones.
+    const bool in_turn = p.grouping != kGroupedK;
+    const int tile_first = in_turn ? unit : p.unit_first[unit];
+    const int tile_end = in_turn ? num_tiles : p.unit_first[unit + 1];
+    const int tile_step = in_turn ? units : 1;
 
+    // The 512-column tile's epilogue holds 128 columns of its row in registers: the four
+    // other warps give theirs up (128 x 56 + 256 x 224 = 384 x 168, the launch's total).
+    // Each role sets its own count, so that the compiler sees the limit it works under.
+    auto give_registers = [&]() {
+        if constexpr (kParts == 2)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    };
     if (warp == 0) {
         // ------------------------------------------------------------ producer
+        give_registers();
         if (lane == 0) {
             int stage = 0;
             uint32_t phase = 0, filled = 0, fill_parity = 0;
             bool ok = true;
             int acquired = -1;     // ragged-K mode: the group whose maps this thread has acquired
             const uint32_t leader_full0 = kPair ? map_to_cta(full_bar(0), 0) : full_bar(0);
-            for (int tile = unit; ok && tile < num_tiles; tile += units) {
+            for (int tile = tile_first; ok && tile < tile_end; tile += tile_step) {
                 const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
                 const void *ma = &map_a, *mb = &map_b;
                 int za = 0, zb = 0;
@@ -476,8 +603,8 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     (kSwap ? za : zb) = w.group;
                 }
                 const int am = w.m0 + static_cast<int>(rank) * OP_BM;
-                const int bn = w.n0 + static_cast<int>(rank) * kBCols;
-                for (int kb = 0; kb < w.nkb; ++kb) {
+                const int bn = w.n0 + static_cast<int>(rank) * kHalfCols;
+                for (int kb = kb_begin; kb < kb_end(w.nkb); ++kb) {
                     // In a pair this wait keeps the fixed limit: both CTAs then stop at the
                     // same stage and the leader's drain covers every copy of either.
                     if (!mbar_wait(empty_bar(stage), phase ^ 1u, kPair ? kWaitLimitNs : p.wait_limit_ns)) {
@@ -487,7 +614,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                     const uint32_t fb = leader_full0 + 8u * stage;
                     if (leader)
-                        mbar_arrive_expect_tx(full_bar(stage), kStageTx);
+                        mbar_arrive_expect_tx(full_bar(stage), kParts == 2 && w.parts == 1 ? kHalfStageTx : kStageTx);
                     const int k = w.k0 + kb * kBK;
                     auto load = [&](uint32_t dst, const void *map, int x, int y, int z) {
                         if constexpr (kPair)
@@ -503,12 +630,18 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     } else {
                         load(sa, ma, k, am, za);
                     }
-                    if constexpr (B_MN) {
 #pragma unroll
-                        for (int j = 0; j < kBCols / kBox; ++j)
-                            load(sb + j * kBoxBytes, mb, bn + j * kBox, k, zb);
-                    } else {
-                        load(sb, mb, k, bn, zb);
+                    for (int h = 0; h < kParts; ++h) {
+                        if (h == w.parts)
+                            break;
+                        const uint32_t sbh = sb + h * kHalfCols * OP_ROW_BYTES;
+                        if constexpr (B_MN) {
+#pragma unroll
+                            for (int j = 0; j < kHalfCols / kBox; ++j)
+                                load(sbh + j * kBoxBytes, mb, bn + h * 256 + j * kBox, k, zb);
+                        } else {
+                            load(sbh, mb, k, bn + h * 256, zb);
+                        }
                     }
                     filled |= 1u << stage;
                     fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
@@ -528,6 +661,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (a pair's leader)
+        give_registers();
         if (leader && lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
@@ -541,35 +675,87 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 else
                     tc_commit(bar);
             };
+            auto arrive_both = [&](uint32_t bar) {
+                if constexpr (kPair) {
+                    mbar_arrive_cluster(map_to_cta(bar, 0));
+                    mbar_arrive_cluster(map_to_cta(bar, 1));
+                } else {
+                    mbar_arrive(bar);
+                }
+            };
+            // The MMAs of the K block in stage s for half h of the accumulator.
+            auto issue_half = [&](uint32_t d_tmem, int s, int h, bool first) {
+                const uint64_t a_desc = a_desc0 + static_cast<uint64_t>(s) * (OP_A_STAGE >> 4);
+                const uint64_t b_desc = b_desc0 + static_cast<uint64_t>(s) * (kBStage >> 4) +
+                                        static_cast<uint64_t>(h) * ((kHalfCols * OP_ROW_BYTES) >> 4);
+#pragma unroll
+                for (int kk = 0; kk < kMmasPerStage; ++kk) {
+                    const uint32_t accumulate = !first || kk != 0 ? 1u : 0u;
+                    const uint32_t d = d_tmem + static_cast<uint32_t>(h * 256);
+                    if constexpr (kPair)
+                        tc_mma_pair<kTF32>(d, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
+                    else
+                        tc_mma<kTF32>(d, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
+                }
+            };
             int acc = 0;
             uint32_t acc_phase = 0;
             bool ok = true;
-            for (int tile = unit; ok && tile < num_tiles; tile += units) {
-                const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
-                if (!mbar_wait(acce_bar(acc), acc_phase ^ 1u, p.wait_limit_ns)) {
+            auto wait_free = [&](int i) {      // the epilogue has read accumulator (half) i
+                if (!mbar_wait(acce_bar(i), acc_phase ^ 1u, p.wait_limit_ns)) {
                     atomicOr(p.status, kOpMmaTimeout);
-                    break;
+                    ok = false;
                 }
                 tc_fence_after();
+                return ok;
+            };
+            for (int tile = tile_first; ok && tile < tile_end; tile += tile_step) {
+                const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
+                if (!wait_free(acc))
+                    break;
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-                for (int kb = 0; kb < w.nkb; ++kb) {
+                const int nkb = kb_end(w.nkb);
+                bool upper_live = false;              // 512 columns: the epilogue has read the upper half
+                int pending = 0, pending_stage = 0;   // 512 columns: K blocks whose upper-half MMAs wait
+                for (int kb = kb_begin; kb < nkb; ++kb) {
                     if (!mbar_wait(full_bar(stage), phase, p.wait_limit_ns)) {
                         atomicOr(p.status, kOpMmaTimeout);
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t a_desc = a_desc0 + static_cast<uint64_t>(stage) * (OP_A_STAGE >> 4);
-                    const uint64_t b_desc = b_desc0 + static_cast<uint64_t>(stage) * (kBStage >> 4);
-#pragma unroll
-                    for (int kk = 0; kk < kMmasPerStage; ++kk) {
-                        const uint32_t accumulate = (kb | kk) != 0 ? 1u : 0u;
-                        if constexpr (kPair)
-                            tc_mma_pair<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
-                        else
-                            tc_mma<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
+                    issue_half(d_tmem, stage, 0, kb == kb_begin);
+                    if (kParts == 1 || w.parts == 1) {
+                        commit(empty_bar(stage));
+                    } else {
+                        // The lower half runs ahead by kDefer K blocks at either end of the tile: its
+                        // epilogue overlaps the upper half's last MMAs, and the upper half's epilogue
+                        // of the tile before overlaps this tile's first ones.
+                        if (kb == nkb - 1)
+                            commit(accf_bar(0));
+                        if (upper_live && kb < nkb - kDefer) {
+                            issue_half(d_tmem, stage, 1, false);
+                            commit(empty_bar(stage));
+                        } else {
+                            if (pending++ == 0)
+                                pending_stage = stage;
+                            if (kb == nkb - 1 || (!upper_live && kb == kDefer - 1)) {
+                                if (!upper_live) {
+                                    if (!wait_free(1))
+                                        break;
+                                    upper_live = true;
+                                }
+                                int s = pending_stage;
+                                for (int j = kb - pending + 1; j <= kb; ++j) {
+                                    issue_half(d_tmem, s, 1, j == 0);
+                                    commit(empty_bar(s));
+                                    if (++s == kStages)
+                                        s = 0;
+                                }
+                                pending = 0;
+                            }
+                        }
                     }
-                    commit(empty_bar(stage));
                     if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
@@ -577,15 +763,17 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 }
                 if (!ok)
                     break;
-                if (w.nkb > 0) {
-                    commit(accf_bar(acc));
-                } else if constexpr (kPair) {     // an empty group: its sum is zero, nothing to wait for
-                    mbar_arrive_cluster(map_to_cta(accf_bar(acc), 0));
-                    mbar_arrive_cluster(map_to_cta(accf_bar(acc), 1));
-                } else {
-                    mbar_arrive(accf_bar(acc));
+                if (nkb > kb_begin) {
+                    commit(accf_bar(kParts == 1 ? acc : w.parts - 1));
+                } else {          // no K block (an empty group or split): a zero sum, nothing to wait for
+                    if (kParts == 2 && w.parts == 2) {
+                        if (!wait_free(1))
+                            break;
+                        arrive_both(accf_bar(0));
+                    }
+                    arrive_both(accf_bar(kParts == 1 ? acc : w.parts - 1));
                 }
-                if (++acc == 2) {
+                if (++acc == kAccs) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
@@ -599,15 +787,17 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 atomicOr(p.status, kOpDrainTimeout);
         }
         __syncwarp();
-    } else {
+    } else if (warp >= Tile::kFirstEpi) {
         // ------------------------------------------------------------ epilogue
+        if constexpr (kParts == 2)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3;                 // TMEM lanes 32 * quarter .. +31
         const int r = quarter * 32 + lane;
-        const int group = (warp - 2) >> 2;            // epilogue warpgroup: D columns group * kGroupCols ..
+        const int group = (warp - Tile::kFirstEpi) >> 2;   // epilogue warpgroup: D columns group * kGroupCols ..
         const int gcol = group * kGroupCols;
-        const int gthread = static_cast<int>(threadIdx.x) - 64 - 128 * group;
+        const int gthread = static_cast<int>(threadIdx.x) - 32 * Tile::kFirstEpi - 128 * group;
         const bool issuer = gthread == 0;
-        const uint32_t s_box = s_epi + group * 2 * OP_BOX;
+        const uint32_t s_box = s_epi + group * kBoxes * OP_BOX;
         auto epilogue_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
         // 1 only if every thread of the warpgroup passes 1.
         auto epilogue_all = [&](int ok) {
@@ -626,304 +816,352 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         uint32_t acc_phase = 0, stores = 0;
         int failed_tile = -1;
         int acquired = -1;
-        // Releases the accumulator after this warp's last read of it.
+        // Releases the accumulator (half) after this warp's last read of it.
+        int part = 0;
         auto release = [&]() {
+            const uint32_t bar = acce_bar(kAccs == 2 ? acc : part);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
                 if constexpr (kPair)
-                    mbar_arrive_cluster(map_to_cta(acce_bar(acc), 0));
+                    mbar_arrive_remote(map_to_cta(bar, 0));
                 else
-                    mbar_arrive(acce_bar(acc));
+                    mbar_arrive(bar);
             }
         };
-        for (int tile = unit; tile < num_tiles; tile += units) {
+        for (int tile = tile_first; tile < tile_end; tile += tile_step) {
             const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
             const int row0 = w.m0 + static_cast<int>(rank) * OP_BM;     // D's first row in this CTA
-            const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                   static_cast<uint32_t>(acc * BN + gcol);
-            if constexpr (EPI == kEpiStore) {
-                if (p.bias) {       // the tile's bias, read once into shared memory
-                    epilogue_sync();
-                    for (int c = gcol + gthread; c < gcol + kGroupCols; c += 128) {
-                        const int col = w.n0 + c;
-                        float b = 0.0f;
-                        if (col < p.n)
-                            b = load_bias(col);
-                        bias_s[c] = b;
-                    }
-                    epilogue_sync();
-                }
-            }
-            // Per-row values of the loss epilogues.
-            int label = -1;
-            float row_lse = 0.0f, row_grad = 0.0f;
-            if constexpr (EPI == kEpiLse || EPI == kEpiSoftmaxGrad) {
-                if (row0 + r < p.m) {
-                    label = op_label(p, row0 + r);
-                    if constexpr (EPI == kEpiSoftmaxGrad) {
-                        row_lse = p.lse[row0 + r];
-                        row_grad = p.grad[row0 + r];
+            for (part = 0; part < w.parts; ++part) {
+                const int n0 = w.n0 + part * 256;     // this half's first column
+                const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                       static_cast<uint32_t>(acc * BN + part * 256 + gcol);
+                if constexpr (EPI == kEpiStore) {
+                    if (p.bias) {       // this part's bias, read once into shared memory
+                        epilogue_sync();
+                        for (int c = gcol + gthread; c < gcol + kGroupCols; c += 128) {
+                            const int col = n0 + c;
+                            float b = 0.0f;
+                            if (col < p.n)
+                                b = load_bias(col);
+                            bias_s[c] = b;
+                        }
+                        epilogue_sync();
                     }
                 }
-            }
-            int ok = 1;
-            if (lane == 0)
-                ok = mbar_wait(accf_bar(acc), acc_phase, p.wait_limit_ns) ? 1 : 0;
-            ok = epilogue_all(__shfl_sync(0xffffffffu, ok, 0));
-            if (!ok) {
-                if (lane == 0)
-                    atomicOr(p.status, kOpEpilogueTimeout);
-                failed_tile = tile;
-                break;
-            }
-            tc_fence_after();
-
-            if constexpr (EPI == kEpiStore || EPI == kEpiSoftmaxGrad) {
-                const void *mc = &map_c;
-                if (p.grouping == kGroupedRows && p.out_tma) {
-                    mc = p.group_maps + w.group;
-                    if (issuer && acquired != w.group) {
-                        tensormap_acquire(mc);
-                        acquired = w.group;
+                // Per-row values of the loss epilogues.
+                int label = -1;
+                float row_lse = 0.0f, row_grad = 0.0f;
+                if constexpr (EPI == kEpiLse || EPI == kEpiSoftmaxGrad) {
+                    if (row0 + r < p.m) {
+                        label = op_label(p, row0 + r);
+                        if constexpr (EPI == kEpiSoftmaxGrad) {
+                            row_lse = p.lse[row0 + r];
+                            row_grad = p.grad[row0 + r];
+                        }
                     }
                 }
-                const int zc = p.grouping == kGroupedK ? w.group : 0;
-                // Puts 128 bytes of this thread's row into a box of 128 rows.
-                auto fill = [&](uint32_t box, const uint32_t (&words)[32]) {
-                    const uint32_t row_addr = box + r * 128;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        st_shared_v4(row_addr + ((j ^ (r & 7)) << 4), words[4 * j], words[4 * j + 1], words[4 * j + 2],
-                                     words[4 * j + 3]);
-                };
-                // A box of 32 FP32 or 64 16-bit columns, stored by TMA.
-                auto emit = [&](const uint32_t (&words)[32], const void *map, int z, int col0) {
-                    const uint32_t box = s_box + (stores & 1u) * OP_BOX;
-                    if (issuer)
-                        bulk_wait_group_read<1>();      // the store that last read this box
-                    epilogue_sync();
-                    fill(box, words);
-                    fence_proxy_async_shared();
-                    epilogue_sync();
+                int ok = 1;
+                if (issuer)       // one thread polls, the others wait at the barrier
+                    ok = mbar_wait(accf_bar(kAccs == 2 ? acc : part), acc_phase, p.wait_limit_ns) ? 1 : 0;
+                ok = epilogue_all(ok);
+                if (!ok) {
                     if (issuer) {
-                        tma_store_3d(map, box, col0, row0, z);
-                        bulk_commit_group();
+                        atomicOr(p.status, kOpEpilogueTimeout);
+                        *fail_flag_ptr = 1u;
                     }
-                    ++stores;
-                };
-                // A box of 32 FP32 columns written out row by row (lane = column) where TMA cannot
-                // write, in either format; the residual is added on the way, coalesced.
-                auto emit_rows = [&](const uint32_t (&words)[32], bool half, void *dst, long long at0, long long pitch,
-                                     int col0, const void *residual) {
-                    const uint32_t box = s_box + (stores & 1u) * OP_BOX;
-                    epilogue_sync();
-                    fill(box, words);
-                    epilogue_sync();
-                    ++stores;
-                    const uint8_t *box_p = smem_raw + (box - raw);
-                    const int rows = min(OP_BM, w.row_end - row0);
-                    if (col0 + lane >= p.n)
-                        return;
-                    const long long at = at0 + row0 * pitch + col0 + lane;
-#pragma unroll 1
-                    for (int first = quarter; first < rows; first += 32) {
-                        float x[8];
+                    failed_tile = tile;
+                    break;
+                }
+                tc_fence_after();
+                if (splits > 1)
+                    break;     // one tile; its partial sums are exchanged below
+
+                if constexpr (EPI == kEpiStore || EPI == kEpiSoftmaxGrad) {
+                    const void *mc = &map_c;
+                    if (p.grouping == kGroupedRows && p.out_tma && row0 + OP_BM > w.row_end && row0 < w.row_end) {
+                        // Rows of the next group in this tile: the group's own map clips them.
+                        mc = p.group_maps + w.group;
+                        if (issuer && acquired != w.group) {
+                            tensormap_acquire(mc);
+                            acquired = w.group;
+                        }
+                    }
+                    const int zc = p.grouping == kGroupedK ? w.group : 0;
+                    // Puts 128 bytes of this thread's row into a box of 128 rows.
+                    auto fill = [&](uint32_t box, const uint32_t (&words)[32]) {
+                        const uint32_t row_addr = box + r * 128;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int rr = first + 4 * i;
-                            if (rr < rows) {
-                                x[i] = *reinterpret_cast<const float *>(box_p + rr * 128 + (((lane >> 2) ^ (rr & 7)) << 4) +
-                                                                        (lane & 3) * 4);
-                                if (residual)
-                                    x[i] += p.residual_half ? Type::to(static_cast<const T *>(residual)[at + rr * pitch])
-                                                            : static_cast<const float *>(residual)[at + rr * pitch];
+                        for (int j = 0; j < 8; ++j)
+                            st_shared_v4(row_addr + ((j ^ (r & 7)) << 4), words[4 * j], words[4 * j + 1], words[4 * j + 2],
+                                         words[4 * j + 3]);
+                    };
+                    // A box of 32 FP32 or 64 16-bit columns, stored by TMA.
+                    auto emit = [&](const uint32_t (&words)[32], const void *map, int z, int col0) {
+                        const uint32_t box = s_box + stores % kBoxes * OP_BOX;
+                        if (issuer)
+                            bulk_wait_group_read<kBoxes - 1>();      // the store that last read this box
+                        epilogue_sync();
+                        fill(box, words);
+                        fence_proxy_async_shared();
+                        epilogue_sync();
+                        if (issuer) {
+                            tma_store_3d(map, box, col0, row0, z);
+                            bulk_commit_group();
+                        }
+                        ++stores;
+                    };
+                    // A box of 32 FP32 columns written out row by row (lane = column) where TMA cannot
+                    // write, in either format; the residual is added on the way, coalesced.
+                    auto emit_rows = [&](const uint32_t (&words)[32], bool half, void *dst, long long at0, long long pitch,
+                                         int col0, const void *residual) {
+                        const uint32_t box = s_box + stores % kBoxes * OP_BOX;
+                        if (issuer) {
+                            bulk_wait_group_read<kBoxes - 1>();
+                            bulk_commit_group();            // an empty group: one per box, whoever writes it out
+                        }
+                        epilogue_sync();
+                        fill(box, words);
+                        epilogue_sync();
+                        ++stores;
+                        const uint8_t *box_p = smem_raw + (box - raw);
+                        const int rows = min(OP_BM, w.row_end - row0);
+                        if (col0 + lane >= p.n)
+                            return;
+                        const long long at = at0 + row0 * pitch + col0 + lane;
+#pragma unroll 1
+                        for (int first = quarter; first < rows; first += 32) {
+                            float x[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int rr = first + 4 * i;
+                                if (rr < rows) {
+                                    x[i] = *reinterpret_cast<const float *>(box_p + rr * 128 + (((lane >> 2) ^ (rr & 7)) << 4) +
+                                                                            (lane & 3) * 4);
+                                    if (residual)
+                                        x[i] += p.residual_half ? Type::to(static_cast<const T *>(residual)[at + rr * pitch])
+                                                                : static_cast<const float *>(residual)[at + rr * pitch];
+                                }
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int rr = first + 4 * i;
+                                if (rr < rows) {
+                                    if (half)
+                                        static_cast<T *>(dst)[at + rr * pitch] = Type::from(x[i]);
+                                    else
+                                        static_cast<float *>(dst)[at + rr * pitch] = x[i];
+                                }
                             }
                         }
+                    };
+                    auto emit_columns = [&](const float (&v)[64], const void *map, int z, bool tma, bool half, void *dst,
+                                            long long at0, long long pitch, int col0, const void *residual) {
+                        uint32_t words[32];
+                        if (tma && half) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int rr = first + 4 * i;
-                            if (rr < rows) {
-                                if (half)
-                                    static_cast<T *>(dst)[at + rr * pitch] = Type::from(x[i]);
+                            for (int j = 0; j < 32; ++j)
+                                words[j] = Type::pack(v[2 * j], v[2 * j + 1]);
+                            emit(words, map, z, col0);
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                if (col0 + 32 * h >= p.n)
+                                    break;
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    words[j] = __float_as_uint(v[32 * h + j]);
+                                if (tma)
+                                    emit(words, map, z, col0 + 32 * h);
                                 else
-                                    static_cast<float *>(dst)[at + rr * pitch] = x[i];
+                                    emit_rows(words, half, dst, at0, pitch, col0 + 32 * h, residual);
                             }
                         }
-                    }
-                };
-                auto emit_columns = [&](const float (&v)[64], const void *map, int z, bool tma, bool half, void *dst,
-                                        long long at0, long long pitch, int col0, const void *residual) {
-                    uint32_t words[32];
-                    if (tma && half) {
+                    };
+                    // 64 columns of this thread's row: epilogue arithmetic and stores.
+                    auto process = [&](float (&v)[64], int step) {
+                        const int col0 = n0 + gcol + step * 64;
+                        if (col0 >= p.n || row0 >= w.row_end)      // the same for all four warps
+                            return;
+                        if constexpr (EPI == kEpiSoftmaxGrad) {
+                            // p = exp(z - lse); an ignored row's gradient is zero whatever its logits are.
+                            const int hit = label - p.column0 - col0;
+                            const float scale = label == -2 ? __int_as_float(0x7fc00000) : row_grad;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            words[j] = Type::pack(v[2 * j], v[2 * j + 1]);
-                        emit(words, map, z, col0);
-                    } else {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (col0 + 32 * h >= p.n)
-                                break;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                words[j] = __float_as_uint(v[32 * h + j]);
-                            if (tma)
-                                emit(words, map, z, col0 + 32 * h);
-                            else
-                                emit_rows(words, half, dst, at0, pitch, col0 + 32 * h, residual);
-                        }
-                    }
-                };
-#pragma unroll 1
-                for (int step = 0; step < kGroupCols / 64; ++step) {
-                    float v[64];
-                    {
-                        uint32_t u[32];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (w.nkb > 0)
-                                tmem_load_32cols(t_row + step * 64 + h * 32, u);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                v[32 * h + j] = w.nkb > 0 ? __uint_as_float(u[j]) : 0.0f;
-                        }
-                    }
-                    if (step == kGroupCols / 64 - 1)
-                        release();
-                    const int col0 = w.n0 + gcol + step * 64;
-                    if (col0 >= p.n || row0 >= w.row_end)      // the same for all four warps
-                        continue;
-                    if constexpr (EPI == kEpiSoftmaxGrad) {
-                        // p = exp(z - lse); an ignored row's gradient is zero whatever its logits are.
-                        const int hit = label - p.column0 - col0;
-                        const float scale = label == -2 ? __int_as_float(0x7fc00000) : row_grad;
-#pragma unroll
-                        for (int j = 0; j < 64; ++j) {
-                            const float prob = exp2f((v[j] - row_lse) * 1.4426950408889634f);   // subnormals kept
-                            v[j] = label == -1 ? 0.0f : (prob - (j == hit ? 1.0f : 0.0f)) * scale;
-                        }
-                    } else {
-                        if (p.bias) {
-                            const float4 *b4 = reinterpret_cast<const float4 *>(bias_s + gcol + step * 64);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const float4 b = b4[j];
-                                v[4 * j] += b.x;
-                                v[4 * j + 1] += b.y;
-                                v[4 * j + 2] += b.z;
-                                v[4 * j + 3] += b.w;
+                            for (int j = 0; j < 64; ++j) {
+                                const float prob = exp2f((v[j] - row_lse) * 1.4426950408889634f);   // subnormals kept
+                                v[j] = label == -1 ? 0.0f : (prob - (j == hit ? 1.0f : 0.0f)) * scale;
                             }
-                        }
-                        if (p.preact)
-                            emit_columns(v, &map_z, 0, p.preact_tma != 0, p.preact_half != 0, p.preact, 0, p.n, col0, nullptr);
-                        op_with_activation(p.activation, [&](auto act) {
+                        } else {
+                            if (p.bias) {
+                                const float4 *b4 = reinterpret_cast<const float4 *>(bias_s + gcol + step * 64);
 #pragma unroll
-                            for (int j = 0; j < 64; ++j)
-                                v[j] = op_activation<decltype(act)::value>(v[j]);
-                        });
-                        // Where TMA writes out, each thread reads its own row of the residual (16-byte
-                        // loads where it can); otherwise the row-by-row store adds it.
-                        if (p.residual && p.out_tma && row0 + r < w.row_end) {
-                            const long long at = (row0 + r) * p.out_pitch + col0;
-                            if (col0 + 64 <= p.n) {
-                                if (p.residual_half) {
-                                    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at);
+                                for (int j = 0; j < 16; ++j) {
+                                    const float4 b = b4[j];
+                                    v[4 * j] += b.x;
+                                    v[4 * j + 1] += b.y;
+                                    v[4 * j + 2] += b.z;
+                                    v[4 * j + 3] += b.w;
+                                }
+                            }
+                            if (p.preact)
+                                emit_columns(v, &map_z, 0, p.preact_tma != 0, p.preact_half != 0, p.preact, 0, p.n, col0, nullptr);
+                            op_with_activation(p.activation, [&](auto act) {
 #pragma unroll
-                                    for (int j = 0; j < 8; ++j) {
-                                        const uint4 q = src[j];
-                                        const T *h = reinterpret_cast<const T *>(&q);
-                                        if constexpr (!kTF32) {
+                                for (int j = 0; j < 64; ++j)
+                                    v[j] = op_activation<decltype(act)::value>(v[j]);
+                            });
+                            // Where TMA writes out, each thread reads its own row of the residual (16-byte
+                            // loads where it can); otherwise the row-by-row store adds it.
+                            if (p.residual && p.out_tma && row0 + r < w.row_end) {
+                                const long long at = (row0 + r) * p.out_pitch + col0;
+                                if (col0 + 64 <= p.n) {
+                                    if (p.residual_half) {
+                                        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at);
 #pragma unroll
-                                            for (int e = 0; e < 8; ++e)
-                                                v[8 * j + e] += Type::to(h[e]);
+                                        for (int j = 0; j < 8; ++j) {
+                                            const uint4 q = src[j];
+                                            const T *h = reinterpret_cast<const T *>(&q);
+                                            if constexpr (!kTF32) {
+#pragma unroll
+                                                for (int e = 0; e < 8; ++e)
+                                                    v[8 * j + e] += Type::to(h[e]);
+                                            }
+                                        }
+                                    } else {
+                                        const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.residual) + at);
+#pragma unroll
+                                        for (int j = 0; j < 16; ++j) {
+                                            const float4 q = src[j];
+                                            v[4 * j] += q.x;
+                                            v[4 * j + 1] += q.y;
+                                            v[4 * j + 2] += q.z;
+                                            v[4 * j + 3] += q.w;
                                         }
                                     }
                                 } else {
-                                    const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.residual) + at);
 #pragma unroll
-                                    for (int j = 0; j < 16; ++j) {
-                                        const float4 q = src[j];
-                                        v[4 * j] += q.x;
-                                        v[4 * j + 1] += q.y;
-                                        v[4 * j + 2] += q.z;
-                                        v[4 * j + 3] += q.w;
-                                    }
+                                    for (int j = 0; j < 64; ++j)
+                                        if (col0 + j < p.n)
+                                            v[j] += p.residual_half ? Type::to(static_cast<const T *>(p.residual)[at + j])
+                                                                    : static_cast<const float *>(p.residual)[at + j];
                                 }
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 64; ++j)
-                                    if (col0 + j < p.n)
-                                        v[j] += p.residual_half ? Type::to(static_cast<const T *>(p.residual)[at + j])
-                                                                : static_cast<const float *>(p.residual)[at + j];
                             }
                         }
-                    }
-                    emit_columns(v, mc, zc, p.out_tma != 0, p.out_half != 0, p.out, zc * p.out_slab, p.out_pitch, col0,
-                                 p.residual);
-                }
-            } else if constexpr (EPI == kEpiStoreT) {
-                // D's rows are output columns: one lane per column, one store of 32 consecutive
-                // elements per output row and warp.
-                const int col = row0 + r;
-                const float b = p.bias && col < p.n ? load_bias(col) : 0.0f;
-#pragma unroll 1
-                for (int chunk = 0; chunk < kGroupCols / 16; ++chunk) {
-                    uint32_t u[16];
-                    tmem_load_16cols(t_row + chunk * 16, u);
-                    if (chunk == kGroupCols / 16 - 1)
-                        release();
-                    const int first = w.n0 + gcol + chunk * 16;
-                    const int rows = min(16, w.row_end - first);
-                    if (col >= p.n || rows <= 0)
-                        continue;
-                    float v[16];
+                        emit_columns(v, mc, zc, p.out_tma != 0, p.out_half != 0, p.out, zc * p.out_slab, p.out_pitch, col0,
+                                     p.residual);
+                    };
+                    auto load = [&](float (&v)[64], int step) {
+                        if (w.nkb > 0) {
+                            tmem_load_64cols(t_row + step * 64, v);
+                        } else {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        v[j] = __uint_as_float(u[j]) + b;
-                    store_elements(v, rows, first, col, 1, 0);
-                }
-            } else {
-                // One pass: running maximum and sum of exponentials in base 2 of this row's
-                // columns in the tile; columns past the vocabulary count as -infinity.
-                float top = -INFINITY, sum = 0.0f;
-                const int row = row0 + r;
-#pragma unroll 1
-                for (int chunk = 0; chunk < kGroupCols / 32; ++chunk) {
-                    uint32_t u[32];
-                    tmem_load_32cols(t_row + chunk * 32, u);
-                    if (chunk == kGroupCols / 32 - 1)
+                            for (int j = 0; j < 64; ++j)
+                                v[j] = 0.0f;
+                        }
+                    };
+                    if constexpr (kParts == 2) {
+                        // The half is read into registers at once and given back to the MMAs, whose
+                        // first K blocks of the next tile wait for it.
+                        float v0[64], v1[64];
+                        load(v0, 0);
+                        load(v1, 1);
                         release();
-                    const int col0 = w.n0 + gcol + chunk * 32;
-                    if (col0 >= p.n)
-                        continue;
-                    const int hit = label - col0;
-                    if (label >= 0 && hit >= 0 && hit < 32) {
-                        float z = 0.0f;
+                        process(v0, 0);
+                        process(v1, 1);
+                    } else {
+#pragma unroll 1
+                        for (int step = 0; step < kGroupCols / 64; ++step) {
+                            float v[64];
+                            load(v, step);
+                            if (step == kGroupCols / 64 - 1)
+                                release();
+                            process(v, step);
+                        }
+                    }
+                } else if constexpr (EPI == kEpiStoreT) {
+                    // D's rows are output columns: one lane per column, one store of 32 consecutive
+                    // elements per output row and warp.
+                    const int col = row0 + r;
+                    const float b = p.bias && col < p.n ? load_bias(col) : 0.0f;
+#pragma unroll 1
+                    for (int chunk = 0; chunk < kGroupCols / 16; ++chunk) {
+                        uint32_t u[16];
+                        tmem_load_16cols(t_row + chunk * 16, u);
+                        if (chunk == kGroupCols / 16 - 1)
+                            release();
+                        const int first = w.n0 + gcol + chunk * 16;
+                        const int rows = min(16, w.row_end - first);
+                        if (col >= p.n || rows <= 0)
+                            continue;
+                        float v[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            v[j] = __uint_as_float(u[j]) + b;
+                        store_elements(v, rows, first, col, 1, 0);
+                    }
+                } else {
+                    // One pass: running maximum and sum of exponentials in base 2 of this row's
+                    // columns in the tile; columns past the vocabulary count as -infinity.
+                    float top = -INFINITY, sum = 0.0f;
+                    const int row = row0 + r;
+                    auto reduce = [&](const uint32_t (&u)[32], int chunk) {
+                        const int col0 = n0 + gcol + chunk * 32;
+                        if (col0 >= p.n)
+                            return;
+                        const int hit = label - col0;
+                        if (label >= 0 && hit >= 0 && hit < 32) {
+                            float z = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                z = j == hit ? __uint_as_float(u[j]) : z;
+                            p.label_logit[row] = z;
+                        }
+                        float t[32], chunk_top = -INFINITY;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            t[j] = col0 + j < p.n ? __uint_as_float(u[j]) * 1.4426950408889634f : -INFINITY;
+                            chunk_top = fmaxf(chunk_top, t[j]);
+                        }
+                        const float next = fmaxf(top, chunk_top);
+                        // A row whose logits are all -infinity so far adds nothing; NaN is carried by the sum.
+                        const float origin = next == -INFINITY ? 0.0f : next;
+                        sum *= op_exp2(top - origin);
+                        float part_sum[4] = {};     // four chains
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            z = j == hit ? __uint_as_float(u[j]) : z;
-                        p.label_logit[row] = z;
+                            part_sum[j & 3] += op_exp2(t[j] - origin);
+                        sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+                        top = next;
+                    };
+                    if constexpr (kParts == 2) {
+                        uint32_t u0[32], u1[32], u2[32], u3[32];      // read at once, as above
+                        tmem_load_32cols(t_row, u0);
+                        tmem_load_32cols(t_row + 32, u1);
+                        tmem_load_32cols(t_row + 64, u2);
+                        tmem_load_32cols(t_row + 96, u3);
+                        release();
+                        reduce(u0, 0);
+                        reduce(u1, 1);
+                        reduce(u2, 2);
+                        reduce(u3, 3);
+                    } else {
+#pragma unroll 1
+                        for (int chunk = 0; chunk < kGroupCols / 32; ++chunk) {
+                            uint32_t u[32];
+                            tmem_load_32cols(t_row + chunk * 32, u);
+                            if (chunk == kGroupCols / 32 - 1)
+                                release();
+                            reduce(u, chunk);
+                        }
                     }
-                    float t[32], chunk_top = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        t[j] = col0 + j < p.n ? __uint_as_float(u[j]) * 1.4426950408889634f : -INFINITY;
-                        chunk_top = fmaxf(chunk_top, t[j]);
-                    }
-                    const float next = fmaxf(top, chunk_top);
-                    // A row whose logits are all -infinity so far adds nothing; NaN is carried by the sum.
-                    const float origin = next == -INFINITY ? 0.0f : next;
-                    sum *= op_exp2(top - origin);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        sum += op_exp2(t[j] - origin);
-                    top = next;
+                    if (row < p.m)
+                        p.partial[static_cast<long long>((w.loss_block + part) * kGroups + group) * p.m + row] = make_float2(top, sum);
                 }
-                if (row < p.m)
-                    p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row] = make_float2(top, sum);
             }
-            if (++acc == 2) {
+            if (splits > 1 || failed_tile >= 0)
+                break;
+            if (++acc == kAccs) {
                 acc = 0;
                 acc_phase ^= 1u;
             }
@@ -935,37 +1173,134 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 bulk_wait_group_read<0>();
         }
         __syncwarp();
-        if (failed_tile >= 0) {
+        if (failed_tile >= 0 && splits == 1) {
             // NaN over what this CTA did not finish, so that no later step reads stale values.
             epilogue_sync();
-            const float nan = __int_as_float(0x7fc00000);
-            for (int tile = failed_tile; tile < num_tiles; tile += units) {
+            for (int tile = failed_tile; tile < tile_end; tile += tile_step) {
                 const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
                 const int row0 = w.m0 + static_cast<int>(rank) * OP_BM;
-                if constexpr (EPI == kEpiLse) {
-                    if (row0 + r < p.m)
-                        p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row0 + r] = make_float2(nan, nan);
-                } else {
-                    const int first_row = kSwap ? w.n0 + gcol : row0, rows = kSwap ? kGroupCols : OP_BM;
-                    const int first_col = kSwap ? row0 : w.n0 + gcol, cols = kSwap ? OP_BM : kGroupCols;
-                    const int row_end = min(w.row_end, first_row + rows), col_end = min(p.n, first_col + cols);
-                    for (int row = first_row + quarter; row < row_end; row += 4)
-                        for (int col = first_col + lane; col < col_end; col += 32) {
-                            const long long at =
-                                (p.grouping == kGroupedK ? w.group : 0) * p.out_slab + row * p.out_pitch + col;
-                            if (p.out_half)
-                                static_cast<T *>(p.out)[at] = Type::from(nan);
-                            else
-                                static_cast<float *>(p.out)[at] = nan;
-                            if (EPI != kEpiSoftmaxGrad && p.preact) {
-                                if (p.preact_half)
-                                    static_cast<T *>(p.preact)[row * static_cast<long long>(p.n) + col] = Type::from(nan);
-                                else
-                                    static_cast<float *>(p.preact)[row * static_cast<long long>(p.n) + col] = nan;
-                            }
-                        }
+                for (int h = 0; h < w.parts; ++h) {
+                    if constexpr (EPI == kEpiLse) {
+                        if (row0 + r < p.m)
+                            p.partial[static_cast<long long>((w.loss_block + h) * kGroups + group) * p.m + row0 + r] =
+                                make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+                    } else {
+                        nan_elements(w, kSwap ? w.n0 + gcol : row0, kSwap ? kGroupCols : OP_BM,
+                                     kSwap ? row0 : w.n0 + h * 256 + gcol, kSwap ? OP_BM : kGroupCols, quarter, 4, lane);
+                    }
                 }
             }
+        }
+    } else {
+        give_registers();
+    }
+
+    if constexpr (kSplittable) {
+        constexpr uint32_t kPitch = BN * 4;                          // a D row of FP32 partial sums
+        constexpr uint32_t kPartialBytes = OP_BM * kPitch;
+        constexpr int kSwizzle = BN / 4 - 1 < 7 ? BN / 4 - 1 : 7;    // 16-byte chunks XOR row
+        static_assert(kPartialBytes + 7 * (kPartialBytes / 8) <= kStages * (OP_A_STAGE + kBStage),
+                      "the partial and seven received slices fit the ring");
+        if (splits > 1) {
+            // D rows [j * rows, (j + 1) * rows) of the tile are summed by CTA j.  Every CTA writes its
+            // accumulator into its own idle ring, the bulk-copy engine sends each row slice to
+            // its owner, and the owner adds the slices in the order 0 .. S-1.
+            const int rows = OP_BM / splits;
+            const uint32_t slice_bytes = static_cast<uint32_t>(rows) * kPitch;
+            const int z = static_cast<int>(blockIdx.z);
+            if (threadIdx.x == 0)
+                mbar_arrive_expect_tx(recv_bar, static_cast<uint32_t>(splits - 1) * slice_bytes);
+            cluster_sync_all();     // every CTA of the cluster is past its main loop: rings idle
+            // A CTA whose progress wait ran out has no valid partial: NaN from all of them.
+            uint32_t any_failed = 0;
+            for (int j = 0; j < splits; ++j)
+                any_failed |= ld_shared_cluster_u32(map_to_cta(fail_flag, static_cast<uint32_t>(j)));
+            if (warp >= Tile::kFirstEpi) {
+                const int quarter = warp & 3, r = quarter * 32 + lane;
+                const int first = ((warp - Tile::kFirstEpi) >> 2) * kGroupCols;
+                const uint32_t row_addr = s_a + static_cast<uint32_t>(r) * kPitch;
+                const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+                for (int chunk = first / 16; chunk < (first + kGroupCols) / 16; ++chunk) {
+                    uint32_t v[16];
+                    if (kb_begin < kb_end(p.num_k_blocks)) {
+                        tmem_load_16cols(t_row + chunk * 16, v);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            v[j] = 0u;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        st_shared_v4(row_addr + (((chunk * 4 + j) ^ (r & kSwizzle)) << 4), v[4 * j], v[4 * j + 1],
+                                     v[4 * j + 2], v[4 * j + 3]);
+                }
+                fence_proxy_async_shared();     // the bulk copies below read these stores
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                for (int j = 0; j < splits; ++j) {
+                    if (j == z)
+                        continue;
+                    const uint32_t slot = static_cast<uint32_t>(z < j ? z : z - 1);
+                    bulk_copy_to_cluster(map_to_cta(s_a + kPartialBytes + slot * slice_bytes, static_cast<uint32_t>(j)),
+                                         s_a + static_cast<uint32_t>(j) * slice_bytes, slice_bytes,
+                                         map_to_cta(recv_bar, static_cast<uint32_t>(j)));
+                }
+            }
+            int received = 1;
+            if (lane == 0)
+                received = mbar_wait(recv_bar, 0) ? 1 : 0;
+            received = __shfl_sync(0xffffffffu, received, 0);
+            if (!received && lane == 0)
+                atomicOr(p.status, kOpDrainTimeout);
+            const OpWhere w = op_where<CTAS, BN, kSwap>(unit, row_tile_count, kBK, p);
+            const int first_row = w.m0 + z * rows;        // D's rows of this CTA
+            if (any_failed || !received) {
+                nan_elements(w, kSwap ? w.n0 : first_row, kSwap ? BN : rows, kSwap ? first_row : w.n0, kSwap ? rows : BN,
+                             warp, Tile::kThreads / 32, lane);
+            } else {
+                const uint8_t *ring = smem_raw + (s_a - raw);
+                for (int idx = threadIdx.x; idx < rows * (BN / 4); idx += Tile::kThreads) {
+                    // Neighbouring threads take neighbouring output columns.
+                    const int rl = kSwap ? idx % rows : idx / (BN / 4), q = kSwap ? idx / rows : idx % (BN / 4);
+                    const int r = z * rows + rl;
+                    const uint32_t offset = static_cast<uint32_t>(rl) * kPitch +
+                                            (static_cast<uint32_t>(q ^ (r & kSwizzle)) << 4);
+                    float v[4] = {};
+#pragma unroll
+                    for (int src = 0; src < 8; ++src) {
+                        if (src < splits) {
+                            const uint32_t at = src == z ? static_cast<uint32_t>(z) * slice_bytes
+                                                         : kPartialBytes + static_cast<uint32_t>(src < z ? src : src - 1) *
+                                                                               slice_bytes;
+                            const float4 x = *reinterpret_cast<const float4 *>(ring + at + offset);
+                            v[0] += x.x;
+                            v[1] += x.y;
+                            v[2] += x.z;
+                            v[3] += x.w;
+                        }
+                    }
+                    const int d_row = first_row + rl, d_col = w.n0 + q * 4;
+                    if constexpr (kSwap) {
+                        const float b = p.bias && d_row < p.n ? load_bias(d_row) : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            v[i] += b;
+                        if (d_row < p.n && d_col < w.row_end)
+                            store_elements(v, min(4, w.row_end - d_col), d_col, d_row, 1, 0);
+                    } else if (d_row < w.row_end && d_col < p.n) {
+                        const int count = min(4, p.n - d_col);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (p.bias && i < count)
+                                v[i] += load_bias(d_col + i);
+                        store_elements(v, count, d_row, d_col, 0, 1);
+                    }
+                }
+            }
+            // No CTA leaves while a copy into it (or out of it) may be in flight.
+            cluster_sync_all();
         }
     }
 
