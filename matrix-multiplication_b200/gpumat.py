@@ -43,7 +43,7 @@ from pathlib import Path
 
 import torch
 
-from operators import (ACTIVATION_IDS, validate_cross_entropy, validate_cross_entropy_backward, validate_epilogue,
+from operator_contracts import (ACTIVATION_IDS, validate_cross_entropy, validate_cross_entropy_backward, validate_epilogue,
                        validate_epilogue_backward, validate_grouped, validate_grouped_backward)
 from precision import INPUT_DTYPES, PRECISION_IDS, unsupported_reason, validate_operands
 

@@ -8,8 +8,8 @@ import ctypes
 import pytest
 import torch
 
-import operators as ops
-from operators import (ACTIVATION_IDS, ACTIVATIONS, validate_cross_entropy, validate_cross_entropy_backward,
+import operator_contracts as ops
+from operator_contracts import (ACTIVATION_IDS, ACTIVATIONS, validate_cross_entropy, validate_cross_entropy_backward,
                        validate_epilogue, validate_epilogue_backward, validate_grouped, validate_grouped_backward)
 
 BF16, FP32 = torch.bfloat16, torch.float32

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import operator_reference as ref
-from operators import ACTIVATIONS
+from operator_contracts import ACTIVATIONS
 from operator_reference import DTYPES, assert_within
 
 pytestmark = pytest.mark.gpu
