@@ -58,6 +58,7 @@ struct Matrix {
     const void *ptr = nullptr;
     int64_t rows = 0, cols = 0, pitch = 0;
     int64_t groups = 1, slab = 0;
+    int64_t skipped = 0;     // columns of the rows before `ptr` (a piece of a matrix)
 };
 
 // One call: its context, format, stream and stream-ordered scratch.  Scratch is asked
@@ -103,7 +104,7 @@ struct Call {
 };
 
 // An operand that TMA can address: the caller's matrix, or its copy in scratch with rows
-// padded to 16 bytes (unaligned bases and row pitches).
+// padded to 128 bytes (unaligned bases and row pitches).
 struct Operand {
     Matrix source;
     Matrix ready;
@@ -116,21 +117,34 @@ struct Operand {
         direct = aligned16(ptr) && cols * c.elem() % 16 == 0;
         ready = source;
         if (!direct) {
-            ready.pitch = round_up(cols, 16 / c.elem());
+            ready.pitch = round_up(cols, OP_ROW_BYTES / c.elem());
             ready.slab = rows * ready.pitch;
             at = c.reserve(static_cast<size_t>(groups * ready.slab * c.elem()));
         }
     }
-    int prepare(Call &c)
+    RepackJob job(Call &c)
     {
-        if (direct)
-            return 0;
         ready.ptr = c.scratch + at;
-        const cudaError_t st = c.kernels().repack(source.ptr, c.scratch + at, source.rows * source.groups, source.cols,
-                                                  ready.pitch, c.ctx->sm_count, c.stream);
-        return st == cudaSuccess ? 0 : c.failed(st);
+        return repack_job(source.ptr, c.scratch + at, source.rows * source.groups, source.cols, ready.pitch, c.elem());
     }
 };
+
+// Copies the operands that need it, two to a launch.
+int prepare_operands(Call &c, std::initializer_list<Operand *> operands)
+{
+    RepackJob jobs[4]{};
+    int count = 0;
+    for (Operand *o : operands)
+        if (o->source.ptr && !o->direct)
+            jobs[count++] = o->job(c);
+    for (int i = 0; i < count; i += 2) {
+        const cudaError_t st = c.kernels().repack(jobs[i], i + 1 < count ? jobs[i + 1] : RepackJob{}, c.ctx->sm_count,
+                                                  c.stream);
+        if (st != cudaSuccess)
+            return c.failed(st);
+    }
+    return 0;
+}
 
 bool encode_3d(const Context *ctx, CUtensorMap *map, CUtensorMapDataType type, const Matrix &m, int elem,
                uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle)
@@ -147,15 +161,36 @@ bool encode_3d(const Context *ctx, CUtensorMap *map, CUtensorMapDataType type, c
                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// An operand's map: K-major tiles are boxes of 128 bytes of K x `extent` rows,
-// MN-major tiles boxes of 128 bytes of M/N x one K block of rows.
+// Whether an MN-major operand's columns are whole 128-byte blocks in memory (up to the row
+// pitch, which a copy in scratch has to spare).
+bool whole_blocks(const Call &c, const Matrix &m)
+{
+    const int64_t block = OP_ROW_BYTES / c.elem();
+    return m.skipped + round_up(m.cols, block) <= m.pitch;
+}
+
+// An operand's map: K-major tiles are boxes of 128 bytes of K x `extent` rows; MN-major
+// tiles are boxes of 128 bytes of M/N x one K block of rows, `extent` columns of them in
+// one load where the columns are whole blocks (then the map's inner dimension is a block,
+// its third the blocks of a row).
 bool operand_map(const Call &c, CUtensorMap *map, const Matrix &m, bool mn_major, int extent)
 {
     const uint32_t inner = static_cast<uint32_t>(OP_ROW_BYTES / c.elem());
+    const bool blocked = mn_major && whole_blocks(c, m);
     const CUtensorMapSwizzle swizzle = mn_major && c.precision == kTf32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
                                                                         : CU_TENSOR_MAP_SWIZZLE_128B;
-    return encode_3d(c.ctx, map, operand_type(c.precision), m, c.elem(), inner,
-                     mn_major ? inner : static_cast<uint32_t>(extent), swizzle);
+    const cuuint64_t blocks = static_cast<cuuint64_t>((m.cols + inner - 1) / inner);
+    const cuuint64_t dims[4] = {blocked ? inner : static_cast<cuuint64_t>(m.cols), static_cast<cuuint64_t>(m.rows),
+                                blocked ? blocks : 1, static_cast<cuuint64_t>(m.groups)};
+    const cuuint64_t row = static_cast<cuuint64_t>(m.pitch) * c.elem();
+    const cuuint64_t slab = m.groups > 1 ? static_cast<cuuint64_t>(m.slab) * c.elem() : row * m.rows;
+    const cuuint64_t strides[3] = {row, blocked ? OP_ROW_BYTES : slab, slab};
+    const cuuint32_t box[4] = {inner, mn_major ? inner : static_cast<cuuint32_t>(extent),
+                               blocked ? static_cast<cuuint32_t>(extent) / inner : 1, 1};
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    return c.ctx->encode(map, operand_type(c.precision), 4, const_cast<void *>(m.ptr), dims, strides, box, steps,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Whether TMA can write an output, and its map (boxes of 128 rows x 128 bytes).
@@ -188,28 +223,33 @@ bool is_swap(int tile)
     return tile >= kSwap16;
 }
 
-// Estimated cycles of `tiles` tiles of a kind with K blocks of 128 bytes, K split S ways:
-// the model and the constants of the plain product's plan (matmul_b200.cu): a K block
-// costs the most of its MMA time, its operand bytes into one SM at 55 B/cycle, and all
-// running CTAs' bytes out of L2 at 8 KB/cycle; a split adds its exchange.
-double tile_cycles(const Context *ctx, int tile, int splits, double tiles, double k_blocks)
+// Estimated cycles of `tiles` tiles of a kind with K blocks of 128 bytes, K split S ways,
+// whose epilogue reads and writes `bytes_out` bytes per element.  As in the plain product's
+// plan (matmul_b200.cu) a K block costs the most of its MMA time, its operand bytes into
+// one SM at 55 B/cycle, and all running CTAs' bytes out of L2 at 8 KB/cycle; a split adds
+// its exchange.  A pair's tile also costs no less than its epilogue: 5400 cycles per 256
+// columns of BF16 (measured with K = 256).  Between 512-column tiles the MMAs wait for the
+// second half's read, which follows the first half's stores: 5000 cycles for a BF16 output,
+// 18000 more for each BF16 output or residual beside it (cycle stamps at 4096 x 4096 x 14336:
+// 70.6 k cycles a tile of 65.5 k MMA cycles; two 256-column tiles take 76 k).
+double tile_cycles(const Context *ctx, int tile, int splits, double tiles, double k_blocks, int bytes_out)
 {
     const TileShape &t = kTileShapes[tile];
-    const double units = t.ctas == 2 ? ctx->max_pairs : ctx->sm_count;
+    const bool pair = t.ctas == 2;
+    const double units = pair ? ctx->max_pairs : ctx->sm_count;
     const double active = splits > 1 ? tiles * splits : t.ctas * std::min(tiles, units);
     double rounds = splits > 1 ? 1.0 : std::max(1.0, std::ceil(tiles / units));
     const double bytes = static_cast<double>(OP_BM + t.bn / t.ctas) * OP_ROW_BYTES;
     const double k_cycles = std::max({2.0 * t.bn, bytes / 55.0, active * bytes / 8000.0});
-    // A 512-column tile's second half is read once the first one's outputs are on their way,
-    // and the next tile's MMAs wait for that: about 24000 cycles a tile where a 256-column
-    // tile, whose two accumulators alternate, loses 4000.  So the wide tile is for long K:
-    // 4096 x 14336 x 4096 BF16 316 us against 345 us, but 4096 x 4096 x 14336 380 against 334.
-    const double epilogue = t.bn == 512 ? 24000.0 : 4000.0 * t.bn / 256.0;
+    const double extra = std::max(0.0, bytes_out / 2.0 - 1.0);
+    const double epilogue = t.bn == 512 ? 5000.0 + 18000.0 * extra : pair ? 1000.0 : 4000.0 * t.bn / 256.0;
     // A short last round of 512-column tiles runs as halves (enqueue).
     if (t.bn == 512 && tiles - std::floor(tiles / units) * units <= units / 2)
         rounds = std::floor(tiles / units) + (std::fmod(tiles, units) > 0.0 ? 0.5 : 0.0);
-    return 2000.0 + rounds * (std::ceil(k_blocks / splits) * k_cycles + epilogue) +
-           (t.ctas == 2 ? 10000.0 : 0.0) +
+    double tile_time = std::ceil(k_blocks / splits) * k_cycles + epilogue;
+    if (pair)
+        tile_time = std::max(tile_time, 2700.0 * bytes_out * t.bn / 256.0);
+    return 2000.0 + rounds * tile_time + (pair ? 10000.0 : 0.0) +
            (splits > 1 ? 1000.0 + static_cast<double>(splits - 1) / splits * OP_BM * t.bn * 4.0 / 8.0 : 0.0);
 }
 
@@ -226,7 +266,7 @@ bool can_split(const Context *ctx, int log_splits, int64_t tiles, int64_t k_bloc
 
 // The tile and K split with the fewest estimated cycles for an m x n product (of one of
 // `groups` groups).  Splits are for ungrouped products whose epilogue can take partial sums.
-TileChoice choose_tile(const Context *ctx, int64_t m, int64_t n, int64_t k_blocks, int64_t groups = 1,
+TileChoice choose_tile(const Context *ctx, int64_t m, int64_t n, int64_t k_blocks, int bytes_out, int64_t groups = 1,
                        bool splittable = false)
 {
     TileChoice best{kSingle64, 1};
@@ -239,7 +279,8 @@ TileChoice choose_tile(const Context *ctx, int64_t m, int64_t n, int64_t k_block
         for (int i = 0; i < (splittable && t.ctas == 1 ? 4 : 1); ++i) {
             if (i > 0 && !can_split(ctx, i, tiles, k_blocks))
                 continue;
-            const double cycles = tile_cycles(ctx, tile, 1 << i, static_cast<double>(tiles), static_cast<double>(k_blocks));
+            const double cycles = tile_cycles(ctx, tile, 1 << i, static_cast<double>(tiles), static_cast<double>(k_blocks),
+                                              bytes_out);
             if (best_cycles == 0.0 || cycles < best_cycles) {
                 best = {tile, 1 << i};
                 best_cycles = cycles;
@@ -291,6 +332,9 @@ int enqueue(Call &c, Product &q)
     const bool swap = is_swap(l.tile);
     const bool a_mn = l.layout == kTN, b_mn = l.layout != kNT;
     const int b_cols = std::min(t.bn, 256) / t.ctas;     // rows of a K-major box of Bop
+    // Every blocked load takes whole columns, OP_BM of Aop or a half's share of Bop.
+    l.p.a_blocked = whole_blocks(c, swap ? q.b : q.a) ? 1 : 0;
+    l.p.b_blocked = whole_blocks(c, q.b) ? 1 : 0;
     bool ok;
     if (swap)     // D = B^T A^T: B's columns on the M side, A's rows on the N side
         ok = operand_map(c, &l.map_a, q.b, true, OP_BM) && operand_map(c, &l.map_b, q.a, false, b_cols);
@@ -424,7 +468,7 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     Operand oa, ob;
     oa.plan(c, a, m, k);
     ob.plan(c, b, k, n);
-    if (c.allocate() || oa.prepare(c) || ob.prepare(c))
+    if (c.allocate() || prepare_operands(c, {&oa, &ob}))
         return 1;
     Product q;
     q.a = oa.ready;
@@ -435,11 +479,12 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     OpLaunch &l = q.launch;
     const int bk = OP_ROW_BYTES / e;
     const int64_t k_blocks = (static_cast<int64_t>(k) + bk - 1) / bk;
+    const int bytes_out = (out_half ? 2 : 4) * (residual ? 2 : 1) + (preact ? (preact_half ? 2 : 4) : 0);
     const TileChoice choice = m <= 64 ? choose_few_rows(c.ctx, m, n, k_blocks)
-                                      : choose_tile(c.ctx, m, n, k_blocks, 1, true);
+                                      : choose_tile(c.ctx, m, n, k_blocks, bytes_out, 1, true);
     l.tile = choice.tile;
     l.splits = choice.splits;
-    l.epilogue = m <= 64 ? kEpiStoreT : kEpiStore;
+    l.epilogue = is_swap(choice.tile) ? kEpiStoreT : kEpiStore;
     const Matrix mo{out, m, n, n};
     if (set_output(c, l, mo, out_half))
         return 1;
@@ -469,16 +514,25 @@ namespace {
 // dz = dout * act'(preact) into `dz` (pitch dz_pitch; null without an activation) and
 // dbias, the column sums, through `partial` ([chunks][n]) when there are several chunks.
 struct ActGradPlan {
-    int chunks = 1, rows_per_chunk = 0;
+    int chunks = 1, rows_per_chunk = 0, cluster = 1, clusters = 1;
     void choose(const Context *ctx, int m, int n)
     {
-        // About eight blocks per SM, at least 32 rows each.
+        // Row chunks of at least 32 rows.  Few columns: clusters of eight blocks that add up their
+        // sums, one if its chunks stay below 512 rows; many: about sixteen blocks per SM, summed
+        // by a second kernel (in clusters, 448 blocks of 4096 x 14336 took two waves).
         const int64_t column_blocks = (static_cast<int64_t>(n) + AG_COLS - 1) / AG_COLS;
-        const int64_t wanted = std::max<int64_t>(1, 8LL * ctx->sm_count / column_blocks);
-        int64_t rows = std::max<int64_t>(32, (m + wanted - 1) / wanted);
-        rows = (rows + 7) / 8 * 8;
-        chunks = static_cast<int>((m + rows - 1) / rows);
-        rows_per_chunk = static_cast<int>(rows);
+        const int64_t most = std::max<int64_t>(1, m / 32);
+        int64_t wanted;
+        if (column_blocks * AG_CLUSTER <= ctx->sm_count) {
+            const int64_t all = std::max<int64_t>(1, std::min<int64_t>((m + 4095) / 4096, 2LL * ctx->sm_count / (column_blocks * AG_CLUSTER)));
+            wanted = most >= AG_CLUSTER ? AG_CLUSTER * std::min(all, most / AG_CLUSTER) : most;
+            cluster = static_cast<int>(std::min<int64_t>(wanted, AG_CLUSTER));
+        } else {
+            wanted = std::min<int64_t>(most, std::max<int64_t>(1, 16LL * ctx->sm_count / column_blocks));
+        }
+        clusters = static_cast<int>(wanted / cluster);
+        chunks = static_cast<int>(wanted);
+        rows_per_chunk = static_cast<int>((m + wanted - 1) / wanted);
     }
 };
 
@@ -518,7 +572,7 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
     if (da)
         ob.plan(c, b, k, n);
     size_t dz_at = 0;
-    const int64_t dz_pitch = round_up(n, 16 / e);
+    const int64_t dz_pitch = round_up(n, OP_ROW_BYTES / e);
     if (own_dz)
         dz_at = c.reserve(static_cast<size_t>(m * dz_pitch * e));
     else if (da || db)
@@ -526,10 +580,10 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
     ActGradPlan plan;
     plan.choose(c.ctx, m, n);
     size_t partial_at = 0;
-    const bool partial = dbias && plan.chunks > 1;
+    const bool partial = dbias && plan.clusters > 1;
     if (partial)
-        partial_at = c.reserve(static_cast<size_t>(plan.chunks) * n * sizeof(float));
-    if (c.allocate() || (db && oa.prepare(c)) || (da && ob.prepare(c)) || (!own_dz && (da || db) && od.prepare(c)))
+        partial_at = c.reserve(static_cast<size_t>(plan.clusters) * n * sizeof(float));
+    if (c.allocate() || prepare_operands(c, {&oa, &ob, &od}))
         return 1;
 
     if (own_dz || dbias) {
@@ -550,9 +604,9 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
                 (!g.preact || static_cast<int64_t>(n) * (preact_half ? 2 : 4) % 16 == 0);
         cudaError_t st = c.kernels().act_grad(g, dim3(static_cast<unsigned int>((n + AG_COLS - 1) / AG_COLS),
                                                       static_cast<unsigned int>(plan.chunks)),
-                                              c.stream);
+                                              plan.cluster, c.stream);
         if (st == cudaSuccess && partial)
-            st = c.kernels().bias_grad(g.partial, plan.chunks, n, dbias, g.dbias_half, c.stream);
+            st = c.kernels().bias_grad(g.partial, plan.clusters, n, dbias, g.dbias_half, c.stream);
         if (st != cudaSuccess)
             return c.failed(st);
     }
@@ -566,7 +620,7 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.n = k;
         q.k = n;
         q.launch.layout = kNT;
-        q.set_tile(choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk, 1, true));
+        q.set_tile(choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk, da_half ? 2 : 4, 1, true));
         if (set_output(c, q.launch, Matrix{da, m, k, k}, da_half) || enqueue(c, q))
             return 1;
     }
@@ -578,7 +632,7 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.n = n;
         q.k = m;
         q.launch.layout = kTN;
-        q.set_tile(choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk, 1, true));
+        q.set_tile(choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk, db_half ? 2 : 4, 1, true));
         if (set_output(c, q.launch, Matrix{db, k, n, n}, db_half) || enqueue(c, q))
             return 1;
     }
@@ -605,9 +659,10 @@ struct GroupPlan {
         count_at = c.reserve(sizeof(int));
         units_at = c.reserve(static_cast<size_t>(c.ctx->sm_count + 1) * sizeof(int));
     }
+    // The plan kernel's parameters, and what the product reads of its results.
     // `tiles_per_group`, `max_units`: ragged-K mode's tiles and the CTAs or pairs that share them.
-    int enqueue(Call &c, const void *offsets, int offsets64, int groups, int rows, const CUtensorMap &map0,
-                const CUtensorMap &map1, OpParams &p, int64_t tiles_per_group = 0, int64_t max_units = 0)
+    GroupPlanParams fill(Call &c, const void *offsets, int offsets64, int groups, int rows, OpParams &p,
+                         int64_t tiles_per_group = 0, int64_t max_units = 0) const
     {
         GroupPlanParams g{};
         if (!tile_rows) {
@@ -626,17 +681,26 @@ struct GroupPlan {
         g.count = reinterpret_cast<int *>(c.scratch + count_at);
         g.tiles = reinterpret_cast<OpRowTile *>(c.scratch + tiles_at);
         g.group_maps = reinterpret_cast<CUtensorMap *>(c.scratch + maps_at);
-        // One warp per tensor map, up to sixteen blocks.
-        const unsigned int blocks = static_cast<unsigned int>(std::min(16, std::max(1, groups * maps / (GP_THREADS / 32))));
         p.grouping = tile_rows ? kGroupedRows : kGroupedK;
         p.groups = groups;
         p.row_tile_count = g.count;
         p.row_tiles = g.tiles;
         p.group_maps = g.group_maps;
-        const cudaError_t st = launch_pdl(group_plan_kernel, dim3(blocks), dim3(GP_THREADS), 0, c.stream, map0, map1, g);
-        return st == cudaSuccess ? 0 : c.failed(st);
+        return g;
     }
 };
+
+// One launch for one plan, or for a backward pass's two (`second` with map2 alone).
+int enqueue_plans(Call &c, const CUtensorMap &map0, const CUtensorMap &map1, const CUtensorMap &map2,
+                  const GroupPlanParams &first, const GroupPlanParams *second)
+{
+    // One warp per tensor map, up to sixteen blocks.
+    const int maps = std::max(first.groups * first.maps, second ? second->groups * second->maps : 0);
+    const dim3 grid(static_cast<unsigned int>(std::min(16, std::max(1, maps / GP_WARPS))), second ? 2 : 1);
+    const cudaError_t st = launch_pdl(group_plan_kernel, grid, dim3(GP_THREADS), 0, c.stream, map0, map1, map2, first,
+                                      second ? *second : first);
+    return st == cudaSuccess ? 0 : c.failed(st);
+}
 
 int check_groups(Call &c, int groups, int rows, int k, int n, const void *offsets, int offsets64)
 {
@@ -651,7 +715,7 @@ int check_groups(Call &c, int groups, int rows, int k, int n, const void *offset
 
 // Rows per tile follow the mean group: with few rows they take the MMA's N side (16 to
 // 128 wide) and the weight's columns its M side, so that a tile wastes little.
-int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_t n, int64_t k_blocks)
+int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_t n, int64_t k_blocks, int bytes_out)
 {
     const int64_t mean = (rows + groups - 1) / groups;
     if (mean <= 16)
@@ -662,18 +726,7 @@ int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_
         return kSwap64;
     if (mean <= 128)
         return kSwap128;
-    return choose_tile(ctx, mean, n, k_blocks, groups).tile;
-}
-
-// A product over row groups: out[i] = a[i] . b[g] (layout kNN) or a[i] . b[g]^T (kNT).
-int grouped_rows(Call &c, GroupPlan &plan, Product &q, const void *offsets, int offsets64, int groups, int rows,
-                 const Matrix &out, bool half)
-{
-    if (set_output(c, q.launch, out, half))
-        return 1;
-    if (plan.enqueue(c, offsets, offsets64, groups, rows, q.launch.map_c, q.launch.map_c, q.launch.p))
-        return 1;
-    return enqueue(c, q);
+    return choose_tile(ctx, mean, n, k_blocks, bytes_out, groups).tile;
 }
 
 } // namespace
@@ -700,7 +753,7 @@ extern "C" int matmul_grouped(void *opaque, int precision, const void *a, const 
     const int64_t bk = OP_ROW_BYTES / e;
     Product q;
     OpLaunch &l = q.launch;
-    l.tile = choose_grouped_tile(c.ctx, rows, groups, n, (k + bk - 1) / bk);
+    l.tile = choose_grouped_tile(c.ctx, rows, groups, n, (k + bk - 1) / bk, half ? 2 : 4);
     const bool swap = is_swap(l.tile);
     l.epilogue = swap ? kEpiStoreT : kEpiStore;
     Operand oa, ob;
@@ -710,14 +763,17 @@ extern "C" int matmul_grouped(void *opaque, int precision, const void *a, const 
     GroupPlan plan;
     plan.plan(c, groups, rows, swap ? kTileShapes[l.tile].bn : kTileShapes[l.tile].bm,
               !swap && output_tma(mo, half ? 2 : 4) ? 1 : 0);
-    if (c.allocate() || oa.prepare(c) || ob.prepare(c))
+    if (c.allocate() || prepare_operands(c, {&oa, &ob}))
         return 1;
     q.a = oa.ready;
     q.b = ob.ready;
     q.m = rows;
     q.n = n;
     q.k = k;
-    return grouped_rows(c, plan, q, offsets, offsets64, groups, rows, mo, half);
+    if (set_output(c, l, mo, half))
+        return 1;
+    const GroupPlanParams g = plan.fill(c, offsets, offsets64, groups, rows, l.p);
+    return enqueue_plans(c, l.map_c, l.map_c, l.map_c, g, nullptr) || enqueue(c, q) ? 1 : 0;
 }
 
 extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *dout, const void *a, const void *b,
@@ -752,26 +808,30 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
         ob.plan(c, b, k, n, groups);
         const int64_t mean = (rows + groups - 1) / groups;
         qa.launch.layout = kNT;
-        qa.launch.tile = choose_tile(c.ctx, mean, k, (n + bk - 1) / bk, groups).tile;
+        qa.launch.tile = choose_tile(c.ctx, mean, k, (n + bk - 1) / bk, da_half ? 2 : 4, groups).tile;
         rows_plan.plan(c, groups, rows, kTileShapes[qa.launch.tile].bm, output_tma(ma, da_half ? 2 : 4) ? 1 : 0);
     }
     if (db) {
         oa.plan(c, a, rows, k);
         const int64_t mean = (rows + groups - 1) / groups;
         qb.launch.layout = kTN;
-        qb.launch.tile = choose_tile(c.ctx, k, n, (mean + bk - 1) / bk, groups).tile;
+        qb.launch.tile = choose_tile(c.ctx, k, n, (mean + bk - 1) / bk, db_half ? 2 : 4, groups).tile;
         k_plan.plan(c, groups, rows, 0, 2);
     }
-    if (c.allocate() || od.prepare(c) || (da && ob.prepare(c)) || (db && oa.prepare(c)))
+    if (c.allocate() || prepare_operands(c, {&od, &ob, &oa}))
         return 1;
+    // The plans first, both in one launch, then the two products.
+    GroupPlanParams ga{}, gb{};
+    CUtensorMap map0{}, map1{};
     if (da) {
         qa.a = od.ready;
         qa.b = ob.ready;
         qa.m = rows;
         qa.n = k;
         qa.k = n;
-        if (grouped_rows(c, rows_plan, qa, offsets, offsets64, groups, rows, ma, da_half))
+        if (set_output(c, qa.launch, ma, da_half))
             return 1;
+        ga = rows_plan.fill(c, offsets, offsets64, groups, rows, qa.launch.p);
     }
     if (db) {
         qb.a = oa.ready;
@@ -780,18 +840,23 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
         qb.n = n;
         qb.k = rows;
         const TileShape &t = kTileShapes[qb.launch.tile];
-        CUtensorMap map0, map1;
-        if (!operand_map(c, &map0, qb.a, true, OP_BM) || !operand_map(c, &map1, qb.b, true, std::min(t.bn, 256) / t.ctas)) {
+        if (!operand_map(c, &map0, qb.a, true, OP_BM) ||
+            !operand_map(c, &map1, qb.b, true, std::min(t.bn, 256) / t.ctas)) {
             cudaGetLastError();
             return c.failed("cuTensorMapEncodeTiled rejected an operand");
         }
-        if (set_output(c, qb.launch, Matrix{db, k, n, n, groups, static_cast<int64_t>(k) * n}, db_half) ||
-            k_plan.enqueue(c, offsets, offsets64, groups, rows, map0, map1, qb.launch.p,
-                           ((k + t.bm - 1) / t.bm) * ((static_cast<int64_t>(n) + t.bn - 1) / t.bn),
-                           t.ctas == 2 ? c.ctx->max_pairs : c.ctx->sm_count) ||
-            enqueue(c, qb))
+        if (set_output(c, qb.launch, Matrix{db, k, n, n, groups, static_cast<int64_t>(k) * n}, db_half))
             return 1;
+        gb = k_plan.fill(c, offsets, offsets64, groups, rows, qb.launch.p,
+                         ((k + t.bm - 1) / t.bm) * ((static_cast<int64_t>(n) + t.bn - 1) / t.bn),
+                         t.ctas == 2 ? c.ctx->max_pairs : c.ctx->sm_count);
     }
+    const CUtensorMap &map_da = qa.launch.map_c;
+    if (db ? enqueue_plans(c, map0, map1, map_da, gb, da ? &ga : nullptr)
+           : enqueue_plans(c, map_da, map_da, map_da, ga, nullptr))
+        return 1;
+    if ((da && enqueue(c, qa)) || (db && enqueue(c, qb)))
+        return 1;
     return 0;
 }
 
@@ -832,7 +897,7 @@ extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hid
     Product q;
     OpLaunch &l = q.launch;
     l.epilogue = kEpiLse;
-    l.tile = choose_tile(c.ctx, m, v, (k + bk - 1) / bk).tile;
+    l.tile = choose_tile(c.ctx, m, v, (k + bk - 1) / bk, 2).tile;
     // One (maximum, sum) per row and column range of a tile.
     const int tiles = (v + kTileShapes[l.tile].bn - 1) / kTileShapes[l.tile].bn * loss_parts(l.tile);
     Operand oh, ow;
@@ -840,7 +905,7 @@ extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hid
     ow.plan(c, weight, k, v);
     const size_t partial_at = c.reserve(static_cast<size_t>(tiles) * m * sizeof(float2));
     const size_t logit_at = c.reserve(static_cast<size_t>(m) * sizeof(float));
-    if (c.allocate() || oh.prepare(c) || ow.prepare(c))
+    if (c.allocate() || prepare_operands(c, {&oh, &ow}))
         return 1;
     q.a = oh.ready;
     q.b = ow.ready;
@@ -856,7 +921,8 @@ extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hid
     p.label_logit = reinterpret_cast<float *>(c.scratch + logit_at);
     if (enqueue(c, q))
         return 1;
-    const cudaError_t st = launch_pdl(loss_join_kernel, dim3(static_cast<unsigned int>((m + 31) / 32)), dim3(256), 0,
+    const cudaError_t st = launch_pdl(loss_join_kernel, dim3(static_cast<unsigned int>((m + 31) / 32)),
+                                      dim3(32 * LJ_WARPS), 0,
                                       c.stream, static_cast<const float2 *>(p.partial), tiles,
                                       static_cast<const float *>(p.label_logit), loss, lse, p);
     return st == cudaSuccess ? 0 : c.failed(st);
@@ -903,13 +969,13 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
     // dH is summed over the pieces in FP32: in the output itself where it is FP32.
     const bool own_sum = dhidden && dh_half && pieces > 1;
     const size_t sum_at = own_sum ? c.reserve(static_cast<size_t>(m) * k * sizeof(float)) : 0;
-    if (c.allocate() || oh.prepare(c) || ow.prepare(c))
+    if (c.allocate() || prepare_operands(c, {&oh, &ow}))
         return 1;
     const Matrix dh{dhidden, m, k, k};
     const Matrix sum = own_sum ? Matrix{c.scratch + sum_at, m, k, k} : dh;
     for (int64_t piece = 0; piece < pieces; ++piece) {
         const int64_t v0 = piece * width, cols = std::min<int64_t>(width, v - v0);
-        const Matrix w{static_cast<const uint8_t *>(ow.ready.ptr) + v0 * e, k, cols, ow.ready.pitch};
+        const Matrix w{static_cast<const uint8_t *>(ow.ready.ptr) + v0 * e, k, cols, ow.ready.pitch, 1, 0, v0};
         const Matrix dz{c.scratch + dz_at, m, cols, width};
         {
             Product q;
@@ -919,7 +985,7 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = cols;
             q.k = k;
             q.launch.epilogue = kEpiSoftmaxGrad;
-            q.launch.tile = choose_tile(c.ctx, m, cols, (k + bk - 1) / bk).tile;
+            q.launch.tile = choose_tile(c.ctx, m, cols, (k + bk - 1) / bk, e).tile;
             OpParams &p = q.launch.p;
             p.labels = labels;
             p.labels64 = labels64;
@@ -939,8 +1005,9 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = k;
             q.k = cols;
             q.launch.layout = kNT;
-            q.set_tile(choose_tile(c.ctx, m, k, (cols + bk - 1) / bk, 1, true));
             const bool last = piece == pieces - 1;
+            q.set_tile(choose_tile(c.ctx, m, k, (cols + bk - 1) / bk, (piece > 0 ? 4 : 0) + (last && dh_half ? 2 : 4), 1,
+                                   true));
             if (set_output(c, q.launch, last ? dh : sum, last && dh_half))
                 return 1;
             if (piece > 0) {
@@ -960,7 +1027,7 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = cols;
             q.k = m;
             q.launch.layout = kTN;
-            q.set_tile(choose_tile(c.ctx, k, cols, (m + bk - 1) / bk, 1, true));
+            q.set_tile(choose_tile(c.ctx, k, cols, (m + bk - 1) / bk, dw_half ? 2 : 4, 1, true));
             const Matrix dw{static_cast<uint8_t *>(dweight) + v0 * (dw_half ? 2 : 4), k, cols, v};
             if (set_output(c, q.launch, dw, dw_half) || enqueue(c, q))
                 return 1;

@@ -95,25 +95,37 @@ struct OpInstances {
         });
     }
 
-    static cudaError_t act_grad(const ActGradParams &params, dim3 grid, cudaStream_t stream)
+    static cudaError_t act_grad(const ActGradParams &params, dim3 grid, int cluster, cudaStream_t stream)
     {
-        return launch_pdl(act_grad_kernel<FMT>, grid, dim3(AG_THREADS), 0, stream, params);
+        cudaLaunchConfig_t config{};
+        config.gridDim = grid;
+        config.blockDim = dim3(AG_THREADS);
+        config.stream = stream;
+        cudaLaunchAttribute attributes[2]{};
+        attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[0].val.programmaticStreamSerializationAllowed = 1;
+        attributes[1].id = cudaLaunchAttributeClusterDimension;
+        attributes[1].val.clusterDim.x = 1;
+        attributes[1].val.clusterDim.y = static_cast<unsigned int>(cluster);
+        attributes[1].val.clusterDim.z = 1;
+        config.attrs = attributes;
+        config.numAttrs = 2;
+        return cudaLaunchKernelEx(&config, act_grad_kernel<FMT>, params);
     }
 
-    static cudaError_t bias_grad(const float *partial, int chunks, int n, void *dbias, int dbias_half,
+    static cudaError_t bias_grad(const float *partial, int count, int n, void *dbias, int dbias_half,
                                  cudaStream_t stream)
     {
         return launch_pdl(bias_grad_kernel<FMT>, dim3(static_cast<unsigned int>((n + 255) / 256)), dim3(256), 0, stream,
-                          partial, chunks, n, dbias, dbias_half);
+                          partial, count, n, dbias, dbias_half);
     }
 
-    static cudaError_t repack(const void *src, void *dst, int64_t rows, int64_t cols, int64_t pitch, int sms,
-                              cudaStream_t stream)
+    static cudaError_t repack(const RepackJob &job0, const RepackJob &job1, int sms, cudaStream_t stream)
     {
-        const RepackPlan plan = repack_plan(rows, pitch, static_cast<int>(sizeof(T)), sms);
-        return launch_pdl(repack_kernel<static_cast<int>(sizeof(T))>, dim3(plan.grid), dim3(RP_THREADS), 0, stream,
-                          static_cast<const uint8_t *>(src), static_cast<uint8_t *>(dst), rows, cols, pitch,
-                          plan.log_lanes);
+        const int64_t units = job0.units + job1.units, cap = 32LL * sms;
+        return launch_pdl(repack_kernel<static_cast<int>(sizeof(T))>,
+                          dim3(static_cast<unsigned int>(units < cap ? units : cap)), dim3(RP_THREADS), 0, stream, job0,
+                          job1);
     }
 
     static constexpr OpKernels kTable{setup, product, act_grad, bias_grad, repack};

@@ -46,8 +46,12 @@ constexpr int GP_EPILOGUE_BLOCKS = 6;
 // tables, all blocks share the maps.
 __global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_constant__ CUtensorMap map0,
                                                                 const __grid_constant__ CUtensorMap map1,
-                                                                const GroupPlanParams p)
+                                                                const __grid_constant__ CUtensorMap map2,
+                                                                const __grid_constant__ GroupPlanParams first_plan,
+                                                                const __grid_constant__ GroupPlanParams second_plan)
 {
+    // Blocks of the second row make the second plan (a backward pass has two), with map2 alone.
+    const GroupPlanParams &p = blockIdx.y ? second_plan : first_plan;
     __shared__ int warp_max[GP_WARPS], warp_sum[GP_WARPS];
     __shared__ int carry_max, carry_sum;
     __shared__ int ends[GP_THREADS];
@@ -113,7 +117,9 @@ __global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_con
              i < GP_THREADS * p.maps && g0 + i / p.maps < p.groups; i += GP_WARPS * static_cast<int>(gridDim.x)) {
             const uint32_t s = smem_addr(map_s[warp]);
             const int local = i / p.maps;
-            const uint32_t *src = reinterpret_cast<const uint32_t *>(i - local * p.maps ? &map1 : &map0);
+            const uint32_t *src = reinterpret_cast<const uint32_t *>(blockIdx.y               ? &map2
+                                                                    : i - local * p.maps ? &map1
+                                                                                         : &map0);
             reinterpret_cast<uint32_t *>(map_s[warp])[lane] = src[lane];
             __syncwarp();
             if (lane == 0) {
@@ -165,36 +171,46 @@ __global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_con
 }
 
 // ---------------------------------------------------------------- loss
-// lse = log sum exp over the column tiles' (maximum, sum) pairs in base 2, loss = lse -
-// the label's logit; 32 rows per block, eight warps each take every eighth tile and
-// join in a fixed order.
-__global__ void __launch_bounds__(256) loss_join_kernel(const float2 *partial, int tiles, const float *label_logit,
-                                                        float *loss, float *lse, const OpParams p)
+constexpr int LJ_WARPS = 32;
+
+// lse = log sum exp over the column ranges' (maximum, sum) pairs in base 2, loss = lse -
+// the label's logit.  A block takes 32 rows, each warp every 32nd range: the maximum
+// first, then the sums scaled to it (loads and exponentials without a chain through
+// them), joined over the warps in a fixed order.  A range's sum is NaN where a logit was.
+__global__ void __launch_bounds__(32 * LJ_WARPS) loss_join_kernel(const float2 *partial, int ranges,
+                                                                  const float *label_logit, float *loss, float *lse,
+                                                                  const OpParams p)
 {
-    __shared__ float tops[8][32], sums[8][32];
+    __shared__ float tops[LJ_WARPS][32], sums[LJ_WARPS][32];
     wait_for_prior_grid();
     allow_next_grid();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = static_cast<int>(blockIdx.x) * 32 + lane;
-    float top = -INFINITY, sum = 0.0f;
-    auto join = [&](float t, float s) {
-        const float next = fmaxf(top, t);
-        const float origin = next == -INFINITY ? 0.0f : next;
-        sum = sum * exp2f(top - origin) + s * exp2f(t - origin);
-        top = next;
-    };
-    if (row < p.m)
-        for (int i = warp; i < tiles; i += 8) {
-            const float2 v = partial[static_cast<long long>(i) * p.m + row];
-            join(v.x, v.y);
-        }
+    const float2 *column = partial + min(row, p.m - 1);
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int i = warp; i < ranges; i += LJ_WARPS)
+        top = fmaxf(top, column[static_cast<long long>(i) * p.m].x);
     tops[warp][lane] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < LJ_WARPS; ++i)
+        top = fmaxf(top, tops[i][lane]);
+    const float origin = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int i = warp; i < ranges; i += LJ_WARPS) {
+        const float2 v = column[static_cast<long long>(i) * p.m];
+        sum += v.y * exp2f(v.x - origin);
+    }
     sums[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && row < p.m) {
-        for (int i = 1; i < 8; ++i)
-            join(tops[i][lane], sums[i][lane]);
-        const float total = (top + log2f(sum)) * 0.69314718055994531f;
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < LJ_WARPS; ++i)
+            sum += sums[i][lane];
+        const float total = (origin + log2f(sum)) * 0.69314718055994531f;
         const int label = op_label(p, row);
         lse[row] = total;
         loss[row] = label == -1 ? 0.0f : label == -2 ? __int_as_float(0x7fc00000) : total - label_logit[row];

@@ -15,8 +15,10 @@
 //
 // Roles, rings, bounded waits and the pair protocol are those of tc2_gemm.cuh (CTAS
 // = 2: one 256 x BN tile per CTA pair, each CTA staging half of either operand) and
-// tc_gemm.cuh (CTAS = 1: 128 x BN).  All maps are three-dimensional (inner, rows,
-// group): a coordinate past a group's own K rows reads zeros, not the next group.
+// tc_gemm.cuh (CTAS = 1: 128 x BN).  Operand maps are four-dimensional (inner, rows,
+// column block, group): a coordinate past a group's own K rows reads zeros, not the next
+// group.  An MN-major operand whose columns are whole 128-byte blocks is one load per
+// stage.
 //
 // Measured choices stand at the host's plan (ops.cu).
 #pragma once
@@ -80,6 +82,20 @@ struct OpRowTile {
     int group, row0, row_end, unused;
 };
 
+// One lane of a converged warp.  The roles that issue TMA and tensor-core instructions
+// branch on this rather than on a lane number, so that the compiler knows that a single
+// thread holds their operands.
+__device__ __forceinline__ bool op_elect_one()
+{
+    uint32_t elected;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(elected));
+    return elected != 0;
+}
+
 // Division by a divisor the host knows (Granlund and Montgomery's multiply-and-shift for
 // 32-bit numbers): quotients of numbers below 2^31.
 struct OpDivisor {
@@ -102,6 +118,7 @@ struct OpParams {
     OpDivisor per_raster;     // raster x N-side tiles (transposed epilogue: M-side tiles)
     OpDivisor per_group;      // ragged-K mode: tiles of one group
     int grouping;             // OpGrouping
+    int a_blocked, b_blocked; // MN-major operands: 1 when their map sees blocks of 128 bytes of columns
     const int *row_tile_count;        // rows mode: number of row tiles (device)
     const OpRowTile *row_tiles;       // rows mode: table of row tiles; ragged-K mode: one entry per group
     const CUtensorMap *group_maps;    // rows mode: out's map per group; ragged-K mode: Aop's and Bop's
@@ -132,22 +149,22 @@ struct OpParams {
     unsigned long long wait_limit_ns;
 };
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z)
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z, int w)
 {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
 
 // The load of a CTA pair: `bar` may be the other CTA's barrier.
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z)
+__device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z, int w)
 {
     asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
 
@@ -581,7 +598,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (warp == 0) {
         // ------------------------------------------------------------ producer
         give_registers();
-        if (lane == 0) {
+        if (op_elect_one()) {
             int stage = 0;
             uint32_t phase = 0, filled = 0, fill_parity = 0;
             bool ok = true;
@@ -616,32 +633,35 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     if (leader)
                         mbar_arrive_expect_tx(full_bar(stage), kParts == 2 && w.parts == 1 ? kHalfStageTx : kStageTx);
                     const int k = w.k0 + kb * kBK;
-                    auto load = [&](uint32_t dst, const void *map, int x, int y, int z) {
+                    auto load = [&](uint32_t dst, const void *map, int x, int y, int block, int z) {
                         if constexpr (kPair)
-                            tma_load_3d_pair(dst, map, fb, x, y, z);
+                            tma_load_4d_pair(dst, map, fb, x, y, block, z);
                         else
-                            tma_load_3d(dst, map, fb, x, y, z);
+                            tma_load_4d(dst, map, fb, x, y, block, z);
+                    };
+                    // `cols` M/N columns from `mn` on, as MN-major boxes: one load, or one per box.
+                    auto load_mn = [&](uint32_t dst, const void *map, bool blocked, int mn, int cols, int z) {
+                        if (blocked) {
+                            load(dst, map, 0, k, mn / kBox, z);
+                        } else {
+                            for (int j = 0; j < cols / kBox; ++j)
+                                load(dst + j * kBoxBytes, map, mn + j * kBox, k, 0, z);
+                        }
                     };
                     const uint32_t sa = s_a + stage * OP_A_STAGE, sb = s_b + stage * kBStage;
-                    if constexpr (A_MN) {
-#pragma unroll
-                        for (int j = 0; j < OP_BM / kBox; ++j)
-                            load(sa + j * kBoxBytes, ma, am + j * kBox, k, za);
-                    } else {
-                        load(sa, ma, k, am, za);
-                    }
+                    if constexpr (A_MN)
+                        load_mn(sa, ma, p.a_blocked != 0, am, OP_BM, za);
+                    else
+                        load(sa, ma, k, am, 0, za);
 #pragma unroll
                     for (int h = 0; h < kParts; ++h) {
                         if (h == w.parts)
                             break;
                         const uint32_t sbh = sb + h * kHalfCols * OP_ROW_BYTES;
-                        if constexpr (B_MN) {
-#pragma unroll
-                            for (int j = 0; j < kHalfCols / kBox; ++j)
-                                load(sbh + j * kBoxBytes, mb, bn + h * 256 + j * kBox, k, zb);
-                        } else {
-                            load(sbh, mb, k, bn + h * 256, zb);
-                        }
+                        if constexpr (B_MN)
+                            load_mn(sbh, mb, p.b_blocked != 0, bn + h * 256, kHalfCols, zb);
+                        else
+                            load(sbh, mb, k, bn + h * 256, 0, zb);
                     }
                     filled |= 1u << stage;
                     fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
@@ -662,7 +682,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (a pair's leader)
         give_registers();
-        if (leader && lane == 0) {
+        if (leader && op_elect_one()) {
             int stage = 0;
             uint32_t phase = 0;
             const uint64_t a_desc0 = A_MN ? smem_desc_mn<kTF32>(s_a, kBoxBytes) : smem_desc_sw128(s_a, 16, 1024);
@@ -955,14 +975,62 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                             }
                         }
                     };
+                    // The same for a box of 64 16-bit columns: a lane's two elements go out as one word
+                    // where the row starts on 4 bytes; where it starts on 2, words are shifted by one
+                    // element with the neighbour's and the two ends go out alone.
+                    auto emit_rows_half = [&](const uint32_t (&words)[32], void *dst, long long at0, long long pitch,
+                                              int col0) {
+                        const uint32_t box = s_box + stores % kBoxes * OP_BOX;
+                        if (issuer) {
+                            bulk_wait_group_read<kBoxes - 1>();
+                            bulk_commit_group();
+                        }
+                        epilogue_sync();
+                        fill(box, words);
+                        epilogue_sync();
+                        ++stores;
+                        const uint8_t *box_p = smem_raw + (box - raw);
+                        const int rows = min(OP_BM, w.row_end - row0), cols = p.n - col0;
+                        T *base_row = static_cast<T *>(dst) + at0 + (row0 + quarter) * pitch + col0;
+#pragma unroll 1
+                        for (int first = quarter; first < rows; first += 32) {
+                            uint32_t x[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int rr = first + 4 * i;      // below 128: rows past the end are read, not stored
+                                x[i] = *reinterpret_cast<const uint32_t *>(box_p + (rr & 127) * 128 +
+                                                                           (((lane >> 2) ^ (rr & 7)) << 4) + (lane & 3) * 4);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const uint32_t next = __shfl_down_sync(0xffffffffu, x[i], 1);
+                                T *to = base_row + i * 4 * pitch;
+                                if (first + 4 * i >= rows)
+                                    continue;
+                                uint16_t *h = reinterpret_cast<uint16_t *>(to);
+                                const bool odd = (reinterpret_cast<uintptr_t>(to) & 2u) != 0;
+                                const int e = 2 * lane + (odd ? 1 : 0);
+                                if (e + 1 < min(cols, 64))
+                                    *reinterpret_cast<uint32_t *>(h + e) = odd ? __funnelshift_r(x[i], next, 16) : x[i];
+                                else if (e < min(cols, 64))
+                                    h[e] = static_cast<uint16_t>(odd ? x[i] >> 16 : x[i]);
+                                if (odd && lane == 0)
+                                    h[0] = static_cast<uint16_t>(x[i]);
+                            }
+                            base_row += 32 * pitch;
+                        }
+                    };
                     auto emit_columns = [&](const float (&v)[64], const void *map, int z, bool tma, bool half, void *dst,
                                             long long at0, long long pitch, int col0, const void *residual) {
                         uint32_t words[32];
-                        if (tma && half) {
+                        if (half && (tma || !residual)) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
                                 words[j] = Type::pack(v[2 * j], v[2 * j + 1]);
-                            emit(words, map, z, col0);
+                            if (tma)
+                                emit(words, map, z, col0);
+                            else
+                                emit_rows_half(words, dst, at0, pitch, col0);
                         } else {
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
