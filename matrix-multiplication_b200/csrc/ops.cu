@@ -208,14 +208,13 @@ bool output_map(const Call &c, CUtensorMap *map, const Matrix &m, bool half)
 struct TileShape {
     int ctas, bm, bn;     // CTAs per tile, D's rows and columns per tile
 };
-constexpr TileShape kTileShapes[] = {{2, 256, 256}, {2, 256, 512}, {1, 128, 128}, {1, 128, 64},
-                                     {1, 128, 16},  {1, 128, 32},  {1, 128, 64},  {1, 128, 128}};
+constexpr TileShape kTileShapes[] = {{2, 256, 256}, {1, 128, 128}, {1, 128, 64}, {1, 128, 16},
+                                     {1, 128, 32},  {1, 128, 64},  {1, 128, 128}};
 
-// Column ranges of a tile that the loss reduces on its own (halves x epilogue warpgroups).
+// Column ranges of a tile that the loss reduces on its own: one per epilogue warpgroup.
 int loss_parts(int tile)
 {
-    const int bn = kTileShapes[tile].bn;
-    return bn > 256 ? 4 : bn >= 128 ? 2 : 1;
+    return kTileShapes[tile].bn >= 128 ? 2 : 1;
 }
 
 bool is_swap(int tile)
@@ -223,34 +222,42 @@ bool is_swap(int tile)
     return tile >= kSwap16;
 }
 
-// Estimated cycles of `tiles` tiles of a kind with K blocks of 128 bytes, K split S ways,
-// whose epilogue reads and writes `bytes_out` bytes per element.  As in the plain product's
-// plan (matmul_b200.cu) a K block costs the most of its MMA time, its operand bytes into
-// one SM at 55 B/cycle, and all running CTAs' bytes out of L2 at 8 KB/cycle; a split adds
-// its exchange.  A pair's tile also costs no less than its epilogue: 5400 cycles per 256
-// columns of BF16 (measured with K = 256).  Between 512-column tiles the MMAs wait for the
-// second half's read, which follows the first half's stores: 5000 cycles for a BF16 output,
-// 18000 more for each BF16 output or residual beside it (cycle stamps at 4096 x 4096 x 14336:
-// 70.6 k cycles a tile of 65.5 k MMA cycles; two 256-column tiles take 76 k).
-double tile_cycles(const Context *ctx, int tile, int splits, double tiles, double k_blocks, int bytes_out)
+// What the choice of a tile knows of a product: sizes, K blocks of 128 bytes, groups, bytes
+// read and written per output element, whether TMA writes the output, and whether the
+// epilogue can take partial sums (K splits) and run transposed.
+struct TileProblem {
+    int64_t m, n, k_blocks, groups = 1;
+    int bytes_out = 2;
+    bool out_tma = true, splittable = false, transposable = false;
+};
+
+// Estimated cycles of a tile kind with K split S ways.  A K block costs the most of its MMA
+// time (2 cycles a column, 140 at least), its operand bytes into one SM at 70 B/cycle and
+// all running CTAs' bytes out of L2 at 9.3 KB/cycle; a tile's epilogue adds the kind's own
+// cycles, more where rows are stored without TMA, and a pair's tile costs no less than 2500
+// cycles per byte of an output element (5050 measured for BF16 with K = 256).  A split adds
+// its exchange.  The constants are fitted to 1170 times of every kind and split over 95
+// BF16 products of 33 to 2048 rows (10 % rms; the kind chosen is 0.3 % slower than the
+// fastest on average, 7 % at worst).
+double tile_cycles(const Context *ctx, int tile, int splits, const TileProblem &q)
 {
+    constexpr double kEpilogue[] = {4400.0, 1100.0, 1140.0, 810.0, 800.0, 1170.0, 1170.0};
+    constexpr double kRowStores[] = {17800.0, 6100.0, 3050.0, 200.0, 400.0, 800.0, 1700.0};
     const TileShape &t = kTileShapes[tile];
-    const bool pair = t.ctas == 2;
-    const double units = pair ? ctx->max_pairs : ctx->sm_count;
+    const bool swap = is_swap(tile);
+    const int64_t side_m = swap ? q.n : q.m, side_n = swap ? q.m : q.n;
+    const double tiles = static_cast<double>((side_m + t.bm - 1) / t.bm * ((side_n + t.bn - 1) / t.bn) * q.groups);
+    const double units = t.ctas == 2 ? ctx->max_pairs : ctx->sm_count;
     const double active = splits > 1 ? tiles * splits : t.ctas * std::min(tiles, units);
-    double rounds = splits > 1 ? 1.0 : std::max(1.0, std::ceil(tiles / units));
+    const double rounds = splits > 1 ? 1.0 : std::max(1.0, std::ceil(tiles / units));
     const double bytes = static_cast<double>(OP_BM + t.bn / t.ctas) * OP_ROW_BYTES;
-    const double k_cycles = std::max({2.0 * t.bn, bytes / 55.0, active * bytes / 8000.0});
-    const double extra = std::max(0.0, bytes_out / 2.0 - 1.0);
-    const double epilogue = t.bn == 512 ? 5000.0 + 18000.0 * extra : pair ? 1000.0 : 4000.0 * t.bn / 256.0;
-    // A short last round of 512-column tiles runs as halves (enqueue).
-    if (t.bn == 512 && tiles - std::floor(tiles / units) * units <= units / 2)
-        rounds = std::floor(tiles / units) + (std::fmod(tiles, units) > 0.0 ? 0.5 : 0.0);
-    double tile_time = std::ceil(k_blocks / splits) * k_cycles + epilogue;
-    if (pair)
-        tile_time = std::max(tile_time, 2700.0 * bytes_out * t.bn / 256.0);
-    return 2000.0 + rounds * tile_time + (pair ? 10000.0 : 0.0) +
-           (splits > 1 ? 1000.0 + static_cast<double>(splits - 1) / splits * OP_BM * t.bn * 4.0 / 8.0 : 0.0);
+    const double k_cycles = std::max({2.0 * t.bn, 140.0, bytes / 70.0, active * bytes / 9300.0});
+    const double epilogue = kEpilogue[tile] + (q.out_tma ? 0.0 : kRowStores[tile]);
+    double tile_time = std::ceil(static_cast<double>(q.k_blocks) / splits) * k_cycles + epilogue;
+    if (t.ctas == 2)
+        tile_time = std::max(tile_time, 2500.0 * q.bytes_out);
+    return rounds * tile_time +
+           (splits > 1 ? 3700.0 + 0.093 * static_cast<double>(splits - 1) / splits * OP_BM * t.bn * 4.0 : 0.0);
 }
 
 struct TileChoice {
@@ -264,23 +271,26 @@ bool can_split(const Context *ctx, int log_splits, int64_t tiles, int64_t k_bloc
     return tiles * splits <= ctx->max_split_ctas[log_splits] && (splits - 1) * per < k_blocks;
 }
 
-// The tile and K split with the fewest estimated cycles for an m x n product (of one of
-// `groups` groups).  Splits are for ungrouped products whose epilogue can take partial sums.
-TileChoice choose_tile(const Context *ctx, int64_t m, int64_t n, int64_t k_blocks, int bytes_out, int64_t groups = 1,
-                       bool splittable = false)
+// The tile kind and K split with the fewest estimated cycles.  Transposed kinds are
+// considered where one wave holds all their tiles: their stores go element by element
+// (2048 x 256 x 45056 with a residual took 1236 us on 128 x 128 tiles transposed, 146 us not).
+TileChoice choose_tile(const Context *ctx, const TileProblem &q)
 {
     TileChoice best{kSingle64, 1};
     double best_cycles = 0.0;
-    for (int tile : {kPair256, kPair512, kSingle128, kSingle64}) {
+    for (int tile = kPair256; tile <= (q.transposable ? kSwap128 : kSingle64); ++tile) {
         const TileShape &t = kTileShapes[tile];
-        if (t.ctas == 2 && (ctx->max_pairs < 1 || m <= OP_BM || (tile == kPair512 && n <= 256)))
+        const bool swap = is_swap(tile);
+        if (t.ctas == 2 && (ctx->max_pairs < 1 || q.m <= OP_BM))
             continue;
-        const int64_t tiles = (m + t.bm - 1) / t.bm * ((n + t.bn - 1) / t.bn) * groups;
-        for (int i = 0; i < (splittable && t.ctas == 1 ? 4 : 1); ++i) {
-            if (i > 0 && !can_split(ctx, i, tiles, k_blocks))
+        const int64_t side_m = swap ? q.n : q.m, side_n = swap ? q.m : q.n;
+        const int64_t tiles = (side_m + t.bm - 1) / t.bm * ((side_n + t.bn - 1) / t.bn) * q.groups;
+        if (swap && tiles > ctx->sm_count)
+            continue;
+        for (int i = 0; i < (q.splittable && t.ctas == 1 ? 4 : 1); ++i) {
+            if (i > 0 && !can_split(ctx, i, tiles, q.k_blocks))
                 continue;
-            const double cycles = tile_cycles(ctx, tile, 1 << i, static_cast<double>(tiles), static_cast<double>(k_blocks),
-                                              bytes_out);
+            const double cycles = tile_cycles(ctx, tile, 1 << i, q);
             if (best_cycles == 0.0 || cycles < best_cycles) {
                 best = {tile, 1 << i};
                 best_cycles = cycles;
@@ -331,8 +341,7 @@ int enqueue(Call &c, Product &q)
     const TileShape &t = kTileShapes[l.tile];
     const bool swap = is_swap(l.tile);
     const bool a_mn = l.layout == kTN, b_mn = l.layout != kNT;
-    const int b_cols = std::min(t.bn, 256) / t.ctas;     // rows of a K-major box of Bop
-    // Every blocked load takes whole columns, OP_BM of Aop or a half's share of Bop.
+    const int b_cols = t.bn / t.ctas;     // Bop columns per CTA
     l.p.a_blocked = whole_blocks(c, swap ? q.b : q.a) ? 1 : 0;
     l.p.b_blocked = whole_blocks(c, q.b) ? 1 : 0;
     bool ok;
@@ -366,17 +375,6 @@ int enqueue(Call &c, Product &q)
     const int64_t per_group = static_cast<int64_t>(p.num_m_blocks) * p.num_n_blocks;
     p.per_raster = divisor(std::min<int64_t>(per_raster, 0x7fffffff));
     p.per_group = divisor(std::min<int64_t>(per_group, 0x7fffffff));
-    // 512 columns: when the last round has few tiles, they run as halves on twice the pairs
-    // (4096 x 4096 x 14336: 448 tiles on 74 pairs, 6.5 rounds in place of 7).
-    p.full_tiles = p.num_tiles;
-    if (l.tile == kPair512 && p.grouping == kUngrouped) {
-        const int rest = p.num_tiles % c.ctx->max_pairs;
-        if (2 * rest <= c.ctx->max_pairs) {
-            p.full_tiles = p.num_tiles - rest;
-            p.num_tiles += rest;
-            tiles = p.num_tiles;
-        }
-    }
     p.status = c.ctx->status;
     p.wait_limit_ns = wait_limit(c.ctx);
     const int64_t units = t.ctas == 2 ? c.ctx->max_pairs : c.ctx->sm_count;
@@ -480,12 +478,13 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     const int bk = OP_ROW_BYTES / e;
     const int64_t k_blocks = (static_cast<int64_t>(k) + bk - 1) / bk;
     const int bytes_out = (out_half ? 2 : 4) * (residual ? 2 : 1) + (preact ? (preact_half ? 2 : 4) : 0);
+    const Matrix mo{out, m, n, n};
+    const bool out_tma = output_tma(mo, out_half ? 2 : 4) && (!residual || aligned16(residual));
     const TileChoice choice = m <= 64 ? choose_few_rows(c.ctx, m, n, k_blocks)
-                                      : choose_tile(c.ctx, m, n, k_blocks, bytes_out, 1, true);
+                                      : choose_tile(c.ctx, {m, n, k_blocks, 1, bytes_out, out_tma, true, true});
     l.tile = choice.tile;
     l.splits = choice.splits;
     l.epilogue = is_swap(choice.tile) ? kEpiStoreT : kEpiStore;
-    const Matrix mo{out, m, n, n};
     if (set_output(c, l, mo, out_half))
         return 1;
     OpParams &p = l.p;
@@ -494,8 +493,7 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     p.activation = activation;
     p.residual = residual;
     p.residual_half = p.out_half;
-    if (residual && !aligned16(residual))
-        p.out_tma = 0;
+    p.out_tma = out_tma ? 1 : 0;
     if (preact) {
         const Matrix mz{preact, m, n, n};
         p.preact = preact;
@@ -620,7 +618,8 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.n = k;
         q.k = n;
         q.launch.layout = kNT;
-        q.set_tile(choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk, da_half ? 2 : 4, 1, true));
+        q.set_tile(choose_tile(c.ctx, {q.m, q.n, (q.k + bk - 1) / bk, 1, da_half ? 2 : 4,
+                                       output_tma(Matrix{da, m, k, k}, da_half ? 2 : 4), true}));
         if (set_output(c, q.launch, Matrix{da, m, k, k}, da_half) || enqueue(c, q))
             return 1;
     }
@@ -632,7 +631,8 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.n = n;
         q.k = m;
         q.launch.layout = kTN;
-        q.set_tile(choose_tile(c.ctx, q.m, q.n, (q.k + bk - 1) / bk, db_half ? 2 : 4, 1, true));
+        q.set_tile(choose_tile(c.ctx, {q.m, q.n, (q.k + bk - 1) / bk, 1, db_half ? 2 : 4,
+                                       output_tma(Matrix{db, k, n, n}, db_half ? 2 : 4), true}));
         if (set_output(c, q.launch, Matrix{db, k, n, n}, db_half) || enqueue(c, q))
             return 1;
     }
@@ -715,7 +715,8 @@ int check_groups(Call &c, int groups, int rows, int k, int n, const void *offset
 
 // Rows per tile follow the mean group: with few rows they take the MMA's N side (16 to
 // 128 wide) and the weight's columns its M side, so that a tile wastes little.
-int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_t n, int64_t k_blocks, int bytes_out)
+int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_t n, int64_t k_blocks, int bytes_out,
+                        bool out_tma)
 {
     const int64_t mean = (rows + groups - 1) / groups;
     if (mean <= 16)
@@ -726,7 +727,7 @@ int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_
         return kSwap64;
     if (mean <= 128)
         return kSwap128;
-    return choose_tile(ctx, mean, n, k_blocks, bytes_out, groups).tile;
+    return choose_tile(ctx, {mean, n, k_blocks, groups, bytes_out, out_tma}).tile;
 }
 
 } // namespace
@@ -753,13 +754,13 @@ extern "C" int matmul_grouped(void *opaque, int precision, const void *a, const 
     const int64_t bk = OP_ROW_BYTES / e;
     Product q;
     OpLaunch &l = q.launch;
-    l.tile = choose_grouped_tile(c.ctx, rows, groups, n, (k + bk - 1) / bk, half ? 2 : 4);
+    const Matrix mo{out, rows, n, n};
+    l.tile = choose_grouped_tile(c.ctx, rows, groups, n, (k + bk - 1) / bk, half ? 2 : 4, output_tma(mo, half ? 2 : 4));
     const bool swap = is_swap(l.tile);
     l.epilogue = swap ? kEpiStoreT : kEpiStore;
     Operand oa, ob;
     oa.plan(c, a, rows, k);
     ob.plan(c, b, k, n, groups);
-    const Matrix mo{out, rows, n, n};
     GroupPlan plan;
     plan.plan(c, groups, rows, swap ? kTileShapes[l.tile].bn : kTileShapes[l.tile].bm,
               !swap && output_tma(mo, half ? 2 : 4) ? 1 : 0);
@@ -808,14 +809,17 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
         ob.plan(c, b, k, n, groups);
         const int64_t mean = (rows + groups - 1) / groups;
         qa.launch.layout = kNT;
-        qa.launch.tile = choose_tile(c.ctx, mean, k, (n + bk - 1) / bk, da_half ? 2 : 4, groups).tile;
+        qa.launch.tile = choose_tile(c.ctx, {mean, k, (n + bk - 1) / bk, groups, da_half ? 2 : 4,
+                                           output_tma(ma, da_half ? 2 : 4)}).tile;
         rows_plan.plan(c, groups, rows, kTileShapes[qa.launch.tile].bm, output_tma(ma, da_half ? 2 : 4) ? 1 : 0);
     }
     if (db) {
         oa.plan(c, a, rows, k);
         const int64_t mean = (rows + groups - 1) / groups;
         qb.launch.layout = kTN;
-        qb.launch.tile = choose_tile(c.ctx, k, n, (mean + bk - 1) / bk, db_half ? 2 : 4, groups).tile;
+        qb.launch.tile = choose_tile(c.ctx, {k, n, (mean + bk - 1) / bk, groups, db_half ? 2 : 4,
+                                           output_tma(Matrix{db, k, n, n, groups, static_cast<int64_t>(k) * n},
+                                                      db_half ? 2 : 4)}).tile;
         k_plan.plan(c, groups, rows, 0, 2);
     }
     if (c.allocate() || prepare_operands(c, {&od, &ob, &oa}))
@@ -841,7 +845,7 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
         qb.k = rows;
         const TileShape &t = kTileShapes[qb.launch.tile];
         if (!operand_map(c, &map0, qb.a, true, OP_BM) ||
-            !operand_map(c, &map1, qb.b, true, std::min(t.bn, 256) / t.ctas)) {
+            !operand_map(c, &map1, qb.b, true, t.bn / t.ctas)) {
             cudaGetLastError();
             return c.failed("cuTensorMapEncodeTiled rejected an operand");
         }
@@ -897,7 +901,7 @@ extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hid
     Product q;
     OpLaunch &l = q.launch;
     l.epilogue = kEpiLse;
-    l.tile = choose_tile(c.ctx, m, v, (k + bk - 1) / bk, 2).tile;
+    l.tile = choose_tile(c.ctx, {m, v, (k + bk - 1) / bk}).tile;
     // One (maximum, sum) per row and column range of a tile.
     const int tiles = (v + kTileShapes[l.tile].bn - 1) / kTileShapes[l.tile].bn * loss_parts(l.tile);
     Operand oh, ow;
@@ -985,7 +989,7 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = cols;
             q.k = k;
             q.launch.epilogue = kEpiSoftmaxGrad;
-            q.launch.tile = choose_tile(c.ctx, m, cols, (k + bk - 1) / bk, e).tile;
+            q.launch.tile = choose_tile(c.ctx, {m, cols, (k + bk - 1) / bk, 1, e}).tile;
             OpParams &p = q.launch.p;
             p.labels = labels;
             p.labels64 = labels64;
@@ -1006,9 +1010,10 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.k = cols;
             q.launch.layout = kNT;
             const bool last = piece == pieces - 1;
-            q.set_tile(choose_tile(c.ctx, m, k, (cols + bk - 1) / bk, (piece > 0 ? 4 : 0) + (last && dh_half ? 2 : 4), 1,
-                                   true));
-            if (set_output(c, q.launch, last ? dh : sum, last && dh_half))
+            const Matrix &to = last ? dh : sum;
+            q.set_tile(choose_tile(c.ctx, {m, k, (cols + bk - 1) / bk, 1, (piece > 0 ? 4 : 0) + (last && dh_half ? 2 : 4),
+                                           output_tma(to, last && dh_half ? 2 : 4), true}));
+            if (set_output(c, q.launch, to, last && dh_half))
                 return 1;
             if (piece > 0) {
                 q.launch.p.residual = sum.ptr;
@@ -1027,8 +1032,9 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = cols;
             q.k = m;
             q.launch.layout = kTN;
-            q.set_tile(choose_tile(c.ctx, k, cols, (m + bk - 1) / bk, dw_half ? 2 : 4, 1, true));
             const Matrix dw{static_cast<uint8_t *>(dweight) + v0 * (dw_half ? 2 : 4), k, cols, v};
+            q.set_tile(choose_tile(c.ctx, {k, cols, (m + bk - 1) / bk, 1, dw_half ? 2 : 4,
+                                           output_tma(dw, dw_half ? 2 : 4), true}));
             if (set_output(c, q.launch, dw, dw_half) || enqueue(c, q))
                 return 1;
         }

@@ -13,11 +13,9 @@ namespace b200 {
 // How a product's operands are stored: A.B, A.B^T, A^T.B of row-major matrices.
 enum OpLayout : int { kNN = 0, kNT = 1, kTN = 2 };
 
-// Tiles: a CTA pair's 256 x 256 or 256 x 512, one CTA's 128 x 128 or 128 x 64, or,
-// transposed (few rows), 128 columns x 16 / 32 / 64 / 128 rows.
-enum OpTileKind : int {
-    kPair256 = 0, kPair512 = 1, kSingle128 = 2, kSingle64 = 3, kSwap16 = 4, kSwap32 = 5, kSwap64 = 6, kSwap128 = 7
-};
+// Tiles: a CTA pair's 256 x 256, one CTA's 128 x 128 or 128 x 64, or, transposed, 128
+// columns x 16 / 32 / 64 / 128 rows.
+enum OpTileKind : int { kPair256 = 0, kSingle128 = 1, kSingle64 = 2, kSwap16 = 3, kSwap32 = 4, kSwap64 = 5, kSwap128 = 6 };
 
 struct OpLaunch {
     CUtensorMap map_a{}, map_b{}, map_c{}, map_z{};

@@ -23,7 +23,6 @@ struct OpInstances {
     {
         switch (tile) {
         case kPair256: return with<2, 256, A_MN, B_MN, EPI>(f);
-        case kPair512: return with<2, 512, A_MN, B_MN, EPI>(f);
         case kSingle128: return with<1, 128, A_MN, B_MN, EPI>(f);
         case kSingle64: return with<1, 64, A_MN, B_MN, EPI>(f);
         }

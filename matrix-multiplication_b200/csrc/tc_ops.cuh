@@ -52,28 +52,27 @@ constexpr int OP_A_STAGE = OP_BM * OP_ROW_BYTES;
 constexpr int OP_BOX = 128 * 128;             // epilogue box: 128 rows x 128 bytes
 constexpr int OP_BAR_BYTES = 512;
 
-// Geometry of a tile of BN N columns on one CTA or a pair.  A 512-column tile is two
-// halves of 256 that share one accumulator set, freed half by half (tc2_gemm.cuh); the
-// others have two accumulators.  Tiles of 128 columns and more have two epilogue
-// warpgroups, each with half of the columns: one warpgroup needs longer for an
-// activation and two outputs than the MMAs of a 4096-deep 256 x 256 tile (4096 x 4096 x
-// 14336 BF16 with gelu, bias and pre-activation: 609 us with one, 496 us with two).
+// Geometry of a tile of BN N columns on one CTA or a pair, with two accumulators.  Tiles
+// of 128 columns and more have two epilogue warpgroups, each with half of the columns:
+// one warpgroup needs longer for an activation and two outputs than the MMAs of a
+// 4096-deep 256 x 256 tile (4096 x 4096 x 14336 BF16 with gelu, bias and pre-activation:
+// 609 us with one, 496 us with two).  A 256 x 512 pair tile (one accumulator, freed half
+// by half, as in tc2_gemm.cuh) was built and taken out: 311 us against 323 us at 4096 x
+// 4096 x 14336 BF16, 695 against 714 us at 8192^3, ahead by 1 % at most where its count
+// of tiles fits the pairs better.
 template <int CTAS, int BN>
 struct OpTile {
-    static constexpr int kParts = BN > 256 ? 2 : 1;            // 256-column halves
-    static constexpr int kPartCols = BN / kParts;
-    static constexpr int kAccs = BN > 256 ? 1 : 2;
     static constexpr int kBCols = BN / CTAS;                   // N columns staged per CTA
     static constexpr int kBStage = kBCols * OP_ROW_BYTES;
-    static constexpr int kStages = kBCols >= 256 ? 4 : kBCols >= 128 ? 6 : 8;
+    static constexpr int kStages = kBCols >= 128 ? 6 : 8;
     static constexpr int kGroups = BN >= 128 ? 2 : 1;          // epilogue warpgroups
     static constexpr int kFirstEpi = kGroups == 2 ? 4 : 2;     // first epilogue warp (after TMA, MMA, two idle ones)
     static constexpr int kThreads = 32 * (kFirstEpi + 4 * kGroups);
     static constexpr int kBoxes = 3 - kGroups;                 // boxes per epilogue warpgroup: two in all
     static constexpr int kEpiBytes = kBoxes * kGroups * OP_BOX;
-    static constexpr int kBiasBytes = kPartCols * 4 < 256 ? 256 : kPartCols * 4;
+    static constexpr int kBiasBytes = BN * 4 < 256 ? 256 : BN * 4;
     static constexpr int kSmem = 1024 + kStages * (OP_A_STAGE + kBStage) + kEpiBytes + OP_BAR_BYTES + kBiasBytes;
-    static constexpr uint32_t kTmemColumns = kAccs * BN < 32 ? 32 : kAccs * BN;
+    static constexpr uint32_t kTmemColumns = 2 * BN < 32 ? 32 : 2 * BN;   // two accumulators
     static_assert(kSmem <= 227 * 1024, "tile exceeds shared memory");
 };
 
@@ -113,7 +112,6 @@ struct OpParams {
     int m, n;                 // rows and columns of the output (of one group in ragged-K mode)
     int num_m_blocks, num_n_blocks, num_k_blocks;   // M- and N-side tiles of D, K blocks
     int num_tiles;
-    int full_tiles;           // 512 columns: tiles from here on are halves of a tile (two indices a tile)
     int log_raster;           // log2 of the M-side tiles per raster group
     OpDivisor per_raster;     // raster x N-side tiles (transposed epilogue: M-side tiles)
     OpDivisor per_group;      // ragged-K mode: tiles of one group
@@ -347,23 +345,14 @@ __device__ __forceinline__ int op_label(const OpParams &p, int row)
 // the end of the output rows it may write.
 struct OpWhere {
     int m0, n0, group, nkb, k0, row_end;
-    int parts;         // 256-column halves
-    int loss_block;    // index of the first half among all column tiles' halves
+    int n_block;
 };
 
 template <int CTAS, int BN, bool SWAP>
 __device__ __forceinline__ OpWhere op_where(int tile, int row_tile_count, int bk, const OpParams &p)
 {
     constexpr int kBM = OP_BM * CTAS;
-    constexpr bool kHalves = BN > 256;
     OpWhere w;
-    int half = 0;
-    w.parts = kHalves ? 2 : 1;
-    if (kHalves && tile >= p.full_tiles) {
-        half = (tile - p.full_tiles) & 1;
-        tile = p.full_tiles + ((tile - p.full_tiles) >> 1);
-        w.parts = 1;
-    }
     int local = tile;
     w.group = 0;
     w.k0 = 0;
@@ -396,8 +385,8 @@ __device__ __forceinline__ OpWhere op_where(int tile, int row_tile_count, int bk
         }
     }
     w.m0 = mb * kBM;
-    w.n0 = nb * BN + half * 256;
-    w.loss_block = nb * (kHalves ? 2 : 1) + half;
+    w.n0 = nb * BN;
+    w.n_block = nb;
     if (p.grouping == kGroupedRows) {
         const OpRowTile t = p.row_tiles[SWAP ? nb : mb];
         w.group = t.group;
@@ -429,23 +418,16 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     constexpr int kBStage = Tile::kBStage;
     constexpr int kBCols = Tile::kBCols;
     constexpr int kGroups = Tile::kGroups;
-    constexpr int kParts = Tile::kParts;
-    constexpr int kAccs = Tile::kAccs;
     constexpr int kBoxes = Tile::kBoxes;
-    constexpr int kHalfCols = kBCols / kParts;            // N columns staged per CTA and half
-    constexpr int kMmaN = Tile::kPartCols;
-    constexpr int kDefer = 2;     // 512 columns: K blocks at each end of a tile run on one half first
-    static_assert(kParts == 1 || kDefer < kStages, "deferred K blocks must leave the producer a stage");
     constexpr bool kSplittable = CTAS == 1 && (EPI == kEpiStore || EPI == kEpiStoreT);
-    constexpr int kGroupCols = Tile::kPartCols / kGroups; // D columns per epilogue warpgroup (and half)
+    constexpr int kGroupCols = BN / kGroups;              // D columns per epilogue warpgroup
     constexpr uint32_t kStageTx = static_cast<uint32_t>(CTAS) * (OP_A_STAGE + kBStage);
-    constexpr uint32_t kHalfStageTx = static_cast<uint32_t>(CTAS) * (OP_A_STAGE + kBStage / 2);
     // FP32 accumulator, formats, A MN-major (bit 15), B MN-major (bit 16), N >> 3, M >> 4.
     constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(FMT) << 7) | (static_cast<uint32_t>(FMT) << 10) |
                                 ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
-                                (static_cast<uint32_t>(kMmaN >> 3) << 17) |
+                                (static_cast<uint32_t>(BN >> 3) << 17) |
                                 (static_cast<uint32_t>((OP_BM * CTAS) >> 4) << 24);
-    static_assert(!B_MN || kHalfCols % kBox == 0, "whole MN-major boxes");
+    static_assert(!B_MN || kBCols % kBox == 0, "whole MN-major boxes");
     static_assert(!kPair || !kSwap, "the transposed epilogue runs on single CTAs");
 
     extern __shared__ uint8_t smem_raw[];
@@ -588,16 +570,8 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const int tile_end = in_turn ? num_tiles : p.unit_first[unit + 1];
     const int tile_step = in_turn ? units : 1;
 
-    // The 512-column tile's epilogue holds 128 columns of its row in registers: the four
-    // other warps give theirs up (128 x 56 + 256 x 224 = 384 x 168, the launch's total).
-    // Each role sets its own count, so that the compiler sees the limit it works under.
-    auto give_registers = [&]() {
-        if constexpr (kParts == 2)
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    };
     if (warp == 0) {
         // ------------------------------------------------------------ producer
-        give_registers();
         if (op_elect_one()) {
             int stage = 0;
             uint32_t phase = 0, filled = 0, fill_parity = 0;
@@ -620,7 +594,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     (kSwap ? za : zb) = w.group;
                 }
                 const int am = w.m0 + static_cast<int>(rank) * OP_BM;
-                const int bn = w.n0 + static_cast<int>(rank) * kHalfCols;
+                const int bn = w.n0 + static_cast<int>(rank) * kBCols;
                 for (int kb = kb_begin; kb < kb_end(w.nkb); ++kb) {
                     // In a pair this wait keeps the fixed limit: both CTAs then stop at the
                     // same stage and the leader's drain covers every copy of either.
@@ -631,7 +605,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                     const uint32_t fb = leader_full0 + 8u * stage;
                     if (leader)
-                        mbar_arrive_expect_tx(full_bar(stage), kParts == 2 && w.parts == 1 ? kHalfStageTx : kStageTx);
+                        mbar_arrive_expect_tx(full_bar(stage), kStageTx);
                     const int k = w.k0 + kb * kBK;
                     auto load = [&](uint32_t dst, const void *map, int x, int y, int block, int z) {
                         if constexpr (kPair)
@@ -653,16 +627,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         load_mn(sa, ma, p.a_blocked != 0, am, OP_BM, za);
                     else
                         load(sa, ma, k, am, 0, za);
-#pragma unroll
-                    for (int h = 0; h < kParts; ++h) {
-                        if (h == w.parts)
-                            break;
-                        const uint32_t sbh = sb + h * kHalfCols * OP_ROW_BYTES;
-                        if constexpr (B_MN)
-                            load_mn(sbh, mb, p.b_blocked != 0, bn + h * 256, kHalfCols, zb);
-                        else
-                            load(sbh, mb, k, bn + h * 256, 0, zb);
-                    }
+                    if constexpr (B_MN)
+                        load_mn(sb, mb, p.b_blocked != 0, bn, kBCols, zb);
+                    else
+                        load(sb, mb, k, bn, 0, zb);
                     filled |= 1u << stage;
                     fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
                     if (++stage == kStages) {
@@ -681,7 +649,6 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer (a pair's leader)
-        give_registers();
         if (leader && op_elect_one()) {
             int stage = 0;
             uint32_t phase = 0;
@@ -703,40 +670,18 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     mbar_arrive(bar);
                 }
             };
-            // The MMAs of the K block in stage s for half h of the accumulator.
-            auto issue_half = [&](uint32_t d_tmem, int s, int h, bool first) {
-                const uint64_t a_desc = a_desc0 + static_cast<uint64_t>(s) * (OP_A_STAGE >> 4);
-                const uint64_t b_desc = b_desc0 + static_cast<uint64_t>(s) * (kBStage >> 4) +
-                                        static_cast<uint64_t>(h) * ((kHalfCols * OP_ROW_BYTES) >> 4);
-#pragma unroll
-                for (int kk = 0; kk < kMmasPerStage; ++kk) {
-                    const uint32_t accumulate = !first || kk != 0 ? 1u : 0u;
-                    const uint32_t d = d_tmem + static_cast<uint32_t>(h * 256);
-                    if constexpr (kPair)
-                        tc_mma_pair<kTF32>(d, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
-                    else
-                        tc_mma<kTF32>(d, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
-                }
-            };
             int acc = 0;
             uint32_t acc_phase = 0;
             bool ok = true;
-            auto wait_free = [&](int i) {      // the epilogue has read accumulator (half) i
-                if (!mbar_wait(acce_bar(i), acc_phase ^ 1u, p.wait_limit_ns)) {
-                    atomicOr(p.status, kOpMmaTimeout);
-                    ok = false;
-                }
-                tc_fence_after();
-                return ok;
-            };
             for (int tile = tile_first; ok && tile < tile_end; tile += tile_step) {
                 const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
-                if (!wait_free(acc))
+                if (!mbar_wait(acce_bar(acc), acc_phase ^ 1u, p.wait_limit_ns)) {
+                    atomicOr(p.status, kOpMmaTimeout);
                     break;
+                }
+                tc_fence_after();
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
                 const int nkb = kb_end(w.nkb);
-                bool upper_live = false;              // 512 columns: the epilogue has read the upper half
-                int pending = 0, pending_stage = 0;   // 512 columns: K blocks whose upper-half MMAs wait
                 for (int kb = kb_begin; kb < nkb; ++kb) {
                     if (!mbar_wait(full_bar(stage), phase, p.wait_limit_ns)) {
                         atomicOr(p.status, kOpMmaTimeout);
@@ -744,38 +689,17 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         break;
                     }
                     tc_fence_after();
-                    issue_half(d_tmem, stage, 0, kb == kb_begin);
-                    if (kParts == 1 || w.parts == 1) {
-                        commit(empty_bar(stage));
-                    } else {
-                        // The lower half runs ahead by kDefer K blocks at either end of the tile: its
-                        // epilogue overlaps the upper half's last MMAs, and the upper half's epilogue
-                        // of the tile before overlaps this tile's first ones.
-                        if (kb == nkb - 1)
-                            commit(accf_bar(0));
-                        if (upper_live && kb < nkb - kDefer) {
-                            issue_half(d_tmem, stage, 1, false);
-                            commit(empty_bar(stage));
-                        } else {
-                            if (pending++ == 0)
-                                pending_stage = stage;
-                            if (kb == nkb - 1 || (!upper_live && kb == kDefer - 1)) {
-                                if (!upper_live) {
-                                    if (!wait_free(1))
-                                        break;
-                                    upper_live = true;
-                                }
-                                int s = pending_stage;
-                                for (int j = kb - pending + 1; j <= kb; ++j) {
-                                    issue_half(d_tmem, s, 1, j == 0);
-                                    commit(empty_bar(s));
-                                    if (++s == kStages)
-                                        s = 0;
-                                }
-                                pending = 0;
-                            }
-                        }
+                    const uint64_t a_desc = a_desc0 + static_cast<uint64_t>(stage) * (OP_A_STAGE >> 4);
+                    const uint64_t b_desc = b_desc0 + static_cast<uint64_t>(stage) * (kBStage >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < kMmasPerStage; ++kk) {
+                        const uint32_t accumulate = kb != kb_begin || kk != 0 ? 1u : 0u;
+                        if constexpr (kPair)
+                            tc_mma_pair<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
+                        else
+                            tc_mma<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
                     }
+                    commit(empty_bar(stage));
                     if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
@@ -784,16 +708,11 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 if (!ok)
                     break;
                 if (nkb > kb_begin) {
-                    commit(accf_bar(kParts == 1 ? acc : w.parts - 1));
+                    commit(accf_bar(acc));
                 } else {          // no K block (an empty group or split): a zero sum, nothing to wait for
-                    if (kParts == 2 && w.parts == 2) {
-                        if (!wait_free(1))
-                            break;
-                        arrive_both(accf_bar(0));
-                    }
-                    arrive_both(accf_bar(kParts == 1 ? acc : w.parts - 1));
+                    arrive_both(accf_bar(acc));
                 }
-                if (++acc == kAccs) {
+                if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1u;
                 }
@@ -809,14 +728,15 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         __syncwarp();
     } else if (warp >= Tile::kFirstEpi) {
         // ------------------------------------------------------------ epilogue
-        if constexpr (kParts == 2)
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3;                 // TMEM lanes 32 * quarter .. +31
         const int r = quarter * 32 + lane;
         const int group = (warp - Tile::kFirstEpi) >> 2;   // epilogue warpgroup: D columns group * kGroupCols ..
         const int gcol = group * kGroupCols;
         const int gthread = static_cast<int>(threadIdx.x) - 32 * Tile::kFirstEpi - 128 * group;
-        const bool issuer = gthread == 0;
+        // One thread of the warpgroup issues and waits for its TMA stores: the same lane at
+        // every election (elect.sync is deterministic for a mask).
+        const bool issuer_warp = gthread < 32;
+        const bool issuer = issuer_warp && op_elect_one();
         const uint32_t s_box = s_epi + group * kBoxes * OP_BOX;
         auto epilogue_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
         // 1 only if every thread of the warpgroup passes 1.
@@ -836,10 +756,9 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         uint32_t acc_phase = 0, stores = 0;
         int failed_tile = -1;
         int acquired = -1;
-        // Releases the accumulator (half) after this warp's last read of it.
-        int part = 0;
+        // Releases the accumulator after this warp's last read of it.
         auto release = [&]() {
-            const uint32_t bar = acce_bar(kAccs == 2 ? acc : part);
+            const uint32_t bar = acce_bar(acc);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -852,384 +771,357 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         for (int tile = tile_first; tile < tile_end; tile += tile_step) {
             const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
             const int row0 = w.m0 + static_cast<int>(rank) * OP_BM;     // D's first row in this CTA
-            for (part = 0; part < w.parts; ++part) {
-                const int n0 = w.n0 + part * 256;     // this half's first column
-                const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                       static_cast<uint32_t>(acc * BN + part * 256 + gcol);
-                if constexpr (EPI == kEpiStore) {
-                    if (p.bias) {       // this part's bias, read once into shared memory
-                        epilogue_sync();
-                        for (int c = gcol + gthread; c < gcol + kGroupCols; c += 128) {
-                            const int col = n0 + c;
-                            float b = 0.0f;
-                            if (col < p.n)
-                                b = load_bias(col);
-                            bias_s[c] = b;
-                        }
-                        epilogue_sync();
+            const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                   static_cast<uint32_t>(acc * BN + gcol);
+            if constexpr (EPI == kEpiStore) {
+                if (p.bias) {       // the tile's bias, read once into shared memory
+                    epilogue_sync();
+                    for (int c = gcol + gthread; c < gcol + kGroupCols; c += 128) {
+                        const int col = w.n0 + c;
+                        float b = 0.0f;
+                        if (col < p.n)
+                            b = load_bias(col);
+                        bias_s[c] = b;
+                    }
+                    epilogue_sync();
+                }
+            }
+            // Per-row values of the loss epilogues.
+            int label = -1;
+            float row_lse = 0.0f, row_grad = 0.0f;
+            if constexpr (EPI == kEpiLse || EPI == kEpiSoftmaxGrad) {
+                if (row0 + r < p.m) {
+                    label = op_label(p, row0 + r);
+                    if constexpr (EPI == kEpiSoftmaxGrad) {
+                        row_lse = p.lse[row0 + r];
+                        row_grad = p.grad[row0 + r];
                     }
                 }
-                // Per-row values of the loss epilogues.
-                int label = -1;
-                float row_lse = 0.0f, row_grad = 0.0f;
-                if constexpr (EPI == kEpiLse || EPI == kEpiSoftmaxGrad) {
-                    if (row0 + r < p.m) {
-                        label = op_label(p, row0 + r);
-                        if constexpr (EPI == kEpiSoftmaxGrad) {
-                            row_lse = p.lse[row0 + r];
-                            row_grad = p.grad[row0 + r];
-                        }
-                    }
+            }
+            int ok = 1;
+            if (issuer)       // one thread polls, the others wait at the barrier
+                ok = mbar_wait(accf_bar(acc), acc_phase, p.wait_limit_ns) ? 1 : 0;
+            ok = epilogue_all(ok);
+            if (!ok) {
+                if (issuer) {
+                    atomicOr(p.status, kOpEpilogueTimeout);
+                    *fail_flag_ptr = 1u;
                 }
-                int ok = 1;
-                if (issuer)       // one thread polls, the others wait at the barrier
-                    ok = mbar_wait(accf_bar(kAccs == 2 ? acc : part), acc_phase, p.wait_limit_ns) ? 1 : 0;
-                ok = epilogue_all(ok);
-                if (!ok) {
-                    if (issuer) {
-                        atomicOr(p.status, kOpEpilogueTimeout);
-                        *fail_flag_ptr = 1u;
-                    }
-                    failed_tile = tile;
-                    break;
-                }
-                tc_fence_after();
-                if (splits > 1)
-                    break;     // one tile; its partial sums are exchanged below
+                failed_tile = tile;
+                break;
+            }
+            tc_fence_after();
+            if (splits > 1)
+                break;     // one tile; its partial sums are exchanged below
 
-                if constexpr (EPI == kEpiStore || EPI == kEpiSoftmaxGrad) {
-                    const void *mc = &map_c;
-                    if (p.grouping == kGroupedRows && p.out_tma && row0 + OP_BM > w.row_end && row0 < w.row_end) {
-                        // Rows of the next group in this tile: the group's own map clips them.
-                        mc = p.group_maps + w.group;
-                        if (issuer && acquired != w.group) {
-                            tensormap_acquire(mc);
-                            acquired = w.group;
+            if constexpr (EPI == kEpiStore || EPI == kEpiSoftmaxGrad) {
+                const void *mc = &map_c;
+                if (p.grouping == kGroupedRows && p.out_tma && row0 + OP_BM > w.row_end && row0 < w.row_end) {
+                    // Rows of the next group in this tile: the group's own map clips them.
+                    mc = p.group_maps + w.group;
+                    if (issuer && acquired != w.group) {
+                        tensormap_acquire(mc);
+                        acquired = w.group;
+                    }
+                }
+                const int zc = p.grouping == kGroupedK ? w.group : 0;
+                // Puts 128 bytes of this thread's row into a box of 128 rows.
+                auto fill = [&](uint32_t box, const uint32_t (&words)[32]) {
+                    const uint32_t row_addr = box + r * 128;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        st_shared_v4(row_addr + ((j ^ (r & 7)) << 4), words[4 * j], words[4 * j + 1], words[4 * j + 2],
+                                     words[4 * j + 3]);
+                };
+                // A box of 32 FP32 or 64 16-bit columns, stored by TMA.
+                auto emit = [&](const uint32_t (&words)[32], const void *map, int z, int col0) {
+                    const uint32_t box = s_box + stores % kBoxes * OP_BOX;
+                    if (issuer)
+                        bulk_wait_group_read<kBoxes - 1>();      // the store that last read this box
+                    epilogue_sync();
+                    fill(box, words);
+                    fence_proxy_async_shared();
+                    epilogue_sync();
+                    __syncwarp();
+                    if (issuer_warp && op_elect_one()) {
+                        tma_store_3d(map, box, col0, row0, z);
+                        bulk_commit_group();
+                    }
+                    __syncwarp();
+                    ++stores;
+                };
+                // A box of 32 FP32 columns written out row by row (lane = column) where TMA cannot
+                // write, in either format; the residual is added on the way, coalesced.
+                auto emit_rows = [&](const uint32_t (&words)[32], bool half, void *dst, long long at0, long long pitch,
+                                     int col0, const void *residual) {
+                    const uint32_t box = s_box + stores % kBoxes * OP_BOX;
+                    if (issuer) {
+                        bulk_wait_group_read<kBoxes - 1>();
+                        bulk_commit_group();            // an empty group: one per box, whoever writes it out
+                    }
+                    epilogue_sync();
+                    fill(box, words);
+                    epilogue_sync();
+                    ++stores;
+                    const uint8_t *box_p = smem_raw + (box - raw);
+                    const int rows = min(OP_BM, w.row_end - row0);
+                    if (col0 + lane >= p.n)
+                        return;
+                    const long long at = at0 + row0 * pitch + col0 + lane;
+#pragma unroll 1
+                    for (int first = quarter; first < rows; first += 32) {
+                        float x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int rr = first + 4 * i;
+                            if (rr < rows) {
+                                x[i] = *reinterpret_cast<const float *>(box_p + rr * 128 + (((lane >> 2) ^ (rr & 7)) << 4) +
+                                                                        (lane & 3) * 4);
+                                if (residual)
+                                    x[i] += p.residual_half ? Type::to(static_cast<const T *>(residual)[at + rr * pitch])
+                                                            : static_cast<const float *>(residual)[at + rr * pitch];
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int rr = first + 4 * i;
+                            if (rr < rows) {
+                                if (half)
+                                    static_cast<T *>(dst)[at + rr * pitch] = Type::from(x[i]);
+                                else
+                                    static_cast<float *>(dst)[at + rr * pitch] = x[i];
+                            }
                         }
                     }
-                    const int zc = p.grouping == kGroupedK ? w.group : 0;
-                    // Puts 128 bytes of this thread's row into a box of 128 rows.
-                    auto fill = [&](uint32_t box, const uint32_t (&words)[32]) {
-                        const uint32_t row_addr = box + r * 128;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            st_shared_v4(row_addr + ((j ^ (r & 7)) << 4), words[4 * j], words[4 * j + 1], words[4 * j + 2],
-                                         words[4 * j + 3]);
-                    };
-                    // A box of 32 FP32 or 64 16-bit columns, stored by TMA.
-                    auto emit = [&](const uint32_t (&words)[32], const void *map, int z, int col0) {
-                        const uint32_t box = s_box + stores % kBoxes * OP_BOX;
-                        if (issuer)
-                            bulk_wait_group_read<kBoxes - 1>();      // the store that last read this box
-                        epilogue_sync();
-                        fill(box, words);
-                        fence_proxy_async_shared();
-                        epilogue_sync();
-                        if (issuer) {
-                            tma_store_3d(map, box, col0, row0, z);
-                            bulk_commit_group();
-                        }
-                        ++stores;
-                    };
-                    // A box of 32 FP32 columns written out row by row (lane = column) where TMA cannot
-                    // write, in either format; the residual is added on the way, coalesced.
-                    auto emit_rows = [&](const uint32_t (&words)[32], bool half, void *dst, long long at0, long long pitch,
-                                         int col0, const void *residual) {
-                        const uint32_t box = s_box + stores % kBoxes * OP_BOX;
-                        if (issuer) {
-                            bulk_wait_group_read<kBoxes - 1>();
-                            bulk_commit_group();            // an empty group: one per box, whoever writes it out
-                        }
-                        epilogue_sync();
-                        fill(box, words);
-                        epilogue_sync();
-                        ++stores;
-                        const uint8_t *box_p = smem_raw + (box - raw);
-                        const int rows = min(OP_BM, w.row_end - row0);
-                        if (col0 + lane >= p.n)
-                            return;
-                        const long long at = at0 + row0 * pitch + col0 + lane;
+                };
+                // The same for a box of 64 16-bit columns: a lane's two elements go out as one word
+                // where the row starts on 4 bytes; where it starts on 2, words are shifted by one
+                // element with the neighbour's and the two ends go out alone.
+                auto emit_rows_half = [&](const uint32_t (&words)[32], void *dst, long long at0, long long pitch,
+                                          int col0) {
+                    const uint32_t box = s_box + stores % kBoxes * OP_BOX;
+                    if (issuer) {
+                        bulk_wait_group_read<kBoxes - 1>();
+                        bulk_commit_group();
+                    }
+                    epilogue_sync();
+                    fill(box, words);
+                    epilogue_sync();
+                    ++stores;
+                    const uint8_t *box_p = smem_raw + (box - raw);
+                    const int rows = min(OP_BM, w.row_end - row0), cols = p.n - col0;
+                    T *base_row = static_cast<T *>(dst) + at0 + (row0 + quarter) * pitch + col0;
 #pragma unroll 1
-                        for (int first = quarter; first < rows; first += 32) {
-                            float x[8];
+                    for (int first = quarter; first < rows; first += 32) {
+                        uint32_t x[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const int rr = first + 4 * i;
-                                if (rr < rows) {
-                                    x[i] = *reinterpret_cast<const float *>(box_p + rr * 128 + (((lane >> 2) ^ (rr & 7)) << 4) +
-                                                                            (lane & 3) * 4);
-                                    if (residual)
-                                        x[i] += p.residual_half ? Type::to(static_cast<const T *>(residual)[at + rr * pitch])
-                                                                : static_cast<const float *>(residual)[at + rr * pitch];
-                                }
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const int rr = first + 4 * i;
-                                if (rr < rows) {
-                                    if (half)
-                                        static_cast<T *>(dst)[at + rr * pitch] = Type::from(x[i]);
-                                    else
-                                        static_cast<float *>(dst)[at + rr * pitch] = x[i];
-                                }
-                            }
+                        for (int i = 0; i < 8; ++i) {
+                            const int rr = first + 4 * i;      // below 128: rows past the end are read, not stored
+                            x[i] = *reinterpret_cast<const uint32_t *>(box_p + (rr & 127) * 128 +
+                                                                       (((lane >> 2) ^ (rr & 7)) << 4) + (lane & 3) * 4);
                         }
-                    };
-                    // The same for a box of 64 16-bit columns: a lane's two elements go out as one word
-                    // where the row starts on 4 bytes; where it starts on 2, words are shifted by one
-                    // element with the neighbour's and the two ends go out alone.
-                    auto emit_rows_half = [&](const uint32_t (&words)[32], void *dst, long long at0, long long pitch,
-                                              int col0) {
-                        const uint32_t box = s_box + stores % kBoxes * OP_BOX;
-                        if (issuer) {
-                            bulk_wait_group_read<kBoxes - 1>();
-                            bulk_commit_group();
-                        }
-                        epilogue_sync();
-                        fill(box, words);
-                        epilogue_sync();
-                        ++stores;
-                        const uint8_t *box_p = smem_raw + (box - raw);
-                        const int rows = min(OP_BM, w.row_end - row0), cols = p.n - col0;
-                        T *base_row = static_cast<T *>(dst) + at0 + (row0 + quarter) * pitch + col0;
-#pragma unroll 1
-                        for (int first = quarter; first < rows; first += 32) {
-                            uint32_t x[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const int rr = first + 4 * i;      // below 128: rows past the end are read, not stored
-                                x[i] = *reinterpret_cast<const uint32_t *>(box_p + (rr & 127) * 128 +
-                                                                           (((lane >> 2) ^ (rr & 7)) << 4) + (lane & 3) * 4);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const uint32_t next = __shfl_down_sync(0xffffffffu, x[i], 1);
-                                T *to = base_row + i * 4 * pitch;
-                                if (first + 4 * i >= rows)
-                                    continue;
-                                uint16_t *h = reinterpret_cast<uint16_t *>(to);
-                                const bool odd = (reinterpret_cast<uintptr_t>(to) & 2u) != 0;
-                                const int e = 2 * lane + (odd ? 1 : 0);
-                                if (e + 1 < min(cols, 64))
-                                    *reinterpret_cast<uint32_t *>(h + e) = odd ? __funnelshift_r(x[i], next, 16) : x[i];
-                                else if (e < min(cols, 64))
-                                    h[e] = static_cast<uint16_t>(odd ? x[i] >> 16 : x[i]);
-                                if (odd && lane == 0)
-                                    h[0] = static_cast<uint16_t>(x[i]);
-                            }
-                            base_row += 32 * pitch;
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t next = __shfl_down_sync(0xffffffffu, x[i], 1);
+                            T *to = base_row + i * 4 * pitch;
+                            if (first + 4 * i >= rows)
+                                continue;
+                            uint16_t *h = reinterpret_cast<uint16_t *>(to);
+                            const bool odd = (reinterpret_cast<uintptr_t>(to) & 2u) != 0;
+                            const int e = 2 * lane + (odd ? 1 : 0);
+                            if (e + 1 < min(cols, 64))
+                                *reinterpret_cast<uint32_t *>(h + e) = odd ? __funnelshift_r(x[i], next, 16) : x[i];
+                            else if (e < min(cols, 64))
+                                h[e] = static_cast<uint16_t>(odd ? x[i] >> 16 : x[i]);
+                            if (odd && lane == 0)
+                                h[0] = static_cast<uint16_t>(x[i]);
                         }
-                    };
-                    auto emit_columns = [&](const float (&v)[64], const void *map, int z, bool tma, bool half, void *dst,
-                                            long long at0, long long pitch, int col0, const void *residual) {
-                        uint32_t words[32];
-                        if (half && (tma || !residual)) {
+                        base_row += 32 * pitch;
+                    }
+                };
+                auto emit_columns = [&](const float (&v)[64], const void *map, int z, bool tma, bool half, void *dst,
+                                        long long at0, long long pitch, int col0, const void *residual) {
+                    uint32_t words[32];
+                    if (half && (tma || !residual)) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            words[j] = Type::pack(v[2 * j], v[2 * j + 1]);
+                        if (tma)
+                            emit(words, map, z, col0);
+                        else
+                            emit_rows_half(words, dst, at0, pitch, col0);
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (col0 + 32 * h >= p.n)
+                                break;
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                words[j] = Type::pack(v[2 * j], v[2 * j + 1]);
+                                words[j] = __float_as_uint(v[32 * h + j]);
                             if (tma)
-                                emit(words, map, z, col0);
+                                emit(words, map, z, col0 + 32 * h);
                             else
-                                emit_rows_half(words, dst, at0, pitch, col0);
-                        } else {
+                                emit_rows(words, half, dst, at0, pitch, col0 + 32 * h, residual);
+                        }
+                    }
+                };
+                // 64 columns of this thread's row: epilogue arithmetic and stores.
+                auto process = [&](float (&v)[64], int step) {
+                    const int col0 = w.n0 + gcol + step * 64;
+                    if (col0 >= p.n || row0 >= w.row_end)      // the same for all four warps
+                        return;
+                    if constexpr (EPI == kEpiSoftmaxGrad) {
+                        // p = exp(z - lse); an ignored row's gradient is zero whatever its logits are.
+                        const int hit = label - p.column0 - col0;
+                        const float scale = label == -2 ? __int_as_float(0x7fc00000) : row_grad;
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                if (col0 + 32 * h >= p.n)
-                                    break;
+                        for (int j = 0; j < 64; ++j) {
+                            const float prob = exp2f((v[j] - row_lse) * 1.4426950408889634f);   // subnormals kept
+                            v[j] = label == -1 ? 0.0f : (prob - (j == hit ? 1.0f : 0.0f)) * scale;
+                        }
+                    } else {
+                        if (p.bias) {
+                            const float4 *b4 = reinterpret_cast<const float4 *>(bias_s + gcol + step * 64);
 #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    words[j] = __float_as_uint(v[32 * h + j]);
-                                if (tma)
-                                    emit(words, map, z, col0 + 32 * h);
-                                else
-                                    emit_rows(words, half, dst, at0, pitch, col0 + 32 * h, residual);
+                            for (int j = 0; j < 16; ++j) {
+                                const float4 b = b4[j];
+                                v[4 * j] += b.x;
+                                v[4 * j + 1] += b.y;
+                                v[4 * j + 2] += b.z;
+                                v[4 * j + 3] += b.w;
                             }
                         }
-                    };
-                    // 64 columns of this thread's row: epilogue arithmetic and stores.
-                    auto process = [&](float (&v)[64], int step) {
-                        const int col0 = n0 + gcol + step * 64;
-                        if (col0 >= p.n || row0 >= w.row_end)      // the same for all four warps
-                            return;
-                        if constexpr (EPI == kEpiSoftmaxGrad) {
-                            // p = exp(z - lse); an ignored row's gradient is zero whatever its logits are.
-                            const int hit = label - p.column0 - col0;
-                            const float scale = label == -2 ? __int_as_float(0x7fc00000) : row_grad;
+                        if (p.preact)
+                            emit_columns(v, &map_z, 0, p.preact_tma != 0, p.preact_half != 0, p.preact, 0, p.n, col0, nullptr);
+                        op_with_activation(p.activation, [&](auto act) {
 #pragma unroll
-                            for (int j = 0; j < 64; ++j) {
-                                const float prob = exp2f((v[j] - row_lse) * 1.4426950408889634f);   // subnormals kept
-                                v[j] = label == -1 ? 0.0f : (prob - (j == hit ? 1.0f : 0.0f)) * scale;
-                            }
-                        } else {
-                            if (p.bias) {
-                                const float4 *b4 = reinterpret_cast<const float4 *>(bias_s + gcol + step * 64);
+                            for (int j = 0; j < 64; ++j)
+                                v[j] = op_activation<decltype(act)::value>(v[j]);
+                        });
+                        // Where TMA writes out, each thread reads its own row of the residual (16-byte
+                        // loads where it can); otherwise the row-by-row store adds it.
+                        if (p.residual && p.out_tma && row0 + r < w.row_end) {
+                            const long long at = (row0 + r) * p.out_pitch + col0;
+                            if (col0 + 64 <= p.n) {
+                                if (p.residual_half) {
+                                    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at);
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) {
-                                    const float4 b = b4[j];
-                                    v[4 * j] += b.x;
-                                    v[4 * j + 1] += b.y;
-                                    v[4 * j + 2] += b.z;
-                                    v[4 * j + 3] += b.w;
-                                }
-                            }
-                            if (p.preact)
-                                emit_columns(v, &map_z, 0, p.preact_tma != 0, p.preact_half != 0, p.preact, 0, p.n, col0, nullptr);
-                            op_with_activation(p.activation, [&](auto act) {
+                                    for (int j = 0; j < 8; ++j) {
+                                        const uint4 q = src[j];
+                                        const T *h = reinterpret_cast<const T *>(&q);
+                                        if constexpr (!kTF32) {
 #pragma unroll
-                                for (int j = 0; j < 64; ++j)
-                                    v[j] = op_activation<decltype(act)::value>(v[j]);
-                            });
-                            // Where TMA writes out, each thread reads its own row of the residual (16-byte
-                            // loads where it can); otherwise the row-by-row store adds it.
-                            if (p.residual && p.out_tma && row0 + r < w.row_end) {
-                                const long long at = (row0 + r) * p.out_pitch + col0;
-                                if (col0 + 64 <= p.n) {
-                                    if (p.residual_half) {
-                                        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at);
-#pragma unroll
-                                        for (int j = 0; j < 8; ++j) {
-                                            const uint4 q = src[j];
-                                            const T *h = reinterpret_cast<const T *>(&q);
-                                            if constexpr (!kTF32) {
-#pragma unroll
-                                                for (int e = 0; e < 8; ++e)
-                                                    v[8 * j + e] += Type::to(h[e]);
-                                            }
-                                        }
-                                    } else {
-                                        const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.residual) + at);
-#pragma unroll
-                                        for (int j = 0; j < 16; ++j) {
-                                            const float4 q = src[j];
-                                            v[4 * j] += q.x;
-                                            v[4 * j + 1] += q.y;
-                                            v[4 * j + 2] += q.z;
-                                            v[4 * j + 3] += q.w;
+                                            for (int e = 0; e < 8; ++e)
+                                                v[8 * j + e] += Type::to(h[e]);
                                         }
                                     }
                                 } else {
+                                    const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.residual) + at);
 #pragma unroll
-                                    for (int j = 0; j < 64; ++j)
-                                        if (col0 + j < p.n)
-                                            v[j] += p.residual_half ? Type::to(static_cast<const T *>(p.residual)[at + j])
-                                                                    : static_cast<const float *>(p.residual)[at + j];
+                                    for (int j = 0; j < 16; ++j) {
+                                        const float4 q = src[j];
+                                        v[4 * j] += q.x;
+                                        v[4 * j + 1] += q.y;
+                                        v[4 * j + 2] += q.z;
+                                        v[4 * j + 3] += q.w;
+                                    }
                                 }
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 64; ++j)
+                                    if (col0 + j < p.n)
+                                        v[j] += p.residual_half ? Type::to(static_cast<const T *>(p.residual)[at + j])
+                                                                : static_cast<const float *>(p.residual)[at + j];
                             }
                         }
-                        emit_columns(v, mc, zc, p.out_tma != 0, p.out_half != 0, p.out, zc * p.out_slab, p.out_pitch, col0,
-                                     p.residual);
-                    };
-                    auto load = [&](float (&v)[64], int step) {
-                        if (w.nkb > 0) {
-                            tmem_load_64cols(t_row + step * 64, v);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 64; ++j)
-                                v[j] = 0.0f;
-                        }
-                    };
-                    if constexpr (kParts == 2) {
-                        // The half is read into registers at once and given back to the MMAs, whose
-                        // first K blocks of the next tile wait for it.
-                        float v0[64], v1[64];
-                        load(v0, 0);
-                        load(v1, 1);
-                        release();
-                        process(v0, 0);
-                        process(v1, 1);
+                    }
+                    emit_columns(v, mc, zc, p.out_tma != 0, p.out_half != 0, p.out, zc * p.out_slab, p.out_pitch, col0,
+                                 p.residual);
+                };
+                auto load = [&](float (&v)[64], int step) {
+                    if (w.nkb > 0) {
+                        tmem_load_64cols(t_row + step * 64, v);
                     } else {
-#pragma unroll 1
-                        for (int step = 0; step < kGroupCols / 64; ++step) {
-                            float v[64];
-                            load(v, step);
-                            if (step == kGroupCols / 64 - 1)
-                                release();
-                            process(v, step);
-                        }
+#pragma unroll
+                        for (int j = 0; j < 64; ++j)
+                            v[j] = 0.0f;
                     }
-                } else if constexpr (EPI == kEpiStoreT) {
-                    // D's rows are output columns: one lane per column, one store of 32 consecutive
-                    // elements per output row and warp.
-                    const int col = row0 + r;
-                    const float b = p.bias && col < p.n ? load_bias(col) : 0.0f;
+                };
 #pragma unroll 1
-                    for (int chunk = 0; chunk < kGroupCols / 16; ++chunk) {
-                        uint32_t u[16];
-                        tmem_load_16cols(t_row + chunk * 16, u);
-                        if (chunk == kGroupCols / 16 - 1)
-                            release();
-                        const int first = w.n0 + gcol + chunk * 16;
-                        const int rows = min(16, w.row_end - first);
-                        if (col >= p.n || rows <= 0)
-                            continue;
-                        float v[16];
+                for (int step = 0; step < kGroupCols / 64; ++step) {
+                    float v[64];
+                    load(v, step);
+                    if (step == kGroupCols / 64 - 1)
+                        release();
+                    process(v, step);
+                }
+            } else if constexpr (EPI == kEpiStoreT) {
+                // D's rows are output columns: one lane per column, one store of 32 consecutive
+                // elements per output row and warp.
+                const int col = row0 + r;
+                const float b = p.bias && col < p.n ? load_bias(col) : 0.0f;
+#pragma unroll 1
+                for (int chunk = 0; chunk < kGroupCols / 16; ++chunk) {
+                    uint32_t u[16];
+                    tmem_load_16cols(t_row + chunk * 16, u);
+                    if (chunk == kGroupCols / 16 - 1)
+                        release();
+                    const int first = w.n0 + gcol + chunk * 16;
+                    const int rows = min(16, w.row_end - first);
+                    if (col >= p.n || rows <= 0)
+                        continue;
+                    float v[16];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            v[j] = __uint_as_float(u[j]) + b;
-                        store_elements(v, rows, first, col, 1, 0);
-                    }
-                } else {
-                    // One pass: running maximum and sum of exponentials in base 2 of this row's
-                    // columns in the tile; columns past the vocabulary count as -infinity.
-                    float top = -INFINITY, sum = 0.0f;
-                    const int row = row0 + r;
-                    auto reduce = [&](const uint32_t (&u)[32], int chunk) {
-                        const int col0 = n0 + gcol + chunk * 32;
-                        if (col0 >= p.n)
-                            return;
-                        const int hit = label - col0;
-                        if (label >= 0 && hit >= 0 && hit < 32) {
-                            float z = 0.0f;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                z = j == hit ? __uint_as_float(u[j]) : z;
-                            p.label_logit[row] = z;
-                        }
-                        float t[32], chunk_top = -INFINITY;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            t[j] = col0 + j < p.n ? __uint_as_float(u[j]) * 1.4426950408889634f : -INFINITY;
-                            chunk_top = fmaxf(chunk_top, t[j]);
-                        }
-                        const float next = fmaxf(top, chunk_top);
-                        // A row whose logits are all -infinity so far adds nothing; NaN is carried by the sum.
-                        const float origin = next == -INFINITY ? 0.0f : next;
-                        sum *= op_exp2(top - origin);
-                        float part_sum[4] = {};     // four chains
+                    for (int j = 0; j < 16; ++j)
+                        v[j] = __uint_as_float(u[j]) + b;
+                    store_elements(v, rows, first, col, 1, 0);
+                }
+            } else {
+                // One pass: running maximum and sum of exponentials in base 2 of this row's
+                // columns in the tile; columns past the vocabulary count as -infinity.
+                float top = -INFINITY, sum = 0.0f;
+                const int row = row0 + r;
+                auto reduce = [&](const uint32_t (&u)[32], int chunk) {
+                    const int col0 = w.n0 + gcol + chunk * 32;
+                    if (col0 >= p.n)
+                        return;
+                    const int hit = label - col0;
+                    if (label >= 0 && hit >= 0 && hit < 32) {
+                        float z = 0.0f;
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            part_sum[j & 3] += op_exp2(t[j] - origin);
-                        sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
-                        top = next;
-                    };
-                    if constexpr (kParts == 2) {
-                        uint32_t u0[32], u1[32], u2[32], u3[32];      // read at once, as above
-                        tmem_load_32cols(t_row, u0);
-                        tmem_load_32cols(t_row + 32, u1);
-                        tmem_load_32cols(t_row + 64, u2);
-                        tmem_load_32cols(t_row + 96, u3);
-                        release();
-                        reduce(u0, 0);
-                        reduce(u1, 1);
-                        reduce(u2, 2);
-                        reduce(u3, 3);
-                    } else {
-#pragma unroll 1
-                        for (int chunk = 0; chunk < kGroupCols / 32; ++chunk) {
-                            uint32_t u[32];
-                            tmem_load_32cols(t_row + chunk * 32, u);
-                            if (chunk == kGroupCols / 32 - 1)
-                                release();
-                            reduce(u, chunk);
-                        }
+                            z = j == hit ? __uint_as_float(u[j]) : z;
+                        p.label_logit[row] = z;
                     }
-                    if (row < p.m)
-                        p.partial[static_cast<long long>((w.loss_block + part) * kGroups + group) * p.m + row] = make_float2(top, sum);
+                    float t[32], chunk_top = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        t[j] = col0 + j < p.n ? __uint_as_float(u[j]) * 1.4426950408889634f : -INFINITY;
+                        chunk_top = fmaxf(chunk_top, t[j]);
+                    }
+                    const float next = fmaxf(top, chunk_top);
+                    // A row whose logits are all -infinity so far adds nothing; NaN is carried by the sum.
+                    const float origin = next == -INFINITY ? 0.0f : next;
+                    sum *= op_exp2(top - origin);
+                    float part_sum[4] = {};     // four chains
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        part_sum[j & 3] += op_exp2(t[j] - origin);
+                    sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+                    top = next;
+                };
+#pragma unroll 1
+                for (int chunk = 0; chunk < kGroupCols / 32; ++chunk) {
+                    uint32_t u[32];
+                    tmem_load_32cols(t_row + chunk * 32, u);
+                    if (chunk == kGroupCols / 32 - 1)
+                        release();
+                    reduce(u, chunk);
                 }
+                if (row < p.m)
+                    p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row] = make_float2(top, sum);
             }
-            if (splits > 1 || failed_tile >= 0)
-                break;
-            if (++acc == kAccs) {
+            if (++acc == 2) {
                 acc = 0;
                 acc_phase ^= 1u;
             }
@@ -1247,20 +1139,16 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             for (int tile = failed_tile; tile < tile_end; tile += tile_step) {
                 const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
                 const int row0 = w.m0 + static_cast<int>(rank) * OP_BM;
-                for (int h = 0; h < w.parts; ++h) {
-                    if constexpr (EPI == kEpiLse) {
-                        if (row0 + r < p.m)
-                            p.partial[static_cast<long long>((w.loss_block + h) * kGroups + group) * p.m + row0 + r] =
-                                make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
-                    } else {
-                        nan_elements(w, kSwap ? w.n0 + gcol : row0, kSwap ? kGroupCols : OP_BM,
-                                     kSwap ? row0 : w.n0 + h * 256 + gcol, kSwap ? OP_BM : kGroupCols, quarter, 4, lane);
-                    }
+                if constexpr (EPI == kEpiLse) {
+                    if (row0 + r < p.m)
+                        p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row0 + r] =
+                            make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+                } else {
+                    nan_elements(w, kSwap ? w.n0 + gcol : row0, kSwap ? kGroupCols : OP_BM, kSwap ? row0 : w.n0 + gcol,
+                                 kSwap ? OP_BM : kGroupCols, quarter, 4, lane);
                 }
             }
         }
-    } else {
-        give_registers();
     }
 
     if constexpr (kSplittable) {
