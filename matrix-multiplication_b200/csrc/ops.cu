@@ -383,6 +383,21 @@ int enqueue(Call &c, Product &q)
     return st == cudaSuccess ? 0 : c.failed(st);
 }
 
+// Gives a product's epilogue its residual (rows as the output's), after set_output and the
+// pre-activation.
+int set_residual(Call &c, OpLaunch &l, const Matrix &residual, bool half)
+{
+    OpParams &p = l.p;
+    p.residual = residual.ptr;
+    p.residual_half = half ? 1 : 0;
+    p.residual_tma = p.out_tma && !p.preact && p.residual_half == p.out_half && !is_swap(l.tile) && l.splits == 1 ? 1 : 0;
+    if (p.residual_tma && !output_map(c, &l.map_z, residual, half)) {
+        cudaGetLastError();
+        return c.failed("cuTensorMapEncodeTiled rejected the residual");
+    }
+    return 0;
+}
+
 // Points a product's epilogue at an output matrix.
 int set_output(Call &c, OpLaunch &l, const Matrix &out, bool half)
 {
@@ -491,8 +506,6 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     p.bias = bias;
     p.bias_half = bias_half ? 1 : 0;
     p.activation = activation;
-    p.residual = residual;
-    p.residual_half = p.out_half;
     p.out_tma = out_tma ? 1 : 0;
     if (preact) {
         const Matrix mz{preact, m, n, n};
@@ -504,6 +517,8 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
             return c.failed("cuTensorMapEncodeTiled rejected an output");
         }
     }
+    if (residual && set_residual(c, l, Matrix{residual, m, n, n}, out_half))
+        return 1;
     return enqueue(c, q);
 }
 
@@ -1016,10 +1031,10 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             if (set_output(c, q.launch, to, last && dh_half))
                 return 1;
             if (piece > 0) {
-                q.launch.p.residual = sum.ptr;
-                q.launch.p.residual_half = 0;
                 if (!output_tma(sum, 4))
                     q.launch.p.out_tma = 0;
+                if (set_residual(c, q.launch, sum, false))
+                    return 1;
             }
             if (enqueue(c, q))
                 return 1;

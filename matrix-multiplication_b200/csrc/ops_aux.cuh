@@ -167,10 +167,14 @@ __global__ void __launch_bounds__(AG_THREADS) act_grad_kernel(const ActGradParam
                 if (row + 8 * i >= row_end)
                     break;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
+                for (int e = 0; e < 8; e += 2) {
+                    float2 dz = make_float2(d[i][e], d[i][e + 1]);
                     if (ACT != kActNone)
-                        d[i][e] *= op_activation_slope<ACT>(z[i][e]);
-                    sum[e] += d[i][e];
+                        dz = __fmul2_rn(dz, op_activation_slope<ACT>(make_float2(z[i][e], z[i][e + 1])));
+                    d[i][e] = dz.x;
+                    d[i][e + 1] = dz.y;
+                    sum[e] += dz.x;
+                    sum[e + 1] += dz.y;
                 }
                 if (p.dz) {
                     T *dst = static_cast<T *>(p.dz) + (row + 8 * i) * p.dz_pitch + col0;

@@ -64,11 +64,11 @@ template <int CTAS, int BN>
 struct OpTile {
     static constexpr int kBCols = BN / CTAS;                   // N columns staged per CTA
     static constexpr int kBStage = kBCols * OP_ROW_BYTES;
-    static constexpr int kStages = kBCols >= 128 ? 6 : 8;
+    static constexpr int kStages = kBCols >= 128 ? 5 : 8;
     static constexpr int kGroups = BN >= 128 ? 2 : 1;          // epilogue warpgroups
     static constexpr int kFirstEpi = kGroups == 2 ? 4 : 2;     // first epilogue warp (after TMA, MMA, two idle ones)
     static constexpr int kThreads = 32 * (kFirstEpi + 4 * kGroups);
-    static constexpr int kBoxes = 3 - kGroups;                 // boxes per epilogue warpgroup: two in all
+    static constexpr int kBoxes = 2;                           // boxes per epilogue warpgroup
     static constexpr int kEpiBytes = kBoxes * kGroups * OP_BOX;
     static constexpr int kBiasBytes = BN * 4 < 256 ? 256 : BN * 4;
     static constexpr int kSmem = 1024 + kStages * (OP_A_STAGE + kBStage) + kEpiBytes + OP_BAR_BYTES + kBiasBytes;
@@ -131,6 +131,7 @@ struct OpParams {
     int preact_half, preact_tma;
     const void *residual;             // null, or added after the activation (pitch out_pitch)
     int residual_half;
+    int residual_tma;                 // 1: TMA brings it (map_z; out's format, no pre-activation)
     const void *bias;                 // n values or null
     int bias_half;
     int activation;
@@ -163,6 +164,15 @@ __device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const void *map, 
         "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *map, uint32_t bar, int x, int y, int z)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 
@@ -254,67 +264,91 @@ __device__ __forceinline__ float op_exp2(float x)
     return y;
 }
 
-__device__ __forceinline__ float op_exp(float x)
-{
-    return op_exp2(x * 1.4426950408889634f);
-}
-
 // The normal distribution function by Abramowitz and Stegun's rational approximation of
 // erf (Handbook of Mathematical Functions, 7.1.26; absolute error of erf 1.5e-7), half
 // the instructions of erff: with x = |z| / sqrt 2 and t = 1 / (1 + 0.3275911 x), 1 -
-// erf(x) = t (a1 + t (a2 + ... )) exp(-x^2).  `e` receives exp(-z^2 / 2).
-__device__ __forceinline__ float op_normal_cdf(float z, float &e)
+// erf(x) = t (a1 + t (a2 + ... )) exp(-x^2).  Two values at a time: the polynomial and
+// products are packed FP32 instructions.  `e` receives exp(-z^2 / 2).
+__device__ __forceinline__ float2 op_normal_cdf(float2 z, float2 &e)
 {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-    e = op_exp(-x * x);
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(t, q, 1.421413741f);
-    q = fmaf(t, q, -0.284496736f);
-    q = fmaf(t, q, 0.254829592f);
-    const float half_tail = 0.5f * t * q * e;
-    return z < 0.0f ? half_tail : 1.0f - half_tail;
+    const float2 a = make_float2(fabsf(z.x), fabsf(z.y));
+    const float2 d = __ffma2_rn(make_float2(0.23164189f, 0.23164189f), a, make_float2(1.0f, 1.0f));
+    const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+    const float2 x = __fmul2_rn(__fmul2_rn(a, make_float2(-0.72134752f, -0.72134752f)), a);   // -z^2 / 2 log2 e
+    e = make_float2(op_exp2(x.x), op_exp2(x.y));
+    float2 q = __ffma2_rn(t, make_float2(0.5307027145f, 0.5307027145f), make_float2(-0.7265760135f, -0.7265760135f));
+    q = __ffma2_rn(t, q, make_float2(0.7107068705f, 0.7107068705f));
+    q = __ffma2_rn(t, q, make_float2(-0.142248368f, -0.142248368f));
+    q = __ffma2_rn(t, q, make_float2(0.127414796f, 0.127414796f));
+    const float2 tail = __fmul2_rn(__fmul2_rn(t, q), e);       // half of 1 - erf
+    return make_float2(z.x < 0.0f ? tail.x : 1.0f - tail.x, z.y < 0.0f ? tail.y : 1.0f - tail.y);
 }
 
-// act(z) in FP32.  relu keeps NaN; gelu_tanh uses 0.5 (1 + tanh u) = 1 / (1 + exp(-2u)).
+// act(z) of two values in FP32.  relu keeps NaN; gelu_tanh uses 0.5 (1 + tanh u) = 1 / (1
+// + exp(-2u)).
 template <int ACT>
-__device__ __forceinline__ float op_activation(float z)
+__device__ __forceinline__ float2 op_activation(float2 z)
 {
     if constexpr (ACT == kActRelu)
-        return z < 0.0f ? 0.0f : z;
+        return make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);
     if constexpr (ACT == kActGelu) {
-        float e;
-        return z * op_normal_cdf(z, e);
+        float2 e;
+        return __fmul2_rn(z, op_normal_cdf(z, e));
     }
     if constexpr (ACT == kActGeluTanh) {
-        const float u = 0.79788456080286536f * fmaf(0.044715f * z * z, z, z);
-        return __fdividef(z, 1.0f + op_exp(-2.0f * u));
+        // -2 u log2 e = z (-2.3022082 - 0.10294324 z^2)
+        const float2 p = __ffma2_rn(__fmul2_rn(z, z), make_float2(-0.10294324f, -0.10294324f),
+                                    make_float2(-2.3022082f, -2.3022082f));
+        const float2 x = __fmul2_rn(z, p);
+        return make_float2(__fdividef(z.x, 1.0f + op_exp2(x.x)), __fdividef(z.y, 1.0f + op_exp2(x.y)));
     }
-    if constexpr (ACT == kActSilu)
-        return __fdividef(z, 1.0f + op_exp(-z));
+    if constexpr (ACT == kActSilu) {
+        const float2 x = __fmul2_rn(z, make_float2(-1.44269504f, -1.44269504f));
+        return make_float2(__fdividef(z.x, 1.0f + op_exp2(x.x)), __fdividef(z.y, 1.0f + op_exp2(x.y)));
+    }
     return z;
 }
 
-// act'(z) in FP32.
+// act'(z) of two values in FP32.
 template <int ACT>
-__device__ __forceinline__ float op_activation_slope(float z)
+__device__ __forceinline__ float2 op_activation_slope(float2 z)
 {
+    const float2 one = make_float2(1.0f, 1.0f);
     if constexpr (ACT == kActRelu)
-        return z > 0.0f ? 1.0f : 0.0f;
+        return make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
     if constexpr (ACT == kActGelu) {
-        float e;
-        const float cdf = op_normal_cdf(z, e);
-        return fmaf(z * 0.39894228040143268f, e, cdf);
+        float2 e;
+        const float2 cdf = op_normal_cdf(z, e);
+        return __ffma2_rn(__fmul2_rn(z, make_float2(0.39894228f, 0.39894228f)), e, cdf);
     }
     if constexpr (ACT == kActGeluTanh) {
-        const float s = __fdividef(1.0f, 1.0f + op_exp(-1.5957691216057308f * fmaf(0.044715f * z * z, z, z)));
-        return fmaf(z * s * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f), s);
+        const float2 zz = __fmul2_rn(z, z);
+        const float2 x = __fmul2_rn(z, __ffma2_rn(zz, make_float2(-0.10294324f, -0.10294324f),
+                                                  make_float2(-2.3022082f, -2.3022082f)));
+        const float2 s = make_float2(__fdividef(1.0f, 1.0f + op_exp2(x.x)), __fdividef(1.0f, 1.0f + op_exp2(x.y)));
+        const float2 du = __ffma2_rn(zz, make_float2(0.21406446f, 0.21406446f), make_float2(1.59576912f, 1.59576912f));
+        const float2 rest = __ffma2_rn(make_float2(-s.x, -s.y), s, s);         // s (1 - s)
+        return __ffma2_rn(__fmul2_rn(z, rest), du, s);
     }
     if constexpr (ACT == kActSilu) {
-        const float s = __fdividef(1.0f, 1.0f + op_exp(-z));
-        return s * fmaf(z, 1.0f - s, 1.0f);
+        const float2 x = __fmul2_rn(z, make_float2(-1.44269504f, -1.44269504f));
+        const float2 s = make_float2(__fdividef(1.0f, 1.0f + op_exp2(x.x)), __fdividef(1.0f, 1.0f + op_exp2(x.y)));
+        const float2 rest = __ffma2_rn(make_float2(-s.x, -s.y), s, s);
+        return __ffma2_rn(z, rest, s);
     }
-    return 1.0f;
+    return one;
+}
+
+// The activation of N values (N even).
+template <int ACT, int N>
+__device__ __forceinline__ void op_activate(float (&v)[N])
+{
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        const float2 y = op_activation<ACT>(make_float2(v[j], v[j + 1]));
+        v[j] = y.x;
+        v[j + 1] = y.y;
+    }
 }
 
 // Calls f with the activation as a constant, so that loops over it hold no branch (with
@@ -474,6 +508,8 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         mbar_init(drain_bar, 1);
         mbar_init(recv_bar, 1);
+        for (int i = 0; i < kGroups * Tile::kBoxes; ++i)
+            mbar_init(s_bar + 8u * (2 * kStages + 8 + i), 1);
         *fail_flag_ptr = 0u;
         fence_mbarrier_init();
     }
@@ -519,9 +555,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 }
         }
         op_with_activation(p.activation, [&](auto act) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                v[i] = op_activation<decltype(act)::value>(v[i]);
+            op_activate<decltype(act)::value>(v);
         });
         if (p.residual) {
 #pragma unroll
@@ -756,6 +790,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         uint32_t acc_phase = 0, stores = 0;
         int failed_tile = -1;
         int acquired = -1;
+        // Residual boxes: loads issued and used, the parity of each box's next load, and boxes of
+        // the current tile already stored.
+        uint32_t res_issued = 0, res_used = 0, res_parity = 0, box_done = 0;
+        auto res_bar = [&](uint32_t b) { return s_bar + 8u * (2 * kStages + 8 + group * kBoxes + b); };
         // Releases the accumulator after this warp's last read of it.
         auto release = [&]() {
             const uint32_t bar = acce_bar(acc);
@@ -798,6 +836,26 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                 }
             }
+            // Residual by TMA: box u of this tile (32 FP32 or 64 16-bit columns) is loaded into the
+            // shared-memory box that its result will leave from, one box ahead.
+            const int box_cols = p.out_half ? 64 : 32;
+            auto fetch = [&](int u) {
+                const int col0 = w.n0 + gcol + u * box_cols;
+                if (u * box_cols >= kGroupCols || col0 >= p.n || row0 >= w.row_end)
+                    return;
+                const uint32_t b = (stores + static_cast<uint32_t>(u) - box_done) % kBoxes;
+                if (issuer_warp && op_elect_one()) {
+                    bulk_wait_group_read<0>();      // the stores that last read the boxes
+                    mbar_arrive_expect_tx(res_bar(b), OP_BOX);
+                    tma_load_3d(s_box + b * OP_BOX, &map_z, res_bar(b), col0, row0, 0);
+                }
+                __syncwarp();
+                ++res_issued;
+            };
+            box_done = 0;
+            if constexpr (EPI == kEpiStore)
+                if (p.residual_tma && splits == 1)
+                    fetch(0);
             int ok = 1;
             if (issuer)       // one thread polls, the others wait at the barrier
                 ok = mbar_wait(accf_bar(acc), acc_phase, p.wait_limit_ns) ? 1 : 0;
@@ -849,6 +907,48 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                     __syncwarp();
                     ++stores;
+                };
+                // The same with the residual already in the box: each thread adds its own row to `v`,
+                // puts the result in its place and the box is stored.
+                auto emit_residual = [&](auto &v, const void *map, int col0) {
+                    constexpr bool kHalfBox = std::extent<std::remove_reference_t<decltype(v)>>::value == 64;
+                    const uint32_t b = stores % kBoxes;
+                    fetch(static_cast<int>(box_done) + 1);
+                    if (!mbar_wait(res_bar(b), (res_parity >> b) & 1u)) {
+                        atomicOr(p.status, kOpDrainTimeout);
+                        v[0] = __int_as_float(0x7fc00000);
+                    }
+                    res_parity ^= 1u << b;
+                    ++res_used;
+                    const uint32_t row_addr = s_box + b * OP_BOX + r * 128;
+                    uint32_t words[32];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint4 q = *reinterpret_cast<const uint4 *>(smem_raw + (row_addr + ((j ^ (r & 7)) << 4) - raw));
+                        if constexpr (kHalfBox) {
+                            const T *h = reinterpret_cast<const T *>(&q);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                words[4 * j + e] = Type::pack(v[8 * j + 2 * e] + Type::to(h[2 * e]),
+                                                              v[8 * j + 2 * e + 1] + Type::to(h[2 * e + 1]));
+                        } else {
+                            words[4 * j] = __float_as_uint(v[4 * j] + __uint_as_float(q.x));
+                            words[4 * j + 1] = __float_as_uint(v[4 * j + 1] + __uint_as_float(q.y));
+                            words[4 * j + 2] = __float_as_uint(v[4 * j + 2] + __uint_as_float(q.z));
+                            words[4 * j + 3] = __float_as_uint(v[4 * j + 3] + __uint_as_float(q.w));
+                        }
+                    }
+                    fill(s_box + b * OP_BOX, words);
+                    fence_proxy_async_shared();
+                    epilogue_sync();
+                    __syncwarp();
+                    if (issuer_warp && op_elect_one()) {
+                        tma_store_3d(map, s_box + b * OP_BOX, col0, row0, 0);
+                        bulk_commit_group();
+                    }
+                    __syncwarp();
+                    ++stores;
+                    ++box_done;
                 };
                 // A box of 32 FP32 columns written out row by row (lane = column) where TMA cannot
                 // write, in either format; the residual is added on the way, coalesced.
@@ -994,22 +1094,32 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         if (p.preact)
                             emit_columns(v, &map_z, 0, p.preact_tma != 0, p.preact_half != 0, p.preact, 0, p.n, col0, nullptr);
                         op_with_activation(p.activation, [&](auto act) {
-#pragma unroll
-                            for (int j = 0; j < 64; ++j)
-                                v[j] = op_activation<decltype(act)::value>(v[j]);
+                            op_activate<decltype(act)::value>(v);
                         });
-                        // Where TMA writes out, each thread reads its own row of the residual (16-byte
-                        // loads where it can); otherwise the row-by-row store adds it.
+                        if (p.residual_tma) {
+                            if (p.out_half) {
+                                if constexpr (!kTF32)
+                                    emit_residual(v, mc, col0);
+                            } else {
+                                emit_residual(reinterpret_cast<float(&)[32]>(v[0]), mc, col0);
+                                if (col0 + 32 < p.n)
+                                    emit_residual(reinterpret_cast<float(&)[32]>(v[32]), mc, col0 + 32);
+                            }
+                            return;
+                        }
+                        // Where TMA writes out but does not bring the residual (a pre-activation takes its
+                        // boxes, or it has another format), each thread reads its own row of it; without
+                        // TMA the row-by-row store adds it.
                         if (p.residual && p.out_tma && row0 + r < w.row_end) {
                             const long long at = (row0 + r) * p.out_pitch + col0;
                             if (col0 + 64 <= p.n) {
                                 if (p.residual_half) {
-                                    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at);
+                                    if constexpr (!kTF32) {
+                                        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at);
 #pragma unroll
-                                    for (int j = 0; j < 8; ++j) {
-                                        const uint4 q = src[j];
-                                        const T *h = reinterpret_cast<const T *>(&q);
-                                        if constexpr (!kTF32) {
+                                        for (int j = 0; j < 8; ++j) {
+                                            const uint4 q = src[j];
+                                            const T *h = reinterpret_cast<const T *>(&q);
 #pragma unroll
                                             for (int e = 0; e < 8; ++e)
                                                 v[8 * j + e] += Type::to(h[e]);
@@ -1125,6 +1235,13 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 acc = 0;
                 acc_phase ^= 1u;
             }
+        }
+        // A residual box that was fetched and not used (an accumulator that never came) lands
+        // before the CTA can exit.
+        if (res_issued != res_used) {
+            const uint32_t b = stores % kBoxes;
+            if (!mbar_wait(res_bar(b), (res_parity >> b) & 1u))
+                atomicOr(p.status, kOpDrainTimeout);
         }
         if (issuer) {
             if (failed_tile >= 0)
