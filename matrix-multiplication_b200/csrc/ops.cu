@@ -228,21 +228,22 @@ bool is_swap(int tile)
 struct TileProblem {
     int64_t m, n, k_blocks, groups = 1;
     int bytes_out = 2;
-    bool out_tma = true, splittable = false, transposable = false;
+    bool out_tma = true, splittable = false, transposable = false, ragged_k = false;
 };
 
 // Estimated cycles of a tile kind with K split S ways.  A K block costs the most of its MMA
 // time (2 cycles a column, 140 at least), its operand bytes into one SM at 70 B/cycle and
 // all running CTAs' bytes out of L2 at 9.3 KB/cycle; a tile's epilogue adds the kind's own
-// cycles, more where rows are stored without TMA, and a pair's tile costs no less than 2500
-// cycles per byte of an output element (5050 measured for BF16 with K = 256).  A split adds
-// its exchange.  The constants are fitted to 1170 times of every kind and split over 95
+// cycles, more where rows are stored without TMA, and a tile costs no less than its stores
+// (a pair's 5050 cycles, one CTA's 128 x 128 2960 for BF16, measured with K = 256).  A split
+// adds its exchange.  The constants are fitted to 1170 times of every kind and split over 95
 // BF16 products of 33 to 2048 rows (10 % rms; the kind chosen is 0.3 % slower than the
 // fastest on average, 7 % at worst).
 double tile_cycles(const Context *ctx, int tile, int splits, const TileProblem &q)
 {
     constexpr double kEpilogue[] = {4400.0, 1100.0, 1140.0, 810.0, 800.0, 1170.0, 1170.0};
     constexpr double kRowStores[] = {17800.0, 6100.0, 3050.0, 200.0, 400.0, 800.0, 1700.0};
+    constexpr double kFloor[] = {2500.0, 1480.0, 900.0, 0.0, 0.0, 0.0, 0.0};
     const TileShape &t = kTileShapes[tile];
     const bool swap = is_swap(tile);
     const int64_t side_m = swap ? q.n : q.m, side_n = swap ? q.m : q.n;
@@ -254,8 +255,12 @@ double tile_cycles(const Context *ctx, int tile, int splits, const TileProblem &
     const double k_cycles = std::max({2.0 * t.bn, 140.0, bytes / 70.0, active * bytes / 9300.0});
     const double epilogue = kEpilogue[tile] + (q.out_tma ? 0.0 : kRowStores[tile]);
     double tile_time = std::ceil(static_cast<double>(q.k_blocks) / splits) * k_cycles + epilogue;
-    if (t.ctas == 2)
-        tile_time = std::max(tile_time, 2500.0 * q.bytes_out);
+    // In ragged-K mode one CTA's tile also waits for its group's tables and tensor maps, which a
+    // pair's longer tile hides (32 groups of 256 rows, 2048 x 1408 outputs: 4800 cycles a
+    // 128 x 128 tile, 3000 ungrouped; 80 us in pairs, 107 us without).
+    if (q.ragged_k && t.ctas == 1)
+        tile_time += 1800.0;
+    tile_time = std::max(tile_time, kFloor[tile] * q.bytes_out);
     return rounds * tile_time +
            (splits > 1 ? 3700.0 + 0.093 * static_cast<double>(splits - 1) / splits * OP_BM * t.bn * 4.0 : 0.0);
 }
@@ -398,6 +403,45 @@ int set_residual(Call &c, OpLaunch &l, const Matrix &residual, bool half)
     return 0;
 }
 
+// An output that TMA cannot write (odd row pitch or base) and that is large is computed
+// into scratch rows of whole 128 bytes and copied from there: the products' own
+// row-by-row stores cost more (768 x 32001 BF16 from K = 200: 79 us, of which 10 us are
+// its bytes).  Small ones keep them, without the second launch.
+struct PaddedOutput {
+    Matrix target, padded;
+    bool used = false, half = false;
+    size_t at = 0;
+
+    void plan(Call &c, const Matrix &out, bool out_half)
+    {
+        constexpr int64_t kSmallest = int64_t{4} << 20;       // bytes
+        const int elem = out_half ? 2 : 4;
+        target = out;
+        half = out_half;
+        padded = out;
+        used = !output_tma(out, elem) && out.pitch == out.cols && out.rows * out.groups * out.cols * elem >= kSmallest;
+        if (!used)
+            return;
+        padded.pitch = round_up(out.cols, 128 / elem);
+        padded.slab = padded.pitch * out.rows;
+        at = c.reserve(static_cast<size_t>(padded.slab * out.groups * elem));
+    }
+    const Matrix &matrix(Call &c)
+    {
+        if (used)
+            padded.ptr = c.scratch + at;
+        return padded;
+    }
+    int finish(Call &c) const
+    {
+        if (!used)
+            return 0;
+        const cudaError_t st = c.kernels().unpack(padded.ptr, const_cast<void *>(target.ptr), target.rows * target.groups,
+                                                  target.cols, padded.pitch, !half, c.ctx->sm_count, c.stream);
+        return st == cudaSuccess ? 0 : c.failed(st);
+    }
+};
+
 // Points a product's epilogue at an output matrix.
 int set_output(Call &c, OpLaunch &l, const Matrix &out, bool half)
 {
@@ -481,6 +525,12 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     Operand oa, ob;
     oa.plan(c, a, m, k);
     ob.plan(c, b, k, n);
+    // A residual is added by the row-by-row stores, so its output takes no padded rows.
+    PaddedOutput po, pz;
+    if (m > 64 && !residual)
+        po.plan(c, Matrix{out, m, n, n}, out_half);
+    if (m > 64 && preact && !residual)
+        pz.plan(c, Matrix{preact, m, n, n}, preact_half);
     if (c.allocate() || prepare_operands(c, {&oa, &ob}))
         return 1;
     Product q;
@@ -493,10 +543,10 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     const int bk = OP_ROW_BYTES / e;
     const int64_t k_blocks = (static_cast<int64_t>(k) + bk - 1) / bk;
     const int bytes_out = (out_half ? 2 : 4) * (residual ? 2 : 1) + (preact ? (preact_half ? 2 : 4) : 0);
-    const Matrix mo{out, m, n, n};
+    const Matrix mo = po.used ? po.matrix(c) : Matrix{out, m, n, n};
     const bool out_tma = output_tma(mo, out_half ? 2 : 4) && (!residual || aligned16(residual));
     const TileChoice choice = m <= 64 ? choose_few_rows(c.ctx, m, n, k_blocks)
-                                      : choose_tile(c.ctx, {m, n, k_blocks, 1, bytes_out, out_tma, true, true});
+                                      : choose_tile(c.ctx, {m, n, k_blocks, 1, bytes_out, out_tma, true, !po.used && !pz.used});
     l.tile = choice.tile;
     l.splits = choice.splits;
     l.epilogue = is_swap(choice.tile) ? kEpiStoreT : kEpiStore;
@@ -508,8 +558,9 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     p.activation = activation;
     p.out_tma = out_tma ? 1 : 0;
     if (preact) {
-        const Matrix mz{preact, m, n, n};
-        p.preact = preact;
+        const Matrix mz = pz.used ? pz.matrix(c) : Matrix{preact, m, n, n};
+        p.preact = const_cast<void *>(mz.ptr);
+        p.preact_pitch = mz.pitch;
         p.preact_half = preact_half ? 1 : 0;
         p.preact_tma = output_tma(mz, preact_half ? 2 : 4) ? 1 : 0;
         if (p.preact_tma && !output_map(c, &l.map_z, mz, preact_half)) {
@@ -519,7 +570,7 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     }
     if (residual && set_residual(c, l, Matrix{residual, m, n, n}, out_half))
         return 1;
-    return enqueue(c, q);
+    return enqueue(c, q) || po.finish(c) || pz.finish(c) ? 1 : 0;
 }
 
 namespace {
@@ -530,19 +581,14 @@ struct ActGradPlan {
     int chunks = 1, rows_per_chunk = 0, cluster = 1, clusters = 1;
     void choose(const Context *ctx, int m, int n)
     {
-        // Row chunks of at least 32 rows.  Few columns: clusters of eight blocks that add up their
-        // sums, one if its chunks stay below 512 rows; many: about sixteen blocks per SM, summed
-        // by a second kernel (in clusters, 448 blocks of 4096 x 14336 took two waves).
+        // Eight row chunks of at least 32 rows, a cluster whose blocks add up their sums; where
+        // the columns are few and the rows many, several clusters and a second kernel.
         const int64_t column_blocks = (static_cast<int64_t>(n) + AG_COLS - 1) / AG_COLS;
         const int64_t most = std::max<int64_t>(1, m / 32);
-        int64_t wanted;
-        if (column_blocks * AG_CLUSTER <= ctx->sm_count) {
-            const int64_t all = std::max<int64_t>(1, std::min<int64_t>((m + 4095) / 4096, 2LL * ctx->sm_count / (column_blocks * AG_CLUSTER)));
-            wanted = most >= AG_CLUSTER ? AG_CLUSTER * std::min(all, most / AG_CLUSTER) : most;
-            cluster = static_cast<int>(std::min<int64_t>(wanted, AG_CLUSTER));
-        } else {
-            wanted = std::min<int64_t>(most, std::max<int64_t>(1, 16LL * ctx->sm_count / column_blocks));
-        }
+        const int64_t fill = std::max<int64_t>(1, 4LL * ctx->sm_count / (column_blocks * AG_CLUSTER));
+        const int64_t all = std::min<int64_t>((m + 2047) / 2048, fill);
+        const int64_t wanted = most >= AG_CLUSTER ? AG_CLUSTER * std::min(all, most / AG_CLUSTER) : most;
+        cluster = static_cast<int>(std::min<int64_t>(wanted, AG_CLUSTER));
         clusters = static_cast<int>(wanted / cluster);
         chunks = static_cast<int>(wanted);
         rows_per_chunk = static_cast<int>((m + wanted - 1) / wanted);
@@ -590,6 +636,11 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         dz_at = c.reserve(static_cast<size_t>(m * dz_pitch * e));
     else if (da || db)
         od.plan(c, dout, m, n);
+    PaddedOutput pa, pb;
+    if (da)
+        pa.plan(c, Matrix{da, m, k, k}, da_half);
+    if (db)
+        pb.plan(c, Matrix{db, k, n, n}, db_half);
     ActGradPlan plan;
     plan.choose(c.ctx, m, n);
     size_t partial_at = 0;
@@ -634,8 +685,8 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.k = n;
         q.launch.layout = kNT;
         q.set_tile(choose_tile(c.ctx, {q.m, q.n, (q.k + bk - 1) / bk, 1, da_half ? 2 : 4,
-                                       output_tma(Matrix{da, m, k, k}, da_half ? 2 : 4), true}));
-        if (set_output(c, q.launch, Matrix{da, m, k, k}, da_half) || enqueue(c, q))
+                                       output_tma(pa.matrix(c), da_half ? 2 : 4), true}));
+        if (set_output(c, q.launch, pa.matrix(c), da_half) || enqueue(c, q) || pa.finish(c))
             return 1;
     }
     if (db) {
@@ -647,8 +698,8 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.k = m;
         q.launch.layout = kTN;
         q.set_tile(choose_tile(c.ctx, {q.m, q.n, (q.k + bk - 1) / bk, 1, db_half ? 2 : 4,
-                                       output_tma(Matrix{db, k, n, n}, db_half ? 2 : 4), true}));
-        if (set_output(c, q.launch, Matrix{db, k, n, n}, db_half) || enqueue(c, q))
+                                       output_tma(pb.matrix(c), db_half ? 2 : 4), true}));
+        if (set_output(c, q.launch, pb.matrix(c), db_half) || enqueue(c, q) || pb.finish(c))
             return 1;
     }
     return 0;
@@ -828,13 +879,15 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
                                            output_tma(ma, da_half ? 2 : 4)}).tile;
         rows_plan.plan(c, groups, rows, kTileShapes[qa.launch.tile].bm, output_tma(ma, da_half ? 2 : 4) ? 1 : 0);
     }
+    PaddedOutput pb;
     if (db) {
         oa.plan(c, a, rows, k);
+        pb.plan(c, Matrix{db, k, n, n, groups, static_cast<int64_t>(k) * n}, db_half);
         const int64_t mean = (rows + groups - 1) / groups;
         qb.launch.layout = kTN;
         qb.launch.tile = choose_tile(c.ctx, {k, n, (mean + bk - 1) / bk, groups, db_half ? 2 : 4,
-                                           output_tma(Matrix{db, k, n, n, groups, static_cast<int64_t>(k) * n},
-                                                      db_half ? 2 : 4)}).tile;
+                                           pb.used || output_tma(pb.padded, db_half ? 2 : 4), false, false,
+                                           true}).tile;
         k_plan.plan(c, groups, rows, 0, 2);
     }
     if (c.allocate() || prepare_operands(c, {&od, &ob, &oa}))
@@ -864,7 +917,7 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
             cudaGetLastError();
             return c.failed("cuTensorMapEncodeTiled rejected an operand");
         }
-        if (set_output(c, qb.launch, Matrix{db, k, n, n, groups, static_cast<int64_t>(k) * n}, db_half))
+        if (set_output(c, qb.launch, pb.matrix(c), db_half))
             return 1;
         gb = k_plan.fill(c, offsets, offsets64, groups, rows, qb.launch.p,
                          ((k + t.bm - 1) / t.bm) * ((static_cast<int64_t>(n) + t.bn - 1) / t.bn),
@@ -874,7 +927,7 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
     if (db ? enqueue_plans(c, map0, map1, map_da, gb, da ? &ga : nullptr)
            : enqueue_plans(c, map_da, map_da, map_da, ga, nullptr))
         return 1;
-    if ((da && enqueue(c, qa)) || (db && enqueue(c, qb)))
+    if ((da && enqueue(c, qa)) || (db && (enqueue(c, qb) || pb.finish(c))))
         return 1;
     return 0;
 }
@@ -984,6 +1037,9 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
     Operand oh, ow;
     oh.plan(c, hidden, m, k);
     ow.plan(c, weight, k, v);
+    PaddedOutput pw;
+    if (dweight)
+        pw.plan(c, Matrix{dweight, k, v, v}, dw_half);
     const size_t dz_at = c.reserve(static_cast<size_t>(m) * width * e);
     // dH is summed over the pieces in FP32: in the output itself where it is FP32.
     const bool own_sum = dhidden && dh_half && pieces > 1;
@@ -1047,12 +1103,13 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = cols;
             q.k = m;
             q.launch.layout = kTN;
-            const Matrix dw{static_cast<uint8_t *>(dweight) + v0 * (dw_half ? 2 : 4), k, cols, v};
+            const Matrix &all = pw.matrix(c);
+            const Matrix dw{static_cast<const uint8_t *>(all.ptr) + v0 * (dw_half ? 2 : 4), k, cols, all.pitch};
             q.set_tile(choose_tile(c.ctx, {k, cols, (m + bk - 1) / bk, 1, dw_half ? 2 : 4,
                                            output_tma(dw, dw_half ? 2 : 4), true}));
             if (set_output(c, q.launch, dw, dw_half) || enqueue(c, q))
                 return 1;
         }
     }
-    return 0;
+    return pw.finish(c);
 }

@@ -4,11 +4,38 @@
 
 #include <cuda.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "ptx.cuh"
 #include "tc_ops.cuh"
 
 namespace b200 {
+
+// 16 bytes from an address aligned to ELEM bytes: words where it starts on 4 bytes, else a
+// half word, three words and a half word shifted into place, so that nothing outside the
+// 16 bytes is read.
+template <int ELEM>
+__device__ __forceinline__ uint4 load_16_bytes(const uint8_t *from)
+{
+    uint4 q;
+    if (ELEM == 2 && (reinterpret_cast<uintptr_t>(from) & 2u)) {
+        const uint32_t w0 = *reinterpret_cast<const uint16_t *>(from);
+        const uint32_t w1 = *reinterpret_cast<const uint32_t *>(from + 2);
+        const uint32_t w2 = *reinterpret_cast<const uint32_t *>(from + 6);
+        const uint32_t w3 = *reinterpret_cast<const uint32_t *>(from + 10);
+        const uint32_t w4 = *reinterpret_cast<const uint16_t *>(from + 14);
+        q.x = w0 | (w1 << 16);
+        q.y = (w1 >> 16) | (w2 << 16);
+        q.z = (w2 >> 16) | (w3 << 16);
+        q.w = (w3 >> 16) | (w4 << 16);
+    } else {
+        q.x = reinterpret_cast<const uint32_t *>(from)[0];
+        q.y = reinterpret_cast<const uint32_t *>(from)[1];
+        q.z = reinterpret_cast<const uint32_t *>(from)[2];
+        q.w = reinterpret_cast<const uint32_t *>(from)[3];
+    }
+    return q;
+}
 
 // ---------------------------------------------------------------- operand copy
 constexpr int RP_THREADS = 256;
@@ -33,9 +60,7 @@ inline RepackJob repack_job(const void *src, void *dst, int64_t rows, int64_t co
 }
 
 // rows x cols of ELEM-byte elements at any element alignment -> rows x pitch with pitch a
-// multiple of 16 bytes, zero in the added columns.  Each thread writes 16-byte chunks; a
-// source that starts between two 4-byte words is read as a half word, three words and a
-// half word and shifted into place, so that nothing outside the matrix is read.
+// multiple of 16 bytes, zero in the added columns; each thread writes 16-byte chunks.
 // Up to two matrices in one launch.
 template <int ELEM>
 __global__ void __launch_bounds__(RP_THREADS) repack_kernel(const RepackJob job0, const RepackJob job1)
@@ -57,22 +82,7 @@ __global__ void __launch_bounds__(RP_THREADS) repack_kernel(const RepackJob job0
         const uint8_t *from = job.src + (row * cols + c * kPer) * ELEM;
         uint4 q;
         if ((c + 1) * kPer <= cols) {
-            if (ELEM == 2 && (reinterpret_cast<uintptr_t>(from) & 2u)) {
-                const uint32_t w0 = *reinterpret_cast<const uint16_t *>(from);
-                const uint32_t w1 = *reinterpret_cast<const uint32_t *>(from + 2);
-                const uint32_t w2 = *reinterpret_cast<const uint32_t *>(from + 6);
-                const uint32_t w3 = *reinterpret_cast<const uint32_t *>(from + 10);
-                const uint32_t w4 = *reinterpret_cast<const uint16_t *>(from + 14);
-                q.x = w0 | (w1 << 16);
-                q.y = (w1 >> 16) | (w2 << 16);
-                q.z = (w2 >> 16) | (w3 << 16);
-                q.w = (w3 >> 16) | (w4 << 16);
-            } else {
-                q.x = reinterpret_cast<const uint32_t *>(from)[0];
-                q.y = reinterpret_cast<const uint32_t *>(from)[1];
-                q.z = reinterpret_cast<const uint32_t *>(from)[2];
-                q.w = reinterpret_cast<const uint32_t *>(from)[3];
-            }
+            q = load_16_bytes<ELEM>(from);
         } else {
             uint32_t words[4] = {};
 #pragma unroll
@@ -89,10 +99,49 @@ __global__ void __launch_bounds__(RP_THREADS) repack_kernel(const RepackJob job0
     }
 }
 
+// The way back for outputs that TMA cannot write: rows x pitch in scratch (rows on 16
+// bytes) -> rows x cols without padding at any element alignment.  Each thread writes
+// aligned 16-byte chunks of the destination, which may hold the end of one row and the
+// start of the next, element by element where they do or at either end of the matrix.
+template <int ELEM>
+__global__ void __launch_bounds__(RP_THREADS) unpack_kernel(const uint8_t *src, uint8_t *dst, int64_t rows,
+                                                            int64_t cols, int64_t pitch)
+{
+    using Word = std::conditional_t<ELEM == 2, uint16_t, uint32_t>;
+    constexpr int kPer = 16 / ELEM;
+    wait_for_prior_grid();
+    allow_next_grid();
+    const int64_t total = rows * cols;
+    const int64_t head = (16 - (reinterpret_cast<uintptr_t>(dst) & 15u)) % 16 / ELEM;     // elements before the first chunk
+    const int64_t chunks = (total - head + kPer - 1) / kPer + (head ? 1 : 0);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * RP_THREADS + threadIdx.x; i < chunks;
+         i += static_cast<int64_t>(gridDim.x) * RP_THREADS) {
+        const int64_t first = head + (i - (head ? 1 : 0)) * kPer;       // negative in the chunk before the first whole one
+        const int64_t begin = first < 0 ? 0 : first, end = min(first + kPer, total);
+        const int64_t row = total < (int64_t{1} << 31) ? static_cast<int64_t>(static_cast<uint32_t>(begin) /
+                                                                              static_cast<uint32_t>(cols))
+                                                       : begin / cols;
+        const int64_t col = begin - row * cols;
+        if (end - first == kPer && begin == first && col + kPer <= cols) {
+            *reinterpret_cast<uint4 *>(dst + first * ELEM) = load_16_bytes<ELEM>(src + (row * pitch + col) * ELEM);
+        } else {
+            int64_t r = row, c = col;
+            for (int64_t e = begin; e < end; ++e) {
+                reinterpret_cast<Word *>(dst)[e] = reinterpret_cast<const Word *>(src)[r * pitch + c];
+                if (++c == cols) {
+                    c = 0;
+                    ++r;
+                }
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------- activation and bias gradient
 constexpr int AG_THREADS = 256;
-constexpr int AG_COLS = 256;      // columns per block: 32 lanes x 8
-constexpr int AG_ROWS = 2;        // rows a thread has in flight
+constexpr int AG_COLS = 64;       // columns per block: 8 lanes x 8, so that a warp covers four rows
+constexpr int AG_PASS = 32;       // rows of one pass of a block
+constexpr int AG_ROWS = 4;        // rows a thread has in flight
 constexpr int AG_CLUSTER = 8;     // row chunks whose sums are joined in one cluster
 
 struct ActGradParams {
@@ -108,115 +157,140 @@ struct ActGradParams {
 };
 
 // dz = dout * act'(z) in the input format, and the column sums of the unrounded FP32
-// values: each thread takes 8 columns and every eighth row of its block's chunk, two rows
-// in flight; a block's eight warps join through its shared memory and the blocks of a
-// cluster (along y) through each other's, both in a fixed order.
+// values: each thread takes 8 columns and every 32nd row of its block's chunk, four rows in
+// flight; a block's 32 row positions join through its shared memory and the blocks of a
+// cluster (along y) through each other's, both in a fixed order.  Bound by HBM: two reads
+// and a write.
 template <int FMT>
-__global__ void __launch_bounds__(AG_THREADS) act_grad_kernel(const ActGradParams p)
+__global__ void __launch_bounds__(AG_THREADS, 4) act_grad_kernel(const ActGradParams p)
 {
     using Type = OpType<FMT>;
     using T = typename Type::T;
-    __shared__ float sums[8][AG_COLS];
-    __shared__ __align__(16) float block_sums[AG_COLS];
+    __shared__ float sums[AG_PASS][AG_COLS + 1];
+    __shared__ float block_sums[AG_COLS];
     wait_for_prior_grid();
     allow_next_grid();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int col0 = static_cast<int>(blockIdx.x) * AG_COLS + lane * 8;
-    const long long row_begin = static_cast<long long>(blockIdx.y) * p.rows_per_chunk;
-    const int row_end = static_cast<int>(min(static_cast<long long>(p.m), row_begin + p.rows_per_chunk));
-    const bool vec = p.vec && col0 + 8 <= p.n;
+    const int place = threadIdx.x >> 3;            // row within a pass
+    const int local = (threadIdx.x & 7) * 8;       // first column within the block
+    const int col0 = static_cast<int>(blockIdx.x) * AG_COLS + local;
+    const int64_t row_begin = static_cast<int64_t>(blockIdx.y) * p.rows_per_chunk;
+    const int row_end = static_cast<int>(min(static_cast<int64_t>(p.m), row_begin + p.rows_per_chunk));
+    const bool whole = col0 + 8 <= p.n;
     float sum[8] = {};
-    auto read = [&](const void *src, bool half, int row, float (&x)[8]) {
-        const long long at = static_cast<long long>(row) * p.n + col0;
-        if (vec && half) {
-            if constexpr (FMT != kOpTF32) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(static_cast<const T *>(src) + at);
-                const T *h = reinterpret_cast<const T *>(&q);
+    auto widen = [&](const uint4 &q, float (&x)[8]) {
+        if constexpr (FMT != kOpTF32) {
+            const T *h = reinterpret_cast<const T *>(&q);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] = Type::to(h[e]);
-            }
-        } else if (vec) {
-            const float4 q0 = reinterpret_cast<const float4 *>(static_cast<const float *>(src) + at)[0];
-            const float4 q1 = reinterpret_cast<const float4 *>(static_cast<const float *>(src) + at)[1];
-            x[0] = q0.x, x[1] = q0.y, x[2] = q0.z, x[3] = q0.w;
-            x[4] = q1.x, x[5] = q1.y, x[6] = q1.z, x[7] = q1.w;
-        } else {
+            for (int e = 0; e < 8; ++e)
+                x[e] = Type::to(h[e]);
+        }
+    };
+    auto read = [&](const void *src, bool half, int row, float (&x)[8]) {
+        const int64_t at = static_cast<int64_t>(row) * p.n + col0;
+        if (!whole) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 x[e] = col0 + e < p.n ? (half ? Type::to(static_cast<const T *>(src)[at + e])
                                               : static_cast<const float *>(src)[at + e])
                                       : 0.0f;
+        } else if (half) {
+            const uint8_t *from = static_cast<const uint8_t *>(src) + at * 2;
+            widen(p.vec ? *reinterpret_cast<const uint4 *>(from) : load_16_bytes<2>(from), x);
+        } else {
+            const uint8_t *from = static_cast<const uint8_t *>(src) + at * 4;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint4 q = p.vec ? reinterpret_cast<const uint4 *>(from)[h] : load_16_bytes<4>(from + 16 * h);
+                x[4 * h] = __uint_as_float(q.x);
+                x[4 * h + 1] = __uint_as_float(q.y);
+                x[4 * h + 2] = __uint_as_float(q.z);
+                x[4 * h + 3] = __uint_as_float(q.w);
+            }
         }
     };
     op_with_activation(p.preact ? p.activation : kActNone, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
         if (col0 >= p.n)
             return;
-        for (int row = static_cast<int>(row_begin) + warp; row < row_end; row += 8 * AG_ROWS) {
-            float d[AG_ROWS][8], z[AG_ROWS][8];
+        // dz of 8 columns of a row: summed, and stored rounded.
+        auto finish = [&](int row, float (&d)[8], float (&z)[8]) {
 #pragma unroll
-            for (int i = 0; i < AG_ROWS; ++i)
-                if (row + 8 * i < row_end) {
-                    read(p.dout, FMT != kOpTF32, row + 8 * i, d[i]);
-                    if (ACT != kActNone)
-                        read(p.preact, p.preact_half != 0, row + 8 * i, z[i]);
-                }
-#pragma unroll
-            for (int i = 0; i < AG_ROWS; ++i) {
-                if (row + 8 * i >= row_end)
-                    break;
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    float2 dz = make_float2(d[i][e], d[i][e + 1]);
-                    if (ACT != kActNone)
-                        dz = __fmul2_rn(dz, op_activation_slope<ACT>(make_float2(z[i][e], z[i][e + 1])));
-                    d[i][e] = dz.x;
-                    d[i][e + 1] = dz.y;
-                    sum[e] += dz.x;
-                    sum[e + 1] += dz.y;
-                }
-                if (p.dz) {
-                    T *dst = static_cast<T *>(p.dz) + (row + 8 * i) * p.dz_pitch + col0;
-                    if (col0 + 8 <= p.dz_pitch) {       // rows are padded to 16 bytes
-                        if constexpr (FMT == kOpTF32) {
-                            reinterpret_cast<float4 *>(dst)[0] = make_float4(d[i][0], d[i][1], d[i][2], d[i][3]);
-                            reinterpret_cast<float4 *>(dst)[1] = make_float4(d[i][4], d[i][5], d[i][6], d[i][7]);
-                        } else {
-                            *reinterpret_cast<uint4 *>(dst) =
-                                make_uint4(Type::pack(d[i][0], d[i][1]), Type::pack(d[i][2], d[i][3]),
-                                           Type::pack(d[i][4], d[i][5]), Type::pack(d[i][6], d[i][7]));
-                        }
-                    } else {
-                        for (int e = 0; e < 8 && col0 + e < p.dz_pitch; ++e)
-                            dst[e] = Type::from(d[i][e]);
-                    }
+            for (int e = 0; e < 8; e += 2) {
+                float2 dz = make_float2(d[e], d[e + 1]);
+                if (ACT != kActNone)
+                    dz = __fmul2_rn(dz, op_activation_slope<ACT>(make_float2(z[e], z[e + 1])));
+                d[e] = dz.x;
+                d[e + 1] = dz.y;
+                sum[e] += dz.x;
+                sum[e + 1] += dz.y;
+            }
+            if (p.dz) {
+                T *dst = static_cast<T *>(p.dz) + row * p.dz_pitch + col0;
+                // Rows in scratch are padded to 128 bytes: 8 columns always fit.
+                if constexpr (FMT == kOpTF32) {
+                    reinterpret_cast<float4 *>(dst)[0] = make_float4(d[0], d[1], d[2], d[3]);
+                    reinterpret_cast<float4 *>(dst)[1] = make_float4(d[4], d[5], d[6], d[7]);
+                } else {
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(Type::pack(d[0], d[1]), Type::pack(d[2], d[3]),
+                                                                 Type::pack(d[4], d[5]), Type::pack(d[6], d[7]));
                 }
             }
+        };
+        int row = static_cast<int>(row_begin) + place;
+        if (FMT != kOpTF32 && whole && p.vec && (ACT == kActNone || p.preact_half)) {
+            // All loads of AG_ROWS rows before the first use: with a branch around each load a
+            // thread waited for one at a time (4096 x 14336: 132 us against 97 us).
+            for (; row + AG_PASS * (AG_ROWS - 1) < row_end; row += AG_PASS * AG_ROWS) {
+                uint4 dq[AG_ROWS], zq[AG_ROWS];
+#pragma unroll
+                for (int i = 0; i < AG_ROWS; ++i) {
+                    const int64_t at = static_cast<int64_t>(row + AG_PASS * i) * p.n + col0;
+                    dq[i] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.dout) + at);
+                    if (ACT != kActNone)
+                        zq[i] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.preact) + at);
+                }
+#pragma unroll
+                for (int i = 0; i < AG_ROWS; ++i) {
+                    float d[8], z[8];
+                    widen(dq[i], d);
+                    if (ACT != kActNone)
+                        widen(zq[i], z);
+                    finish(row + AG_PASS * i, d, z);
+                }
+            }
+        }
+        for (; row < row_end; row += AG_PASS) {
+            float d[8], z[8];
+            read(p.dout, FMT != kOpTF32, row, d);
+            if (ACT != kActNone)
+                read(p.preact, p.preact_half != 0, row, z);
+            finish(row, d, z);
         }
     });
     if (!p.dbias)
         return;      // the same for the whole cluster
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-        sums[warp][lane * 8 + e] = sum[e];
+        sums[place][local + e] = sum[e];
     __syncthreads();
-    float total = 0.0f;
+    if (threadIdx.x < AG_COLS) {
+        float total = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        total += sums[i][threadIdx.x];
-    block_sums[threadIdx.x] = total;
+        for (int i = 0; i < AG_PASS; ++i)
+            total += sums[i][threadIdx.x];
+        block_sums[threadIdx.x] = total;
+    }
     // The cluster's first block adds its blocks' sums in order.
     cluster_sync_all();
     uint32_t blocks;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
     const int col = static_cast<int>(blockIdx.x) * AG_COLS + threadIdx.x;
-    if (cluster_cta_rank() == 0 && col < p.n) {
-        total = 0.0f;
+    if (cluster_cta_rank() == 0 && threadIdx.x < AG_COLS && col < p.n) {
+        float total = 0.0f;
         for (uint32_t j = 0; j < blocks; ++j)
             total += __uint_as_float(ld_shared_cluster_u32(map_to_cta(smem_addr(block_sums + threadIdx.x), j)));
         if (p.partial)
-            p.partial[static_cast<long long>(blockIdx.y / blocks) * p.n + col] = total;
+            p.partial[static_cast<int64_t>(blockIdx.y / blocks) * p.n + col] = total;
         else if (p.dbias_half)
             static_cast<T *>(p.dbias)[col] = Type::from(total);
         else

@@ -127,7 +127,8 @@ struct OpParams {
     long long out_pitch, out_slab;    // elements between rows / between groups' outputs
     int out_half;                     // 1: the 16-bit input format, 0: FP32
     int out_tma;                      // 1: TMA can write out, and its rows and the residual's start on 16 bytes
-    void *preact;                     // D + bias before the activation, or null (pitch n)
+    void *preact;                     // D + bias before the activation, or null
+    long long preact_pitch;
     int preact_half, preact_tma;
     const void *residual;             // null, or added after the activation (pitch out_pitch)
     int residual_half;
@@ -264,6 +265,15 @@ __device__ __forceinline__ float op_exp2(float x)
     return y;
 }
 
+// 1 / x by the hardware's approximation (1 ulp; zero for results below the smallest normal
+// number).
+__device__ __forceinline__ float op_reciprocal(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // The normal distribution function by Abramowitz and Stegun's rational approximation of
 // erf (Handbook of Mathematical Functions, 7.1.26; absolute error of erf 1.5e-7), half
 // the instructions of erff: with x = |z| / sqrt 2 and t = 1 / (1 + 0.3275911 x), 1 -
@@ -273,7 +283,7 @@ __device__ __forceinline__ float2 op_normal_cdf(float2 z, float2 &e)
 {
     const float2 a = make_float2(fabsf(z.x), fabsf(z.y));
     const float2 d = __ffma2_rn(make_float2(0.23164189f, 0.23164189f), a, make_float2(1.0f, 1.0f));
-    const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+    const float2 t = make_float2(op_reciprocal(d.x), op_reciprocal(d.y));
     const float2 x = __fmul2_rn(__fmul2_rn(a, make_float2(-0.72134752f, -0.72134752f)), a);   // -z^2 / 2 log2 e
     e = make_float2(op_exp2(x.x), op_exp2(x.y));
     float2 q = __ffma2_rn(t, make_float2(0.5307027145f, 0.5307027145f), make_float2(-0.7265760135f, -0.7265760135f));
@@ -300,11 +310,11 @@ __device__ __forceinline__ float2 op_activation(float2 z)
         const float2 p = __ffma2_rn(__fmul2_rn(z, z), make_float2(-0.10294324f, -0.10294324f),
                                     make_float2(-2.3022082f, -2.3022082f));
         const float2 x = __fmul2_rn(z, p);
-        return make_float2(__fdividef(z.x, 1.0f + op_exp2(x.x)), __fdividef(z.y, 1.0f + op_exp2(x.y)));
+        return make_float2(z.x * op_reciprocal(1.0f + op_exp2(x.x)), z.y * op_reciprocal(1.0f + op_exp2(x.y)));
     }
     if constexpr (ACT == kActSilu) {
         const float2 x = __fmul2_rn(z, make_float2(-1.44269504f, -1.44269504f));
-        return make_float2(__fdividef(z.x, 1.0f + op_exp2(x.x)), __fdividef(z.y, 1.0f + op_exp2(x.y)));
+        return make_float2(z.x * op_reciprocal(1.0f + op_exp2(x.x)), z.y * op_reciprocal(1.0f + op_exp2(x.y)));
     }
     return z;
 }
@@ -325,14 +335,14 @@ __device__ __forceinline__ float2 op_activation_slope(float2 z)
         const float2 zz = __fmul2_rn(z, z);
         const float2 x = __fmul2_rn(z, __ffma2_rn(zz, make_float2(-0.10294324f, -0.10294324f),
                                                   make_float2(-2.3022082f, -2.3022082f)));
-        const float2 s = make_float2(__fdividef(1.0f, 1.0f + op_exp2(x.x)), __fdividef(1.0f, 1.0f + op_exp2(x.y)));
+        const float2 s = make_float2(op_reciprocal(1.0f + op_exp2(x.x)), op_reciprocal(1.0f + op_exp2(x.y)));
         const float2 du = __ffma2_rn(zz, make_float2(0.21406446f, 0.21406446f), make_float2(1.59576912f, 1.59576912f));
         const float2 rest = __ffma2_rn(make_float2(-s.x, -s.y), s, s);         // s (1 - s)
         return __ffma2_rn(__fmul2_rn(z, rest), du, s);
     }
     if constexpr (ACT == kActSilu) {
         const float2 x = __fmul2_rn(z, make_float2(-1.44269504f, -1.44269504f));
-        const float2 s = make_float2(__fdividef(1.0f, 1.0f + op_exp2(x.x)), __fdividef(1.0f, 1.0f + op_exp2(x.y)));
+        const float2 s = make_float2(op_reciprocal(1.0f + op_exp2(x.x)), op_reciprocal(1.0f + op_exp2(x.y)));
         const float2 rest = __ffma2_rn(make_float2(-s.x, -s.y), s, s);
         return __ffma2_rn(z, rest, s);
     }
@@ -545,13 +555,14 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         constexpr int N = std::extent<std::remove_reference_t<decltype(v)>>::value;
         const long long at = row * p.out_pitch + col, step = row_step * p.out_pitch + col_step;
         if (p.preact) {
+            const long long z_at = row * p.preact_pitch + col, z_step = row_step * p.preact_pitch + col_step;
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 if (i < count) {
                     if (p.preact_half)
-                        static_cast<T *>(p.preact)[at + i * step] = Type::from(v[i]);
+                        static_cast<T *>(p.preact)[z_at + i * z_step] = Type::from(v[i]);
                     else
-                        static_cast<float *>(p.preact)[at + i * step] = v[i];
+                        static_cast<float *>(p.preact)[z_at + i * z_step] = v[i];
                 }
         }
         op_with_activation(p.activation, [&](auto act) {
@@ -587,10 +598,11 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 else
                     static_cast<float *>(p.out)[at] = nan;
                 if (EPI != kEpiSoftmaxGrad && p.preact) {
+                    const long long z_at = row * p.preact_pitch + col;
                     if (p.preact_half)
-                        static_cast<T *>(p.preact)[at] = Type::from(nan);
+                        static_cast<T *>(p.preact)[z_at] = Type::from(nan);
                     else
-                        static_cast<float *>(p.preact)[at] = nan;
+                        static_cast<float *>(p.preact)[z_at] = nan;
                 }
             }
     };
@@ -1092,7 +1104,8 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                             }
                         }
                         if (p.preact)
-                            emit_columns(v, &map_z, 0, p.preact_tma != 0, p.preact_half != 0, p.preact, 0, p.n, col0, nullptr);
+                            emit_columns(v, &map_z, 0, p.preact_tma != 0, p.preact_half != 0, p.preact, 0,
+                                         p.preact_pitch, col0, nullptr);
                         op_with_activation(p.activation, [&](auto act) {
                             op_activate<decltype(act)::value>(v);
                         });
