@@ -250,7 +250,10 @@ double tile_cycles(const Context *ctx, int tile, int splits, const TileProblem &
     const double tiles = static_cast<double>((side_m + t.bm - 1) / t.bm * ((side_n + t.bn - 1) / t.bn) * q.groups);
     const double units = t.ctas == 2 ? ctx->max_pairs : ctx->sm_count;
     const double active = splits > 1 ? tiles * splits : t.ctas * std::min(tiles, units);
-    const double rounds = splits > 1 ? 1.0 : std::max(1.0, std::ceil(tiles / units));
+    double rounds = splits > 1 ? 1.0 : std::max(1.0, std::ceil(tiles / units));
+    // A pair's short last round runs as half tiles (enqueue).
+    if (t.ctas == 2 && q.groups == 1 && std::fmod(tiles, units) > 0.0 && std::fmod(tiles, units) <= units / 2)
+        rounds = std::floor(tiles / units) + 0.6;
     const double bytes = static_cast<double>(OP_BM + t.bn / t.ctas) * OP_ROW_BYTES;
     const double k_cycles = std::max({2.0 * t.bn, 140.0, bytes / 70.0, active * bytes / 9300.0});
     const double epilogue = kEpilogue[tile] + (q.out_tma ? 0.0 : kRowStores[tile]);
@@ -277,8 +280,9 @@ bool can_split(const Context *ctx, int log_splits, int64_t tiles, int64_t k_bloc
 }
 
 // The tile kind and K split with the fewest estimated cycles.  Transposed kinds are
-// considered where one wave holds all their tiles: their stores go element by element
-// (2048 x 256 x 45056 with a residual took 1236 us on 128 x 128 tiles transposed, 146 us not).
+// considered for up to 64 rows, and where one wave holds all their tiles: their stores go
+// element by element (2048 x 256 x 45056 with a residual took 1236 us on 128 x 128 tiles
+// transposed, 146 us not).
 TileChoice choose_tile(const Context *ctx, const TileProblem &q)
 {
     TileChoice best{kSingle64, 1};
@@ -290,7 +294,7 @@ TileChoice choose_tile(const Context *ctx, const TileProblem &q)
             continue;
         const int64_t side_m = swap ? q.n : q.m, side_n = swap ? q.m : q.n;
         const int64_t tiles = (side_m + t.bm - 1) / t.bm * ((side_n + t.bn - 1) / t.bn) * q.groups;
-        if (swap && tiles > ctx->sm_count)
+        if (swap && q.m > 64 && tiles > ctx->sm_count)
             continue;
         for (int i = 0; i < (q.splittable && t.ctas == 1 ? 4 : 1); ++i) {
             if (i > 0 && !can_split(ctx, i, tiles, q.k_blocks))
@@ -302,18 +306,6 @@ TileChoice choose_tile(const Context *ctx, const TileProblem &q)
             }
         }
     }
-    return best;
-}
-
-// At most 64 rows: the transposed tile that holds them, and the most K splits that fit with
-// four K blocks each (bound by the weight's bytes: more SMs streaming them is what counts).
-TileChoice choose_few_rows(const Context *ctx, int64_t m, int64_t n, int64_t k_blocks)
-{
-    TileChoice best{m <= 16 ? kSwap16 : m <= 32 ? kSwap32 : kSwap64, 1};
-    const int64_t tiles = (n + OP_BM - 1) / OP_BM;
-    for (int i = 1; i < 4; ++i)
-        if (can_split(ctx, i, tiles, k_blocks) && (k_blocks >> i) >= 4)
-            best.splits = 1 << i;
     return best;
 }
 
@@ -380,6 +372,18 @@ int enqueue(Call &c, Product &q)
     const int64_t per_group = static_cast<int64_t>(p.num_m_blocks) * p.num_n_blocks;
     p.per_raster = divisor(std::min<int64_t>(per_raster, 0x7fffffff));
     p.per_group = divisor(std::min<int64_t>(per_group, 0x7fffffff));
+    // A last round that leaves half of the pairs without a tile runs as half tiles on twice as
+    // many of them (4096 x 14336 . 14336 x 4096: 256 tiles on 74 pairs, 3.5 rounds in place
+    // of 4).
+    p.full_tiles = p.num_tiles;
+    if (l.tile == kPair256 && p.grouping == kUngrouped && l.epilogue != kEpiLse) {
+        const int rest = p.num_tiles % c.ctx->max_pairs;
+        if (2 * rest <= c.ctx->max_pairs) {
+            p.full_tiles = p.num_tiles - rest;
+            p.num_tiles += rest;
+            tiles = p.num_tiles;
+        }
+    }
     p.status = c.ctx->status;
     p.wait_limit_ns = wait_limit(c.ctx);
     const int64_t units = t.ctas == 2 ? c.ctx->max_pairs : c.ctx->sm_count;
@@ -545,8 +549,7 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     const int bytes_out = (out_half ? 2 : 4) * (residual ? 2 : 1) + (preact ? (preact_half ? 2 : 4) : 0);
     const Matrix mo = po.used ? po.matrix(c) : Matrix{out, m, n, n};
     const bool out_tma = output_tma(mo, out_half ? 2 : 4) && (!residual || aligned16(residual));
-    const TileChoice choice = m <= 64 ? choose_few_rows(c.ctx, m, n, k_blocks)
-                                      : choose_tile(c.ctx, {m, n, k_blocks, 1, bytes_out, out_tma, true, !po.used && !pz.used});
+    const TileChoice choice = choose_tile(c.ctx, {m, n, k_blocks, 1, bytes_out, out_tma, true, !po.used && !pz.used});
     l.tile = choice.tile;
     l.splits = choice.splits;
     l.epilogue = is_swap(choice.tile) ? kEpiStoreT : kEpiStore;
@@ -779,8 +782,11 @@ int check_groups(Call &c, int groups, int rows, int k, int n, const void *offset
     return 0;
 }
 
-// Rows per tile follow the mean group: with few rows they take the MMA's N side (16 to
-// 128 wide) and the weight's columns its M side, so that a tile wastes little.
+// Rows per tile follow the mean group: with few rows they take the MMA's N side (16 to 128
+// wide) and the weight's columns its M side, so that a tile wastes little (64 groups, 2048 x
+// 2816 BF16, one box: mean 50 rows 100 us on 64-row transposed tiles, 118 us on pairs; mean
+// 100 rows 124 us on 128-row ones, 129 us on pairs; mean 200 rows 198 and 163 us).  Larger
+// groups go by the cycles of a mean group.
 int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_t n, int64_t k_blocks, int bytes_out,
                         bool out_tma)
 {
@@ -793,7 +799,7 @@ int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_
         return kSwap64;
     if (mean <= 128)
         return kSwap128;
-    return choose_tile(ctx, {mean, n, k_blocks, groups, bytes_out, out_tma}).tile;
+    return choose_tile(ctx, {mean, n, k_blocks, groups, bytes_out, out_tma, false, true}).tile;
 }
 
 } // namespace

@@ -112,6 +112,7 @@ struct OpParams {
     int m, n;                 // rows and columns of the output (of one group in ragged-K mode)
     int num_m_blocks, num_n_blocks, num_k_blocks;   // M- and N-side tiles of D, K blocks
     int num_tiles;
+    int full_tiles;           // pairs: from here on two indices name the column halves of one tile
     int log_raster;           // log2 of the M-side tiles per raster group
     OpDivisor per_raster;     // raster x N-side tiles (transposed epilogue: M-side tiles)
     OpDivisor per_group;      // ragged-K mode: tiles of one group
@@ -390,6 +391,7 @@ __device__ __forceinline__ int op_label(const OpParams &p, int row)
 struct OpWhere {
     int m0, n0, group, nkb, k0, row_end;
     int n_block;
+    int cols;          // columns of the tile: BN, or half of it
 };
 
 template <int CTAS, int BN, bool SWAP>
@@ -397,6 +399,13 @@ __device__ __forceinline__ OpWhere op_where(int tile, int row_tile_count, int bk
 {
     constexpr int kBM = OP_BM * CTAS;
     OpWhere w;
+    int half = 0;
+    w.cols = BN;
+    if (CTAS == 2 && tile >= p.full_tiles) {
+        half = (tile - p.full_tiles) & 1;
+        tile = p.full_tiles + ((tile - p.full_tiles) >> 1);
+        w.cols = BN / 2;
+    }
     int local = tile;
     w.group = 0;
     w.k0 = 0;
@@ -429,7 +438,7 @@ __device__ __forceinline__ OpWhere op_where(int tile, int row_tile_count, int bk
         }
     }
     w.m0 = mb * kBM;
-    w.n0 = nb * BN;
+    w.n0 = nb * BN + half * (BN / 2);
     w.n_block = nb;
     if (p.grouping == kGroupedRows) {
         const OpRowTile t = p.row_tiles[SWAP ? nb : mb];
@@ -466,6 +475,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     constexpr bool kSplittable = CTAS == 1 && (EPI == kEpiStore || EPI == kEpiStoreT);
     constexpr int kGroupCols = BN / kGroups;              // D columns per epilogue warpgroup
     constexpr uint32_t kStageTx = static_cast<uint32_t>(CTAS) * (OP_A_STAGE + kBStage);
+    constexpr uint32_t kIdescHalfN = static_cast<uint32_t>((BN / 2) >> 3) << 17;
     // FP32 accumulator, formats, A MN-major (bit 15), B MN-major (bit 16), N >> 3, M >> 4.
     constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(FMT) << 7) | (static_cast<uint32_t>(FMT) << 10) |
                                 ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
@@ -639,8 +649,13 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 } else if (p.grouping == kGroupedRows) {
                     (kSwap ? za : zb) = w.group;
                 }
-                const int am = w.m0 + static_cast<int>(rank) * OP_BM;
-                const int bn = w.n0 + static_cast<int>(rank) * kBCols;
+                int am = w.m0 + static_cast<int>(rank) * OP_BM;
+                // Half a pair's tile past its group's rows: a coordinate past the matrix reads zeros, no
+                // memory, where the next group's rows would cost loads and power for nothing.
+                if (!A_MN && p.grouping == kGroupedRows && !kSwap && am >= w.row_end)
+                    am = p.m;
+                // Half a tile's columns are the first halves of the same boxes.
+                const int bn = w.n0 + static_cast<int>(rank) * (w.cols / CTAS);
                 for (int kb = kb_begin; kb < kb_end(w.nkb); ++kb) {
                     // In a pair this wait keeps the fixed limit: both CTAs then stop at the
                     // same stage and the leader's drain covers every copy of either.
@@ -727,6 +742,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+                const uint32_t idesc = kPair && w.cols != BN ? kIdesc - kIdescHalfN : kIdesc;     // half the N
                 const int nkb = kb_end(w.nkb);
                 for (int kb = kb_begin; kb < nkb; ++kb) {
                     if (!mbar_wait(full_bar(stage), phase, p.wait_limit_ns)) {
@@ -741,9 +757,9 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     for (int kk = 0; kk < kMmasPerStage; ++kk) {
                         const uint32_t accumulate = kb != kb_begin || kk != 0 ? 1u : 0u;
                         if constexpr (kPair)
-                            tc_mma_pair<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
+                            tc_mma_pair<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, idesc, accumulate);
                         else
-                            tc_mma<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, kIdesc, accumulate);
+                            tc_mma<kTF32>(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, idesc, accumulate);
                     }
                     commit(empty_bar(stage));
                     if (++stage == kStages) {
@@ -777,7 +793,6 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const int quarter = warp & 3;                 // TMEM lanes 32 * quarter .. +31
         const int r = quarter * 32 + lane;
         const int group = (warp - Tile::kFirstEpi) >> 2;   // epilogue warpgroup: D columns group * kGroupCols ..
-        const int gcol = group * kGroupCols;
         const int gthread = static_cast<int>(threadIdx.x) - 32 * Tile::kFirstEpi - 128 * group;
         // One thread of the warpgroup issues and waits for its TMA stores: the same lane at
         // every election (elect.sync is deterministic for a mask).
@@ -821,12 +836,14 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         for (int tile = tile_first; tile < tile_end; tile += tile_step) {
             const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
             const int row0 = w.m0 + static_cast<int>(rank) * OP_BM;     // D's first row in this CTA
+            const int group_cols = kPair ? w.cols / kGroups : kGroupCols;
+            const int gcol = group * group_cols;
             const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
                                    static_cast<uint32_t>(acc * BN + gcol);
             if constexpr (EPI == kEpiStore) {
                 if (p.bias) {       // the tile's bias, read once into shared memory
                     epilogue_sync();
-                    for (int c = gcol + gthread; c < gcol + kGroupCols; c += 128) {
+                    for (int c = gcol + gthread; c < gcol + group_cols; c += 128) {
                         const int col = w.n0 + c;
                         float b = 0.0f;
                         if (col < p.n)
@@ -853,7 +870,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             const int box_cols = p.out_half ? 64 : 32;
             auto fetch = [&](int u) {
                 const int col0 = w.n0 + gcol + u * box_cols;
-                if (u * box_cols >= kGroupCols || col0 >= p.n || row0 >= w.row_end)
+                if (u * box_cols >= group_cols || col0 >= p.n || row0 >= w.row_end)
                     return;
                 const uint32_t b = (stores + static_cast<uint32_t>(u) - box_done) % kBoxes;
                 if (issuer_warp && op_elect_one()) {
@@ -1171,10 +1188,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                 };
 #pragma unroll 1
-                for (int step = 0; step < kGroupCols / 64; ++step) {
+                for (int step = 0; step < group_cols / 64; ++step) {
                     float v[64];
                     load(v, step);
-                    if (step == kGroupCols / 64 - 1)
+                    if (step == group_cols / 64 - 1)
                         release();
                     process(v, step);
                 }
@@ -1274,8 +1291,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row0 + r] =
                             make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
                 } else {
-                    nan_elements(w, kSwap ? w.n0 + gcol : row0, kSwap ? kGroupCols : OP_BM, kSwap ? row0 : w.n0 + gcol,
-                                 kSwap ? OP_BM : kGroupCols, quarter, 4, lane);
+                    const int group_cols = kPair ? w.cols / kGroups : kGroupCols;
+                    const int first = w.n0 + group * group_cols;
+                    nan_elements(w, kSwap ? first : row0, kSwap ? group_cols : OP_BM, kSwap ? row0 : first,
+                                 kSwap ? OP_BM : group_cols, quarter, 4, lane);
                 }
             }
         }
