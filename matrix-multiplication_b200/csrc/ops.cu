@@ -242,7 +242,7 @@ struct TileProblem {
 double tile_cycles(const Context *ctx, int tile, int splits, const TileProblem &q)
 {
     constexpr double kEpilogue[] = {4400.0, 1100.0, 1140.0, 810.0, 800.0, 1170.0, 1170.0};
-    constexpr double kRowStores[] = {17800.0, 6100.0, 3050.0, 200.0, 400.0, 800.0, 1700.0};
+    constexpr double kRowStores[] = {6000.0, 2000.0, 1000.0, 200.0, 400.0, 800.0, 1700.0};
     constexpr double kFloor[] = {2500.0, 1480.0, 900.0, 0.0, 0.0, 0.0, 0.0};
     const TileShape &t = kTileShapes[tile];
     const bool swap = is_swap(tile);
@@ -407,45 +407,6 @@ int set_residual(Call &c, OpLaunch &l, const Matrix &residual, bool half)
     return 0;
 }
 
-// An output that TMA cannot write (odd row pitch or base) and that is large is computed
-// into scratch rows of whole 128 bytes and copied from there: the products' own
-// row-by-row stores cost more (768 x 32001 BF16 from K = 200: 79 us, of which 10 us are
-// its bytes).  Small ones keep them, without the second launch.
-struct PaddedOutput {
-    Matrix target, padded;
-    bool used = false, half = false;
-    size_t at = 0;
-
-    void plan(Call &c, const Matrix &out, bool out_half)
-    {
-        constexpr int64_t kSmallest = int64_t{4} << 20;       // bytes
-        const int elem = out_half ? 2 : 4;
-        target = out;
-        half = out_half;
-        padded = out;
-        used = !output_tma(out, elem) && out.pitch == out.cols && out.rows * out.groups * out.cols * elem >= kSmallest;
-        if (!used)
-            return;
-        padded.pitch = round_up(out.cols, 128 / elem);
-        padded.slab = padded.pitch * out.rows;
-        at = c.reserve(static_cast<size_t>(padded.slab * out.groups * elem));
-    }
-    const Matrix &matrix(Call &c)
-    {
-        if (used)
-            padded.ptr = c.scratch + at;
-        return padded;
-    }
-    int finish(Call &c) const
-    {
-        if (!used)
-            return 0;
-        const cudaError_t st = c.kernels().unpack(padded.ptr, const_cast<void *>(target.ptr), target.rows * target.groups,
-                                                  target.cols, padded.pitch, !half, c.ctx->sm_count, c.stream);
-        return st == cudaSuccess ? 0 : c.failed(st);
-    }
-};
-
 // Points a product's epilogue at an output matrix.
 int set_output(Call &c, OpLaunch &l, const Matrix &out, bool half)
 {
@@ -529,12 +490,6 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     Operand oa, ob;
     oa.plan(c, a, m, k);
     ob.plan(c, b, k, n);
-    // A residual is added by the row-by-row stores, so its output takes no padded rows.
-    PaddedOutput po, pz;
-    if (m > 64 && !residual)
-        po.plan(c, Matrix{out, m, n, n}, out_half);
-    if (m > 64 && preact && !residual)
-        pz.plan(c, Matrix{preact, m, n, n}, preact_half);
     if (c.allocate() || prepare_operands(c, {&oa, &ob}))
         return 1;
     Product q;
@@ -547,9 +502,9 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     const int bk = OP_ROW_BYTES / e;
     const int64_t k_blocks = (static_cast<int64_t>(k) + bk - 1) / bk;
     const int bytes_out = (out_half ? 2 : 4) * (residual ? 2 : 1) + (preact ? (preact_half ? 2 : 4) : 0);
-    const Matrix mo = po.used ? po.matrix(c) : Matrix{out, m, n, n};
+    const Matrix mo{out, m, n, n};
     const bool out_tma = output_tma(mo, out_half ? 2 : 4) && (!residual || aligned16(residual));
-    const TileChoice choice = choose_tile(c.ctx, {m, n, k_blocks, 1, bytes_out, out_tma, true, !po.used && !pz.used});
+    const TileChoice choice = choose_tile(c.ctx, {m, n, k_blocks, 1, bytes_out, out_tma, true, true});
     l.tile = choice.tile;
     l.splits = choice.splits;
     l.epilogue = is_swap(choice.tile) ? kEpiStoreT : kEpiStore;
@@ -561,8 +516,8 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     p.activation = activation;
     p.out_tma = out_tma ? 1 : 0;
     if (preact) {
-        const Matrix mz = pz.used ? pz.matrix(c) : Matrix{preact, m, n, n};
-        p.preact = const_cast<void *>(mz.ptr);
+        const Matrix mz{preact, m, n, n};
+        p.preact = preact;
         p.preact_pitch = mz.pitch;
         p.preact_half = preact_half ? 1 : 0;
         p.preact_tma = output_tma(mz, preact_half ? 2 : 4) ? 1 : 0;
@@ -573,7 +528,7 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     }
     if (residual && set_residual(c, l, Matrix{residual, m, n, n}, out_half))
         return 1;
-    return enqueue(c, q) || po.finish(c) || pz.finish(c) ? 1 : 0;
+    return enqueue(c, q);
 }
 
 namespace {
@@ -639,11 +594,7 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         dz_at = c.reserve(static_cast<size_t>(m * dz_pitch * e));
     else if (da || db)
         od.plan(c, dout, m, n);
-    PaddedOutput pa, pb;
-    if (da)
-        pa.plan(c, Matrix{da, m, k, k}, da_half);
-    if (db)
-        pb.plan(c, Matrix{db, k, n, n}, db_half);
+    const Matrix ma{da, m, k, k}, mb{db, k, n, n};
     ActGradPlan plan;
     plan.choose(c.ctx, m, n);
     size_t partial_at = 0;
@@ -688,8 +639,8 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.k = n;
         q.launch.layout = kNT;
         q.set_tile(choose_tile(c.ctx, {q.m, q.n, (q.k + bk - 1) / bk, 1, da_half ? 2 : 4,
-                                       output_tma(pa.matrix(c), da_half ? 2 : 4), true}));
-        if (set_output(c, q.launch, pa.matrix(c), da_half) || enqueue(c, q) || pa.finish(c))
+                                       output_tma(ma, da_half ? 2 : 4), true}));
+        if (set_output(c, q.launch, ma, da_half) || enqueue(c, q))
             return 1;
     }
     if (db) {
@@ -701,8 +652,8 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         q.k = m;
         q.launch.layout = kTN;
         q.set_tile(choose_tile(c.ctx, {q.m, q.n, (q.k + bk - 1) / bk, 1, db_half ? 2 : 4,
-                                       output_tma(pb.matrix(c), db_half ? 2 : 4), true}));
-        if (set_output(c, q.launch, pb.matrix(c), db_half) || enqueue(c, q) || pb.finish(c))
+                                       output_tma(mb, db_half ? 2 : 4), true}));
+        if (set_output(c, q.launch, mb, db_half) || enqueue(c, q))
             return 1;
     }
     return 0;
@@ -784,7 +735,7 @@ int check_groups(Call &c, int groups, int rows, int k, int n, const void *offset
 
 // Rows per tile follow the mean group: with few rows they take the MMA's N side (16 to 128
 // wide) and the weight's columns its M side, so that a tile wastes little (64 groups, 2048 x
-// 2816 BF16, one box: mean 50 rows 100 us on 64-row transposed tiles, 118 us on pairs; mean
+// 2816 BF16: mean 50 rows 100 us on 64-row transposed tiles, 118 us on pairs; mean
 // 100 rows 124 us on 128-row ones, 129 us on pairs; mean 200 rows 198 and 163 us).  Larger
 // groups go by the cycles of a mean group.
 int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_t n, int64_t k_blocks, int bytes_out,
@@ -885,14 +836,13 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
                                            output_tma(ma, da_half ? 2 : 4)}).tile;
         rows_plan.plan(c, groups, rows, kTileShapes[qa.launch.tile].bm, output_tma(ma, da_half ? 2 : 4) ? 1 : 0);
     }
-    PaddedOutput pb;
+    const Matrix mb{db, k, n, n, groups, static_cast<int64_t>(k) * n};
     if (db) {
         oa.plan(c, a, rows, k);
-        pb.plan(c, Matrix{db, k, n, n, groups, static_cast<int64_t>(k) * n}, db_half);
         const int64_t mean = (rows + groups - 1) / groups;
         qb.launch.layout = kTN;
         qb.launch.tile = choose_tile(c.ctx, {k, n, (mean + bk - 1) / bk, groups, db_half ? 2 : 4,
-                                           pb.used || output_tma(pb.padded, db_half ? 2 : 4), false, false,
+                                           output_tma(mb, db_half ? 2 : 4), false, false,
                                            true}).tile;
         k_plan.plan(c, groups, rows, 0, 2);
     }
@@ -923,7 +873,7 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
             cudaGetLastError();
             return c.failed("cuTensorMapEncodeTiled rejected an operand");
         }
-        if (set_output(c, qb.launch, pb.matrix(c), db_half))
+        if (set_output(c, qb.launch, mb, db_half))
             return 1;
         gb = k_plan.fill(c, offsets, offsets64, groups, rows, qb.launch.p,
                          ((k + t.bm - 1) / t.bm) * ((static_cast<int64_t>(n) + t.bn - 1) / t.bn),
@@ -933,7 +883,7 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
     if (db ? enqueue_plans(c, map0, map1, map_da, gb, da ? &ga : nullptr)
            : enqueue_plans(c, map_da, map_da, map_da, ga, nullptr))
         return 1;
-    if ((da && enqueue(c, qa)) || (db && (enqueue(c, qb) || pb.finish(c))))
+    if ((da && enqueue(c, qa)) || (db && enqueue(c, qb)))
         return 1;
     return 0;
 }
@@ -1043,9 +993,6 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
     Operand oh, ow;
     oh.plan(c, hidden, m, k);
     ow.plan(c, weight, k, v);
-    PaddedOutput pw;
-    if (dweight)
-        pw.plan(c, Matrix{dweight, k, v, v}, dw_half);
     const size_t dz_at = c.reserve(static_cast<size_t>(m) * width * e);
     // dH is summed over the pieces in FP32: in the output itself where it is FP32.
     const bool own_sum = dhidden && dh_half && pieces > 1;
@@ -1109,13 +1056,12 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = cols;
             q.k = m;
             q.launch.layout = kTN;
-            const Matrix &all = pw.matrix(c);
-            const Matrix dw{static_cast<const uint8_t *>(all.ptr) + v0 * (dw_half ? 2 : 4), k, cols, all.pitch};
+            const Matrix dw{static_cast<uint8_t *>(dweight) + v0 * (dw_half ? 2 : 4), k, cols, v};
             q.set_tile(choose_tile(c.ctx, {k, cols, (m + bk - 1) / bk, 1, dw_half ? 2 : 4,
                                            output_tma(dw, dw_half ? 2 : 4), true}));
             if (set_output(c, q.launch, dw, dw_half) || enqueue(c, q))
                 return 1;
         }
     }
-    return pw.finish(c);
+    return 0;
 }

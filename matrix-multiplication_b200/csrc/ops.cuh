@@ -31,8 +31,6 @@ struct OpKernels {
     cudaError_t (*act_grad)(const ActGradParams &params, dim3 grid, int cluster, cudaStream_t stream);
     cudaError_t (*bias_grad)(const float *partial, int count, int n, void *dbias, int dbias_half, cudaStream_t stream);
     cudaError_t (*repack)(const RepackJob &job0, const RepackJob &job1, int sms, cudaStream_t stream);
-    cudaError_t (*unpack)(const void *src, void *dst, int64_t rows, int64_t cols, int64_t pitch, bool fp32, int sms,
-                          cudaStream_t stream);
 };
 
 // Sets every operator kernel's attributes on the current device (matmul_create).

@@ -4,7 +4,6 @@
 
 #include <cuda.h>
 #include <cstdint>
-#include <type_traits>
 
 #include "ptx.cuh"
 #include "tc_ops.cuh"
@@ -96,44 +95,6 @@ __global__ void __launch_bounds__(RP_THREADS) repack_kernel(const RepackJob job0
             q = make_uint4(words[0], words[1], words[2], words[3]);
         }
         *reinterpret_cast<uint4 *>(job.dst + (row * pitch + c * kPer) * ELEM) = q;
-    }
-}
-
-// The way back for outputs that TMA cannot write: rows x pitch in scratch (rows on 16
-// bytes) -> rows x cols without padding at any element alignment.  Each thread writes
-// aligned 16-byte chunks of the destination, which may hold the end of one row and the
-// start of the next, element by element where they do or at either end of the matrix.
-template <int ELEM>
-__global__ void __launch_bounds__(RP_THREADS) unpack_kernel(const uint8_t *src, uint8_t *dst, int64_t rows,
-                                                            int64_t cols, int64_t pitch)
-{
-    using Word = std::conditional_t<ELEM == 2, uint16_t, uint32_t>;
-    constexpr int kPer = 16 / ELEM;
-    wait_for_prior_grid();
-    allow_next_grid();
-    const int64_t total = rows * cols;
-    const int64_t head = (16 - (reinterpret_cast<uintptr_t>(dst) & 15u)) % 16 / ELEM;     // elements before the first chunk
-    const int64_t chunks = (total - head + kPer - 1) / kPer + (head ? 1 : 0);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * RP_THREADS + threadIdx.x; i < chunks;
-         i += static_cast<int64_t>(gridDim.x) * RP_THREADS) {
-        const int64_t first = head + (i - (head ? 1 : 0)) * kPer;       // negative in the chunk before the first whole one
-        const int64_t begin = first < 0 ? 0 : first, end = min(first + kPer, total);
-        const int64_t row = total < (int64_t{1} << 31) ? static_cast<int64_t>(static_cast<uint32_t>(begin) /
-                                                                              static_cast<uint32_t>(cols))
-                                                       : begin / cols;
-        const int64_t col = begin - row * cols;
-        if (end - first == kPer && begin == first && col + kPer <= cols) {
-            *reinterpret_cast<uint4 *>(dst + first * ELEM) = load_16_bytes<ELEM>(src + (row * pitch + col) * ELEM);
-        } else {
-            int64_t r = row, c = col;
-            for (int64_t e = begin; e < end; ++e) {
-                reinterpret_cast<Word *>(dst)[e] = reinterpret_cast<const Word *>(src)[r * pitch + c];
-                if (++c == cols) {
-                    c = 0;
-                    ++r;
-                }
-            }
-        }
     }
 }
 

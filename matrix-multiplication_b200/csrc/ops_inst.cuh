@@ -127,17 +127,7 @@ struct OpInstances {
                           job1);
     }
 
-    static cudaError_t unpack(const void *src, void *dst, int64_t rows, int64_t cols, int64_t pitch, bool fp32, int sms,
-                              cudaStream_t stream)
-    {
-        const int elem = fp32 ? 4 : static_cast<int>(sizeof(T));
-        const int64_t blocks = (rows * cols * elem / 16 + RP_THREADS) / RP_THREADS + 1, cap = 16LL * sms;
-        const dim3 grid(static_cast<unsigned int>(blocks < cap ? blocks : cap));
-        return launch_pdl(elem == 4 ? unpack_kernel<4> : unpack_kernel<2>, grid, dim3(RP_THREADS), 0, stream,
-                          static_cast<const uint8_t *>(src), static_cast<uint8_t *>(dst), rows, cols, pitch);
-    }
-
-    static constexpr OpKernels kTable{setup, product, act_grad, bias_grad, repack, unpack};
+    static constexpr OpKernels kTable{setup, product, act_grad, bias_grad, repack};
 };
 
 } // namespace b200
