@@ -1042,18 +1042,21 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     for (int i = 0; i < 32; ++i)
                         area[r * 33 + i] = words[i];
                     __syncwarp();
-                    const int elem = half ? 2 : 4, per = 16 / elem;
-                    const int cols = min(128 / elem, p.n - col0), rows = min(OP_BM, w.row_end - row0);
-                    const int place = lane & 7;
-                    int rr = quarter * 32 + (lane >> 3);
-                    uint8_t *to = static_cast<uint8_t *>(dst) + (at0 + (row0 + rr) * pitch + col0) * elem;
-#pragma unroll 2
-                    for (int it = 0; it < 8; ++it, rr += 4, to += 4 * pitch * elem) {
+                    const int log_elem = half ? 1 : 2, per = 16 >> log_elem;
+                    const int cols = min(128 >> log_elem, p.n - col0), rows = min(OP_BM, w.row_end - row0);
+                    const int place = lane & 7, row_first = quarter * 32 + (lane >> 3);
+                    uint8_t *base_row = static_cast<uint8_t *>(dst) + ((at0 + (row0 + row_first) * pitch + col0) << log_elem);
+                    const long long row_step = (4 * pitch) << log_elem;
+#pragma unroll 4
+                    for (int it = 0; it < 8; ++it) {
+                        const int rr = row_first + 4 * it;
+                        uint8_t *to = base_row + it * row_step;
                         if (rr >= rows)
-                            break;
+                            continue;
                         const uint32_t *row = area + rr * 33;
-                        const int head = min(static_cast<int>((16u - (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to)) & 15u)) & 15u) / elem, cols);
-                        const int whole = (cols - head) / per;        // aligned 16-byte chunks
+                        const int head = min(static_cast<int>((0u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to))) & 15u) >> log_elem, cols);
+                        const int whole = (cols - head) >> (4 - log_elem);        // aligned 16-byte chunks
+                        const int ends = cols - (whole << (4 - log_elem));
                         if (place < whole) {
                             const int first = head + place * per;
                             uint4 q;
@@ -1068,15 +1071,20 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                                 const uint32_t *x = row + first;
                                 q = make_uint4(x[0], x[1], x[2], x[3]);
                             }
-                            *reinterpret_cast<uint4 *>(to + first * elem) = q;
+                            *reinterpret_cast<uint4 *>(to + (first << log_elem)) = q;
                         }
-                        for (int e = place; e < cols - whole * per; e += 8) {
-                            const int c = e < head ? e : e + whole * per;
+                        // At most 8 elements, one a lane, but in the last columns of the matrix.
+                        auto end_element = [&](int e) {
+                            const int c = e < head ? e : e + (whole << (4 - log_elem));
                             if (half)
                                 reinterpret_cast<uint16_t *>(to)[c] = reinterpret_cast<const uint16_t *>(row)[c];
                             else
                                 reinterpret_cast<uint32_t *>(to)[c] = row[c];
-                        }
+                        };
+                        if (place < ends)
+                            end_element(place);
+                        if (place + 8 < ends)
+                            end_element(place + 8);
                     }
                     __syncwarp();
                 };
@@ -1114,13 +1122,31 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     if (col0 >= p.n || row0 >= w.row_end)      // the same for all four warps
                         return;
                     if constexpr (EPI == kEpiSoftmaxGrad) {
-                        // p = exp(z - lse); an ignored row's gradient is zero whatever its logits are.
-                        const int hit = label - p.column0 - col0;
-                        const float scale = label == -2 ? __int_as_float(0x7fc00000) : row_grad;
+                        // dz = (exp(z - lse) - [column == label]) grad.  The exponential is taken 2^24 times too
+                        // large and grad as much too small, so that only their product, not the
+                        // hardware's exponential, falls below the normal numbers.  An ignored row's
+                        // gradient is zero whatever its logits are.
+                        if (label == -1) {
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) {
-                            const float prob = exp2f((v[j] - row_lse) * 1.4426950408889634f);   // subnormals kept
-                            v[j] = label == -1 ? 0.0f : (prob - (j == hit ? 1.0f : 0.0f)) * scale;
+                            for (int j = 0; j < 64; ++j)
+                                v[j] = 0.0f;
+                        } else {
+                            const float scale = (label == -2 ? __int_as_float(0x7fc00000) : row_grad) * 0x1p-24f;
+                            const float2 shift = make_float2(-row_lse, -row_lse), scale2 = make_float2(scale, scale);
+#pragma unroll
+                            for (int j = 0; j < 64; j += 2) {
+                                const float2 d = __fadd2_rn(make_float2(v[j], v[j + 1]), shift);
+                                const float2 t = __ffma2_rn(d, make_float2(1.44269504f, 1.44269504f), make_float2(24.0f, 24.0f));
+                                const float2 q = __fmul2_rn(make_float2(op_exp2(t.x), op_exp2(t.y)), scale2);
+                                v[j] = q.x;
+                                v[j + 1] = q.y;
+                            }
+                            const int hit = label - p.column0 - col0;
+                            if (hit >= 0 && hit < 64) {
+#pragma unroll
+                                for (int j = 0; j < 64; ++j)
+                                    v[j] -= j == hit ? row_grad : 0.0f;
+                            }
                         }
                     } else {
                         if (p.bias) {
@@ -1231,9 +1257,9 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     store_elements(v, rows, first, col, 1, 0);
                 }
             } else {
-                // One pass: running maximum and sum of exponentials in base 2 of this row's
+                // One pass: running maximum and sum of exponentials, in base 2, of this row's
                 // columns in the tile; columns past the vocabulary count as -infinity.
-                float top = -INFINITY, sum = 0.0f;
+                float top = -INFINITY, origin = -INFINITY, sum = 0.0f;
                 const int row = row0 + r;
                 auto reduce = [&](const uint32_t (&u)[32], int chunk) {
                     const int col0 = w.n0 + gcol + chunk * 32;
@@ -1247,21 +1273,32 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                             z = j == hit ? __uint_as_float(u[j]) : z;
                         p.label_logit[row] = z;
                     }
-                    float t[32], chunk_top = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        t[j] = col0 + j < p.n ? __uint_as_float(u[j]) * 1.4426950408889634f : -INFINITY;
-                        chunk_top = fmaxf(chunk_top, t[j]);
-                    }
-                    const float next = fmaxf(top, chunk_top);
-                    // A row whose logits are all -infinity so far adds nothing; NaN is carried by the sum.
-                    const float origin = next == -INFINITY ? 0.0f : next;
-                    sum *= op_exp2(top - origin);
-                    float part_sum[4] = {};     // four chains
+                    float x[32], chunk_top = -INFINITY;
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        part_sum[j & 3] += op_exp2(t[j] - origin);
-                    sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
+                        x[j] = __uint_as_float(u[j]);
+                    if (col0 + 32 > p.n) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            x[j] = col0 + j < p.n ? x[j] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        chunk_top = fmaxf(chunk_top, x[j]);
+                    const float next = fmaxf(top, chunk_top);
+                    // A row whose logits are all -infinity so far adds nothing; NaN is carried by the sum.
+                    // The origin is rounded once and used for every term and in the result.
+                    const float next_origin = next == -INFINITY ? 0.0f : next * 1.44269504f;
+                    sum *= top == -INFINITY ? 0.0f : op_exp2(origin - next_origin);
+                    origin = next_origin;
+                    const float2 scale = make_float2(1.44269504f, 1.44269504f), minus = make_float2(-origin, -origin);
+                    float2 chain[2] = {};
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 t = __ffma2_rn(make_float2(x[j], x[j + 1]), scale, minus);
+                        chain[(j >> 1) & 1] = __fadd2_rn(chain[(j >> 1) & 1], make_float2(op_exp2(t.x), op_exp2(t.y)));
+                    }
+                    sum += (chain[0].x + chain[0].y) + (chain[1].x + chain[1].y);
                     top = next;
                 };
 #pragma unroll 1
@@ -1273,7 +1310,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     reduce(u, chunk);
                 }
                 if (row < p.m)
-                    p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row] = make_float2(top, sum);
+                    p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row] = make_float2(top == -INFINITY ? top : origin, sum);
             }
             if (++acc == 2) {
                 acc = 0;

@@ -461,6 +461,28 @@ def test_cross_entropy_marks_bad_labels_and_keeps_rows_apart(native):
     assert bool(rows[10:13].all()) and int(rows.sum()) == 3 + int(bad[20])
 
 
+@pytest.mark.parametrize("m", (3, 300))
+def test_cross_entropy_with_logits_of_minus_infinity(native, m):
+    """Whole stretches of -infinity before, between and after logits near -1000: they add nothing, the rest is exact;
+    a row of nothing but -infinity has lse -infinity."""
+    k, v = 64, 2000
+    hidden = randn((m, k), torch.bfloat16, 1).abs() + 0.5
+    weight = randn((k, v), torch.bfloat16, 2, 0.3) - 15.0
+    weight[:, :700] = float("-inf")
+    weight[:, 900:1300] = float("-inf")
+    weight[:, 1999] = float("-inf")
+    labels = torch.full((m,), 800, device="cuda")
+    loss, lse = (torch.empty((m,), dtype=torch.float32, device="cuda") for _ in range(2))
+    native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision="bf16")()
+    live = torch.cat([torch.arange(700, 900), torch.arange(1300, 1999)]).cuda()
+    expected = ref.cross_entropy(hidden, weight[:, live].contiguous(), torch.full_like(labels, 100), "bf16")
+    assert_within(lse, *expected["lse"], "lse")
+    assert_within(loss, *expected["loss"], "loss")
+    weight.fill_(float("-inf"))
+    native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision="bf16")()
+    assert bool((lse == float("-inf")).all())
+
+
 def test_cross_entropy_every_row_ignored(native):
     m, k, v = 40, 64, 500
     hidden, weight, labels, grad = loss_inputs(m, k, v, "bf16")
