@@ -270,6 +270,7 @@ double tile_cycles(const Context *ctx, int tile, int splits, const TileProblem &
 
 struct TileChoice {
     int tile, splits;
+    int chunks = 1;      // K chunks added up by a second kernel (GradientProduct)
 };
 
 // Whether K blocks split S ways leave every CTA some and fit the device in one wave.
@@ -359,7 +360,7 @@ int enqueue(Call &c, Product &q)
     const int bk = OP_ROW_BYTES / c.elem();
     p.num_k_blocks = static_cast<int>((q.k + bk - 1) / bk);
     int64_t tiles = static_cast<int64_t>(p.num_m_blocks) * p.num_n_blocks;
-    if (p.grouping == kGroupedK)
+    if (p.grouping == kGroupedK || p.grouping == kChunkedK)
         tiles *= p.groups;
     else if (p.grouping == kGroupedRows)     // at most this many; the plan on the device has the number
         tiles = (q.m / (swap ? t.bn : t.bm) + std::min<int64_t>(p.groups, q.m)) *
@@ -422,6 +423,107 @@ int set_output(Call &c, OpLaunch &l, const Matrix &out, bool half)
     }
     return 0;
 }
+
+// A product whose epilogue only stores, possibly added to an FP32 matrix: the gradients.
+// Where there are few output tiles and K is long, K is cut into chunks over all SMs.
+struct GradientProduct {
+    static constexpr int64_t kChunkBytes = 64 << 20;     // the chunks' products stay in L2
+    int layout = kNN;
+    int64_t m = 0, n = 0, k = 0;
+    TileChoice choice{kSingle64, 1};
+    size_t at = 0;
+
+    // Before the call's scratch is allocated.  `base`: an FP32 matrix is added.
+    void plan(Call &c, int product_layout, int64_t rows, int64_t cols, int64_t depth, const Matrix &out, bool half,
+              bool base = false)
+    {
+        layout = product_layout;
+        m = rows;
+        n = cols;
+        k = depth;
+        const int64_t bk = OP_ROW_BYTES / c.elem(), k_blocks = (k + bk - 1) / bk;
+        const int out_bytes = half ? 2 : 4;
+        TileProblem q{m, n, k_blocks, 1, out_bytes + (base ? 4 : 0), output_tma(out, out_bytes), true};
+        choice = choose_tile(c.ctx, q);
+        // Chunks cost their FP32 products, written and read once more through L2, and a launch of about
+        // 8000 cycles; the estimate knows nothing of operands that HBM limits, so a gain below 8 % is
+        // not taken (BF16 da: 302 x 20352 . 20352 x 1920 51.9 -> 41.6 us, 1024 x 30000 . 30000 x 512
+        // 50.3 -> 39.5; 27 x 64 x 113300 with its loss's other kernels 91 -> 65).
+        double best = 0.92 * tile_cycles(c.ctx, choice.tile, choice.splits, q);
+        q.bytes_out = 4;
+        q.out_tma = true;
+        for (int chunks : {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+            if (k_blocks < 4 * chunks || chunks * m * round_up(n, 4) * 4 > kChunkBytes)
+                break;
+            q.k_blocks = (k_blocks + chunks - 1) / chunks;
+            if ((chunks - 1) * q.k_blocks >= k_blocks)
+                continue;        // the last chunk would be empty
+            q.groups = chunks;
+            for (int tile : {kPair256, kSingle128, kSingle64}) {
+                if (tile == kPair256 && (c.ctx->max_pairs < 1 || m <= OP_BM))
+                    continue;
+                const double cycles = tile_cycles(c.ctx, tile, 1, q) + 8000.0 +
+                                      static_cast<double>(chunks) * static_cast<double>(m * n) * 8.0 / 4000.0;
+                if (cycles < best) {
+                    best = cycles;
+                    choice = {tile, 1, chunks};
+                }
+            }
+        }
+        if (choice.chunks > 1)
+            at = c.reserve(static_cast<size_t>(choice.chunks) * m * round_up(n, 4) * sizeof(float));
+    }
+
+    // a and b as stored for the layout; depth may be below the planned one (a last piece).
+    int run(Call &c, const Matrix &a, const Matrix &b, int64_t depth, const Matrix &out, bool half, const Matrix *base = nullptr)
+    {
+        Product q;
+        q.a = a;
+        q.b = b;
+        q.m = m;
+        q.n = n;
+        q.k = depth;
+        q.launch.layout = layout;
+        q.set_tile(choice);
+        const int64_t bk = OP_ROW_BYTES / c.elem(), k_blocks = (depth + bk - 1) / bk;
+        int64_t per = (k_blocks + choice.chunks - 1) / choice.chunks;
+        const int chunks = static_cast<int>((k_blocks + per - 1) / per);
+        if (choice.chunks == 1) {
+            if (set_output(c, q.launch, out, half))
+                return 1;
+            if (base) {
+                if (!output_tma(*base, 4))
+                    q.launch.p.out_tma = 0;
+                if (set_residual(c, q.launch, *base, false))
+                    return 1;
+            }
+            return enqueue(c, q);
+        }
+        const int64_t pitch = round_up(n, 4);
+        const Matrix sums{c.scratch + at, m, n, pitch, chunks, m * pitch};
+        OpParams &p = q.launch.p;
+        p.grouping = kChunkedK;
+        p.groups = chunks;
+        p.chunk_blocks = static_cast<int>(per);
+        if (set_output(c, q.launch, sums, false) || enqueue(c, q))
+            return 1;
+        ChunkSumParams g{};
+        g.chunks = static_cast<const float *>(sums.ptr);
+        g.count = chunks;
+        g.rows = static_cast<int>(m);
+        g.cols = static_cast<int>(n);
+        g.slab = sums.slab;
+        g.pitch = pitch;
+        g.base = base ? static_cast<const float *>(base->ptr) : nullptr;
+        g.base_pitch = base ? base->pitch : 0;
+        g.out = const_cast<void *>(out.ptr);
+        g.out_pitch = out.pitch;
+        g.out_half = half ? 1 : 0;
+        g.vec = output_tma(out, half ? 2 : 4) ? 1 : 0;
+        const cudaError_t st = c.kernels().chunk_sum(g, c.ctx->sm_count, c.stream);
+        return st == cudaSuccess ? 0 : c.failed(st);
+    }
+};
 
 // ---------------------------------------------------------------- argument checks
 int check_call(void *opaque, int precision, const char *name, char *error, size_t error_size)
@@ -595,6 +697,11 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
     else if (da || db)
         od.plan(c, dout, m, n);
     const Matrix ma{da, m, k, k}, mb{db, k, n, n};
+    GradientProduct pa, pb;
+    if (da)
+        pa.plan(c, kNT, m, k, n, ma, da_half);
+    if (db)
+        pb.plan(c, kTN, k, n, m, mb, db_half);
     ActGradPlan plan;
     plan.choose(c.ctx, m, n);
     size_t partial_at = 0;
@@ -629,33 +736,10 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
             return c.failed(st);
     }
     const Matrix dz = own_dz ? Matrix{c.scratch + dz_at, m, n, dz_pitch} : od.ready;
-    const int64_t bk = OP_ROW_BYTES / e;
-    if (da) {
-        Product q;
-        q.a = dz;
-        q.b = ob.ready;
-        q.m = m;
-        q.n = k;
-        q.k = n;
-        q.launch.layout = kNT;
-        q.set_tile(choose_tile(c.ctx, {q.m, q.n, (q.k + bk - 1) / bk, 1, da_half ? 2 : 4,
-                                       output_tma(ma, da_half ? 2 : 4), true}));
-        if (set_output(c, q.launch, ma, da_half) || enqueue(c, q))
-            return 1;
-    }
-    if (db) {
-        Product q;
-        q.a = oa.ready;
-        q.b = dz;
-        q.m = k;
-        q.n = n;
-        q.k = m;
-        q.launch.layout = kTN;
-        q.set_tile(choose_tile(c.ctx, {q.m, q.n, (q.k + bk - 1) / bk, 1, db_half ? 2 : 4,
-                                       output_tma(mb, db_half ? 2 : 4), true}));
-        if (set_output(c, q.launch, mb, db_half) || enqueue(c, q))
-            return 1;
-    }
+    if (da && pa.run(c, dz, ob.ready, n, ma, da_half))
+        return 1;
+    if (db && pb.run(c, oa.ready, dz, m, mb, db_half))
+        return 1;
     return 0;
 }
 
@@ -997,9 +1081,14 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
     // dH is summed over the pieces in FP32: in the output itself where it is FP32.
     const bool own_sum = dhidden && dh_half && pieces > 1;
     const size_t sum_at = own_sum ? c.reserve(static_cast<size_t>(m) * k * sizeof(float)) : 0;
+    const Matrix dh{dhidden, m, k, k};
+    GradientProduct ph, pw;
+    if (dhidden)
+        ph.plan(c, kNT, m, k, width, dh, dh_half && !own_sum, pieces > 1);
+    if (dweight)
+        pw.plan(c, kTN, k, width, m, Matrix{dweight, k, width, v}, dw_half);
     if (c.allocate() || prepare_operands(c, {&oh, &ow}))
         return 1;
-    const Matrix dh{dhidden, m, k, k};
     const Matrix sum = own_sum ? Matrix{c.scratch + sum_at, m, k, k} : dh;
     for (int64_t piece = 0; piece < pieces; ++piece) {
         const int64_t v0 = piece * width, cols = std::min<int64_t>(width, v - v0);
@@ -1026,40 +1115,14 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
                 return 1;
         }
         if (dhidden) {
-            Product q;
-            q.a = dz;
-            q.b = w;
-            q.m = m;
-            q.n = k;
-            q.k = cols;
-            q.launch.layout = kNT;
             const bool last = piece == pieces - 1;
-            const Matrix &to = last ? dh : sum;
-            q.set_tile(choose_tile(c.ctx, {m, k, (cols + bk - 1) / bk, 1, (piece > 0 ? 4 : 0) + (last && dh_half ? 2 : 4),
-                                           output_tma(to, last && dh_half ? 2 : 4), true}));
-            if (set_output(c, q.launch, to, last && dh_half))
-                return 1;
-            if (piece > 0) {
-                if (!output_tma(sum, 4))
-                    q.launch.p.out_tma = 0;
-                if (set_residual(c, q.launch, sum, false))
-                    return 1;
-            }
-            if (enqueue(c, q))
+            if (ph.run(c, dz, w, cols, last ? dh : sum, last && dh_half, piece > 0 ? &sum : nullptr))
                 return 1;
         }
         if (dweight) {
-            Product q;
-            q.a = oh.ready;
-            q.b = dz;
-            q.m = k;
-            q.n = cols;
-            q.k = m;
-            q.launch.layout = kTN;
             const Matrix dw{static_cast<uint8_t *>(dweight) + v0 * (dw_half ? 2 : 4), k, cols, v};
-            q.set_tile(choose_tile(c.ctx, {k, cols, (m + bk - 1) / bk, 1, dw_half ? 2 : 4,
-                                           output_tma(dw, dw_half ? 2 : 4), true}));
-            if (set_output(c, q.launch, dw, dw_half) || enqueue(c, q))
+            pw.n = cols;
+            if (pw.run(c, oh.ready, dz, m, dw, dw_half))
                 return 1;
         }
     }

@@ -31,6 +31,7 @@ struct OpKernels {
     cudaError_t (*act_grad)(const ActGradParams &params, dim3 grid, int cluster, cudaStream_t stream);
     cudaError_t (*bias_grad)(const float *partial, int count, int n, void *dbias, int dbias_half, cudaStream_t stream);
     cudaError_t (*repack)(const RepackJob &job0, const RepackJob &job1, int sms, cudaStream_t stream);
+    cudaError_t (*chunk_sum)(const ChunkSumParams &params, int sms, cudaStream_t stream);
 };
 
 // Sets every operator kernel's attributes on the current device (matmul_create).

@@ -260,6 +260,66 @@ __global__ void __launch_bounds__(AG_THREADS, 4) act_grad_kernel(const ActGradPa
     cluster_sync_all();      // no block leaves while its sums are read
 }
 
+// ---------------------------------------------------------------- chunks of K
+struct ChunkSumParams {
+    const float *chunks;          // count slabs of rows x cols, pitch a multiple of 4
+    int count, rows, cols;
+    int64_t slab, pitch;
+    const float *base;            // null, or FP32 to add (pitch base_pitch)
+    int64_t base_pitch;
+    void *out;
+    int64_t out_pitch;
+    int out_half, vec;            // vec: out's and base's rows start on 16 bytes
+};
+
+// out = base + the chunks' products, added in order; four columns a thread.  Bound by the
+// chunks' bytes, which are in L2.
+template <int FMT>
+__global__ void __launch_bounds__(256) chunk_sum_kernel(const ChunkSumParams p)
+{
+    using Type = OpType<FMT>;
+    using T = typename Type::T;
+    wait_for_prior_grid();
+    allow_next_grid();
+    const int quads = (p.cols + 3) / 4;
+    const int64_t total = static_cast<int64_t>(p.rows) * quads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int row = static_cast<int>(i / quads), col = static_cast<int>(i - static_cast<int64_t>(row) * quads) * 4;
+        const int count = min(4, p.cols - col);
+        float v[4] = {};
+        if (p.base) {
+            const float *b = p.base + row * p.base_pitch + col;
+            for (int e = 0; e < count; ++e)
+                v[e] = b[e];
+        }
+        const float *x = p.chunks + row * p.pitch + col;
+#pragma unroll 8
+        for (int j = 0; j < p.count; ++j) {
+            const float4 q = *reinterpret_cast<const float4 *>(x + j * p.slab);
+            v[0] += q.x;
+            v[1] += q.y;
+            v[2] += q.z;
+            v[3] += q.w;
+        }
+        if (p.out_half) {
+            T *to = static_cast<T *>(p.out) + row * p.out_pitch + col;
+            if (p.vec && count == 4 && FMT != kOpTF32)
+                *reinterpret_cast<uint2 *>(to) = make_uint2(Type::pack(v[0], v[1]), Type::pack(v[2], v[3]));
+            else
+                for (int e = 0; e < count; ++e)
+                    to[e] = Type::from(v[e]);
+        } else {
+            float *to = static_cast<float *>(p.out) + row * p.out_pitch + col;
+            if (p.vec && count == 4)
+                *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+            else
+                for (int e = 0; e < count; ++e)
+                    to[e] = v[e];
+        }
+    }
+}
+
 // dbias = the clusters' partial sums, added in order.
 template <int FMT>
 __global__ void __launch_bounds__(256) bias_grad_kernel(const float *partial, int count, int n, void *dbias,

@@ -127,7 +127,14 @@ struct OpInstances {
                           job1);
     }
 
-    static constexpr OpKernels kTable{setup, product, act_grad, bias_grad, repack};
+    static cudaError_t chunk_sum(const ChunkSumParams &params, int sms, cudaStream_t stream)
+    {
+        const int64_t blocks = (static_cast<int64_t>(params.rows) * ((params.cols + 3) / 4) + 255) / 256, cap = 8LL * sms;
+        return launch_pdl(chunk_sum_kernel<FMT>, dim3(static_cast<unsigned int>(blocks < cap ? blocks : cap)), dim3(256), 0,
+                          stream, params);
+    }
+
+    static constexpr OpKernels kTable{setup, product, act_grad, bias_grad, repack, chunk_sum};
 };
 
 } // namespace b200

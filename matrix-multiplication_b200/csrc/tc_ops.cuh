@@ -10,6 +10,8 @@
 //     - ragged-K mode (gradient of B): one product per group over the group's rows.
 //       Operand tensor maps of that group end at its last row, so TMA fills the
 //       rest of a K block with zeros and no value of a neighbour enters a sum;
+//   * a long K may be cut into chunks whose FP32 products are added up by a second
+//     kernel (few output tiles, as in the gradient of a few rows through a vocabulary);
 //   * the epilogue applies bias, activation and residual, reduces each row to a
 //     maximum and a sum of exponentials (loss), or turns logits into gradients.
 //
@@ -41,7 +43,7 @@ enum OpEpilogue : int {
     kEpiSoftmaxGrad = 3 // out = (exp(D - lse) - [column == label]) * grad
 };
 enum OpActivation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
-enum OpGrouping : int { kUngrouped = 0, kGroupedRows = 1, kGroupedK = 2 };
+enum OpGrouping : int { kUngrouped = 0, kGroupedRows = 1, kGroupedK = 2, kChunkedK = 3 };
 
 // Status bits of the device status word (matmul_device_status).
 enum : unsigned int { kOpLoadTimeout = 1u, kOpMmaTimeout = 2u, kOpEpilogueTimeout = 4u, kOpDrainTimeout = 8u };
@@ -115,7 +117,8 @@ struct OpParams {
     int full_tiles;           // pairs: from here on two indices name the column halves of one tile
     int log_raster;           // log2 of the M-side tiles per raster group
     OpDivisor per_raster;     // raster x N-side tiles (transposed epilogue: M-side tiles)
-    OpDivisor per_group;      // ragged-K mode: tiles of one group
+    OpDivisor per_group;      // ragged-K and chunked-K modes: tiles of one group or chunk
+    int chunk_blocks;         // chunked-K mode: K blocks per chunk
     int grouping;             // OpGrouping
     int a_blocked, b_blocked; // MN-major operands: 1 when their map sees blocks of 128 bytes of columns
     const int *row_tile_count;        // rows mode: number of row tiles (device)
@@ -417,6 +420,12 @@ __device__ __forceinline__ OpWhere op_where(int tile, int row_tile_count, int bk
         const OpRowTile t = p.row_tiles[w.group];
         w.k0 = t.row0;
         w.nkb = (t.row_end - t.row0 + bk - 1) / bk;
+    } else if (p.grouping == kChunkedK) {
+        w.group = op_divide(tile, p.per_group);
+        local = tile - w.group * p.per_group.value;
+        const int first = w.group * p.chunk_blocks;
+        w.k0 = first * bk;
+        w.nkb = min(p.chunk_blocks, p.num_k_blocks - first);
     }
     int mb, nb;
     if constexpr (SWAP) {       // all M-side tiles (columns) of a row tile, then the next
@@ -602,7 +611,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const int row_end = min(w.row_end, first_row + rows), col_end = min(p.n, first_col + cols);
         for (int row = first_row + warp_index; row < row_end; row += warps)
             for (int col = first_col + lane_index; col < col_end; col += 32) {
-                const long long at = (p.grouping == kGroupedK ? w.group : 0) * p.out_slab + row * p.out_pitch + col;
+                const long long at = (p.grouping >= kGroupedK ? w.group : 0) * p.out_slab + row * p.out_pitch + col;
                 if (p.out_half)
                     static_cast<T *>(p.out)[at] = Type::from(nan);
                 else
@@ -911,7 +920,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         acquired = w.group;
                     }
                 }
-                const int zc = p.grouping == kGroupedK ? w.group : 0;
+                const int zc = p.grouping >= kGroupedK ? w.group : 0;
                 // Puts 128 bytes of this thread's row into a box of 128 rows.
                 auto fill = [&](uint32_t box, const uint32_t (&words)[32]) {
                     const uint32_t row_addr = box + r * 128;

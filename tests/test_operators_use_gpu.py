@@ -208,8 +208,8 @@ def test_refusals_reach_the_caller(native):
 @pytest.mark.parametrize("n", (1028, 1032, 1037))
 @pytest.mark.parametrize("m", (70, 300, 2100))
 def test_outputs_and_pre_activations_of_other_alignments(native, m, n):
-    """n % 8 == 4: TMA writes FP32 rows and not 16-bit ones, so one kernel stores both ways; large odd outputs go
-    through padded rows in scratch."""
+    """n % 8 == 4: TMA writes FP32 rows and not 16-bit ones, so one kernel stores both ways; odd rows leave
+    in aligned chunks of 16 bytes."""
     k = 136
     a, b, bias = randn((m, k), BF16, 1), randn((k, n), BF16, 2, k ** -0.5), randn((n,), FP32, 3)
     for out_dtype, preact_dtype in ((BF16, FP32), (FP32, BF16), (BF16, BF16), (FP32, FP32)):
@@ -225,7 +225,7 @@ def test_outputs_and_pre_activations_of_other_alignments(native, m, n):
 
 @pytest.mark.parametrize("precision", ("bf16", "tf32"))
 def test_large_odd_gradients(native, precision):
-    """Gradients of 4 MB and more with odd rows leave through padded scratch, at any base alignment."""
+    """Large gradients with odd rows, at any base alignment."""
     dtype = DTYPES[precision]
     m, k, n = 1500, 1501, 1403
     dout, a, b = randn((m, n), dtype, 1), randn((m, k), dtype, 2), randn((k, n), dtype, 3, k ** -0.5)
@@ -259,6 +259,50 @@ def test_large_odd_grouped_and_vocabulary_gradients(native):
     assert_within(dh, *expected["dhidden"], "dhidden")
     assert_within(dw, *expected["dweight"], "dweight")
     ua(), ub()
+
+
+DEEP = [(1, 3, 70001), (20, 130, 9001), (130, 20, 30000), (302, 264, 20352), (9000, 40, 24), (20011, 33, 65),
+        (40000, 200, 3)]
+
+
+@pytest.mark.parametrize("precision", ("bf16", "fp16", "tf32"))
+@pytest.mark.parametrize("shape", DEEP, ids=lambda s: "x".join(map(str, s)))
+def test_few_gradients_from_long_sums(native, precision, shape):
+    """A small da summed over many columns, or a small db over many rows, is added up from chunks of the sum."""
+    m, k, n = shape
+    dtype = DTYPES[precision]
+    dout, a, b = randn((m, n), dtype, 1), randn((m, k), dtype, 2), randn((k, n), dtype, 3)
+    expected = ref.epilogue_backward(dout, a, b, precision)
+    for grad_dtype in dict.fromkeys((dtype, FP32)):
+        (da, ua), (db, ub) = guarded((m, k), grad_dtype), guarded((k, n), grad_dtype)
+        run = native.prepare_epilogue_backward(dout, a, b, precision=precision, da=da, db=db)
+        run()
+        assert_within(da, *expected["da"], "da")
+        assert_within(db, *expected["db"], "db")
+        ua(), ub()
+        first = da.clone(), db.clone()
+        run()
+        assert torch.equal(first[0], da) and torch.equal(first[1], db)
+
+
+@pytest.mark.parametrize("precision", ("bf16", "tf32"))
+@pytest.mark.parametrize("shape", [(3, 65, 40001), (50, 264, 30000), (2100, 40, 18001), (20000, 24, 40)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_vocabulary_gradients_from_long_sums(native, precision, shape):
+    """The same of the loss: one piece of the vocabulary and several, the last one short."""
+    m, k, v = shape
+    dtype = DTYPES[precision]
+    hidden, weight, labels, grad = loss_inputs(m, k, v, precision)
+    loss, lse = torch.zeros(m, device="cuda"), torch.zeros(m, device="cuda")
+    native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision=precision)()
+    expected = ref.cross_entropy_backward(grad, hidden, weight, labels, precision)
+    for grad_dtype in dict.fromkeys((dtype, FP32)):
+        (dh, ua), (dw, ub) = guarded((m, k), grad_dtype), guarded((k, v), grad_dtype)
+        native.prepare_cross_entropy_backward(grad, hidden, weight, labels, lse, precision=precision, dhidden=dh,
+                                              dweight=dw)()
+        assert_within(dh, *expected["dhidden"], "dhidden")
+        assert_within(dw, *expected["dweight"], "dweight")
+        ua(), ub()
 
 
 def test_on_some_of_the_sms(native):
