@@ -173,7 +173,7 @@ int matmul_launch_noalloc(void *context, int implementation, int precision,
  * No counterparts in the reference.  Products with more fused to them, on the
  * tensor cores, in the manner of matmul_launch: asynchronous on `stream`, graph
  * capturable, matrices row-major and owned by the caller, base pointers aligned
- * to their element, any sizes >= 1 that fit in an int.  `precision` is 1 (tf32),
+ * to their element, any sizes from 1 to 2^31 - 1024.  `precision` is 1 (tf32),
  * 2 (fp16) or 3 (bf16) and names the format of the product's operands; sums and
  * everything else inside are FP32.  An output or an auxiliary operand followed by
  * a flag `x_fp32` is FP32 when the flag is not 0, otherwise in the input format

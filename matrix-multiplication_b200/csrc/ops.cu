@@ -16,6 +16,7 @@ namespace {
 using namespace b200;
 
 constexpr int kTf32 = 1, kFp16 = 2, kBf16 = 3;     // precision ids of the ABI
+constexpr int kMaxSize = 0x7fffffff - 1023;        // a tile past the end still has int coordinates
 
 // Makes a device current for a call and puts the caller's back.
 struct DeviceScope {
@@ -76,8 +77,10 @@ struct Call {
 
     ~Call()
     {
-        if (scratch)
+        if (scratch) {
+            DeviceScope device(ctx->device);     // a default stream is the current device's
             cudaFreeAsync(scratch, stream);
+        }
     }
     int failed(const char *detail) { return fail(error, error_size, name, detail); }
     int failed(cudaError_t st) { return fail_cuda(error, error_size, name, st); }
@@ -536,6 +539,17 @@ int check_call(void *opaque, int precision, const char *name, char *error, size_
     return 0;
 }
 
+int check_sizes(Call &c, std::initializer_list<int> sizes)
+{
+    for (int size : sizes) {
+        if (size <= 0)
+            return c.failed("dimensions must be positive");
+        if (size > kMaxSize)
+            return c.failed("dimensions must be at most 2147482624");
+    }
+    return 0;
+}
+
 bool misaligned(const void *ptr, int bytes)
 {
     return reinterpret_cast<uintptr_t>(ptr) % static_cast<uintptr_t>(bytes) != 0;
@@ -577,8 +591,8 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     Call c{static_cast<Context *>(opaque), precision, static_cast<cudaStream_t>(stream), name, error, error_size};
     if (!a || !b || !out)
         return c.failed("matrix pointer is null");
-    if (m <= 0 || k <= 0 || n <= 0)
-        return c.failed("dimensions must be positive");
+    if (check_sizes(c, {m, k, n}))
+        return 1;
     if (activation < kActNone || activation > kActSilu)
         return c.failed("unknown activation");
     const int e = c.elem();
@@ -646,7 +660,7 @@ struct ActGradPlan {
         const int64_t column_blocks = (static_cast<int64_t>(n) + AG_COLS - 1) / AG_COLS;
         const int64_t most = std::max<int64_t>(1, m / 32);
         const int64_t fill = std::max<int64_t>(1, 4LL * ctx->sm_count / (column_blocks * AG_CLUSTER));
-        const int64_t all = std::min<int64_t>((m + 2047) / 2048, fill);
+        const int64_t all = std::min<int64_t>((m + 2047LL) / 2048, fill);
         const int64_t wanted = most >= AG_CLUSTER ? AG_CLUSTER * std::min(all, most / AG_CLUSTER) : most;
         cluster = static_cast<int>(std::min<int64_t>(wanted, AG_CLUSTER));
         clusters = static_cast<int>(wanted / cluster);
@@ -670,8 +684,8 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
         return c.failed("matrix pointer is null");
     if (!da && !db && !dbias)
         return c.failed("no gradient is asked for");
-    if (m <= 0 || k <= 0 || n <= 0)
-        return c.failed("dimensions must be positive");
+    if (check_sizes(c, {m, k, n}))
+        return 1;
     if (activation < kActNone || activation > kActSilu)
         return c.failed("unknown activation");
     const int e = c.elem();
@@ -808,8 +822,8 @@ int enqueue_plans(Call &c, const CUtensorMap &map0, const CUtensorMap &map1, con
 
 int check_groups(Call &c, int groups, int rows, int k, int n, const void *offsets, int offsets64)
 {
-    if (rows <= 0 || k <= 0 || n <= 0 || groups <= 0)
-        return c.failed("dimensions must be positive");
+    if (check_sizes(c, {rows, k, n, groups}))
+        return 1;
     if (!offsets)
         return c.failed("offsets pointer is null");
     if (misaligned(offsets, offsets64 ? 8 : 4))
@@ -976,8 +990,8 @@ namespace {
 
 int check_loss(Call &c, int m, int k, int v, const void *labels, int labels64)
 {
-    if (m <= 0 || k <= 0 || v <= 0)
-        return c.failed("dimensions must be positive");
+    if (check_sizes(c, {m, k, v}))
+        return 1;
     if (!labels)
         return c.failed("labels pointer is null");
     if (misaligned(labels, labels64 ? 8 : 4))

@@ -11,7 +11,7 @@ from precision import INPUT_DTYPES, PRECISIONS
 ACTIVATIONS = ("none", "relu", "gelu", "gelu_tanh", "silu")
 ACTIVATION_IDS = {name: index for index, name in enumerate(ACTIVATIONS)}
 OPERATOR_PRECISIONS = ("tf32", "fp16", "bf16")
-_INT_MAX = 2**31 - 1
+SIZE_MAX = 2**31 - 1024     # a tile past the end still has coordinates of 32 bits
 
 
 def _input_dtype(precision: str):
@@ -45,8 +45,8 @@ def _shape(name: str, tensor, shape: tuple) -> None:
 
 
 def _sizes(*sizes: int) -> None:
-    if any(size <= 0 or size > _INT_MAX for size in sizes):
-        raise ValueError("matrix dimensions must be positive and fit in a C int")
+    if any(size <= 0 or size > SIZE_MAX for size in sizes):
+        raise ValueError(f"matrix dimensions must be positive and at most {SIZE_MAX}")
 
 
 def _range(tensor) -> tuple[int, int]:

@@ -232,6 +232,8 @@ def test_entry_points_refuse_before_any_device_work(lib, name):
         assert rc == 1 and text.startswith(f"{name}: the precision must be")
     rc, text = _call(lib, name, *CALLS[name](ctx, 3, m=0))
     assert (rc, text) == (1, f"{name}: dimensions must be positive")
+    rc, text = _call(lib, name, *CALLS[name](ctx, 3, m=2**31 - 1023))
+    assert (rc, text) == (1, f"{name}: dimensions must be at most 2147482624")
     null = list(CALLS[name](ctx, 3))
     null[2] = None
     rc, text = _call(lib, name, *null)
@@ -259,3 +261,10 @@ def test_entry_points_refuse_more(lib):
     args[6] = 0
     assert "positive" in _call(lib, "matmul_grouped", *args)[1]
     assert "fp16" in _call(lib, "matmul_cross_entropy_backward", *CALLS["matmul_cross_entropy_backward"](ctx, 2))[1]
+
+
+def test_sizes_whose_tiles_would_leave_32_bits_are_refused():
+    ops._sizes(1, ops.SIZE_MAX)
+    for size in (0, -1, ops.SIZE_MAX + 1, 2**31 - 1, 2**40):
+        with pytest.raises(ValueError, match="must be positive and at most 2147482624"):
+            ops._sizes(4, size)

@@ -3,10 +3,13 @@ graphs, after a wait that ran out, on a part of the SMs, with outputs of every a
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
 import operator_reference as ref
+from operator_contracts import SIZE_MAX
 from operator_reference import DTYPES, assert_within
 from test_operators_gpu import guarded, loss_inputs, offset_copy, randn, sizes_to_offsets
 
@@ -417,3 +420,51 @@ def test_offsets_past_32_bits(native):
     picked = z.gather(1, labels.clamp(min=0)[:, None])[:, 0]
     expected = torch.where(labels == -100, torch.zeros_like(exact), exact - picked)
     assert_within(loss, expected, 2 * tlse + ref.U * exact.abs(), "loss")
+
+
+def test_the_longest_rows(native):
+    """The largest size a call takes, as columns and as the length of a sum; exact in FP32."""
+    n = SIZE_MAX
+    b = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(251).to(BF16).view(1, n)
+    a = torch.full((1, 1), 2.0, dtype=BF16, device="cuda")
+    out = torch.empty((1, n), dtype=BF16, device="cuda")
+    native.prepare_epilogue(a, b, out, precision="bf16")()
+    for c in range(0, n, 1 << 28):
+        assert torch.equal(out[:, c:c + (1 << 28)], 2.0 * b[:, c:c + (1 << 28)])
+    out.zero_()
+    native.prepare_epilogue_backward(b, precision="bf16", dbias=out.view(n))()
+    assert torch.equal(out, b)
+    out.zero_()
+    out[0, ::1 << 20] = 3.0
+    da = torch.empty((1, 1), device="cuda")
+    b[0, ::1 << 20] = 5.0
+    native.prepare_epilogue_backward(out, b=b, precision="bf16", da=da)()
+    assert float(da) == 15.0 * len(range(0, n, 1 << 20))
+
+
+def test_threads_share_a_context(native):
+    """Four threads prepare and enqueue on their own streams at once."""
+    eager = list(_unaligned_cases(native))
+    for launch, _ in eager:
+        launch()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            cases = list(_unaligned_cases(native))
+            for _ in range(20):
+                for launch, _ in cases:
+                    launch()
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(1 for (_, outs), (_, want) in zip(cases, eager)
+                         if not all(torch.equal(x, y) for x, y in zip(outs, want)))
+            done.append(1)
+
+    done = []
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(done) == 4 and not wrong
