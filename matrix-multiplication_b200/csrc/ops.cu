@@ -232,7 +232,8 @@ struct TileProblem {
     int64_t m, n, k_blocks, groups = 1;
     int bytes_out = 2;
     bool out_tma = true, splittable = false, transposable = false, ragged_k = false;
-    bool reduced = false;     // the loss's forward pass: rows are reduced, nothing is stored
+    bool exponentials = false;     // the loss: an exponential of every element
+    bool half_tiles = true;        // not in its forward pass
 };
 
 // Estimated cycles of a tile kind with K split S ways.  A K block costs the most of its MMA
@@ -248,7 +249,7 @@ double tile_cycles(const Context *ctx, int tile, int splits, const TileProblem &
     constexpr double kEpilogue[] = {4400.0, 1100.0, 1140.0, 810.0, 800.0, 1170.0, 1170.0};
     constexpr double kRowStores[] = {6000.0, 2000.0, 1000.0, 200.0, 400.0, 800.0, 1700.0};
     constexpr double kFloor[] = {2500.0, 1480.0, 900.0, 0.0, 0.0, 0.0, 0.0};
-    constexpr double kReduction[] = {6300.0, 4300.0, 3050.0, 0.0, 0.0, 0.0, 0.0};
+    constexpr double kExponentials[] = {6300.0, 4300.0, 3050.0, 0.0, 0.0, 0.0, 0.0};
     const TileShape &t = kTileShapes[tile];
     const bool swap = is_swap(tile);
     const int64_t side_m = swap ? q.n : q.m, side_n = swap ? q.m : q.n;
@@ -257,7 +258,7 @@ double tile_cycles(const Context *ctx, int tile, int splits, const TileProblem &
     const double active = splits > 1 ? tiles * splits : t.ctas * std::min(tiles, units);
     double rounds = splits > 1 ? 1.0 : std::max(1.0, std::ceil(tiles / units));
     // A pair's short last round runs as half tiles (enqueue).
-    if (t.ctas == 2 && q.groups == 1 && !q.reduced && std::fmod(tiles, units) > 0.0 && std::fmod(tiles, units) <= units / 2)
+    if (t.ctas == 2 && q.groups == 1 && q.half_tiles && std::fmod(tiles, units) > 0.0 && std::fmod(tiles, units) <= units / 2)
         rounds = std::floor(tiles / units) + 0.6;
     const double bytes = static_cast<double>(OP_BM + t.bn / t.ctas) * OP_ROW_BYTES;
     const double k_cycles = std::max({2.0 * t.bn, 140.0, bytes / 70.0, active * bytes / 9300.0});
@@ -268,9 +269,9 @@ double tile_cycles(const Context *ctx, int tile, int splits, const TileProblem &
     // 128 x 128 tile, 3000 ungrouped; 80 us in pairs, 107 us without).
     if (q.ragged_k && t.ctas == 1)
         tile_time += 1800.0;
-    // The loss's reduction of a tile takes as long whatever K is (1024 x 50304 with K = 64: 37,
-    // 49 and 68 us on the three kinds; K = 256 52 us with one CTA, 39 in pairs).
-    tile_time = std::max(tile_time, q.reduced ? kReduction[tile] : kFloor[tile] * q.bytes_out);
+    // The loss's epilogues take as long whatever K is (forward, 1024 x 50304 with K = 64: 37, 49
+    // and 68 us on the three kinds; K = 256 52 us with one CTA, 39 in pairs).
+    tile_time = std::max(tile_time, q.exponentials ? kExponentials[tile] : kFloor[tile] * q.bytes_out);
     return rounds * tile_time +
            (splits > 1 ? 3700.0 + 0.093 * static_cast<double>(splits - 1) / splits * OP_BM * t.bn * 4.0 : 0.0);
 }
@@ -1028,7 +1029,8 @@ extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hid
     OpLaunch &l = q.launch;
     l.epilogue = kEpiLse;
     TileProblem problem{m, v, (k + bk - 1) / bk};
-    problem.reduced = true;
+    problem.exponentials = true;
+    problem.half_tiles = false;
     l.tile = choose_tile(c.ctx, problem).tile;
     // One (maximum, sum) per row and column range of a tile.
     const int tiles = (v + kTileShapes[l.tile].bn - 1) / kTileShapes[l.tile].bn * loss_parts(l.tile);
@@ -1122,7 +1124,9 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
             q.n = cols;
             q.k = k;
             q.launch.epilogue = kEpiSoftmaxGrad;
-            q.launch.tile = choose_tile(c.ctx, {m, cols, (k + bk - 1) / bk, 1, e}).tile;
+            TileProblem problem{m, cols, (k + bk - 1) / bk, 1, e};
+            problem.exponentials = true;
+            q.launch.tile = choose_tile(c.ctx, problem).tile;
             OpParams &p = q.launch.p;
             p.labels = labels;
             p.labels64 = labels64;
