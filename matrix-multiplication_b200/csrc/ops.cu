@@ -350,11 +350,17 @@ int enqueue(Call &c, Product &q)
     const int b_cols = t.bn / t.ctas;     // Bop columns per CTA
     l.p.a_blocked = whole_blocks(c, swap ? q.b : q.a) ? 1 : 0;
     l.p.b_blocked = whole_blocks(c, q.b) ? 1 : 0;
+    // Where one tile holds all rows of A, its box holds them alone: TMA writes zeros for rows
+    // past the matrix more slowly than it reads rows, and what the shared memory holds there
+    // instead enters only rows of D that are not stored (the loss of 1 x 1024 x 50257, BF16: 76 -> 67 us).
+    const int most = swap ? b_cols : OP_BM;
+    const int box_rows = a_mn || q.m > most ? most : static_cast<int>(round_up(q.m, 8));
+    l.p.stage_tx = static_cast<uint32_t>(OP_ROW_BYTES * (t.ctas * (OP_BM + b_cols) - t.ctas * (most - box_rows)));
     bool ok;
     if (swap)     // D = B^T A^T: B's columns on the M side, A's rows on the N side
-        ok = operand_map(c, &l.map_a, q.b, true, OP_BM) && operand_map(c, &l.map_b, q.a, false, b_cols);
+        ok = operand_map(c, &l.map_a, q.b, true, OP_BM) && operand_map(c, &l.map_b, q.a, false, box_rows);
     else
-        ok = operand_map(c, &l.map_a, q.a, a_mn, OP_BM) && operand_map(c, &l.map_b, q.b, b_mn, b_cols);
+        ok = operand_map(c, &l.map_a, q.a, a_mn, box_rows) && operand_map(c, &l.map_b, q.b, b_mn, b_cols);
     if (!ok) {
         cudaGetLastError();
         return c.failed("cuTensorMapEncodeTiled rejected an operand");

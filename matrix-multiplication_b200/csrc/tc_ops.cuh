@@ -119,6 +119,7 @@ struct OpParams {
     OpDivisor per_raster;     // raster x N-side tiles (transposed epilogue: M-side tiles)
     OpDivisor per_group;      // ragged-K and chunked-K modes: tiles of one group or chunk
     int chunk_blocks;         // chunked-K mode: K blocks per chunk
+    uint32_t stage_tx;        // bytes that the loads of a K block bring
     int grouping;             // OpGrouping
     int a_blocked, b_blocked; // MN-major operands: 1 when their map sees blocks of 128 bytes of columns
     const int *row_tile_count;        // rows mode: number of row tiles (device)
@@ -483,7 +484,6 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     constexpr int kBoxes = Tile::kBoxes;
     constexpr bool kSplittable = CTAS == 1 && (EPI == kEpiStore || EPI == kEpiStoreT);
     constexpr int kGroupCols = BN / kGroups;              // D columns per epilogue warpgroup
-    constexpr uint32_t kStageTx = static_cast<uint32_t>(CTAS) * (OP_A_STAGE + kBStage);
     constexpr uint32_t kIdescHalfN = static_cast<uint32_t>((BN / 2) >> 3) << 17;
     // FP32 accumulator, formats, A MN-major (bit 15), B MN-major (bit 16), N >> 3, M >> 4.
     constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(FMT) << 7) | (static_cast<uint32_t>(FMT) << 10) |
@@ -675,7 +675,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                     const uint32_t fb = leader_full0 + 8u * stage;
                     if (leader)
-                        mbar_arrive_expect_tx(full_bar(stage), kStageTx);
+                        mbar_arrive_expect_tx(full_bar(stage), p.stage_tx);
                     const int k = w.k0 + kb * kBK;
                     auto load = [&](uint32_t dst, const void *map, int x, int y, int block, int z) {
                         if constexpr (kPair)
