@@ -106,6 +106,11 @@ struct Call {
     }
 };
 
+bool tma_addressable(const void *ptr, int64_t cols, int elem)
+{
+    return aligned16(ptr) && cols * elem % 16 == 0;
+}
+
 // An operand that TMA can address: the caller's matrix, or its copy in scratch with rows
 // padded to 128 bytes (unaligned bases and row pitches).
 struct Operand {
@@ -117,7 +122,7 @@ struct Operand {
     void plan(Call &c, const void *ptr, int64_t rows, int64_t cols, int64_t groups = 1)
     {
         source = Matrix{ptr, rows, cols, cols, groups, rows * cols};
-        direct = aligned16(ptr) && cols * c.elem() % 16 == 0;
+        direct = tma_addressable(ptr, cols, c.elem());
         ready = source;
         if (!direct) {
             ready.pitch = round_up(cols, OP_ROW_BYTES / c.elem());
@@ -318,6 +323,23 @@ TileChoice choose_tile(const Context *ctx, const TileProblem &q)
     return best;
 }
 
+// Whether a kernel had better load by itself a B that TMA cannot address (OpTile's DIRECT;
+// one tile of rows, 16-bit) than read a copy: it takes about 860 cycles more for a K block,
+// the copy what its bytes take in L2 and HBM (BF16, copied and direct: product 1 x 1024 x 50257
+// 56.5 and 29.6 us, 64 x 2048 x 18949 50.0 and 39.5, 32 x 300 x 9999 9.1 and 10.5; loss
+// 1 x 1024 x 50257 76 and 40, 128 x 1024 x 50257 73 and 46, 3 x 2000 x 777 15.6 and 25).
+bool direct_pays(const Context *ctx, int precision, const TileProblem &q, const TileChoice &choice, int epilogue)
+{
+    if (precision == kTf32 || (epilogue == kEpiLse ? choice.tile != kSingle128 || q.m > OP_BM
+                                                   : !is_swap(choice.tile) || choice.tile == kSwap128 ||
+                                                         q.m > kTileShapes[choice.tile].bn))
+        return false;
+    const int64_t tiles = (q.n + OP_BM - 1) / OP_BM, per = (q.k_blocks + choice.splits - 1) / choice.splits;
+    const int64_t rounds = choice.splits > 1 ? 1 : (tiles + ctx->sm_count - 1) / ctx->sm_count;
+    const double copied = 2.0 * static_cast<double>(q.k_blocks * OP_ROW_BYTES) * static_cast<double>(q.n);
+    return 1500.0 + 860.0 * static_cast<double>(rounds * per) < copied / 2700.0;
+}
+
 // A product with everything but its tile-dependent parts: operands as stored, sizes, and
 // in `launch` the epilogue's parameters.
 struct Product {
@@ -357,7 +379,11 @@ int enqueue(Call &c, Product &q)
     const int box_rows = a_mn || q.m > most ? most : static_cast<int>(round_up(q.m, 8));
     l.p.stage_tx = static_cast<uint32_t>(OP_ROW_BYTES * (t.ctas * (OP_BM + b_cols) - t.ctas * (most - box_rows)));
     bool ok;
-    if (swap)     // D = B^T A^T: B's columns on the M side, A's rows on the N side
+    if (l.p.direct) {     // B is loaded without TMA
+        l.p.k = static_cast<int>(q.k);
+        l.p.stage_tx = static_cast<uint32_t>(OP_ROW_BYTES * box_rows);
+        ok = operand_map(c, swap ? &l.map_b : &l.map_a, q.a, false, box_rows);
+    } else if (swap)     // D = B^T A^T: B's columns on the M side, A's rows on the N side
         ok = operand_map(c, &l.map_a, q.b, true, OP_BM) && operand_map(c, &l.map_b, q.a, false, box_rows);
     else
         ok = operand_map(c, &l.map_a, q.a, a_mn, box_rows) && operand_map(c, &l.map_b, q.b, b_mn, b_cols);
@@ -614,27 +640,31 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     DeviceScope device(c.ctx->device);
     if (device.status != cudaSuccess)
         return c.failed(device.status);
-    Operand oa, ob;
-    oa.plan(c, a, m, k);
-    ob.plan(c, b, k, n);
-    if (c.allocate() || prepare_operands(c, {&oa, &ob}))
-        return 1;
     Product q;
-    q.a = oa.ready;
-    q.b = ob.ready;
-    q.m = m;
-    q.n = n;
-    q.k = k;
     OpLaunch &l = q.launch;
     const int bk = OP_ROW_BYTES / e;
     const int64_t k_blocks = (static_cast<int64_t>(k) + bk - 1) / bk;
     const int bytes_out = (out_half ? 2 : 4) * (residual ? 2 : 1) + (preact ? (preact_half ? 2 : 4) : 0);
     const Matrix mo{out, m, n, n};
     const bool out_tma = output_tma(mo, out_half ? 2 : 4) && (!residual || aligned16(residual));
-    const TileChoice choice = choose_tile(c.ctx, {m, n, k_blocks, 1, bytes_out, out_tma, true, true});
+    const TileProblem problem{m, n, k_blocks, 1, bytes_out, out_tma, true, true};
+    const TileChoice choice = choose_tile(c.ctx, problem);
     l.tile = choice.tile;
     l.splits = choice.splits;
     l.epilogue = is_swap(choice.tile) ? kEpiStoreT : kEpiStore;
+    Operand oa, ob;
+    oa.plan(c, a, m, k);
+    if (!tma_addressable(b, n, e) && direct_pays(c.ctx, precision, problem, choice, l.epilogue))
+        l.p.direct = b;
+    else
+        ob.plan(c, b, k, n);
+    if (c.allocate() || prepare_operands(c, {&oa, &ob}))
+        return 1;
+    q.a = oa.ready;
+    q.b = ob.ready;
+    q.m = m;
+    q.n = n;
+    q.k = k;
     if (set_output(c, l, mo, out_half))
         return 1;
     OpParams &p = l.p;
@@ -1038,11 +1068,16 @@ extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hid
     problem.exponentials = true;
     problem.half_tiles = false;
     l.tile = choose_tile(c.ctx, problem).tile;
+    if (!tma_addressable(weight, v, e) && direct_pays(c.ctx, precision, problem, {kSingle128, 1}, kEpiLse)) {
+        l.tile = kSingle128;
+        l.p.direct = weight;
+    }
     // One (maximum, sum) per row and column range of a tile.
     const int tiles = (v + kTileShapes[l.tile].bn - 1) / kTileShapes[l.tile].bn * loss_parts(l.tile);
     Operand oh, ow;
     oh.plan(c, hidden, m, k);
-    ow.plan(c, weight, k, v);
+    if (!l.p.direct)
+        ow.plan(c, weight, k, v);
     const size_t partial_at = c.reserve(static_cast<size_t>(tiles) * m * sizeof(float2));
     const size_t logit_at = c.reserve(static_cast<size_t>(m) * sizeof(float));
     if (c.allocate() || prepare_operands(c, {&oh, &ow}))

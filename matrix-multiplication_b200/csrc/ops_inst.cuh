@@ -12,11 +12,27 @@ struct OpInstances {
     static constexpr bool kHalf = FMT != kOpTF32;
 
     // Calls f(kernel, CTAs per tile, threads, shared memory) and shared memory for the kernel of a launch.
-    template <int CTAS, int BN, bool A_MN, bool B_MN, int EPI, typename F>
+    template <int CTAS, int BN, bool A_MN, bool B_MN, int EPI, bool DIRECT = false, typename F>
     static cudaError_t with(F &&f)
     {
-        using Tile = OpTile<CTAS, BN>;
-        return f(&op_kernel<FMT, CTAS, BN, A_MN, B_MN, EPI>, CTAS, Tile::kThreads, Tile::kSmem);
+        using Tile = OpTile<CTAS, BN, DIRECT>;
+        return f(&op_kernel<FMT, CTAS, BN, A_MN, B_MN, EPI, DIRECT>, CTAS, Tile::kThreads, Tile::kSmem);
+    }
+    // Kernels that load B themselves (can_load_directly).
+    template <typename F>
+    static cudaError_t with_direct(int tile, int epilogue, F &&f)
+    {
+        if constexpr (kHalf) {
+            if (epilogue == kEpiLse && tile == kSingle128)
+                return with<1, 128, false, true, kEpiLse, true>(f);
+            if (epilogue == kEpiStoreT && tile == kSwap16)
+                return with<1, 16, true, false, kEpiStoreT, true>(f);
+            if (epilogue == kEpiStoreT && tile == kSwap32)
+                return with<1, 32, true, false, kEpiStoreT, true>(f);
+            if (epilogue == kEpiStoreT && tile == kSwap64)
+                return with<1, 64, true, false, kEpiStoreT, true>(f);
+        }
+        return cudaErrorInvalidValue;
     }
     template <bool A_MN, bool B_MN, int EPI, typename F>
     static cudaError_t with_tile(int tile, F &&f)
@@ -70,12 +86,18 @@ struct OpInstances {
         }
         for (int tile = kSwap16; tile <= kSwap128 && st == cudaSuccess; ++tile)
             st = with_kernel(kNN, tile, kEpiStoreT, set);
+        if (kHalf) {
+            for (int tile = kSwap16; tile <= kSwap64 && st == cudaSuccess; ++tile)
+                st = with_direct(tile, kEpiStoreT, set);
+            if (st == cudaSuccess)
+                st = with_direct(kSingle128, kEpiLse, set);
+        }
         return st;
     }
 
     static cudaError_t product(const OpLaunch &l, cudaStream_t stream)
     {
-        return with_kernel(l.layout, l.tile, l.epilogue, [&](auto kernel, int ctas, int threads, int smem) {
+        auto launch = [&](auto kernel, int ctas, int threads, int smem) {
             cudaLaunchConfig_t config{};
             config.gridDim = dim3(static_cast<unsigned int>(l.grid), 1, static_cast<unsigned int>(l.splits));
             config.blockDim = dim3(static_cast<unsigned int>(threads));
@@ -91,7 +113,8 @@ struct OpInstances {
             config.attrs = attributes;
             config.numAttrs = ctas > 1 || l.splits > 1 ? 2 : 1;
             return cudaLaunchKernelEx(&config, kernel, l.map_a, l.map_b, l.map_c, l.map_z, l.p);
-        });
+        };
+        return l.p.direct ? with_direct(l.tile, l.epilogue, launch) : with_kernel(l.layout, l.tile, l.epilogue, launch);
     }
 
     static cudaError_t act_grad(const ActGradParams &params, dim3 grid, int cluster, cudaStream_t stream)

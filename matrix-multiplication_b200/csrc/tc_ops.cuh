@@ -62,18 +62,31 @@ constexpr int OP_BAR_BYTES = 512;
 // by half, as in tc2_gemm.cuh) was built and taken out: 311 us against 323 us at 4096 x
 // 4096 x 14336 BF16, 695 against 714 us at 8192^3, ahead by 1 % at most where its count
 // of tiles fits the pairs better.
-template <int CTAS, int BN>
+//
+// DIRECT: B (16-bit, 128 columns a tile) has rows that start on any element, which TMA
+// cannot address.  Two more warps fetch the aligned 16-byte pieces that a K block's rows lie
+// in through kRaw buffers, eight more shift them into the place where TMA would have
+// written them.  For few rows of A, whose products are too short to hide a copy of B behind
+// (direct_pays).  Bound by the shifting: 2 to 4 TB/s of B where TMA reads an aligned one at
+// 5.
+template <int CTAS, int BN, bool DIRECT = false>
 struct OpTile {
     static constexpr int kBCols = BN / CTAS;                   // N columns staged per CTA
     static constexpr int kBStage = kBCols * OP_ROW_BYTES;
-    static constexpr int kStages = kBCols >= 128 ? 5 : 8;
+    static constexpr int kStages = DIRECT ? 3 : kBCols >= 128 ? 5 : 8;
     static constexpr int kGroups = BN >= 128 ? 2 : 1;          // epilogue warpgroups
     static constexpr int kFirstEpi = kGroups == 2 ? 4 : 2;     // first epilogue warp (after TMA, MMA, two idle ones)
-    static constexpr int kThreads = 32 * (kFirstEpi + 4 * kGroups);
+    static constexpr int kFirstLoader = kFirstEpi + 4 * kGroups;
+    static constexpr int kFetchers = DIRECT ? 2 : 0, kShifters = DIRECT ? 8 : 0;   // warps
+    static constexpr int kThreads = 32 * (kFirstLoader + kFetchers + kShifters);
+    static constexpr int kRaw = DIRECT ? (BN >= 128 ? 7 : 8) : 0;
+    static constexpr int kRawPitch = 17 * 16;                  // a row's 128 16-bit columns at any skew
+    static constexpr int kRawBytes = 64 * kRawPitch;
     static constexpr int kBoxes = 2;                           // boxes per epilogue warpgroup
-    static constexpr int kEpiBytes = kBoxes * kGroups * OP_BOX;
+    static constexpr int kEpiBytes = DIRECT ? 0 : kBoxes * kGroups * OP_BOX;   // none in these epilogues
     static constexpr int kBiasBytes = BN * 4 < 256 ? 256 : BN * 4;
-    static constexpr int kSmem = 1024 + kStages * (OP_A_STAGE + kBStage) + kEpiBytes + OP_BAR_BYTES + kBiasBytes;
+    static constexpr int kSmem = 1024 + kStages * (OP_A_STAGE + kBStage) + kEpiBytes + OP_BAR_BYTES + kBiasBytes +
+                                 kRaw * kRawBytes;
     static constexpr uint32_t kTmemColumns = 2 * BN < 32 ? 32 : 2 * BN;   // two accumulators
     static_assert(kSmem <= 227 * 1024, "tile exceeds shared memory");
 };
@@ -119,7 +132,9 @@ struct OpParams {
     OpDivisor per_raster;     // raster x N-side tiles (transposed epilogue: M-side tiles)
     OpDivisor per_group;      // ragged-K and chunked-K modes: tiles of one group or chunk
     int chunk_blocks;         // chunked-K mode: K blocks per chunk
-    uint32_t stage_tx;        // bytes that the loads of a K block bring
+    uint32_t stage_tx;        // bytes that the TMA loads of a K block bring
+    const void *direct;       // DIRECT: B (K x n, rows without padding)
+    int k;                    // DIRECT: its rows
     int grouping;             // OpGrouping
     int a_blocked, b_blocked; // MN-major operands: 1 when their map sees blocks of 128 bytes of columns
     const int *row_tile_count;        // rows mode: number of row tiles (device)
@@ -459,18 +474,57 @@ __device__ __forceinline__ OpWhere op_where(int tile, int row_tile_count, int bk
     return w;
 }
 
-template <int FMT, int CTAS, int BN, bool A_MN, bool B_MN, int EPI>
-__global__ void __launch_bounds__(OpTile<CTAS, BN>::kThreads, 1)
+// 16 bytes that start `skew` (even) bytes into lo, the rest from hi.
+__device__ __forceinline__ uint4 skewed_16_bytes(const uint4 &lo, const uint4 &hi, uint32_t skew)
+{
+    uint32_t w0 = lo.x, w1 = lo.y, w2 = lo.z, w3 = lo.w, w4 = hi.x, w5 = hi.y, w6 = hi.z;
+    if (skew & 8) {
+        w0 = w2;
+        w1 = w3;
+        w2 = w4;
+        w3 = w5;
+        w4 = w6;
+        w5 = hi.w;
+    }
+    if (skew & 4) {
+        w0 = w1;
+        w1 = w2;
+        w2 = w3;
+        w3 = w4;
+        w4 = w5;
+    }
+    const uint32_t bits = 8 * (skew & 3);
+    return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                      __funnelshift_r(w3, w4, bits));
+}
+
+// The aligned 16 bytes at `at`; what lies outside [begin, end) is not read and zero.
+__device__ __forceinline__ uint4 load_16_within(uintptr_t at, uintptr_t begin, uintptr_t end)
+{
+    if (at >= begin && at + 16 <= end)
+        return *reinterpret_cast<const uint4 *>(at);
+    uint32_t words[4] = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (at + 2 * e >= begin && at + 2 * e + 2 <= end)
+            words[e / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(at + 2 * e)) << (16 * (e & 1));
+    return make_uint4(words[0], words[1], words[2], words[3]);
+}
+
+template <int FMT, int CTAS, int BN, bool A_MN, bool B_MN, int EPI, bool DIRECT = false>
+__global__ void __launch_bounds__(OpTile<CTAS, BN, DIRECT>::kThreads, 1)
 op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_z,
           const __grid_constant__ OpParams p)
 {
-    using Tile = OpTile<CTAS, BN>;
+    using Tile = OpTile<CTAS, BN, DIRECT>;
     using Type = OpType<FMT>;
     using T = typename Type::T;
     constexpr bool kPair = CTAS == 2;
     constexpr bool kSwap = EPI == kEpiStoreT;
     constexpr bool kTF32 = FMT == kOpTF32;
+    constexpr int kThreads = Tile::kThreads;
+    constexpr int kFirstLoader = Tile::kFirstLoader;
     constexpr int kElem = kTF32 ? 4 : 2;
     constexpr int kBK = OP_ROW_BYTES / kElem;             // K elements per stage (64 or 32)
     constexpr int kMmaK = 32 / kElem;
@@ -492,6 +546,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                                 (static_cast<uint32_t>((OP_BM * CTAS) >> 4) << 24);
     static_assert(!B_MN || kBCols % kBox == 0, "whole MN-major boxes");
     static_assert(!kPair || !kSwap, "the transposed epilogue runs on single CTAs");
+    static_assert(!DIRECT || (!kPair && !kTF32 && (kSwap || (B_MN && BN == 128))), "128 columns of B per CTA");
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
@@ -508,6 +563,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const uint32_t drain_bar = s_bar + 8u * (2 * kStages + 4);
     const uint32_t tmem_slot = s_bar + 8u * (2 * kStages + 5);
     const uint32_t recv_bar = s_bar + 8u * (2 * kStages + 6);   // split K: partial rows received
+    auto direct_bar = [&](int s) { return s_bar + 8u * (2 * kStages + 12 + s); };     // DIRECT: B's part of a stage
+    auto raw_full_bar = [&](int i) { return s_bar + 8u * (3 * kStages + 12 + i); };   // its buffers on the way there
+    auto raw_empty_bar = [&](int i) { return s_bar + 8u * (3 * kStages + 12 + Tile::kRaw + i); };
+    static_assert(8 * (3 * kStages + 12 + 2 * Tile::kRaw) <= OP_BAR_BYTES && kGroups * kBoxes <= 4, "barriers fit");
     const uint32_t fail_flag = s_bar + 8u * (2 * kStages + 7);  // split K: 1 once a progress wait of this CTA ran out
     volatile uint32_t *fail_flag_ptr = reinterpret_cast<volatile uint32_t *>(smem_raw + (fail_flag - raw));
     uint32_t *tmem_slot_ptr = reinterpret_cast<uint32_t *>(smem_raw + (tmem_slot - raw));
@@ -530,6 +589,12 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
+            if constexpr (DIRECT)
+                mbar_init(direct_bar(s), Tile::kShifters / 2);
+        }
+        for (int i = 0; i < Tile::kRaw; ++i) {
+            mbar_init(raw_full_bar(i), 32 * Tile::kFetchers);
+            mbar_init(raw_empty_bar(i), Tile::kShifters / 2);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(accf_bar(i), 1);
@@ -543,8 +608,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         fence_mbarrier_init();
     }
     if (warp == 0 && lane == 0) {
-        tma_prefetch_map(&map_a);
-        tma_prefetch_map(&map_b);
+        if constexpr (!DIRECT || !kSwap)
+            tma_prefetch_map(&map_a);
+        if constexpr (!DIRECT || kSwap)
+            tma_prefetch_map(&map_b);
     }
     if (warp == 1) {
         if constexpr (kPair) {
@@ -693,11 +760,15 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         }
                     };
                     const uint32_t sa = s_a + stage * OP_A_STAGE, sb = s_b + stage * kBStage;
-                    if constexpr (A_MN)
+                    if constexpr (DIRECT && kSwap)
+                        ;
+                    else if constexpr (A_MN)
                         load_mn(sa, ma, p.a_blocked != 0, am, OP_BM, za);
                     else
                         load(sa, ma, k, am, 0, za);
-                    if constexpr (B_MN)
+                    if constexpr (DIRECT && !kSwap)
+                        ;
+                    else if constexpr (B_MN)
                         load_mn(sb, mb, p.b_blocked != 0, bn, kBCols, zb);
                     else
                         load(sb, mb, k, bn, 0, zb);
@@ -754,7 +825,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 const uint32_t idesc = kPair && w.cols != BN ? kIdesc - kIdescHalfN : kIdesc;     // half the N
                 const int nkb = kb_end(w.nkb);
                 for (int kb = kb_begin; kb < nkb; ++kb) {
-                    if (!mbar_wait(full_bar(stage), phase, p.wait_limit_ns)) {
+                    bool here = mbar_wait(full_bar(stage), phase, p.wait_limit_ns);
+                    if constexpr (DIRECT)
+                        here = here && mbar_wait(direct_bar(stage), phase, p.wait_limit_ns);
+                    if (!here) {
                         atomicOr(p.status, kOpMmaTimeout);
                         ok = false;
                         break;
@@ -797,6 +871,155 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 atomicOr(p.status, kOpDrainTimeout);
         }
         __syncwarp();
+    } else if (DIRECT && warp >= kFirstLoader) {
+        // ------------------------------------------------------------ B without TMA
+        // Some warps fetch, others shift: threads that did both (copy, shift, fence.proxy.async) took
+        // 1900 cycles a K block however many were in flight (product 8 x 4096 x 14337: 55 us, 37 so).
+        if constexpr (DIRECT) {
+            constexpr int kRaw = Tile::kRaw, kPieces = 17 * 64;
+            constexpr int kFetching = 32 * Tile::kFetchers, kShifting = 16 * Tile::kShifters;    // threads per K block
+            const uint32_t s_raw = s_bias + Tile::kBiasBytes;
+            const uintptr_t begin = reinterpret_cast<uintptr_t>(p.direct);
+            const uintptr_t row_bytes = static_cast<uintptr_t>(p.n) * 2;
+            const int kb_last = kb_end(p.num_k_blocks);
+            int buffer = 0;
+            uint32_t buffer_phase = 0;
+            bool ok = true;
+            if (warp < kFirstLoader + Tile::kFetchers) {
+                const int thread = static_cast<int>(threadIdx.x) - 32 * kFirstLoader;
+                const uintptr_t end = begin + static_cast<uintptr_t>(p.k) * row_bytes;
+                // 64 rows, and 128 columns, are multiples of 16 bytes: a thread's pieces lie alike in every K
+                // block of every tile.
+                constexpr int kMine = (kPieces + kFetching - 1) / kFetching;
+                uintptr_t source[kMine];
+                uint32_t place[kMine];
+#pragma unroll
+                for (int j = 0; j < kMine; ++j) {
+                    const int at = min(thread + j * kFetching, kPieces - 1), row = at / 17, piece = at - row * 17;
+                    source[j] = ((begin + row * row_bytes) & ~uintptr_t{15}) + 16 * piece;
+                    place[j] = s_raw + row * Tile::kRawPitch + piece * 16;
+                }
+                for (int tile = tile_first; ok && tile < tile_end; tile += tile_step) {
+                    const OpWhere w = op_where<CTAS, BN, kSwap>(tile, row_tile_count, kBK, p);
+                    const int column = kSwap ? w.m0 : w.n0;
+                    for (int kb = kb_begin; kb < kb_last; ++kb) {
+                        if (!mbar_wait(raw_empty_bar(buffer), buffer_phase ^ 1u, p.wait_limit_ns)) {
+                            atomicOr(p.status, kOpLoadTimeout);
+                            ok = false;
+                            break;
+                        }
+                        const uintptr_t block = static_cast<uintptr_t>(kb) * kBK * row_bytes + static_cast<uintptr_t>(column) * 2;
+                        const uint32_t to = buffer * Tile::kRawBytes;
+                        const int rows = min(64, p.k - kb * kBK);
+                        // Away from both ends of the matrix every piece is whole, or behind the last row.
+                        if (block >= 16 && begin + block + (rows - 1) * row_bytes + 17 * 16 <= end) {
+#pragma unroll
+                            for (int j = 0; j < kMine; ++j) {
+                                const int at = thread + j * kFetching;
+                                if (j == kMine - 1 && at >= kPieces)
+                                    break;
+                                const bool inside = rows == 64 || at < 17 * rows;
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place[j] + to),
+                                             "l"(inside ? source[j] + block : source[0]), "r"(inside ? 16 : 0)
+                                             : "memory");
+                            }
+                            asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(raw_full_bar(buffer))
+                                         : "memory");
+                        } else {
+#pragma unroll 1
+                            for (int i = thread; i < kPieces; i += kFetching) {
+                                const int row = i / 17, piece = i - row * 17;
+                                const uintptr_t at = ((begin + row * row_bytes) & ~uintptr_t{15}) + 16 * piece + block;
+                                const uint32_t dst = s_raw + to + row * Tile::kRawPitch + piece * 16;
+                                if (kb * kBK + row < p.k && at >= begin && at + 16 <= end) {
+                                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(at) : "memory");
+                                } else {
+                                    const uint4 v = kb * kBK + row < p.k ? load_16_within(at, begin, end)
+                                                                         : make_uint4(0u, 0u, 0u, 0u);
+                                    st_shared_v4(dst, v.x, v.y, v.z, v.w);
+                                }
+                            }
+                            asm volatile("cp.async.wait_all;" ::: "memory");
+                            mbar_arrive(raw_full_bar(buffer));
+                        }
+                        if (++buffer == kRaw) {
+                            buffer = 0;
+                            buffer_phase ^= 1u;
+                        }
+                    }
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+            } else {
+                // Two sets of warps take K blocks in turn.
+                const int shifter = static_cast<int>(threadIdx.x) - 32 * (kFirstLoader + Tile::kFetchers);
+                const int thread = shifter % kShifting, set = shifter / kShifting;
+                int turn = 0;
+                const uint32_t skew = static_cast<uint32_t>(begin + (thread >> 4) * row_bytes) & 15u;
+                int stage = 0;
+                uint32_t phase = 0;
+                for (int tile = tile_first; ok && tile < tile_end; tile += tile_step) {
+                    for (int kb = kb_begin; kb < kb_last; ++kb) {
+                        const bool mine = turn == set;
+                        turn ^= 1;
+                        if (mine) {
+                            int ready = 0;
+                            if (lane == 0)
+                                ready = mbar_wait(empty_bar(stage), phase ^ 1u, p.wait_limit_ns) &&
+                                                mbar_wait(raw_full_bar(buffer), buffer_phase, p.wait_limit_ns)
+                                            ? 1
+                                            : 0;
+                            ready = __shfl_sync(0xffffffffu, ready, 0);
+                            // Every thread waits by itself for what it reads (this one is complete).
+                            if (!ready || !mbar_wait(raw_full_bar(buffer), buffer_phase, p.wait_limit_ns)) {
+                                if (lane == 0)
+                                    atomicOr(p.status, kOpLoadTimeout);
+                                ok = false;
+                                break;
+                            }
+                            const uint32_t from = s_raw + buffer * Tile::kRawBytes;
+                            const uint32_t to = kSwap ? s_a + stage * OP_A_STAGE : s_b + stage * kBStage;
+#pragma unroll
+                            for (int i0 = 0; i0 < 64 * 16 / kShifting; i0 += 4) {
+                                uint4 lo[4], hi[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const int at = thread + (i0 + i) * kShifting, row = at >> 4, piece = at & 15;
+                                    const uint32_t src = from + row * Tile::kRawPitch + piece * 16;
+                                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                                 : "=r"(lo[i].x), "=r"(lo[i].y), "=r"(lo[i].z), "=r"(lo[i].w)
+                                                 : "r"(src));
+                                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                                 : "=r"(hi[i].x), "=r"(hi[i].y), "=r"(hi[i].z), "=r"(hi[i].w)
+                                                 : "r"(src + 16));
+                                }
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const int at = thread + (i0 + i) * kShifting, row = at >> 4, piece = at & 15;
+                                    const uint4 v = skewed_16_bytes(lo[i], hi[i], skew);
+                                    st_shared_v4(to + (piece >> 3) * kBoxBytes + row * OP_ROW_BYTES +
+                                                     (((piece & 7) ^ (row & 7)) << 4),
+                                                 v.x, v.y, v.z, v.w);
+                                }
+                            }
+                            fence_proxy_async_shared();      // the tensor core reads these stores
+                            __syncwarp();
+                            if (lane == 0) {
+                                mbar_arrive(direct_bar(stage));
+                                mbar_arrive(raw_empty_bar(buffer));
+                            }
+                        }
+                        if (++buffer == kRaw) {
+                            buffer = 0;
+                            buffer_phase ^= 1u;
+                        }
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+            }
+        }
     } else if (warp >= Tile::kFirstEpi) {
         // ------------------------------------------------------------ epilogue
         const int quarter = warp & 3;                 // TMEM lanes 32 * quarter .. +31
@@ -949,7 +1172,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 // The same with the residual already in the box: each thread adds its own row to `v`,
                 // puts the result in its place and the box is stored.
                 auto emit_residual = [&](auto &v, const void *map, int col0) {
-                    constexpr bool kHalfBox = std::extent<std::remove_reference_t<decltype(v)>>::value == 64;
+                    constexpr bool kShiftingBox = std::extent<std::remove_reference_t<decltype(v)>>::value == 64;
                     const uint32_t b = stores % kBoxes;
                     fetch(static_cast<int>(box_done) + 1);
                     if (!mbar_wait(res_bar(b), (res_parity >> b) & 1u)) {
@@ -963,7 +1186,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const uint4 q = *reinterpret_cast<const uint4 *>(smem_raw + (row_addr + ((j ^ (r & 7)) << 4) - raw));
-                        if constexpr (kHalfBox) {
+                        if constexpr (kShiftingBox) {
                             const T *h = reinterpret_cast<const T *>(&q);
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
@@ -1380,7 +1603,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             uint32_t any_failed = 0;
             for (int j = 0; j < splits; ++j)
                 any_failed |= ld_shared_cluster_u32(map_to_cta(fail_flag, static_cast<uint32_t>(j)));
-            if (warp >= Tile::kFirstEpi) {
+            if (warp >= Tile::kFirstEpi && warp < kFirstLoader) {
                 const int quarter = warp & 3, r = quarter * 32 + lane;
                 const int first = ((warp - Tile::kFirstEpi) >> 2) * kGroupCols;
                 const uint32_t row_addr = s_a + static_cast<uint32_t>(r) * kPitch;
@@ -1423,10 +1646,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             const int first_row = w.m0 + z * rows;        // D's rows of this CTA
             if (any_failed || !received) {
                 nan_elements(w, kSwap ? w.n0 : first_row, kSwap ? BN : rows, kSwap ? first_row : w.n0, kSwap ? rows : BN,
-                             warp, Tile::kThreads / 32, lane);
+                             warp, kThreads / 32, lane);
             } else {
                 const uint8_t *ring = smem_raw + (s_a - raw);
-                for (int idx = threadIdx.x; idx < rows * (BN / 4); idx += Tile::kThreads) {
+                for (int idx = threadIdx.x; idx < rows * (BN / 4); idx += kThreads) {
                     // Neighbouring threads take neighbouring output columns.
                     const int rl = kSwap ? idx % rows : idx / (BN / 4), q = kSwap ? idx / rows : idx % (BN / 4);
                     const int r = z * rows + rl;

@@ -468,3 +468,100 @@ def test_threads_share_a_context(native):
     for t in threads:
         t.join()
     assert len(done) == 4 and not wrong
+
+
+def odd_weight(k, n, dtype, offset):
+    """A weight whose rows no 16-byte copy can address, `offset` elements into memory that NaN surrounds."""
+    whole = torch.full((k * n + 64,), float("nan"), dtype=dtype, device="cuda")
+    return whole[16 + offset:16 + offset + k * n].view(k, n).copy_(randn((k, n), dtype, 2, 3.0 * k ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", (BF16, torch.float16), ids=("bf16", "fp16"))
+@pytest.mark.parametrize("shape", [(1, 1024, 20001), (3, 64, 113301), (16, 770, 32003), (17, 128, 40009), (33, 1000, 20007),
+                                   (64, 130, 100002), (64, 2048, 18949)], ids=lambda s: "x".join(map(str, s)))
+def test_few_rows_by_an_unaligned_weight(native, dtype, shape):
+    """Products that read such a weight in place, at both ends of its memory; with a residual in place."""
+    m, k, n = shape
+    precision = "bf16" if dtype == BF16 else "fp16"
+    for offset in (0, 1, 7):
+        a, b = randn((m, k), dtype, 1), odd_weight(k, n, dtype, offset)
+        (out, ua), (preact, ub) = guarded((m, n), dtype), guarded((m, n), FP32)
+        bias = randn((n,), FP32, 3)
+        run = native.prepare_epilogue(a, b, out, precision=precision, bias=bias, activation="gelu", preact=preact)
+        run()
+        expected = ref.epilogue(a, b, precision, bias, "gelu")
+        assert_within(out, *expected["out"], "out")
+        assert_within(preact, *expected["preact"], "preact")
+        ua(), ub()
+        first = out.clone()
+        run()
+        assert torch.equal(first, out)
+        residual = randn((m, n), dtype, 4)
+        out.copy_(residual)
+        native.prepare_epilogue(a, b, out, precision=precision, residual=out)()
+        assert_within(out, *ref.epilogue(a, b, precision, None, "none", residual)["out"], "residual in place")
+
+
+@pytest.mark.parametrize("dtype", (BF16, torch.float16), ids=("bf16", "fp16"))
+@pytest.mark.parametrize("shape", [(1, 1024, 50257), (2, 64, 60001), (40, 200, 50003), (100, 768, 32001), (128, 65, 70002)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_loss_of_few_rows_by_an_unaligned_weight(native, dtype, shape):
+    m, k, v = shape
+    precision = "bf16" if dtype == BF16 else "fp16"
+    hidden, _, labels, _ = loss_inputs(m, k, v, precision)
+    for offset in (0, 1):
+        weight = odd_weight(k, v, dtype, offset)
+        (loss, ul), (lse, us) = guarded((m,), FP32), guarded((m,), FP32)
+        run = native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision=precision)
+        run()
+        expected = ref.cross_entropy(hidden, weight, labels, precision)
+        assert_within(loss, *expected["loss"], "loss")
+        assert_within(lse, *expected["lse"], "lse")
+        ul(), us()
+        first = loss.clone(), lse.clone()
+        run()
+        assert torch.equal(first[0], loss) and torch.equal(first[1], lse)
+
+
+def test_unaligned_weights_in_a_graph_and_after_waits_that_ran_out(native):
+    a, b = randn((16, 2048), BF16, 1), odd_weight(2048, 20001, BF16, 1)
+    hidden, _, labels, _ = loss_inputs(100, 1024, 30001, "bf16")
+    weight = odd_weight(1024, 30001, BF16, 1)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        out = torch.zeros((16, 20001), dtype=BF16, device="cuda")
+        loss, lse = torch.zeros(100, device="cuda"), torch.zeros(100, device="cuda")
+        runs = [(native.prepare_epilogue(a, b, out, precision="bf16"), (out,)),
+                (native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision="bf16"), (lse,))]
+    torch.cuda.synchronize()
+    good = []
+    for run, outs in runs:
+        run()
+        torch.cuda.synchronize()
+        good.append([t.clone() for t in outs])
+        assert native.device_status() == 0
+        native.set_wait_limit(1)
+        try:
+            run()
+            status = native.device_status()
+        finally:
+            native.set_wait_limit(0)
+        assert status & (LOAD | MMA | EPILOGUE) and not status & DRAIN, f"status {status:#x}"
+        assert all(bool(torch.isnan(t).any()) for t in outs)
+        run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(good[-1], outs)) and native.device_status() == 0
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for run, _ in runs:
+            run()
+    for _ in range(3):
+        for _, outs in runs:
+            for t in outs:
+                t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for (_, outs), want in zip(runs, good):
+            assert all(torch.equal(x, y) for x, y in zip(outs, want))
+    del graph
