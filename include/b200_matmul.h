@@ -178,7 +178,8 @@ int matmul_launch_noalloc(void *context, int implementation, int precision,
  * everything else inside are FP32.  An output or an auxiliary operand followed by
  * a flag `x_fp32` is FP32 when the flag is not 0, otherwise in the input format
  * (rounded to it once, to nearest even).  Operands that TMA cannot address are
- * repacked first, and other scratch is stream-ordered, as in matmul_launch.  The
+ * repacked first (or read in place, where few rows meet a 16-bit weight), and
+ * other scratch is stream-ordered, as in matmul_launch.  The
  * caller's current device is the same after the call.  A wait that runs out is
  * reported and leaves NaN as in matmul_set_wait_limit.  Outputs must not overlap
  * inputs or each other unless said otherwise.

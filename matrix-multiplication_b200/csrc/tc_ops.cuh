@@ -20,7 +20,7 @@
 // tc_gemm.cuh (CTAS = 1: 128 x BN).  Operand maps are four-dimensional (inner, rows,
 // column block, group): a coordinate past a group's own K rows reads zeros, not the next
 // group.  An MN-major operand whose columns are whole 128-byte blocks is one load per
-// stage.
+// stage.  A 16-bit weight that TMA cannot address may be loaded by extra warps (DIRECT).
 //
 // Measured choices stand at the host's plan (ops.cu).
 #pragma once
