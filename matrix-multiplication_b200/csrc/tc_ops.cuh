@@ -920,7 +920,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                                     break;
                                 const bool inside = rows == 64 || at < 17 * rows;
                                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place[j] + to),
-                                             "l"(inside ? source[j] + block : source[0]), "r"(inside ? 16 : 0)
+                                             "l"(inside ? source[j] + block : begin & ~uintptr_t{15}), "r"(inside ? 16 : 0)
                                              : "memory");
                             }
                             asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(raw_full_bar(buffer))

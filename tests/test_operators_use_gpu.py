@@ -478,7 +478,7 @@ def odd_weight(k, n, dtype, offset):
 
 @pytest.mark.parametrize("dtype", (BF16, torch.float16), ids=("bf16", "fp16"))
 @pytest.mark.parametrize("shape", [(1, 1024, 20001), (3, 64, 113301), (16, 770, 32003), (17, 128, 40009), (33, 1000, 20007),
-                                   (64, 130, 100002), (64, 2048, 18949)], ids=lambda s: "x".join(map(str, s)))
+                                   (64, 130, 100002), (64, 2048, 18949), (2, 1, 200001), (5, 3, 150001)], ids=lambda s: "x".join(map(str, s)))
 def test_few_rows_by_an_unaligned_weight(native, dtype, shape):
     """Products that read such a weight in place, at both ends of its memory; with a residual in place."""
     m, k, n = shape
