@@ -10,32 +10,6 @@
 
 namespace b200 {
 
-// 16 bytes from an address aligned to ELEM bytes: words where it starts on 4 bytes, else a
-// half word, three words and a half word shifted into place, so that nothing outside the
-// 16 bytes is read.
-template <int ELEM>
-__device__ __forceinline__ uint4 load_16_bytes(const uint8_t *from)
-{
-    uint4 q;
-    if (ELEM == 2 && (reinterpret_cast<uintptr_t>(from) & 2u)) {
-        const uint32_t w0 = *reinterpret_cast<const uint16_t *>(from);
-        const uint32_t w1 = *reinterpret_cast<const uint32_t *>(from + 2);
-        const uint32_t w2 = *reinterpret_cast<const uint32_t *>(from + 6);
-        const uint32_t w3 = *reinterpret_cast<const uint32_t *>(from + 10);
-        const uint32_t w4 = *reinterpret_cast<const uint16_t *>(from + 14);
-        q.x = w0 | (w1 << 16);
-        q.y = (w1 >> 16) | (w2 << 16);
-        q.z = (w2 >> 16) | (w3 << 16);
-        q.w = (w3 >> 16) | (w4 << 16);
-    } else {
-        q.x = reinterpret_cast<const uint32_t *>(from)[0];
-        q.y = reinterpret_cast<const uint32_t *>(from)[1];
-        q.z = reinterpret_cast<const uint32_t *>(from)[2];
-        q.w = reinterpret_cast<const uint32_t *>(from)[3];
-    }
-    return q;
-}
-
 // ---------------------------------------------------------------- operand copy
 constexpr int RP_THREADS = 256;
 

@@ -565,3 +565,24 @@ def test_unaligned_weights_in_a_graph_and_after_waits_that_ran_out(native):
         for (_, outs), want in zip(runs, good):
             assert all(torch.equal(x, y) for x, y in zip(outs, want))
     del graph
+
+
+@pytest.mark.parametrize("precision", ("bf16", "fp16", "tf32"))
+@pytest.mark.parametrize("shape", [(300, 64, 1037), (1000, 300, 515), (2100, 72, 1026), (130, 2000, 33)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_unaligned_residuals_apart_and_in_place(native, precision, shape):
+    m, k, n = shape
+    dtype = DTYPES[precision]
+    a, b = randn((m, k), dtype, 1), randn((k, n), dtype, 2, k ** -0.5)
+    for out_dtype in dict.fromkeys((dtype, FP32)):
+        residual = randn((m, n), out_dtype, 4)
+        expected = ref.epilogue(a, b, precision, None, "silu", residual)
+        for given in (residual, offset_copy(residual), None):
+            (out, untouched), (preact, ub) = guarded((m, n), out_dtype), guarded((m, n), FP32)
+            if given is None:
+                out.copy_(residual)
+            native.prepare_epilogue(a, b, out, precision=precision, activation="silu", preact=preact,
+                                    residual=out if given is None else given)()
+            assert_within(out, *expected["out"], "out")
+            assert_within(preact, *expected["preact"], "preact")
+            untouched(), ub()
