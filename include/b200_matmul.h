@@ -205,9 +205,10 @@ int matmul_epilogue_backward(void *context, int precision, const void *dout, con
 
 /* Products grouped by expert: out[i] = a[i] b[g] for the rows offsets[g] <= i <
  * offsets[g + 1] of a (rows x k), b groups x k x n, out rows x n.  offsets:
- * groups + 1 values on the device (int64 when offsets64, else int32), read when
- * the kernel runs; values outside [0, rows] are clipped and one below an earlier
- * one counts as equal to it.  Rows of no group are not written. */
+ * groups + 1 values on the device (int64 when offsets64, else int32; groups at
+ * most 2^28), read when the kernel runs; values outside [0, rows] are clipped and
+ * one below an earlier one counts as equal to it.  Rows of no group are not
+ * written. */
 int matmul_grouped(void *context, int precision, const void *a, const void *b, const void *offsets, int offsets64,
                    int groups, void *out, int out_fp32, int rows, int k, int n, void *stream, char *error,
                    size_t error_size);

@@ -17,6 +17,12 @@ using namespace b200;
 
 constexpr int kTf32 = 1, kFp16 = 2, kBf16 = 3;     // precision ids of the ABI
 constexpr int kMaxSize = 0x7fffffff - 1023;        // a tile past the end still has int coordinates
+// The plan kernel adds up row tiles (rows / 16 + groups at most) or K blocks and epilogues (rows / 32 +
+// (1 + GP_EPILOGUE_BLOCKS) groups at most) of all groups as ints.
+constexpr int kMaxGroups = 1 << 28;
+static_assert(kMaxSize / 32 + int64_t{kMaxGroups} * (1 + GP_EPILOGUE_BLOCKS) <= 0x7fffffff &&
+                  kMaxSize / 16 + int64_t{kMaxGroups} <= 0x7fffffff,
+              "a plan's sums fit an int");
 
 // Makes a device current for a call and puts the caller's back.
 struct DeviceScope {
@@ -865,6 +871,8 @@ int check_groups(Call &c, int groups, int rows, int k, int n, const void *offset
 {
     if (check_sizes(c, {rows, k, n, groups}))
         return 1;
+    if (groups > kMaxGroups)
+        return c.failed("groups must be at most 268435456");
     if (!offsets)
         return c.failed("offsets pointer is null");
     if (misaligned(offsets, offsets64 ? 8 : 4))

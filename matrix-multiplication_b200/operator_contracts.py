@@ -12,6 +12,7 @@ ACTIVATIONS = ("none", "relu", "gelu", "gelu_tanh", "silu")
 ACTIVATION_IDS = {name: index for index, name in enumerate(ACTIVATIONS)}
 OPERATOR_PRECISIONS = ("tf32", "fp16", "bf16")
 SIZE_MAX = 2**31 - 1024     # a tile past the end still has coordinates of 32 bits
+GROUPS_MAX = 2**28          # sums over all groups' tiles have 32 bits
 
 
 def _input_dtype(precision: str):
@@ -142,6 +143,8 @@ def validate_epilogue_backward(dout, a, b, precision: str, device: int, activati
 def _check_offsets(offsets, groups: int, device: int) -> None:
     import torch
 
+    if groups > GROUPS_MAX:
+        raise ValueError(f"groups must be at most {GROUPS_MAX}")
     _check("offsets", offsets, (torch.int32, torch.int64), 1, device)
     _shape("offsets", offsets, (groups + 1,))
 
