@@ -173,8 +173,8 @@ __global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_con
 // ---------------------------------------------------------------- loss
 constexpr int LJ_WARPS = 32;
 
-// lse = log sum exp over the column ranges' (maximum, sum) pairs in base 2, loss = lse -
-// the label's logit.  A block takes 32 rows, each warp every 32nd range: the maximum
+// lse = log sum exp over the column ranges' (maximum, sum) pairs, loss = lse - the label's
+// logit.  A block takes 32 rows, each warp every 32nd range: the maximum
 // first, then the sums scaled to it (loads and exponentials without a chain through
 // them), joined over the warps in a fixed order.  A range's sum is NaN where a logit was.
 __global__ void __launch_bounds__(32 * LJ_WARPS) loss_join_kernel(const float2 *partial, int ranges,
@@ -196,12 +196,13 @@ __global__ void __launch_bounds__(32 * LJ_WARPS) loss_join_kernel(const float2 *
 #pragma unroll
     for (int i = 0; i < LJ_WARPS; ++i)
         top = fmaxf(top, tops[i][lane]);
-    const float origin = top == -INFINITY ? 0.0f : top;
+    const bool far = op_far(top);
+    const float origin = far ? op_far_origin(top) : op_origin(top);
     float sum = 0.0f;
 #pragma unroll 4
     for (int i = warp; i < ranges; i += LJ_WARPS) {
         const float2 v = column[static_cast<long long>(i) * p.m];
-        sum += v.y * exp2f(v.x - origin);
+        sum += v.y * exp2f(far ? (v.x - origin) * kLog2E : __fmul_rn(v.x, kLog2E) - origin);
     }
     sums[warp][lane] = sum;
     __syncthreads();
@@ -210,10 +211,16 @@ __global__ void __launch_bounds__(32 * LJ_WARPS) loss_join_kernel(const float2 *
 #pragma unroll
         for (int i = 0; i < LJ_WARPS; ++i)
             sum += sums[i][lane];
-        const float total = (origin + log2f(sum)) * 0.69314718055994531f;
+        // Far from zero the logarithm of the sum is below half a step of the maximum: the loss takes
+        // the maximum's distance from the label's logit first.
+        constexpr float kLn2 = 0.69314718055994531f;
+        const float rest = log2f(sum), total = far ? top + rest * kLn2 : (origin + rest) * kLn2;
         const int label = op_label(p, row);
         lse[row] = total;
-        loss[row] = label == -1 ? 0.0f : label == -2 ? __int_as_float(0x7fc00000) : total - label_logit[row];
+        if (label < 0)
+            loss[row] = label == -1 ? 0.0f : __int_as_float(0x7fc00000);
+        else
+            loss[row] = far ? (top - label_logit[row]) + rest * kLn2 : total - label_logit[row];
     }
 }
 

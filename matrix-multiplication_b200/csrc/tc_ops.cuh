@@ -162,7 +162,7 @@ struct OpParams {
     int column0;                      // vocabulary index of column 0
     long long ignore;
     long long classes;                // vocabulary size: labels outside [0, classes) that are not `ignore` give NaN
-    float2 *partial;                  // [n tiles x epilogue groups][m]: maximum (of logit * log2 e) and sum
+    float2 *partial;                  // [n tiles x epilogue groups][m]: maximum logit, sum of exponentials from it
     float *label_logit;               // [m]
     const float *lse, *grad;          // [m]
     unsigned int *status;
@@ -403,6 +403,28 @@ __device__ __forceinline__ int op_label(const OpParams &p, int row)
     if (y == p.ignore)
         return -1;
     return y >= 0 && y < p.classes ? static_cast<int>(y) : -2;
+}
+
+// Exponentials of logits are taken in base 2, exp(z - top) = 2^(z log2 e - origin) with origin = top log2 e: one
+// FMA a logit, and the origin's rounding is in every term and in the result alike.  From 2^126 on a maximum is
+// far: its origin may be infinite, so the maximum is taken off first, exp(z - top) = 2^((z - top) log2 e).
+// Such logits are those of columns masked with the format's lowest value (or -infinity, from which nothing is
+// taken off).  An origin below -2^127 is held there, where its terms are zero.
+constexpr float kLog2E = 1.44269504f;
+
+__device__ __forceinline__ bool op_far(float top)
+{
+    return fabsf(top) > 0x1p126f;
+}
+
+__device__ __forceinline__ float op_origin(float top)
+{
+    return fmaxf(__fmul_rn(top, kLog2E), -0x1p127f);
+}
+
+__device__ __forceinline__ float op_far_origin(float top)
+{
+    return top == -INFINITY ? 0.0f : top;
 }
 
 // Where a tile of D lies: M-side and N-side origin, group, K blocks and K origin, and
@@ -1545,12 +1567,33 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             } else {
                 // One pass: running maximum and sum of exponentials, in base 2, of this row's
                 // columns in the tile; columns past the vocabulary count as -infinity.
-                float top = -INFINITY, origin = -INFINITY, sum = 0.0f;
+                float top = -INFINITY, origin = -0x1p127f, sum = 0.0f;
+                bool held = true;
                 const int row = row0 + r;
-                auto reduce = [&](const uint32_t (&u)[32], int chunk) {
+                const int chunks = min(kGroupCols / 32, (p.n - w.n0 - gcol + 31) / 32);   // below 1: none in the matrix
+                // The same in two passes from the row's maximum in the tile, for far maxima.
+                auto reduce_far = [&]() {
+                    const bool far = op_far(top);
+                    const float from = far ? op_far_origin(top) : op_origin(top);
+                    sum = 0.0f;
+#pragma unroll 1
+                    for (int c = 0; c < 2 * chunks; ++c) {
+                        uint32_t u[16];
+                        tmem_load_16cols(t_row + c * 16, u);
+                        const int cols = p.n - w.n0 - gcol - c * 16;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float x = __uint_as_float(u[j]);
+                            const float t = far ? (x - from) * kLog2E : __fmaf_rn(x, kLog2E, -from);
+                            sum += j < cols ? op_exp2(t) : 0.0f;
+                        }
+                    }
+                };
+#pragma unroll 1
+                for (int chunk = 0; chunk < chunks; ++chunk) {
+                    uint32_t u[32];
+                    tmem_load_32cols(t_row + chunk * 32, u);
                     const int col0 = w.n0 + gcol + chunk * 32;
-                    if (col0 >= p.n)
-                        return;
                     const int hit = label - col0;
                     if (label >= 0 && hit >= 0 && hit < 32) {
                         float z = 0.0f;
@@ -1571,13 +1614,20 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
                         chunk_top = fmaxf(chunk_top, x[j]);
-                    const float next = fmaxf(top, chunk_top);
+                    top = fmaxf(top, chunk_top);
+                    if (chunk == chunks - 1) {
+                        if (__any_sync(0xffffffffu, op_far(top))) {
+                            reduce_far();
+                            break;
+                        }
+                        release();
+                        held = false;
+                    }
                     // A row whose logits are all -infinity so far adds nothing; NaN is carried by the sum.
-                    // The origin is rounded once and used for every term and in the result.
-                    const float next_origin = next == -INFINITY ? 0.0f : next * 1.44269504f;
-                    sum *= top == -INFINITY ? 0.0f : op_exp2(origin - next_origin);
+                    const float next_origin = op_origin(top);
+                    sum *= op_exp2(origin - next_origin);
                     origin = next_origin;
-                    const float2 scale = make_float2(1.44269504f, 1.44269504f), minus = make_float2(-origin, -origin);
+                    const float2 scale = make_float2(kLog2E, kLog2E), minus = make_float2(-origin, -origin);
                     float2 chain[2] = {};
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
@@ -1585,18 +1635,11 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         chain[(j >> 1) & 1] = __fadd2_rn(chain[(j >> 1) & 1], make_float2(op_exp2(t.x), op_exp2(t.y)));
                     }
                     sum += (chain[0].x + chain[0].y) + (chain[1].x + chain[1].y);
-                    top = next;
-                };
-#pragma unroll 1
-                for (int chunk = 0; chunk < kGroupCols / 32; ++chunk) {
-                    uint32_t u[32];
-                    tmem_load_32cols(t_row + chunk * 32, u);
-                    if (chunk == kGroupCols / 32 - 1)
-                        release();
-                    reduce(u, chunk);
                 }
+                if (held)
+                    release();
                 if (row < p.m)
-                    p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row] = make_float2(top == -INFINITY ? top : origin, sum);
+                    p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row] = make_float2(top, sum);
             }
             if (++acc == 2) {
                 acc = 0;

@@ -1,0 +1,99 @@
+"""Edges of the operators next to the matrix product (needs a B200): logits at the ends of FP32's range."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import operator_reference as ref
+from operator_reference import DTYPES, assert_within
+from test_operators_gpu import guarded, loss_inputs, randn
+
+pytestmark = pytest.mark.gpu
+
+FP32 = torch.float32
+LOWEST = float(torch.finfo(torch.bfloat16).min)     # also a TF32 value
+
+
+# ---------------------------------------------------------------- logits at the ends of FP32's range
+# Rows on every tile kind, a vocabulary that TMA addresses and one that it does not (read in place for few
+# rows, copied for more).
+@pytest.mark.parametrize("precision", ("bf16", "tf32"))
+@pytest.mark.parametrize("shape", [(3, 40, 2000), (64, 64, 20001), (200, 33, 1001), (300, 64, 50048), (1100, 24, 33024)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("masked", ("first", "last", "middle", "all but one"))
+def test_loss_of_columns_masked_with_the_lowest_value(native, precision, shape, masked):
+    """A weight row of 0 and the lowest value masks columns for the rows of `hidden` that have a 1 there.
+
+    Masked columns add nothing to a sum: lse is that of the other columns, to the allowance of a product of the other
+    k terms (a masked column's own sum may be off by any amount below its size).
+    """
+    m, k, v = shape
+    hidden, weight, labels, grad = loss_inputs(m, k, v, precision)
+    mask = torch.zeros(v, dtype=torch.bool, device="cuda")
+    if masked == "first":
+        mask[:v // 3] = True
+    elif masked == "last":
+        mask[-(v // 3):] = True
+    elif masked == "middle":
+        mask[70:v - 90] = True
+    else:
+        mask[:] = True
+        mask[v // 2] = False
+    kept = (~mask).nonzero()[:, 0]
+    labels = torch.where(labels == -100, labels, kept[labels % len(kept)])
+    hidden[:, 0], weight[0] = 1.0, torch.where(mask, LOWEST, 0.0)
+    place = torch.zeros(v, dtype=torch.int64, device="cuda")
+    place[kept] = torch.arange(len(kept), device="cuda")
+    seen = torch.where(labels == -100, labels, place[labels.clamp(min=0)])
+    expected = ref.cross_entropy(hidden[:, 1:], weight[1:, kept], seen, precision)
+    # Chains and roundings are those of all v columns and k terms.
+    slack = (v / 128.0) * ref.U + 2 * ref.U * (hidden[:, 1:].double().abs() @ weight[1:, kept].double().abs()).amax(1)
+    (loss, ul), (lse, us) = guarded((m,), FP32), guarded((m,), FP32)
+    native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision=precision)()
+    assert_within(lse, expected["lse"][0], expected["lse"][1] + slack, "lse")
+    assert_within(loss, expected["loss"][0], expected["loss"][1] + 2 * slack, "loss")
+    ul(), us()
+    # The gradients of masked columns are exactly zero.
+    dhidden, dweight = torch.full((m, k), 7.0, device="cuda"), torch.full((k, v), 7.0, device="cuda")
+    native.prepare_cross_entropy_backward(grad, hidden, weight, labels, lse, precision=precision, dhidden=dhidden,
+                                          dweight=dweight)()
+    assert not dweight[:, mask].any() and not dhidden[:, 0].any()
+    assert torch.isfinite(dweight).all() and torch.isfinite(dhidden).all()
+
+
+@pytest.mark.parametrize("precision", ("bf16", "tf32"))
+@pytest.mark.parametrize("m,v", [(5, 3000), (64, 20001), (300, 50048), (1100, 33024)])
+def test_loss_of_rows_without_a_column_left(native, precision, m, v):
+    """Every column of some rows masked: all logits are the lowest value, so lse is it (half a step of it is far above
+    log v) and the loss log v; of one row alone in the tile as of all.  Its logarithm and the sum of v ones, in chains
+    of at most 256 + v / 256 terms, are off by (600 + v / 128) 2^-23 at most."""
+    dtype = DTYPES[precision]
+    hidden, weight = torch.zeros((m, 16), dtype=dtype, device="cuda"), torch.zeros((16, v), dtype=dtype, device="cuda")
+    weight[0] = LOWEST
+    hidden[1::3, 0] = 1.0
+    weight[1], hidden[2::3, 1] = -LOWEST, 1.0      # and rows at the highest value
+    labels = torch.arange(m, device="cuda") % v
+    loss, lse = torch.empty(m, device="cuda"), torch.empty(m, device="cuda")
+    native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision=precision)()
+    log_v = torch.full((m,), float(v), dtype=torch.float64, device="cuda").log()
+    tol = torch.full_like(log_v, (600.0 + v / 128.0) * ref.U) + 4 * ref.U * log_v
+    assert_within(loss, log_v, tol, "loss")
+    expected = log_v.clone()
+    expected[1::3], expected[2::3] = LOWEST, -LOWEST
+    assert_within(lse, expected, tol, "lse")
+
+
+def test_loss_between_the_ends_of_the_range(native):
+    """One logit of the highest value among the lowest: lse is it, the other labels' losses pass FP32's range."""
+    m, v = 9, 4096
+    for where in (0, 31, 32, 2049, v - 1):
+        hidden, weight = torch.ones((m, 8), dtype=torch.bfloat16, device="cuda"), torch.zeros((8, v), dtype=torch.bfloat16, device="cuda")
+        weight[0] = LOWEST
+        weight[0, where] = -LOWEST
+        labels = torch.full((m,), where, device="cuda")
+        labels[3] = (where + 1) % v
+        loss, lse = torch.empty(m, device="cuda"), torch.empty(m, device="cuda")
+        native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision="bf16")()
+        assert bool((lse == -LOWEST).all())
+        assert float(loss[3]) == float("inf") and float(loss.nan_to_num(posinf=0.0).abs().sum()) == 0.0
