@@ -6,6 +6,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <mutex>
@@ -47,6 +48,10 @@ struct Context {
     // (matmul_set_wait_limit); 0 = the default.
     unsigned long long wait_limit_ns = 0;
     unsigned int *status = nullptr;   // device address of the status word (matmul_device_status)
+    // Whether the operators' kernels of a format have their attributes in this context's device
+    // (setup_operators).
+    std::mutex operators_mutex;
+    std::atomic<bool> operators_ready[3] = {};
 };
 
 inline unsigned long long wait_limit(const Context *ctx)

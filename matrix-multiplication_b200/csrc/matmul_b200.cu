@@ -858,18 +858,15 @@ extern "C" void *matmul_create(int device, char *error, size_t error_size)
         }
         ctx->max_split_ctas[i] = clusters * static_cast<int>(size);
     }
-    // The operators' kernels (ops.cu), and the status word they share with this file's.
-    st = setup_operators();
-    if (st == cudaSuccess) {
-        void *status = nullptr;
-        st = cudaGetSymbolAddress(&status, g_device_status);
-        ctx->status = static_cast<unsigned int *>(status);
-    }
+    // The status word, for the operators' kernels (ops.cu).
+    void *status = nullptr;
+    st = cudaGetSymbolAddress(&status, g_device_status);
     if (st != cudaSuccess) {
         delete ctx;
-        fail_cuda(error, error_size, "matmul_create: operators", st);
+        fail_cuda(error, error_size, "matmul_create: status word", st);
         return nullptr;
     }
+    ctx->status = static_cast<unsigned int *>(status);
     ctx->device_sm_count = ctx->sm_count;
     ctx->device_max_pairs = ctx->max_pairs;
     for (int i = 0; i < 4; ++i)

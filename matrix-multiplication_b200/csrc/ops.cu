@@ -606,22 +606,31 @@ bool aligned_to(std::initializer_list<std::pair<const void *, int>> pointers)
     return true;
 }
 
-} // namespace
-
-namespace b200 {
-
-// Called by matmul_create with the device current.
-cudaError_t setup_operators()
+// Sets the attributes of a format's kernels by its first call, with the device current: it loads
+// them, about half a millisecond each, which programs that call no operator need not pay for
+// (matmul_create with all of them: 32 ms, 5 ms without).
+cudaError_t setup_operators(Call &c)
 {
-    for (const OpKernels *k : {&kOpKernelsF16, &kOpKernelsBF16, &kOpKernelsTF32}) {
-        const cudaError_t st = k->setup();
-        if (st != cudaSuccess)
-            return st;
-    }
-    return cudaSuccess;
+    std::atomic<bool> &ready = c.ctx->operators_ready[c.precision - kTf32];
+    if (ready.load(std::memory_order_acquire))
+        return cudaSuccess;
+    std::lock_guard<std::mutex> lock(c.ctx->operators_mutex);
+    const cudaError_t st = c.kernels().setup();
+    if (st == cudaSuccess)
+        ready.store(true, std::memory_order_release);
+    return st;
 }
 
-} // namespace b200
+// Makes the call's device current, and its kernels ready.
+struct CallScope : DeviceScope {
+    explicit CallScope(Call &c) : DeviceScope(c.ctx->device)
+    {
+        if (status == cudaSuccess)
+            status = setup_operators(c);
+    }
+};
+
+} // namespace
 
 extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const void *b, const void *bias,
                                int bias_fp32, int activation, const void *residual, void *out, int out_fp32,
@@ -643,7 +652,7 @@ extern "C" int matmul_epilogue(void *opaque, int precision, const void *a, const
     if (!aligned_to({{a, e}, {b, e}, {out, out_half ? 2 : 4}, {residual, out_half ? 2 : 4},
                      {preact, preact_half ? 2 : 4}, {bias, bias_half ? 2 : 4}}))
         return c.failed("a pointer is not aligned to its element size");
-    DeviceScope device(c.ctx->device);
+    CallScope device(c);
     if (device.status != cudaSuccess)
         return c.failed(device.status);
     Product q;
@@ -741,7 +750,7 @@ extern "C" int matmul_epilogue_backward(void *opaque, int precision, const void 
     if (!aligned_to({{dout, e}, {a, e}, {b, e}, {preact, preact_half ? 2 : 4}, {da, da_half ? 2 : 4},
                      {db, db_half ? 2 : 4}, {dbias, dbias_half ? 2 : 4}}))
         return c.failed("a pointer is not aligned to its element size");
-    DeviceScope device(c.ctx->device);
+    CallScope device(c);
     if (device.status != cudaSuccess)
         return c.failed(device.status);
 
@@ -918,7 +927,7 @@ extern "C" int matmul_grouped(void *opaque, int precision, const void *a, const 
     const bool half = e == 2 && !out_fp32;
     if (!aligned_to({{a, e}, {b, e}, {out, half ? 2 : 4}}))
         return c.failed("a pointer is not aligned to its element size");
-    DeviceScope device(c.ctx->device);
+    CallScope device(c);
     if (device.status != cudaSuccess)
         return c.failed(device.status);
     const int64_t bk = OP_ROW_BYTES / e;
@@ -966,7 +975,7 @@ extern "C" int matmul_grouped_backward(void *opaque, int precision, const void *
     const bool da_half = e == 2 && !da_fp32, db_half = e == 2 && !db_fp32;
     if (!aligned_to({{dout, e}, {a, e}, {b, e}, {da, da_half ? 2 : 4}, {db, db_half ? 2 : 4}}))
         return c.failed("a pointer is not aligned to its element size");
-    DeviceScope device(c.ctx->device);
+    CallScope device(c);
     if (device.status != cudaSuccess)
         return c.failed(device.status);
     const int64_t bk = OP_ROW_BYTES / e;
@@ -1065,7 +1074,7 @@ extern "C" int matmul_cross_entropy(void *opaque, int precision, const void *hid
     const int e = c.elem();
     if (!aligned_to({{hidden, e}, {weight, e}, {loss, 4}, {lse, 4}}))
         return c.failed("a pointer is not aligned to its element size");
-    DeviceScope device(c.ctx->device);
+    CallScope device(c);
     if (device.status != cudaSuccess)
         return c.failed(device.status);
     const int64_t bk = OP_ROW_BYTES / e;
@@ -1134,7 +1143,7 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
     const bool dh_half = e == 2 && !dhidden_fp32, dw_half = e == 2 && !dweight_fp32;
     if (!aligned_to({{hidden, e}, {weight, e}, {grad, 4}, {lse, 4}, {dhidden, dh_half ? 2 : 4}, {dweight, dw_half ? 2 : 4}}))
         return c.failed("a pointer is not aligned to its element size");
-    DeviceScope device(c.ctx->device);
+    CallScope device(c);
     if (device.status != cudaSuccess)
         return c.failed(device.status);
     const int64_t bk = OP_ROW_BYTES / e;

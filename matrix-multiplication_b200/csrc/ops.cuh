@@ -26,16 +26,13 @@ struct OpLaunch {
 };
 
 struct OpKernels {
-    cudaError_t (*setup)();     // kernel attributes; once per device
+    cudaError_t (*setup)();     // kernel attributes; once per context
     cudaError_t (*product)(const OpLaunch &launch, cudaStream_t stream);
     cudaError_t (*act_grad)(const ActGradParams &params, dim3 grid, int cluster, cudaStream_t stream);
     cudaError_t (*bias_grad)(const float *partial, int count, int n, void *dbias, int dbias_half, cudaStream_t stream);
     cudaError_t (*repack)(const RepackJob &job0, const RepackJob &job1, int sms, cudaStream_t stream);
     cudaError_t (*chunk_sum)(const ChunkSumParams &params, int sms, cudaStream_t stream);
 };
-
-// Sets every operator kernel's attributes on the current device (matmul_create).
-cudaError_t setup_operators();
 
 extern const OpKernels kOpKernelsF16, kOpKernelsBF16, kOpKernelsTF32;
 

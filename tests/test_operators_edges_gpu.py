@@ -1,6 +1,11 @@
-"""Edges of the operators next to the matrix product (needs a B200): logits at the ends of FP32's range."""
+"""Edges of the operators next to the matrix product (needs a B200): logits at the ends of FP32's range, and first
+calls."""
 
 from __future__ import annotations
+
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -11,7 +16,7 @@ from test_operators_gpu import guarded, loss_inputs, randn
 
 pytestmark = pytest.mark.gpu
 
-FP32 = torch.float32
+BF16, FP32 = torch.bfloat16, torch.float32
 LOWEST = float(torch.finfo(torch.bfloat16).min)     # also a TF32 value
 
 
@@ -97,3 +102,74 @@ def test_loss_between_the_ends_of_the_range(native):
         native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision="bf16")()
         assert bool((lse == -LOWEST).all())
         assert float(loss[3]) == float("inf") and float(loss.nan_to_num(posinf=0.0).abs().sum()) == 0.0
+
+
+# ---------------------------------------------------------------- first calls
+FIRST_CALLS = """
+import sys, threading
+sys.path[:0] = [{package!r}, {tests!r}]
+import torch
+import operator_reference as ref
+from gpumat import NativeMatmul
+
+torch.manual_seed(1)
+def randn(*shape, dtype=torch.bfloat16):
+    return torch.randn(shape, device="cuda").to(dtype)
+
+native = NativeMatmul()
+stream = torch.cuda.Stream()
+def case(dtype):
+    name = {{torch.bfloat16: "bf16", torch.float16: "fp16", torch.float32: "tf32"}}[dtype]
+    a, b, d, z = (randn(*s, dtype=dtype) for s in ((150, 130), (130, 264), (150, 264), (150, 264)))
+    out, da, db = torch.zeros_like(d), torch.zeros_like(a), torch.zeros_like(b)
+    runs = (native.prepare_epilogue(a, b, out, precision=name, activation="silu"),
+            native.prepare_epilogue_backward(d, a, b, precision=name, activation="silu", preact=z, da=da, db=db))
+    def check():
+        back = ref.epilogue_backward(d, a, b, name, z, "silu")
+        for got, key in ((da, "da"), (db, "db")):
+            ref.assert_within(got, *back[key], f"{{name}} {{key}}")
+        ref.assert_within(out, *ref.epilogue(a, b, name, None, "silu")["out"], name)
+    return runs, check
+
+# The first operator call of the process, in a capture.
+with torch.cuda.stream(stream):
+    runs, check = case(torch.bfloat16)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=stream):
+    for run in runs:
+        run()
+graph.replay()
+torch.cuda.synchronize()
+check()
+# The first calls in a format, from four threads at once.
+checks, errors, gate = [], [], threading.Barrier(4)
+def work(dtype):
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            runs, check = case(dtype)
+            torch.cuda.current_stream().synchronize()
+            gate.wait()
+            for run in runs:
+                run()
+            torch.cuda.current_stream().synchronize()
+        checks.append(check)
+    except BaseException as error:
+        errors.append(error)
+        gate.abort()
+threads = [threading.Thread(target=work, args=(d,)) for d in (torch.float16, torch.float16, torch.float32, torch.float32)]
+for t in threads: t.start()
+for t in threads: t.join()
+assert not errors and len(checks) == 4, errors
+for check in checks: check()
+assert native.device_status() == 0
+print("first calls hold")
+"""
+
+
+def test_first_calls_of_a_process(gpu_ready, library_path):
+    """Kernels get their attributes by a format's first call: in a graph capture, and by four threads at once."""
+    root = Path(__file__).resolve().parents[1]
+    script = FIRST_CALLS.format(package=str(root / "matrix-multiplication_b200"), tests=str(root / "tests"))
+    result = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300)
+    assert result.returncode == 0 and "first calls hold" in result.stdout, result.stdout + result.stderr
