@@ -1,8 +1,9 @@
-"""Edges of the operators next to the matrix product (needs a B200): logits at the ends of FP32's range, and first
-calls."""
+"""Edges of the operators next to the matrix product (needs a B200): logits at the ends of FP32's range, gelu's tails, and
+first calls."""
 
 from __future__ import annotations
 
+import math
 import subprocess
 import sys
 from pathlib import Path
@@ -102,6 +103,37 @@ def test_loss_between_the_ends_of_the_range(native):
         native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision="bf16")()
         assert bool((lse == -LOWEST).all())
         assert float(loss[3]) == float("inf") and float(loss.nan_to_num(posinf=0.0).abs().sum()) == 0.0
+
+
+# ---------------------------------------------------------------- gelu's tails
+@pytest.mark.parametrize("m", (1, 70, 300))
+def test_gelu_keeps_its_relative_precision_in_the_tails(native, m):
+    """gelu(z) = z Phi(z) and its slope Phi(z) + z phi(z) in FP32, at every z in [-12, 12].
+
+    With u = 2^-23 the kernel's Phi(-|z|) is off by at most (12 + z^2 / 2) u of itself: 1.3 u the fit, 0.9 u the
+    coefficients' roundings, 3.5 u those of Horner's seven steps, 2 u those of t (reciprocal 1 ulp), 2 u the hardware's
+    exponential, 1.5 u the products, and z^2 / 2 u the two roundings of the exponent z^2 / 2 log2 e.  phi(z) is within
+    those bounds too.  1 - Phi and each last operation add half a step of their result.
+    """
+    n = 4096
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    z = torch.empty(n, device="cuda").uniform_(-12.0, 12.0, generator=gen)
+    z[:3] = torch.tensor([0.0, -3.0, -5.0])
+    zd = z.double()
+    tail = 0.5 * torch.special.erfc(zd.abs() / math.sqrt(2.0))
+    cdf = 0.5 * torch.special.erfc(-zd / math.sqrt(2.0))
+    peak = torch.exp(-zd * zd / 2.0) / math.sqrt(2.0 * math.pi)
+    bound = (12.0 + zd * zd / 2.0) * ref.U
+    for precision in ("bf16", "tf32"):
+        dtype = DTYPES[precision]
+        a, b = torch.zeros((m, 8), dtype=dtype, device="cuda"), torch.zeros((8, n), dtype=dtype, device="cuda")
+        out = torch.empty((m, n), device="cuda")
+        native.prepare_epilogue(a, b, out, precision=precision, bias=z, activation="gelu")()
+        assert_within(out, (zd * cdf).expand(m, n), (zd.abs() * (bound * tail + ref.U * cdf)).expand(m, n), "gelu")
+        dbias = torch.empty(n, device="cuda")
+        native.prepare_epilogue_backward(torch.ones((1, n), dtype=dtype, device="cuda"), precision=precision,
+                                         activation="gelu", preact=z.view(1, n), dbias=dbias)()
+        assert_within(dbias, cdf + zd * peak, bound * (tail + zd.abs() * peak) + ref.U * cdf, "slope")
 
 
 # ---------------------------------------------------------------- first calls
