@@ -356,13 +356,16 @@ __device__ __forceinline__ float2 op_activation_slope(float2 z)
         return __ffma2_rn(__fmul2_rn(z, make_float2(0.39894228f, 0.39894228f)), e, cdf);
     }
     if constexpr (ACT == kActGeluTanh) {
-        const float2 zz = __fmul2_rn(z, z);
+        // Beyond 64 the slope is 0 or 1 to all its bits: |z| is held there, since z^2 could be infinite. NaN
+        // comes through x.
+        const float2 a = make_float2(fminf(fabsf(z.x), 64.0f), fminf(fabsf(z.y), 64.0f));
+        const float2 zz = __fmul2_rn(a, a);
         const float2 x = __fmul2_rn(z, __ffma2_rn(zz, make_float2(-0.10294324f, -0.10294324f),
                                                   make_float2(-2.3022082f, -2.3022082f)));
         const float2 s = make_float2(op_reciprocal(1.0f + op_exp2(x.x)), op_reciprocal(1.0f + op_exp2(x.y)));
         const float2 du = __ffma2_rn(zz, make_float2(0.21406446f, 0.21406446f), make_float2(1.59576912f, 1.59576912f));
         const float2 rest = __ffma2_rn(make_float2(-s.x, -s.y), s, s);         // s (1 - s)
-        return __ffma2_rn(__fmul2_rn(z, rest), du, s);
+        return __ffma2_rn(__fmul2_rn(make_float2(copysignf(a.x, z.x), copysignf(a.y, z.y)), rest), du, s);
     }
     if constexpr (ACT == kActSilu) {
         const float2 x = __fmul2_rn(z, make_float2(-1.44269504f, -1.44269504f));

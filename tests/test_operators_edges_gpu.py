@@ -1,4 +1,4 @@
-"""Edges of the operators next to the matrix product (needs a B200): logits at the ends of FP32's range, gelu's tails, and
+"""Edges of the operators next to the matrix product (needs a B200): logits at the ends of FP32's range, the activations' ends, and
 first calls."""
 
 from __future__ import annotations
@@ -105,7 +105,7 @@ def test_loss_between_the_ends_of_the_range(native):
         assert float(loss[3]) == float("inf") and float(loss.nan_to_num(posinf=0.0).abs().sum()) == 0.0
 
 
-# ---------------------------------------------------------------- gelu's tails
+# ---------------------------------------------------------------- the activations' ends
 @pytest.mark.parametrize("m", (1, 70, 300))
 def test_gelu_keeps_its_relative_precision_in_the_tails(native, m):
     """gelu(z) = z Phi(z) and its slope Phi(z) + z phi(z) in FP32, at every z in [-12, 12].
@@ -134,6 +134,21 @@ def test_gelu_keeps_its_relative_precision_in_the_tails(native, m):
         native.prepare_epilogue_backward(torch.ones((1, n), dtype=dtype, device="cuda"), precision=precision,
                                          activation="gelu", preact=z.view(1, n), dbias=dbias)()
         assert_within(dbias, cdf + zd * peak, bound * (tail + zd.abs() * peak) + ref.U * cdf, "slope")
+
+
+@pytest.mark.parametrize("act", ("relu", "gelu", "gelu_tanh", "silu"))
+def test_slopes_of_large_values(native, act):
+    """Where an activation is z or 0 to all 24 bits its slope is 1 or 0 exactly, up to the largest finite z; NaN stays
+    NaN (relu has slope 0 there, as the comparison z > 0 says)."""
+    z = torch.tensor([1e2, 1e4, 6e4, 1e10, 1e19, 1.8e19, 1.9e19, 1e20, 1e30, 3.3e38], device="cuda")
+    z = torch.cat([z, -z, torch.tensor([float("nan"), 0.5], device="cuda")])
+    want = torch.cat([torch.ones(10), torch.zeros(10)]).cuda()
+    dbias = torch.empty(22, device="cuda")
+    for dtype, precision in ((BF16, "bf16"), (FP32, "tf32")):
+        native.prepare_epilogue_backward(torch.ones((1, 22), dtype=dtype, device="cuda"), precision=precision,
+                                         activation=act, preact=z.view(1, 22), dbias=dbias)()
+        assert torch.equal(dbias[:20], want), f"{act}: {dbias.tolist()}"
+        assert bool(torch.isnan(dbias[20])) == (act != "relu") and float(dbias[21]) > 0.5
 
 
 # ---------------------------------------------------------------- first calls
