@@ -1225,38 +1225,40 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     ++stores;
                 };
                 // The same with the residual already in the box: each thread adds its own row to `v`,
-                // puts the result in its place and the box is stored.
+                // puts the result in its place and the box is stored.  False where the residual did not come in
+                // time: the box is not stored, and its loads are left to the drain below.
                 auto emit_residual = [&](auto &v, const void *map, int col0) {
                     constexpr bool kShiftingBox = std::extent<std::remove_reference_t<decltype(v)>>::value == 64;
                     const uint32_t b = stores % kBoxes;
                     fetch(static_cast<int>(box_done) + 1);
-                    if (!mbar_wait(res_bar(b), (res_parity >> b) & 1u)) {
-                        atomicOr(p.status, kOpDrainTimeout);
-                        v[0] = __int_as_float(0x7fc00000);
+                    const bool here = mbar_wait(res_bar(b), (res_parity >> b) & 1u, p.wait_limit_ns);
+                    if (here) {
+                        const uint32_t row_addr = s_box + b * OP_BOX + r * 128;
+                        uint32_t words[32];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint4 q =
+                                *reinterpret_cast<const uint4 *>(smem_raw + (row_addr + ((j ^ (r & 7)) << 4) - raw));
+                            if constexpr (kShiftingBox) {
+                                const T *h = reinterpret_cast<const T *>(&q);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    words[4 * j + e] = Type::pack(v[8 * j + 2 * e] + Type::to(h[2 * e]),
+                                                                  v[8 * j + 2 * e + 1] + Type::to(h[2 * e + 1]));
+                            } else {
+                                words[4 * j] = __float_as_uint(v[4 * j] + __uint_as_float(q.x));
+                                words[4 * j + 1] = __float_as_uint(v[4 * j + 1] + __uint_as_float(q.y));
+                                words[4 * j + 2] = __float_as_uint(v[4 * j + 2] + __uint_as_float(q.z));
+                                words[4 * j + 3] = __float_as_uint(v[4 * j + 3] + __uint_as_float(q.w));
+                            }
+                        }
+                        fill(s_box + b * OP_BOX, words);
+                        fence_proxy_async_shared();
                     }
+                    if (!epilogue_all(here ? 1 : 0))
+                        return false;
                     res_parity ^= 1u << b;
                     ++res_used;
-                    const uint32_t row_addr = s_box + b * OP_BOX + r * 128;
-                    uint32_t words[32];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint4 q = *reinterpret_cast<const uint4 *>(smem_raw + (row_addr + ((j ^ (r & 7)) << 4) - raw));
-                        if constexpr (kShiftingBox) {
-                            const T *h = reinterpret_cast<const T *>(&q);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                words[4 * j + e] = Type::pack(v[8 * j + 2 * e] + Type::to(h[2 * e]),
-                                                              v[8 * j + 2 * e + 1] + Type::to(h[2 * e + 1]));
-                        } else {
-                            words[4 * j] = __float_as_uint(v[4 * j] + __uint_as_float(q.x));
-                            words[4 * j + 1] = __float_as_uint(v[4 * j + 1] + __uint_as_float(q.y));
-                            words[4 * j + 2] = __float_as_uint(v[4 * j + 2] + __uint_as_float(q.z));
-                            words[4 * j + 3] = __float_as_uint(v[4 * j + 3] + __uint_as_float(q.w));
-                        }
-                    }
-                    fill(s_box + b * OP_BOX, words);
-                    fence_proxy_async_shared();
-                    epilogue_sync();
                     __syncwarp();
                     if (issuer_warp && op_elect_one()) {
                         tma_store_3d(map, s_box + b * OP_BOX, col0, row0, 0);
@@ -1265,6 +1267,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     __syncwarp();
                     ++stores;
                     ++box_done;
+                    return true;
                 };
                 // 128 bytes of each row, 32 FP32 or 64 16-bit columns, at any element alignment, without TMA.  Each warp puts its own 32 rows into the boxes' memory at a pitch
                 // of 33 words, then eight lanes take a row: a lane moves one 16-byte chunk that is
@@ -1431,11 +1434,12 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         }
                     }
                 };
-                // 64 columns of this thread's row: epilogue arithmetic and stores.
+                // 64 columns of this thread's row: epilogue arithmetic and stores.  False, for the whole
+                // warpgroup, where a residual did not come in time.
                 auto process = [&](float (&v)[64], int step) {
                     const int col0 = w.n0 + gcol + step * 64;
                     if (col0 >= p.n || row0 >= w.row_end)      // the same for all four warps
-                        return;
+                        return true;
                     if constexpr (EPI == kEpiSoftmaxGrad) {
                         // dz = (exp(z - lse) - [column == label]) grad.  The exponential is taken 2^24 times too
                         // large and grad as much too small, so that only their product, not the
@@ -1484,13 +1488,12 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         if (p.residual_tma) {
                             if (p.out_half) {
                                 if constexpr (!kTF32)
-                                    emit_residual(v, mc, col0);
+                                    return emit_residual(v, mc, col0);
                             } else {
-                                emit_residual(reinterpret_cast<float(&)[32]>(v[0]), mc, col0);
-                                if (col0 + 32 < p.n)
-                                    emit_residual(reinterpret_cast<float(&)[32]>(v[32]), mc, col0 + 32);
+                                return emit_residual(reinterpret_cast<float(&)[32]>(v[0]), mc, col0) &&
+                                       (col0 + 32 >= p.n ||
+                                        emit_residual(reinterpret_cast<float(&)[32]>(v[32]), mc, col0 + 32));
                             }
-                            return;
                         }
                         // Where TMA writes out but does not bring the residual (a pre-activation takes its
                         // boxes, or it has another format), each thread reads its own row of it.
@@ -1532,6 +1535,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         }
                     }
                     emit_columns(v, mc, zc, p.out_tma != 0, p.out_half != 0, p.out, zc * p.out_slab, p.out_pitch, col0);
+                    return true;
                 };
                 auto load = [&](float (&v)[64], int step) {
                     if (w.nkb > 0) {
@@ -1542,13 +1546,20 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                             v[j] = 0.0f;
                     }
                 };
+                bool stored = true;
 #pragma unroll 1
-                for (int step = 0; step < group_cols / 64; ++step) {
+                for (int step = 0; stored && step < group_cols / 64; ++step) {
                     float v[64];
                     load(v, step);
                     if (step == group_cols / 64 - 1)
                         release();
-                    process(v, step);
+                    stored = process(v, step);
+                }
+                if (!stored) {
+                    if (issuer)
+                        atomicOr(p.status, kOpEpilogueTimeout);
+                    failed_tile = tile;
+                    break;
                 }
             } else if constexpr (EPI == kEpiStoreT) {
                 // D's rows are output columns: one lane per column, one store of 32 consecutive
@@ -1653,10 +1664,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 acc_phase ^= 1u;
             }
         }
-        // A residual box that was fetched and not used (an accumulator that never came) lands
-        // before the CTA can exit.
-        if (res_issued != res_used) {
-            const uint32_t b = stores % kBoxes;
+        // Residual boxes that were fetched and not used (an accumulator or a residual that did not
+        // come in time) land before the CTA can exit.
+        for (; res_used != res_issued; ++res_used) {
+            const uint32_t b = (stores + res_issued - res_used - 1) % kBoxes;
             if (!mbar_wait(res_bar(b), (res_parity >> b) & 1u))
                 atomicOr(p.status, kOpDrainTimeout);
         }

@@ -1,5 +1,5 @@
-"""Edges of the operators next to the matrix product (needs a B200): logits at the ends of FP32's range, the activations' ends, and
-first calls."""
+"""Edges of the operators next to the matrix product (needs a B200): logits at the ends of FP32's range, the
+activations' ends, first calls, and waits that run out."""
 
 from __future__ import annotations
 
@@ -13,11 +13,13 @@ import torch
 
 import operator_reference as ref
 from operator_reference import DTYPES, assert_within
-from test_operators_gpu import guarded, loss_inputs, randn
+from test_operators_gpu import guarded, loss_inputs, randn, sizes_to_offsets
+from test_operators_use_gpu import odd_weight
 
 pytestmark = pytest.mark.gpu
 
 BF16, FP32 = torch.bfloat16, torch.float32
+LOAD, MMA, EPILOGUE, DRAIN = 1, 2, 4, 8
 LOWEST = float(torch.finfo(torch.bfloat16).min)     # also a TF32 value
 
 
@@ -220,3 +222,94 @@ def test_first_calls_of_a_process(gpu_ready, library_path):
     script = FIRST_CALLS.format(package=str(root / "matrix-multiplication_b200"), tests=str(root / "tests"))
     result = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300)
     assert result.returncode == 0 and "first calls hold" in result.stdout, result.stdout + result.stderr
+
+
+# ---------------------------------------------------------------- waits that run out
+def _limited_cases(native):
+    """(name, launch, outputs, what the outputs hold before the call) for every kind of tile, epilogue and layout."""
+    def filled(*shape, dtype=BF16):
+        return torch.empty(shape, dtype=dtype, device="cuda")
+
+    for m, k, n in ((16, 4096, 512), (16, 512, 16384), (100, 4096, 4096), (128, 64, 40000), (120, 64, 40001), (260, 320, 1000)):
+        a, b = randn((m, k), BF16, 1), randn((k, n), BF16, 2, k ** -0.5)
+        out, z = filled(m, n), filled(m, n, dtype=FP32)
+        yield f"epilogue {m}x{k}x{n}", native.prepare_epilogue(a, b, out, precision="bf16", preact=z), (out, z), None
+        dout, da, db, dbias = randn((m, n), BF16, 3), filled(m, k), filled(k, n), filled(n, dtype=FP32)
+        yield (f"backward {m}x{k}x{n}",
+               native.prepare_epilogue_backward(dout, a, b, precision="bf16", activation="silu", preact=dout, da=da, db=db,
+                                                dbias=dbias), (da, db, dbias), None)
+    for m, k, n in ((128, 64, 40000), (120, 64, 40001), (3000, 64, 8192), (3000, 64, 8190)):
+        a, b = randn((m, k), BF16, 1), randn((k, n), BF16, 2, k ** -0.5)
+        for dtype in (BF16, FP32):
+            residual, place = randn((m, n), dtype, 4), filled(m, n, dtype=dtype)
+            if m < 1000:
+                out = filled(m, n, dtype=dtype)
+                yield (f"residual {m}x{k}x{n} {dtype}",
+                       native.prepare_epilogue(a, b, out, precision="bf16", activation="relu", residual=residual), (out,), None)
+            yield (f"residual in place {m}x{k}x{n} {dtype}",
+                   native.prepare_epilogue(a, b, place, precision="bf16", residual=place), (place,), residual)
+    b, dout, da = randn((256, 20352), BF16, 2), randn((30, 20352), BF16, 3), filled(30, 256)
+    yield "chunks of a long sum", native.prepare_epilogue_backward(dout, b=b, precision="bf16", da=da), (da,), None
+    for sizes in ((10, 6), (500, 0, 600), (3, 1000, 1, 40)):
+        ends, offsets = sizes_to_offsets(sizes)
+        a, w = randn((ends[-1], 1024), BF16, 5), randn((len(sizes), 1024, 512), BF16, 6, 0.03)
+        out, dout = filled(ends[-1], 512), randn((ends[-1], 512), BF16, 7)
+        yield f"grouped {sizes}", native.prepare_grouped(a, w, offsets, out, precision="bf16"), (out,), None
+        da, dw = filled(ends[-1], 1024), filled(len(sizes), 1024, 512)
+        yield (f"grouped backward {sizes}",
+               native.prepare_grouped_backward(dout, a, w, offsets, precision="bf16", da=da, db=dw), (da, dw), None)
+    for m, k, v in ((100, 512, 20000), (100, 1024, 30001), (700, 64, 70000)):
+        hidden, weight, labels, grad = loss_inputs(m, k, v, "bf16")
+        loss, lse = filled(m, dtype=FP32), filled(m, dtype=FP32)
+        yield f"loss {m}x{k}x{v}", native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision="bf16"), (loss, lse), None
+        known = torch.logsumexp(hidden.float() @ weight.float(), 1)
+        dh, dw = filled(m, k), filled(k, v)
+        yield (f"loss backward {m}x{k}x{v}",
+               native.prepare_cross_entropy_backward(grad, hidden, weight, labels, known, precision="bf16", dhidden=dh,
+                                                     dweight=dw), (dh, dw), None)
+    a, b, out = randn((16, 2048), BF16, 1), odd_weight(2048, 20001, BF16, 1), filled(16, 20001)
+    yield "weight read in place", native.prepare_epilogue(a, b, out, precision="bf16"), (out,), None
+
+
+def check_limited(native, limits):
+    """For each limit and case: every element is NaN or what it is without a limit, NaN comes with a status, and the
+    next call is right.  Returns the status words met."""
+    reached = set()
+    for name, run, outs, before in _limited_cases(native):
+        def prepare():
+            for t in outs:
+                t.fill_(-12345.0) if before is None else t.copy_(before)
+            torch.cuda.synchronize()
+
+        prepare()
+        run()
+        torch.cuda.synchronize()
+        good = [t.clone() for t in outs]
+        assert native.device_status() == 0 and not any(bool(torch.isnan(t).any()) for t in good), name
+        for limit in limits:
+            prepare()
+            native.set_wait_limit(limit)
+            try:
+                run()
+                status = native.device_status()
+            finally:
+                native.set_wait_limit(0)
+            reached.add(status)
+            assert not status & DRAIN, f"{name}, {limit} ns: a drain wait ran out ({status:#x})"
+            lost = 0
+            for t, want in zip(outs, good):
+                nan = torch.isnan(t)
+                stale = ~nan & (t != want)
+                assert not bool(stale.any()), f"{name}, {limit} ns: {int(stale.sum())} of {t.numel()} elements are neither"
+                lost += int(nan.sum())
+            assert lost == 0 or status, f"{name}, {limit} ns: NaN without a status"
+        prepare()
+        run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(good, outs)) and native.device_status() == 0, name
+    return reached
+
+
+def test_every_element_that_a_short_wait_left_unfinished_is_nan(native):
+    """From one poll to a few microseconds (a pair of CTAs that gave up waits two seconds for copies under way)."""
+    assert any(status & (LOAD | MMA | EPILOGUE) for status in check_limited(native, (1, 2500)))
