@@ -1173,8 +1173,13 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 if (p.residual_tma && splits == 1)
                     fetch(0);
             int ok = 1;
-            if (issuer)       // one thread polls, the others wait at the barrier
-                ok = mbar_wait(accf_bar(acc), acc_phase, p.wait_limit_ns) ? 1 : 0;
+            if (issuer) {     // one thread polls, the others wait at the barrier
+                // The tile's whole K loop: a microsecond a K block on top of the default limit (the longest
+                // sums take 2^26 of them).
+                const int blocks = max(kb_end(w.nkb) - kb_begin, 0);
+                const uint64_t limit = p.wait_limit_ns < kWaitLimitNs ? p.wait_limit_ns : kWaitLimitNs + 1000ull * blocks;
+                ok = mbar_wait(accf_bar(acc), acc_phase, limit) ? 1 : 0;
+            }
             ok = epilogue_all(ok);
             if (!ok) {
                 if (issuer) {

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 import operator_reference as ref
+from operator_contracts import SIZE_MAX
 from operator_reference import DTYPES, assert_within
 from test_operators_gpu import guarded, loss_inputs, randn, sizes_to_offsets
 from test_operators_use_gpu import odd_weight
@@ -313,3 +314,27 @@ def check_limited(native, limits):
 def test_every_element_that_a_short_wait_left_unfinished_is_nan(native):
     """From one poll to a few microseconds (a pair of CTAs that gave up waits two seconds for copies under way)."""
     assert any(status & (LOAD | MMA | EPILOGUE) for status in check_limited(native, (1, 2500)))
+
+
+def test_a_tile_whose_sum_takes_seconds(native):
+    """Sums of the largest length that are not split over CTAs: one tile runs 2^25 K blocks, longer than the limit of
+    waits for progress.  Exact in FP32."""
+    k, v = SIZE_MAX, 8
+    at = torch.tensor([0, 63, 64, 12345, 1 << 30, k - 1], device="cuda")
+    tall, row = torch.ones((k, v), dtype=BF16, device="cuda"), torch.zeros((1, k), dtype=BF16, device="cuda")
+    row[0, at] = 1.0
+    tall[at] = torch.arange(48, device="cuda").to(BF16).view(6, 8) / 16
+    want = tall[at].sum(0, dtype=FP32)
+    loss, lse = torch.empty(1, device="cuda"), torch.empty(1, device="cuda")
+    native.prepare_cross_entropy(row, tall, torch.tensor([2], device="cuda"), loss, lse, precision="bf16")()
+    assert native.device_status() == 0
+    assert_within(lse, torch.logsumexp(want.double(), 0)[None], torch.full((1,), 600 * ref.U, device="cuda").double(), "lse")
+    offsets = torch.tensor([0, 1], device="cuda")
+    out = torch.zeros((1, v), device="cuda")
+    native.prepare_grouped(row, tall.view(1, k, v), offsets, out, precision="bf16")()
+    assert native.device_status() == 0 and torch.equal(out[0], want)
+    column, db = row.view(k, 1).expand(k, 8).contiguous(), torch.zeros((1, 8, v), device="cuda")
+    del row
+    offsets[1] = k
+    native.prepare_grouped_backward(tall, column, None, offsets, precision="bf16", db=db)()
+    assert native.device_status() == 0 and torch.equal(db[0], want.expand(8, v))
