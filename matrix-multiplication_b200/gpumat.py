@@ -352,6 +352,9 @@ class NativeMatmul:
         """
         precision_id = self._operator_precision(precision)
         m, k, n = validate_epilogue_backward(dout, a, b, precision, self._device, activation, preact, da, db, dbias)
+        # What no gradient reads was not checked: it does not reach the library.
+        a, b = a if db is not None else None, b if da is not None else None
+        preact = preact if activation != "none" else None
         return self._operator("matmul_epilogue_backward",
                               (precision_id, _ptr(dout), _ptr(a), _ptr(b), _ptr(preact), _fp32(preact),
                                ACTIVATION_IDS[activation], _ptr(da), _fp32(da), _ptr(db), _fp32(db), _ptr(dbias),
@@ -382,6 +385,7 @@ class NativeMatmul:
         """
         precision_id = self._operator_precision(precision)
         rows, groups, k, n = validate_grouped_backward(dout, a, b, offsets, precision, self._device, da, db)
+        a, b = a if db is not None else None, b if da is not None else None      # as in prepare_epilogue_backward
         return self._operator("matmul_grouped_backward",
                               (precision_id, _ptr(dout), _ptr(a), _ptr(b), _ptr(offsets),
                                int(offsets.dtype == torch.int64), groups, _ptr(da), _fp32(da), _ptr(db), _fp32(db),

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import operator_contracts as ops
-from gpumat import load_library
+from gpumat import NativeMatmul, load_library
 
 
 def _call(library, name, *args):
@@ -36,3 +36,26 @@ def test_more_groups_than_a_plan_counts_are_refused(library_path, monkeypatch, g
         ops.validate_grouped(rows, b, offsets, rows, "bf16", 0)
     with pytest.raises(ValueError, match="groups must be at most 268435456"):
         ops.validate_grouped_backward(rows, rows, None, offsets, "bf16", 0, db=b)
+
+
+def test_operands_that_no_gradient_reads_may_be_anything(monkeypatch):
+    """They are not checked, so they do not reach the library either: a tensor on another device could not be recorded
+    on the stream, and what is no tensor has no pointer."""
+    monkeypatch.setattr(ops, "_check", lambda *args: None)
+    taken = []
+    native = object.__new__(NativeMatmul)
+    native._device = 0
+    monkeypatch.setattr(NativeMatmul, "_operator_precision", lambda self, precision: 3)
+    monkeypatch.setattr(NativeMatmul, "_operator",
+                        lambda self, name, arguments, tensors, outputs: taken.append([t for t in tensors if t is not None]))
+    a, b, dout = torch.ones((4, 8)), torch.ones((8, 16)), torch.ones((4, 16))
+    da, db, dbias = torch.empty((4, 8)), torch.empty((8, 16)), torch.empty(16)
+    for unread in (torch.ones(3), "no tensor", 7):
+        native.prepare_epilogue_backward(dout, a, unread, precision="bf16", preact=unread, db=db)
+        native.prepare_epilogue_backward(dout, unread, b, precision="bf16", preact=unread, da=da)
+        native.prepare_epilogue_backward(dout, unread, unread, precision="bf16", preact=unread, dbias=dbias)
+        experts, offsets = torch.ones((2, 8, 16)), torch.zeros(3, dtype=torch.int32)
+        native.prepare_grouped_backward(dout, a, unread, offsets, precision="bf16", db=torch.empty((2, 8, 16)))
+        native.prepare_grouped_backward(dout, unread, experts, offsets, precision="bf16", da=da)
+        assert len(taken) == 5 and not any(t is unread for tensors in taken for t in tensors)
+        taken.clear()
