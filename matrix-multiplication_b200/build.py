@@ -35,10 +35,15 @@ def nvcc() -> str:
     return str(candidate) if candidate.exists() else (shutil.which("nvcc") or "nvcc")
 
 
+COMPILE_FLAGS = ["-O3", "-std=c++17", *ARCH_FLAGS, "-lineinfo", "-Xcompiler", "-fPIC", "-I", str(ROOT / "include")]
+LINK_FLAGS = [*ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-cudart", "static"]
+
+
 def command(output: Path = OUTPUT, verbose_ptxas: bool = False) -> list[str]:
-    """The one-step form of the build: every source into the shared library."""
-    cmd = [nvcc(), "-O3", "-std=c++17", *ARCH_FLAGS, "-lineinfo", "-shared", "-Xcompiler", "-fPIC",
-           "-cudart", "static", "-I", str(ROOT / "include"), "-o", str(output), *map(str, SOURCES)]
+    """The one-step form of the build, with the flags of both of its steps (``build`` itself compiles the sources in
+    parallel)."""
+    cmd = [nvcc(), *COMPILE_FLAGS, *(flag for flag in LINK_FLAGS if flag not in COMPILE_FLAGS), "-o", str(output),
+           *map(str, SOURCES)]
     if verbose_ptxas:
         cmd[1:1] = ["-Xptxas", "-v"]
     return cmd
@@ -46,16 +51,14 @@ def command(output: Path = OUTPUT, verbose_ptxas: bool = False) -> list[str]:
 
 def compile_command(source: Path, target: Path, verbose_ptxas: bool = False) -> list[str]:
     """One source into an object file."""
-    cmd = [nvcc(), "-O3", "-std=c++17", *ARCH_FLAGS, "-lineinfo", "-Xcompiler", "-fPIC", "-I", str(ROOT / "include"),
-           "-c", "-o", str(target), str(source)]
+    cmd = [nvcc(), *COMPILE_FLAGS, "-c", "-o", str(target), str(source)]
     if verbose_ptxas:
         cmd[1:1] = ["-Xptxas", "-v"]
     return cmd
 
 
 def link_command(objects: list[Path], output: Path) -> list[str]:
-    return [nvcc(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-cudart", "static", "-o", str(output),
-            *map(str, objects)]
+    return [nvcc(), *LINK_FLAGS, "-o", str(output), *map(str, objects)]
 
 
 def up_to_date(output: Path = OUTPUT) -> bool:

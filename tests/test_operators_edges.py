@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+from pathlib import Path
 
 import pytest
 import torch
@@ -59,3 +60,26 @@ def test_operands_that_no_gradient_reads_may_be_anything(monkeypatch):
         native.prepare_grouped_backward(dout, unread, experts, offsets, precision="bf16", da=da)
         assert len(taken) == 5 and not any(t is unread for tensors in taken for t in tensors)
         taken.clear()
+
+
+def test_every_command_of_the_build_is_sm100a_only(monkeypatch, tmp_path):
+    """The commands that build() runs, and no others: each source compiled once, all objects linked, for one
+    architecture."""
+    import build
+
+    ran = []
+
+    def run(cmd):
+        ran.append(cmd)
+        Path(cmd[cmd.index("-o") + 1]).touch()
+        return ""
+
+    monkeypatch.setattr(build, "_run", run)
+    output = build.build(force=True, output=tmp_path / "library.so")
+    assert output.exists() and len(ran) == len(build.SOURCES) + 1
+    compiles, link = ran[:-1], ran[-1]
+    assert sorted(cmd[-1] for cmd in compiles) == sorted(map(str, build.SOURCES)) and all("-c" in cmd for cmd in compiles)
+    assert sorted(link[link.index("-o") + 2:]) == sorted(cmd[cmd.index("-o") + 1] for cmd in compiles) and "-shared" in link
+    for cmd in (*ran, build.command()):
+        assert cmd.count("-gencode") == 1 and cmd[cmd.index("-gencode") + 1] == "arch=compute_100a,code=sm_100a"
+        assert not any(flag.startswith(("-arch", "--gpu", "-code", "--generate-code", "-gencode=")) for flag in cmd)
