@@ -338,3 +338,26 @@ def test_a_tile_whose_sum_takes_seconds(native):
     offsets[1] = k
     native.prepare_grouped_backward(tall, column, None, offsets, precision="bf16", db=db)()
     assert native.device_status() == 0 and torch.equal(db[0], want.expand(8, v))
+
+
+# ---------------------------------------------------------------- uneven groups
+@pytest.mark.parametrize("precision", ("bf16", "tf32"))
+@pytest.mark.parametrize("groups,rows,hot", [(400, 3001, 2900), (300, 700, 690), (64, 2048, 1024), (513, 20000, 19480)])
+def test_one_group_with_most_of_the_rows(native, precision, groups, rows, hot):
+    """Tiles follow the mean group; a group of many times the mean is cut into as many of them as it takes, in both
+    directions, wherever it stands."""
+    k, n, dtype = 136, 200, DTYPES[precision]
+    a, b, dout = randn((rows, k), dtype, 1), randn((groups, k, n), dtype, 2, k ** -0.5), randn((rows, n), dtype, 3)
+    for where in (0, groups // 2, groups - 1):
+        gen = torch.Generator().manual_seed(where)
+        sizes = torch.bincount(torch.randint(0, groups, (rows - hot,), generator=gen), minlength=groups)
+        sizes[where] += hot
+        ends, offsets = sizes_to_offsets(sizes.tolist())
+        (out, uo), (da, ua), (db, ub) = guarded((rows, n), FP32), guarded((rows, k), FP32), guarded((groups, k, n), FP32)
+        native.prepare_grouped(a, b, offsets, out, precision=precision)()
+        native.prepare_grouped_backward(dout, a, b, offsets, precision=precision, da=da, db=db)()
+        assert_within(out, *ref.grouped(a, b, ends, precision, out), "out")
+        (eda, tda), (edb, tdb) = ref.grouped_backward(dout, a, b, ends, precision, da)
+        assert_within(da, eda, tda, "da")
+        assert_within(db, edb, tdb, "db")
+        uo(), ua(), ub()
