@@ -124,7 +124,8 @@ int matmul_set_sm_limit(void *context, int sms, char *error, size_t error_size);
  * matmul_device_status), writes NaN over every output element it did not
  * finish, releases its tensor memory and returns, so that the context stays
  * usable and an FP64 check of C fails.  For watchdog tests and for callers that
- * want a kernel to give up sooner.  The FFMA kernel's TMA-staged 128 x 128 tile
+ * want a kernel to give up sooner.  The operators' wait for a tile's sum has a
+ * microsecond per 128-byte block of it on top of the default.  The FFMA kernel's TMA-staged 128 x 128 tile
  * (16-byte aligned operands) bounds its stage waits the same way; its cp.async
  * forms have no waits. */
 int matmul_set_wait_limit(void *context, unsigned long long nanoseconds, char *error, size_t error_size);

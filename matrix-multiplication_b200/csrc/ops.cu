@@ -893,7 +893,10 @@ int check_groups(Call &c, int groups, int rows, int k, int n, const void *offset
 // wide) and the weight's columns its M side, so that a tile wastes little (64 groups, 2048 x
 // 2816 BF16: mean 50 rows 100 us on 64-row transposed tiles, 118 us on pairs; mean
 // 100 rows 124 us on 128-row ones, 129 us on pairs; mean 200 rows 198 and 163 us).  Larger
-// groups go by the cycles of a mean group.
+// groups go by the cycles of a mean group.  The loads themselves are known on the device
+// alone, so a group of many times the mean runs on its narrow tiles and reads its weight once
+// for each (4096 rows over 64 experts, 2048 x 2816: 122 us evenly spread, 151 with half of the
+// rows in one expert, 179 with nine tenths; 8192 over 512, 1024 x 1024: 168, 213 and 254).
 int choose_grouped_tile(const Context *ctx, int64_t rows, int64_t groups, int64_t n, int64_t k_blocks, int bytes_out,
                         bool out_tma)
 {
@@ -1147,8 +1150,10 @@ extern "C" int matmul_cross_entropy_backward(void *opaque, int precision, const 
     if (device.status != cudaSuccess)
         return c.failed(device.status);
     const int64_t bk = OP_ROW_BYTES / e;
-    // Vocabulary pieces: the logits' gradients of one piece (m x width, input format) take
-    // about 64 MB, so that the two products that read them find them in L2.
+    // Vocabulary pieces: the logits' gradients of one piece (m x width, input format) take at
+    // most 64 MB, so that the two products that read them find them in L2, but a piece has
+    // 4096 columns at least (fewer would make dhidden's sum over the pieces dear): from 8193
+    // BF16 or 4097 TF32 rows on its scratch is 8 or 16 KB a row, and L2 holds a part of it.
     constexpr int64_t kPieceBytes = int64_t{64} << 20;
     int64_t width = kPieceBytes / (static_cast<int64_t>(m) * e) / 256 * 256;
     width = std::max<int64_t>(width, 4096);

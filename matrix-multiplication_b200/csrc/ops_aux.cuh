@@ -91,8 +91,10 @@ struct ActGradParams {
     int vec;                      // rows of dout and preact start on 16 bytes
 };
 
-// dz = dout * act'(z) in the input format, and the column sums of the unrounded FP32
-// values: each thread takes 8 columns and every 32nd row of its block's chunk, four rows in
+// dz = dout * act'(z) in the input format, which both products that read it need (an FP32
+// dz would take two of each, for its high and its low part; as it is, da and db are off by
+// about the square root of two of their own rounding), and the column sums of the unrounded
+// FP32 values: each thread takes 8 columns and every 32nd row of its block's chunk, four rows in
 // flight; a block's 32 row positions join through its shared memory and the blocks of a
 // cluster (along y) through each other's, both in a fixed order.  Bound by HBM: two reads
 // and a write.

@@ -18,7 +18,7 @@ struct OpInstances {
         using Tile = OpTile<CTAS, BN, DIRECT>;
         return f(&op_kernel<FMT, CTAS, BN, A_MN, B_MN, EPI, DIRECT>, CTAS, Tile::kThreads, Tile::kSmem);
     }
-    // Kernels that load B themselves (can_load_directly).
+    // Kernels that load B themselves (chosen by direct_pays).
     template <typename F>
     static cudaError_t with_direct(int tile, int epilogue, F &&f)
     {

@@ -59,9 +59,9 @@ constexpr int OP_BAR_BYTES = 512;
 // one warpgroup needs longer for an activation and two outputs than the MMAs of a
 // 4096-deep 256 x 256 tile (4096 x 4096 x 14336 BF16 with gelu, bias and pre-activation:
 // 609 us with one, 496 us with two).  A 256 x 512 pair tile (one accumulator, freed half
-// by half, as in tc2_gemm.cuh) was built and taken out: 311 us against 323 us at 4096 x
-// 4096 x 14336 BF16, 695 against 714 us at 8192^3, ahead by 1 % at most where its count
-// of tiles fits the pairs better.
+// by half, as in tc2_gemm.cuh) was built and taken out: once one elected thread issued the
+// instructions it was ahead of 256 x 256 by 1 % at most, where its count of tiles fits the
+// pairs better.
 //
 // DIRECT: B (16-bit, 128 columns a tile) has rows that start on any element, which TMA
 // cannot address.  Two more warps fetch the aligned 16-byte pieces that a K block's rows lie
@@ -1274,12 +1274,13 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     ++box_done;
                     return true;
                 };
-                // 128 bytes of each row, 32 FP32 or 64 16-bit columns, at any element alignment, without TMA.  Each warp puts its own 32 rows into the boxes' memory at a pitch
-                // of 33 words, then eight lanes take a row: a lane moves one 16-byte chunk that is
-                // aligned in memory (words from shared memory, shifted by half a word where the row
-                // starts on an odd element), and the up to 15 bytes at either end go element by
-                // element.  No bank conflicts either way.  (One row per instruction with 4-byte words
-                // took 13000 cycles for a 128 x 128 tile of 16-bit outputs.)
+                // 128 bytes of each row, 32 FP32 or 64 16-bit columns, at any element alignment, without
+                // TMA.  Each warp puts its own 32 rows into the boxes' memory at a pitch of 33 words,
+                // then eight lanes take a row: a lane moves one 16-byte chunk that is aligned in memory
+                // (words from shared memory, shifted by half a word where the row starts on an odd
+                // element), and the up to 15 bytes at either end go element by element.  No bank
+                // conflicts either way.  (One row per instruction with 4-byte words took 13000 cycles
+                // for a 128 x 128 tile of 16-bit outputs.)
                 auto emit_unaligned = [&](const uint32_t (&words)[32], bool half, void *dst, long long at0,
                                           long long pitch, int col0) {
                     if (p.out_tma | p.preact_tma) {       // the other output's boxes leave by TMA
@@ -1446,7 +1447,10 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     if (col0 >= p.n || row0 >= w.row_end)      // the same for all four warps
                         return true;
                     if constexpr (EPI == kEpiSoftmaxGrad) {
-                        // dz = (exp(z - lse) - [column == label]) grad.  The exponential is taken 2^24 times too
+                        // dz = (exp(z - lse) - [column == label]) grad, rounded to the input format because
+                        // both products that read it take operands of that format (an FP32 dz would take
+                        // two of each, for its high and its low part); the gradients are off by about the
+                        // square root of two of their own rounding.  The exponential is taken 2^24 times too
                         // large and grad as much too small, so that only their product, not the
                         // hardware's exponential, falls below the normal numbers.  An ignored row's
                         // gradient is zero whatever its logits are.

@@ -6,9 +6,11 @@ The allowances follow from the arithmetic, not from observed errors:
   (k + 2) u |A||B|;
 * a rounding to a format is off by at most half a step, finfo.eps / 2 of the value, or half its smallest
   subnormal;
-* the exponential the kernels call has an error of 2 + 1.2 |x| ulp, erf one of 2 ulp, and an activation is a few
-  FP32 operations on them: (8 + 4 |z| + |z|^3) u |z| covers each of them (the cube from gelu_tanh's argument),
-  twice that with |z| + 1 its slope; both have slopes below 1.2.
+* the kernels' exponential and reciprocal are the hardware's approximations (2 u and u, and the rounding of the
+  exponent, 1.2 |x| u), their normal distribution function is off by (12 + z^2 / 2) u of its smaller side, and an
+  activation is a few FP32 operations on them: (8 + 4 |z| + |z|^3) u |z| covers each of them (the cube from gelu_tanh's
+  argument; gelu's own error is largest against it at z = 0, where 12 u Phi(-|z|) is 6 u), twice that with |z| + 1 its
+  slope; both have slopes below 1.2.
 """
 
 from __future__ import annotations
