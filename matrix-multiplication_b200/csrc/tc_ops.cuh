@@ -1086,6 +1086,9 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const bool issuer_warp = gthread < 32;
         const bool issuer = issuer_warp && op_elect_one();
         const uint32_t s_box = s_epi + group * kBoxes * OP_BOX;
+        // A warpgroup's own part whatever a tile's width is: the warpgroups do not wait for each other, so
+        // one may be at the half tile after the other's whole one.
+        float *group_bias = bias_s + group * kGroupCols;
         auto epilogue_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
         // 1 only if every thread of the warpgroup passes 1.
         auto epilogue_all = [&](int ok) {
@@ -1130,12 +1133,12 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             if constexpr (EPI == kEpiStore) {
                 if (p.bias) {       // the tile's bias, read once into shared memory
                     epilogue_sync();
-                    for (int c = gcol + gthread; c < gcol + group_cols; c += 128) {
-                        const int col = w.n0 + c;
+                    for (int c = gthread; c < group_cols; c += 128) {
+                        const int col = w.n0 + gcol + c;
                         float b = 0.0f;
                         if (col < p.n)
                             b = load_bias(col);
-                        bias_s[c] = b;
+                        group_bias[c] = b;
                     }
                     epilogue_sync();
                 }
@@ -1478,7 +1481,7 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                         }
                     } else {
                         if (p.bias) {
-                            const float4 *b4 = reinterpret_cast<const float4 *>(bias_s + gcol + step * 64);
+                            const float4 *b4 = reinterpret_cast<const float4 *>(group_bias + step * 64);
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
                                 const float4 b = b4[j];

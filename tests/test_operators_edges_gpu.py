@@ -361,3 +361,32 @@ def test_one_group_with_most_of_the_rows(native, precision, groups, rows, hot):
         assert_within(da, eda, tda, "da")
         assert_within(db, edb, tdb, "db")
         uo(), ua(), ub()
+
+
+# ---------------------------------------------------------------- bias of whole and half tiles
+@pytest.mark.parametrize("precision", ("bf16", "fp16", "tf32"))
+@pytest.mark.parametrize("m,k,n", [(2304, 2048, 384), (4352, 1024, 384), (2304, 2048, 640), (2100, 600, 1400)])
+def test_bias_where_half_tiles_follow_whole_ones(native, precision, m, k, n):
+    """Eight pairs of CTAs, whose last round runs as halves of tiles in other columns than the tiles before them.  A
+    warpgroup without columns in the last whole tile is at its half tile while the other still adds the whole
+    tile's bias: each reads its own."""
+    dtype = DTYPES[precision]
+    a, b, bias = randn((m, k), dtype, 1), randn((k, n), dtype, 2, k ** -0.5), randn((n,), FP32, 3, 5.0)
+    native.set_sm_limit(16)
+    try:
+        for act, out_dtype, has_preact in (("gelu", dtype, True), ("none", dtype, False), ("silu", FP32, False)):
+            out = torch.empty((m, n), dtype=out_dtype, device="cuda")
+            preact = torch.empty((m, n), device="cuda") if has_preact else None
+            run = native.prepare_epilogue(a, b, out, precision=precision, bias=bias, activation=act, preact=preact)
+            run()
+            expected = ref.epilogue(a, b, precision, bias, act)
+            assert_within(out, *expected["out"], f"out {act}")
+            first = out.clone()
+            for _ in range(40):
+                out.zero_()
+                run()
+                assert torch.equal(out, first)
+            if has_preact:
+                assert_within(preact, *expected["preact"], "preact")
+    finally:
+        native.set_sm_limit(0)
