@@ -1601,24 +1601,6 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 bool held = true;
                 const int row = row0 + r;
                 const int chunks = min(kGroupCols / 32, (p.n - w.n0 - gcol + 31) / 32);   // below 1: none in the matrix
-                // The same in two passes from the row's maximum in the tile, for far maxima.
-                auto reduce_far = [&]() {
-                    const bool far = op_far(top);
-                    const float from = far ? op_far_origin(top) : op_origin(top);
-                    sum = 0.0f;
-#pragma unroll 1
-                    for (int c = 0; c < 2 * chunks; ++c) {
-                        uint32_t u[16];
-                        tmem_load_16cols(t_row + c * 16, u);
-                        const int cols = p.n - w.n0 - gcol - c * 16;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const float x = __uint_as_float(u[j]);
-                            const float t = far ? (x - from) * kLog2E : __fmaf_rn(x, kLog2E, -from);
-                            sum += j < cols ? op_exp2(t) : 0.0f;
-                        }
-                    }
-                };
 #pragma unroll 1
                 for (int chunk = 0; chunk < chunks; ++chunk) {
                     uint32_t u[32];
@@ -1645,11 +1627,8 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     for (int j = 0; j < 32; ++j)
                         chunk_top = fmaxf(chunk_top, x[j]);
                     top = fmaxf(top, chunk_top);
-                    if (chunk == chunks - 1) {
-                        if (__any_sync(0xffffffffu, op_far(top))) {
-                            reduce_far();
-                            break;
-                        }
+                    // (Lanes past the matrix may hold anything.)
+                    if (chunk == chunks - 1 && !__any_sync(0xffffffffu, op_far(top) && row < p.m)) {
                         release();
                         held = false;
                     }
@@ -1666,8 +1645,24 @@ op_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                     }
                     sum += (chain[0].x + chain[0].y) + (chain[1].x + chain[1].y);
                 }
-                if (held)
+                if (held) {
+                    // Rows with a far maximum take a second pass from it; the others keep their sums, so that
+                    // no row's result depends on another row.
+                    const float from = op_far_origin(top);
+                    float far_sum = 0.0f;
+#pragma unroll 1
+                    for (int c = 0; c < 2 * chunks; ++c) {
+                        uint32_t u[16];
+                        tmem_load_16cols(t_row + c * 16, u);
+                        const int cols = p.n - w.n0 - gcol - c * 16;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            far_sum += j < cols ? op_exp2((__uint_as_float(u[j]) - from) * kLog2E) : 0.0f;
+                    }
+                    if (op_far(top))
+                        sum = far_sum;
                     release();
+                }
                 if (row < p.m)
                     p.partial[static_cast<long long>(w.n_block * kGroups + group) * p.m + row] = make_float2(top, sum);
             }

@@ -108,6 +108,32 @@ def test_loss_between_the_ends_of_the_range(native):
         assert float(loss[3]) == float("inf") and float(loss.nan_to_num(posinf=0.0).abs().sum()) == 0.0
 
 
+@pytest.mark.parametrize("m,k,v", [(1, 16, 11), (5, 98, 222), (24, 267, 2408), (56, 109, 5175), (200, 64, 33000), (90, 64, 20001)])
+def test_loss_of_a_row_depends_on_its_own_logits_alone(native, m, k, v):
+    """Bit by bit the same after other calls, which leave other values in the memory behind the last row, and beside rows
+    whose logits are at the ends of FP32's range."""
+    hidden, weight, labels, _ = loss_inputs(m, k, v, "bf16")
+    other = torch.full((200, k), 3e38, dtype=BF16, device="cuda")
+    big = torch.full((k, v), 1.0, dtype=BF16, device="cuda")
+    junk = torch.empty((200, v), dtype=BF16, device="cuda")
+    loss, lse = torch.empty(m, device="cuda"), torch.empty(m, device="cuda")
+    run = native.prepare_cross_entropy(hidden, weight, labels, loss, lse, precision="bf16")
+    dirty = native.prepare_epilogue(other, big, junk, precision="bf16")
+    run()
+    first = loss.clone(), lse.clone()
+    for _ in range(20):
+        loss.zero_(), lse.zero_()
+        torch.cuda.synchronize()
+        dirty()
+        run()
+        assert torch.equal(loss, first[0]) and torch.equal(lse, first[1])
+    if m > 2:
+        hidden[m // 2] = 1e38
+        run()
+        rows = torch.arange(m, device="cuda") != m // 2
+        assert torch.equal(loss[rows], first[0][rows]) and torch.equal(lse[rows], first[1][rows])
+
+
 # ---------------------------------------------------------------- the activations' ends
 @pytest.mark.parametrize("m", (1, 70, 300))
 def test_gelu_keeps_its_relative_precision_in_the_tails(native, m):
