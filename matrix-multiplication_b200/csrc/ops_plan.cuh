@@ -40,12 +40,11 @@ constexpr int GP_EPILOGUE_BLOCKS = 6;
 // Group g's rows are [max(offsets[0..g]), max(offsets[0..g+1])) clipped to
 // [0, rows], so that whatever the offsets hold, groups are disjoint, in order and in
 // range.  Rows mode writes ceil(rows of g / tile_rows) entries per group, in order, one
-// thread a group;
-// ragged-K mode one entry per group (`unused` = K blocks and epilogues of a tile of each
-// group before it, summed) and each unit's share: consecutive tiles of about the same
-// total weight, so that a unit meets few groups (each costs it two tensor-map fences
-// before its loads can start: with tiles dealt out in turn, 64 groups of 256 rows took
-// 420 us on 2048 x 2816 outputs).  Each group's tensor maps are the templates with the
+// thread a group; ragged-K mode one entry per group (`unused` = K blocks and epilogues of a
+// tile of each group before it, summed) and each unit's share: consecutive tiles of about
+// the same total weight, so that a unit meets few groups (each costs it two tensor-map
+// fences before its loads can start: with tiles dealt out in turn, 64 groups of 256 rows
+// took 420 us on 2048 x 2816 outputs).  Each group's tensor maps are the templates with the
 // row extent cut at the group's end.  Every block computes the ends; block 0 writes the
 // tables, all blocks share the maps.
 __global__ void __launch_bounds__(GP_THREADS) group_plan_kernel(const __grid_constant__ CUtensorMap map0,
